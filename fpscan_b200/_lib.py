@@ -15,6 +15,7 @@ LIB_PATH = _build.LIB_PATH
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
+_c_float = ctypes.c_float
 _vp = ctypes.c_void_p
 
 # name -> argtypes; every function returns int except fpscan_last_error
@@ -34,6 +35,16 @@ SIGNATURES = {
     "fpscan_scan_fwd_cl": [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp],
     "fpscan_scan_bwd_cl": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _c_i64,
                            _vp],
+    "fpscan_scan_fwd_cl8": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _c_i64,
+                            _vp],
+    "fpscan_scan_bwd_cl8": [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp,
+                            _c_i64, _vp],
+    "fpscan_quantize8": [_vp, _vp, _vp, _c_i64, _c_int, _vp],
+    "fpscan_dequantize8": [_vp, _vp, _vp, _c_i64, _c_int, _vp],
+    "fpscan_delta_workspace_bytes": [_c_i64] * 6 + [_c_int] * 3,
+    "fpscan_delta_fwd": [_vp] * 8 + [_c_i64] * 6 + [_c_float, _c_int, _c_int, _vp, _c_i64, _vp],
+    "fpscan_delta_bwd": [_vp] * 14 + [_c_i64] * 6 + [_c_float, _c_int, _c_int, _vp, _c_i64, _vp],
+    "fpscan_delta_step": [_vp] * 8 + [_c_i64] * 6 + [_c_float, _c_int, _vp],
     "fpscan_scan_bwd": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp],
     "fpscan_scan_bwd_workspace_bytes": [_c_i64, _c_i64, _c_i64, _c_int],
     "fpscan_scan_bwd_ws": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _c_i64,
@@ -74,6 +85,7 @@ _RESTYPES = {"fpscan_last_error": ctypes.c_char_p,
              "fpscan_scan_fwd_workspace_bytes": ctypes.c_int64,
              "fpscan_scan_bwd_workspace_bytes": ctypes.c_int64,
              "fpscan_cl_workspace_bytes": ctypes.c_int64,
+             "fpscan_delta_workspace_bytes": ctypes.c_int64,
              "fpscan_link_bytes": ctypes.c_int64}
 
 

@@ -780,6 +780,316 @@ int fpscan_scan_bwd_cl(const void* gates, const void* y, const void* grad_out, v
 
 }  // extern "C"
 
+// ------------------------------------------------------------------ gated delta rule
+namespace {
+
+// One tensor of a call: its name, address, bytes, and whether it is written.
+struct Operand {
+  const char* name;
+  const void* ptr;
+  int64_t bytes;
+  bool written;
+};
+
+// Every operand present (ptr non-null), 16-byte aligned, and none that is
+// written overlapping another.
+template <size_t N>
+int check_operands(const Operand (&ops)[N]) {
+  for (const Operand& o : ops)
+    if (o.bytes > 0) FPSCAN_TRY(check_ptr(o.ptr, o.name));
+  for (size_t i = 0; i < N; ++i)
+    for (size_t j = 0; j < i; ++j) {
+      const Operand &a = ops[i], &b = ops[j];
+      if ((!a.written && !b.written) || a.bytes <= 0 || b.bytes <= 0) continue;
+      const Span x{a.name, (uintptr_t)a.ptr, (uintptr_t)a.ptr + (uintptr_t)a.bytes};
+      const Span y{b.name, (uintptr_t)b.ptr, (uintptr_t)b.ptr + (uintptr_t)b.bytes};
+      if (overlaps(x, y)) return fail(FPSCAN_ERR_INVALID, "%s overlaps %s", a.name, b.name);
+    }
+  return FPSCAN_OK;
+}
+
+int check_delta(int64_t batch, int64_t seqlen, int64_t key_heads, int64_t heads, int64_t dk,
+                int64_t dv, int dtype) {
+  FPSCAN_TRY(check_dtype(dtype));
+  if (batch < 0 || seqlen < 1)
+    return fail(FPSCAN_ERR_INVALID, "batch (%lld) must be non-negative and seqlen (%lld) >= 1",
+                (long long)batch, (long long)seqlen);
+  if (key_heads < 1 || heads < 1 || heads % key_heads != 0)
+    return fail(FPSCAN_ERR_INVALID, "heads (%lld) must be a positive multiple of key_heads (%lld)",
+                (long long)heads, (long long)key_heads);
+  if (dk < 8 || dk > 128 || dk % 8 != 0)
+    return fail(FPSCAN_ERR_INVALID, "dk must be a multiple of 8 in [8, 128] (got %lld)",
+                (long long)dk);
+  if (dv < 8 || dv > 65536 || dv % 8 != 0)
+    return fail(FPSCAN_ERR_INVALID, "dv must be a multiple of 8 in [8, 65536] (got %lld)",
+                (long long)dv);
+  const int64_t kMax = int64_t(1) << 31;
+  if (batch >= kMax || seqlen >= kMax || heads >= (int64_t(1) << 16))
+    return fail(FPSCAN_ERR_INVALID, "batch and seqlen must be below 2^31 and heads below 2^16");
+  // one CTA per (chunk, head) and per (32 values, head) at most
+  const int64_t bh = batch * heads, chunks = (seqlen + 63) / 64;
+  if (bh != 0 && (chunks >= kMax / bh || (dv + 31) / 32 >= kMax / bh))
+    return fail(FPSCAN_ERR_INVALID, "batch * heads too large for the launch grid");
+  return FPSCAN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fpscan_delta_workspace_bytes(int64_t batch, int64_t seqlen, int64_t key_heads,
+                                     int64_t heads, int64_t dk, int64_t dv, int dtype, int wide,
+                                     int backward) {
+  if (check_delta(batch, seqlen, key_heads, heads, dk, dv, dtype) != FPSCAN_OK || batch == 0)
+    return 0;
+  return delta_plan(batch, seqlen, key_heads, heads, dk, dv, dtype, wide != 0, backward != 0).bytes;
+}
+
+int fpscan_delta_fwd(const void* q, const void* k, const void* v, const void* log_decay,
+                     const void* beta, const float* initial, void* out, float* final_state,
+                     int64_t batch, int64_t seqlen, int64_t key_heads, int64_t heads, int64_t dk,
+                     int64_t dv, float scale, int dtype, int wide, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  FPSCAN_TRY(check_delta(batch, seqlen, key_heads, heads, dk, dv, dtype));
+  if (batch == 0) return ok();
+  const DeltaPlan pl =
+      delta_plan(batch, seqlen, key_heads, heads, dk, dv, dtype, wide != 0, false);
+  if (workspace_bytes < pl.bytes)
+    return fail(FPSCAN_ERR_INVALID, "workspace too small: %lld bytes, need %lld",
+                (long long)workspace_bytes, (long long)pl.bytes);
+  const int64_t es = dtype_size(dtype), tok = batch * seqlen, st = batch * heads * dv * dk * 4;
+  const Operand ops[] = {{"q", q, tok * key_heads * dk * es, false},
+                         {"k", k, tok * key_heads * dk * es, false},
+                         {"v", v, tok * heads * dv * es, false},
+                         {"log_decay", log_decay, tok * heads * es, false},
+                         {"beta", beta, tok * heads * es, false},
+                         {"initial", initial, initial ? st : 0, false},
+                         {"out", out, tok * heads * dv * es, true},
+                         {"final_state", final_state, final_state ? st : 0, true},
+                         {"workspace", workspace, pl.bytes, true}};
+  FPSCAN_TRY(check_operands(ops));
+  DeltaArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.log_decay = log_decay;
+  a.beta = beta;
+  a.initial = initial;
+  a.out = out;
+  a.final_state = final_state;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  a.batch = batch;
+  a.seqlen = seqlen;
+  a.key_heads = key_heads;
+  a.heads = heads;
+  a.dk = dk;
+  a.dv = dv;
+  a.scale = scale;
+  a.dtype = dtype;
+  a.wide = wide != 0;
+  a.num_sms = num_sms_current();
+  a.stream = static_cast<cudaStream_t>(stream);
+  return cuda_result(launch_delta_fwd(a), "fpscan_delta_fwd launch");
+}
+
+int fpscan_delta_bwd(const void* q, const void* k, const void* v, const void* log_decay,
+                     const void* beta, const float* initial, const void* grad_out,
+                     const float* grad_final, void* dq, void* dk_out, void* dv_out,
+                     void* dlog_decay, void* dbeta, float* dinitial, int64_t batch, int64_t seqlen,
+                     int64_t key_heads, int64_t heads, int64_t dk, int64_t dv, float scale,
+                     int dtype, int wide, void* workspace, int64_t workspace_bytes, void* stream) {
+  FPSCAN_TRY(check_delta(batch, seqlen, key_heads, heads, dk, dv, dtype));
+  if (batch == 0) return ok();
+  const DeltaPlan pl = delta_plan(batch, seqlen, key_heads, heads, dk, dv, dtype, wide != 0, true);
+  if (workspace_bytes < pl.bytes)
+    return fail(FPSCAN_ERR_INVALID, "workspace too small: %lld bytes, need %lld",
+                (long long)workspace_bytes, (long long)pl.bytes);
+  const int64_t es = dtype_size(dtype), tok = batch * seqlen, st = batch * heads * dv * dk * 4;
+  const int64_t nk = tok * key_heads * dk * es, nv = tok * heads * dv * es, ng = tok * heads * es;
+  const Operand ops[] = {{"q", q, nk, false},
+                         {"k", k, nk, false},
+                         {"v", v, nv, false},
+                         {"log_decay", log_decay, ng, false},
+                         {"beta", beta, ng, false},
+                         {"initial", initial, initial ? st : 0, false},
+                         {"grad_out", grad_out, nv, false},
+                         {"grad_final", grad_final, grad_final ? st : 0, false},
+                         {"dq", dq, nk, true},
+                         {"dk", dk_out, nk, true},
+                         {"dv", dv_out, nv, true},
+                         {"dlog_decay", dlog_decay, ng, true},
+                         {"dbeta", dbeta, ng, true},
+                         {"dinitial", dinitial, dinitial ? st : 0, true},
+                         {"workspace", workspace, pl.bytes, true}};
+  FPSCAN_TRY(check_operands(ops));
+  DeltaArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.log_decay = log_decay;
+  a.beta = beta;
+  a.initial = initial;
+  a.grad_out = grad_out;
+  a.grad_final = grad_final;
+  a.dq = dq;
+  a.dk_out = dk_out;
+  a.dv_out = dv_out;
+  a.dlog_decay = dlog_decay;
+  a.dbeta = dbeta;
+  a.dinitial = dinitial;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  a.batch = batch;
+  a.seqlen = seqlen;
+  a.key_heads = key_heads;
+  a.heads = heads;
+  a.dk = dk;
+  a.dv = dv;
+  a.scale = scale;
+  a.dtype = dtype;
+  a.wide = wide != 0;
+  a.num_sms = num_sms_current();
+  a.stream = static_cast<cudaStream_t>(stream);
+  return cuda_result(launch_delta_bwd(a), "fpscan_delta_bwd launch");
+}
+
+int fpscan_delta_step(const void* q, const void* k, const void* v, const void* log_decay,
+                      const void* beta, const float* initial, void* out, float* final_state,
+                      int64_t batch, int64_t seqlen, int64_t key_heads, int64_t heads, int64_t dk,
+                      int64_t dv, float scale, int dtype, void* stream) {
+  FPSCAN_TRY(check_delta(batch, seqlen, key_heads, heads, dk, dv, dtype));
+  if (batch == 0) return ok();
+  const int64_t es = dtype_size(dtype), tok = batch * seqlen, st = batch * heads * dv * dk * 4;
+  const bool in_place = initial != nullptr && initial == final_state;
+  const Operand ops[] = {{"q", q, tok * key_heads * dk * es, false},
+                         {"k", k, tok * key_heads * dk * es, false},
+                         {"v", v, tok * heads * dv * es, false},
+                         {"log_decay", log_decay, tok * heads * es, false},
+                         {"beta", beta, tok * heads * es, false},
+                         {"initial", initial, initial && !in_place ? st : 0, false},
+                         {"out", out, tok * heads * dv * es, true},
+                         {"final_state", final_state, final_state ? st : 0, true}};
+  FPSCAN_TRY(check_operands(ops));
+  DeltaArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.log_decay = log_decay;
+  a.beta = beta;
+  a.initial = initial;
+  a.out = out;
+  a.final_state = final_state;
+  a.batch = batch;
+  a.seqlen = seqlen;
+  a.key_heads = key_heads;
+  a.heads = heads;
+  a.dk = dk;
+  a.dv = dv;
+  a.scale = scale;
+  a.dtype = dtype;
+  a.num_sms = num_sms_current();
+  a.stream = static_cast<cudaStream_t>(stream);
+  return cuda_result(launch_delta_step(a), "fpscan_delta_step launch");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ 8-bit checkpoints
+static int quant8_call(const void* x, void* out, int8_t* codes, float* steps, int64_t n, int dtype,
+                       void* stream, const char* what) {
+  FPSCAN_TRY(check_dtype(dtype));
+  if (n < 0 || n > (int64_t(1) << 60)) return fail(FPSCAN_ERR_INVALID, "n (%lld) out of range", (long long)n);
+  if (n == 0) return ok();
+  const bool write = x != nullptr;
+  const Operand ops[] = {{write ? "x" : "out", write ? x : out, n * dtype_size(dtype), !write},
+                         {"codes", codes, n, write},
+                         {"steps", steps, (n + 63) / 64 * 4, write}};
+  FPSCAN_TRY(check_operands(ops));
+  const Quant8Args a{x, out, codes, steps, n, dtype, num_sms_current(),
+                     static_cast<cudaStream_t>(stream)};
+  return cuda_result(launch_quant8(a), what);
+}
+
+// Operands of the channel-last calls that keep their output in 8 bits.
+static int scan_cl8(const void* gates, const void* tokens, void* out, const void* grad_out,
+                    void* dgates, void* dtokens, void* codes, float* steps, int64_t batch,
+                    int64_t seqlen, int64_t dim, int dtype, void* workspace,
+                    int64_t workspace_bytes, void* stream, bool backward, const char* what) {
+  FPSCAN_TRY(check_cl(batch, seqlen, dim, dtype));
+  if (batch == 0 || dim == 0) return ok();
+  const int64_t need = cl_workspace_bytes(batch, seqlen, dim, dtype, backward);
+  if (workspace_bytes < need)
+    return fail(FPSCAN_ERR_INVALID, "workspace too small: %lld bytes, need %lld",
+                (long long)workspace_bytes, (long long)need);
+  const int64_t bytes = batch * seqlen * dim * dtype_size(dtype);
+  const int64_t stride = (dim + 15) / 16 * 16, vecs = dim / (16 / dtype_size(dtype));
+  const int64_t code_bytes = batch * seqlen * stride, step_bytes = batch * ((seqlen + 7) / 8) * vecs * 4;
+  if (backward) {
+    const Operand ops[] = {{"gates", gates, bytes, false},       {"codes", codes, code_bytes, false},
+                           {"steps", steps, step_bytes, false},  {"grad_out", grad_out, bytes, false},
+                           {"dgates", dgates, bytes, true},      {"dtokens", dtokens, bytes, true},
+                           {"workspace", workspace, need, true}};
+    FPSCAN_TRY(check_operands(ops));
+  } else {
+    const Operand ops[] = {{"gates", gates, bytes, false},      {"tokens", tokens, bytes, false},
+                           {"out", out, bytes, true},           {"codes", codes, code_bytes, true},
+                           {"steps", steps, step_bytes, true},  {"workspace", workspace, need, true}};
+    FPSCAN_TRY(check_operands(ops));
+  }
+  ClArgs a{};
+  a.gates = gates;
+  a.tokens = tokens;
+  a.out = out;
+  a.grad_out = grad_out;
+  a.dgates = dgates;
+  a.dtokens = dtokens;
+  a.codes = static_cast<int8_t*>(codes);
+  a.steps = steps;
+  a.code_stride = stride;
+  a.workspace = workspace;
+  a.workspace_bytes = (uint64_t)workspace_bytes;
+  a.batch = batch;
+  a.seqlen = seqlen;
+  a.dim = dim;
+  a.dtype = dtype;
+  a.backward = backward ? 1 : 0;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return cuda_result(launch_cl(a), what);
+}
+
+extern "C" {
+
+int fpscan_quantize8(const void* x, void* codes, float* steps, int64_t n, int dtype, void* stream) {
+  if (n > 0 && x == nullptr) return fail(FPSCAN_ERR_INVALID, "x is NULL");
+  return quant8_call(x, nullptr, static_cast<int8_t*>(codes), steps, n, dtype, stream,
+                     "fpscan_quantize8 launch");
+}
+
+int fpscan_dequantize8(const void* codes, const float* steps, void* out, int64_t n, int dtype,
+                       void* stream) {
+  return quant8_call(nullptr, out, static_cast<int8_t*>(const_cast<void*>(codes)),
+                     const_cast<float*>(steps), n, dtype, stream, "fpscan_dequantize8 launch");
+}
+
+int fpscan_scan_fwd_cl8(const void* gates, const void* tokens, void* out, void* codes, float* steps,
+                        int64_t batch, int64_t seqlen, int64_t dim, int dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  return scan_cl8(gates, tokens, out, nullptr, nullptr, nullptr, codes, steps, batch, seqlen, dim,
+                  dtype, workspace, workspace_bytes, stream, false, "fpscan_scan_fwd_cl8 launch");
+}
+
+int fpscan_scan_bwd_cl8(const void* gates, const void* codes, const float* steps,
+                        const void* grad_out, void* dgates, void* dtokens, int64_t batch,
+                        int64_t seqlen, int64_t dim, int dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  return scan_cl8(gates, nullptr, nullptr, grad_out, dgates, dtokens, const_cast<void*>(codes),
+                  const_cast<float*>(steps), batch, seqlen, dim, dtype, workspace, workspace_bytes,
+                  stream, true, "fpscan_scan_bwd_cl8 launch");
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------------ rank links
 // Mailbox of one rank (cudaMalloc'd once per (rows, depth); 256-byte aligned
 // regions):

@@ -1,0 +1,255 @@
+// Shared device helpers of the gated delta rule kernels (sm_100a).
+//
+// For one head with a state S of (Dv, Dk) and a = exp(log_decay),
+//     e_t = v_t - a_t S_{t-1} k_t,  S_t = a_t S_{t-1} + beta_t e_t k_t^T,
+//     o_t = scale S_t q_t.
+// The sequence is cut into chunks of C = 64 tokens.  With G the running sum
+// of log_decay inside a chunk, D_ij = exp(G_i - G_j), M_ij = D_ij k_i.k_j
+// (i > j) and S0 the state entering the chunk:
+//     N = (I + M diag(beta))^-1,  E = N (V - exp(G) K S0^T),
+//     O = scale exp(G) Q S0^T + P E,   P_ij = scale D_ij (q_i.k_j) beta_j (i >= j),
+//     S_C = exp(G_C) S0 + E^T diag(beta exp(G_C - G)) K.
+//
+// Matrix products run on bf16 tensor-core instructions with fp32 sums.  An
+// operand of more than 8 bits is cut into bf16 parts, x = x0 + x1 (+ x2),
+// each the rounding of what the parts before it leave, and a product of two
+// operands is the sum of the products of their parts i, j with i + j <= LV:
+//   LV = 1: relative error near 2^-16 per product, for outputs of 16 bits
+//           (a single bf16 rounding, 2^-9, would show in them);
+//   LV = 2: near 2^-24, the level of fp32 products, for outputs of 32 bits.
+// bf16 inputs are one part, fp16 two, fp32 three, each exactly.  tf32
+// products (11 bits) cost as much as LV = 1 and hold less.
+#pragma once
+
+#include "common.cuh"
+
+namespace fpscan {
+
+constexpr int kChunk = 64;
+
+// Below this log_decay counts as -inf: exp of anything near it is 0, and
+// differences of running sums stay finite.
+constexpr float kDecayFloor = -10000.f;
+
+// Per-chunk vectors kept by delta_prep_kernel, kChunk floats each.
+enum DeltaVec : int {
+  kVecEnter = 0,  // exp(G_i)
+  kVecLeave = 1,  // exp(G_C - G_i)
+  kVecBeta = 2,
+  kVecCumHi = 3,  // G_i as a sum of two floats
+  kVecCumLo = 4,
+  kVecCount = 5
+};
+
+template <typename T> constexpr int kParts = 1;
+template <> constexpr int kParts<__half> = 2;
+template <> constexpr int kParts<float> = 3;
+
+// ---------------------------------------------------------------- tensor-core fragments
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+      " {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// N accumulator tiles of one step (16 values of k) of a product.  The tensor
+// core truncates its fp32 sums, and a chain of many truncated sums drifts by
+// more than 32-bit results may be off.  So wide products (LV = 2) sum each
+// step from zero, smallest parts first, and add it to the accumulator with
+// a rounded fp32 add; the others sum in the accumulator itself.
+template <bool WIDE, int N>
+struct Step {
+  float t[WIDE ? N : 1][4];
+  __device__ __forceinline__ Step() {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[n][e] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void mma(int n, float (&acc)[4], const uint32_t (&a)[4], uint32_t b0,
+                                      uint32_t b1) {
+    if constexpr (WIDE) mma_bf16(t[n], a, b0, b1);
+    else mma_bf16(acc, a, b0, b1);
+  }
+  __device__ __forceinline__ void add(int n, float (&acc)[4]) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += t[n][e];
+    }
+  }
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// Transposes an 8 x 8 matrix of 16-bit elements held by a warp.
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Tiles in shared memory: rows of ROWB bytes (a multiple of 128), 16-byte
+// units exchanged by the low bits of the row, so that 8 rows of one unit
+// column (an ldmatrix) fall on 8 different bank groups.
+template <int ROWB>
+__device__ __forceinline__ uint32_t tile_at(uint32_t base, int row, int unit) {
+  return base + row * ROWB + ((unit ^ (row & 7)) << 4);
+}
+
+// The four ways a lane addresses an x4 load; `lane` picks the row and unit.
+// B operand from [n][k] rows: n tiles n0 and n0 + 8, 16 values of k.
+template <int ROWB>
+__device__ __forceinline__ uint32_t at_b(uint32_t base, int lane, int n0, int kk) {
+  const int m = lane >> 3, r = lane & 7;
+  return tile_at<ROWB>(base, n0 + (m >> 1) * 8 + r, kk * 2 + (m & 1));
+}
+// B operand from [k][n] rows (transposing load): n tiles n0 and n0 + 8.
+template <int ROWB>
+__device__ __forceinline__ uint32_t at_bt(uint32_t base, int lane, int n0, int kk) {
+  const int m = lane >> 3, r = lane & 7;
+  return tile_at<ROWB>(base, kk * 16 + (m & 1) * 8 + r, n0 / 8 + (m >> 1));
+}
+// A operand from [m][k] rows.
+template <int ROWB>
+__device__ __forceinline__ uint32_t at_a(uint32_t base, int lane, int m0, int kk) {
+  const int m = lane >> 3, r = lane & 7;
+  return tile_at<ROWB>(base, m0 + (m & 1) * 8 + r, kk * 2 + (m >> 1));
+}
+// A operand from [k][m] rows (transposing load).
+template <int ROWB>
+__device__ __forceinline__ uint32_t at_at(uint32_t base, int lane, int m0, int kk) {
+  const int m = lane >> 3, r = lane & 7;
+  return tile_at<ROWB>(base, kk * 16 + (m >> 1) * 8 + r, m0 / 8 + (m & 1));
+}
+
+// ---------------------------------------------------------------- bf16 parts
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// P parts of the pair (x, y), each packed as bf16 x 2.
+template <int P>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    out[p] = pack_bf16(x, y);
+    if (p + 1 < P) {
+      x -= bf16_lo(out[p]);
+      y -= bf16_hi(out[p]);
+    }
+  }
+}
+
+// A-operand parts of 16 columns held as two accumulator tiles.
+template <int P>
+__device__ __forceinline__ void split_frag(const float (&lo)[4], const float (&hi)[4],
+                                           uint32_t (&a)[P][4]) {
+  uint32_t t[P];
+  split_pair<P>(lo[0], lo[1], t);
+#pragma unroll
+  for (int p = 0; p < P; ++p) a[p][0] = t[p];
+  split_pair<P>(lo[2], lo[3], t);
+#pragma unroll
+  for (int p = 0; p < P; ++p) a[p][1] = t[p];
+  split_pair<P>(hi[0], hi[1], t);
+#pragma unroll
+  for (int p = 0; p < P; ++p) a[p][2] = t[p];
+  split_pair<P>(hi[2], hi[3], t);
+#pragma unroll
+  for (int p = 0; p < P; ++p) a[p][3] = t[p];
+}
+
+// ---------------------------------------------------------------- asynchronous copies
+// 16 bytes global -> shared; zeros when `in` is false (then src is not read).
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Tile of ROWS rows of ROWB bytes: row r from src + r * stride (bytes), the
+// first `rows` rows and `units` units of each; the rest is zeros.  src must
+// be a valid pointer even where nothing of it is read.
+template <int ROWS, int ROWB, int NTH>
+__device__ __forceinline__ void load_tile(uint32_t dst, const void* src, int64_t stride, int rows,
+                                          int units, int tid) {
+  constexpr int U = ROWB / 16;
+  const char* s = static_cast<const char*>(src);
+#pragma unroll 4
+  for (int i = tid; i < ROWS * U; i += NTH) {
+    const int r = i / U, u = i % U;
+    const bool in = r < rows && u < units;
+    cp16(tile_at<ROWB>(dst, r, u), in ? s + r * stride + u * 16 : s, in);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  return pack_bf16(x, y);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(bf16_lo(v), bf16_hi(v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// Stores an accumulator tile that holds 16 rows of values (dv) x 8 tokens as
+// token rows: element (token, dv) at out[token * stride + dv].  Tokens
+// [0, ntok) and values [0, nval) of the tile are written.
+template <typename T>
+__device__ __forceinline__ void store_t(T* out, int64_t stride, const float (&c)[4], int lane,
+                                        int ntok, int nval) {
+  const int g = lane >> 2, t = lane & 3;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int tok = 2 * t + (q & 1), val = g + (q >> 1) * 8;
+      if (tok < ntok && val < nval) out[tok * stride + val] = c[q];
+    }
+  } else {
+    const uint32_t lo = movmatrix_t(pack2<T>(c[0], c[1]));
+    const uint32_t hi = movmatrix_t(pack2<T>(c[2], c[3]));
+    if (g < ntok) {
+      T* p = out + g * stride + 2 * t;
+      if (nval > 0) *reinterpret_cast<uint32_t*>(p) = lo;
+      if (nval > 8) *reinterpret_cast<uint32_t*>(p + 8) = hi;
+    }
+  }
+}
+
+}  // namespace fpscan

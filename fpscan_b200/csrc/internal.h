@@ -190,7 +190,82 @@ struct ClArgs {
   int reverse;
   int backward;
   cudaStream_t stream;
+  // Output kept in 8 bits (quant8.cuh), one step per 8 timesteps x 16 bytes
+  // of channels: written by the forward, read by the backward in place of y.
+  int8_t* codes = nullptr;   // (batch, seqlen, code_stride)
+  float* steps = nullptr;    // (batch, ceil(seqlen / 8), dim vectors)
+  int64_t code_stride = 0;   // dim rounded up to a multiple of 16
 };
+
+// quantize8 (x given) / dequantize8 (out given), n values.
+struct Quant8Args {
+  const void* x;
+  void* out;
+  int8_t* codes;
+  float* steps;
+  int64_t n;
+  int dtype;
+  int num_sms;
+  cudaStream_t stream;
+};
+cudaError_t launch_quant8(const Quant8Args& a);
+
+// Gated delta rule (delta_fwd.cu, delta_bwd.cu, delta_step.cu).  q, k are
+// (batch, seqlen, key_heads, dk), v, out and grad_out (batch, seqlen, heads,
+// dv), log_decay and beta (batch, seqlen, heads); states are fp32 (batch,
+// heads, dv, dk).
+struct DeltaArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* log_decay;
+  const void* beta;
+  const float* initial;   // nullptr: zero
+  void* out;              // forward, step
+  float* final_state;     // forward: may be nullptr; step: may equal initial
+  const void* grad_out;       // backward
+  const float* grad_final;    // backward: nullptr: zero
+  void* dq;
+  void* dk_out;
+  void* dv_out;
+  void* dlog_decay;
+  void* dbeta;
+  float* dinitial;            // nullptr: not wanted
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t batch;
+  int64_t seqlen;
+  int64_t key_heads;
+  int64_t heads;
+  int64_t dk;
+  int64_t dv;
+  float scale;
+  int dtype;
+  int wide;               // products to 2^-24 (fp32 results) instead of 2^-16
+  int num_sms;
+  cudaStream_t stream;
+};
+
+// Offsets (bytes) of what the delta kernels keep in the caller's workspace,
+// for `batch` sequences at a time.  C = 64 tokens, chunks = heads x ceil(L/C).
+struct DeltaPlan {
+  int64_t chunks;    // per head and sequence
+  int64_t batch;     // sequences per pass (the passes share the workspace)
+  int np, ns;        // bf16 parts of the inputs / of fp32 operands
+  int dkp;           // dk padded to 64 or 128
+  int64_t q_parts, k_parts, do_parts;  // [np][batch x seqlen x ...] bf16 (np > 1)
+  int64_t n_mat, p_mat;                // [head][chunk][ns][64][64] bf16
+  int64_t vecs;                        // [head][chunk][kVecCount][64] fp32
+  int64_t e_parts, dv_parts;           // [head][chunk][ns][64][dv] bf16 (backward)
+  int64_t s_parts, ds_parts;           // [head][chunk][ns][dv][dkp] bf16 (backward)
+  int64_t dq_part, dk_part;            // [batch x seqlen][heads][dk] fp32 (backward, shared heads)
+  int64_t bytes;
+};
+DeltaPlan delta_plan(int64_t batch, int64_t seqlen, int64_t key_heads, int64_t heads, int64_t dk,
+                     int64_t dv, int dtype, bool wide, bool backward);
+cudaError_t launch_delta_fwd(const DeltaArgs& a);
+cudaError_t launch_delta_bwd(const DeltaArgs& a);
+cudaError_t launch_delta_step(const DeltaArgs& a);
 
 // Launches `kern` on `stream` with programmatic stream serialization (the
 // kernel calls pdl_wait() before its first global access), so its prologue

@@ -1,0 +1,127 @@
+// quantize8 / dequantize8: a tensor kept in 8 bits for the backward pass, in
+// blocks of 64 consecutive values (format in quant8.cuh).
+//
+// Bound by memory: the value's bytes and one more in each direction.  Eight
+// lanes share a block, eight values each, so a lane reads 16 (fp32: 32)
+// bytes and writes 8, a block's magnitude is three shuffles, and no shared
+// memory or second pass is needed.
+#include <algorithm>
+
+#include "internal.h"
+#include "quant8.cuh"
+
+namespace fpscan {
+
+namespace {
+
+constexpr int kBlock8 = 64;
+
+struct Quant8Params {
+  const void* x;
+  void* out;
+  int8_t* codes;
+  const int8_t* codes_in;
+  float* steps;
+  const float* steps_in;
+  int64_t n;
+};
+
+// Eight values from p; those at or past `left` are 0.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t left, float (&x)[8]) {
+  constexpr int V = Elem<T>::kVec;
+  if (left >= 8) {
+#pragma unroll
+    for (int j = 0; j < 8 / V; ++j) {
+      Vec16<T> v;
+      v.raw = *reinterpret_cast<const uint4*>(p + j * V);
+#pragma unroll
+      for (int c = 0; c < V; ++c) x[j * V + c] = Elem<T>::load(v.e[c]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) x[c] = c < left ? Elem<T>::load(p[c]) : 0.f;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) quantize8_kernel(const Quant8Params p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t units = (p.n + kBlock8 - 1) / kBlock8 * 8;  // whole blocks: all lanes of a group stay
+  const int64_t step = (int64_t)gridDim.x * blockDim.x;
+  const T* src = static_cast<const T*>(p.x);
+  // the loop's bound is a multiple of 8 lanes, not of 32: the shuffles name their group
+  const unsigned mask = 0xffu << (threadIdx.x & 24);
+  for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += step) {
+    const int64_t i = u * 8, left = p.n - i;
+    float x[8];
+    load8(src + i, left, x);
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) most = max(most, __float_as_uint(x[c]) & 0x7fffffffu);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) most = max(most, __shfl_xor_sync(mask, most, d));
+    const Quant8 q = quant8_block(most);
+    int code[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) code[c] = quant8_code(q, x[c]);
+    if (left >= 8)
+      *reinterpret_cast<uint2*>(p.codes + i) =
+          make_uint2(quant8_pack4(code[0], code[1], code[2], code[3]),
+                     quant8_pack4(code[4], code[5], code[6], code[7]));
+    else
+      for (int c = 0; c < left; ++c) p.codes[i + c] = (int8_t)code[c];
+    if ((u & 7) == 0) p.steps[u / 8] = q.step;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize8_kernel(const Quant8Params p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t units = (p.n + 7) / 8, step = (int64_t)gridDim.x * blockDim.x;
+  T* dst = static_cast<T*>(p.out);
+  for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += step) {
+    const int64_t i = u * 8, left = p.n - i;
+    const float s = p.steps_in[u / 8];
+    if (left >= 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p.codes_in + i);
+      float x[8];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        x[c] = quant8_value(w.x, c, s);
+        x[4 + c] = quant8_value(w.y, c, s);
+      }
+#pragma unroll
+      for (int j = 0; j < 8 / Elem<T>::kVec; ++j)
+        *reinterpret_cast<uint4*>(dst + i + j * Elem<T>::kVec) = pack_vec<T>(x + j * Elem<T>::kVec);
+    } else {
+      for (int c = 0; c < left; ++c) dst[i + c] = Elem<T>::store((float)p.codes_in[i + c] * s);
+    }
+  }
+}
+
+template <typename T>
+cudaError_t run8(const Quant8Args& a) {
+  Quant8Params p{a.x, a.out, a.codes, a.codes, a.steps, a.steps, a.n};
+  const int64_t ctas = (a.n + 2047) / 2048;
+  const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)a.num_sms * 32);
+  return a.x != nullptr ? launch_pdl(quantize8_kernel<T>, grid, 256, 0, a.stream, p)
+                        : launch_pdl(dequantize8_kernel<T>, grid, 256, 0, a.stream, p);
+}
+
+}  // namespace
+
+cudaError_t launch_quant8(const Quant8Args& a) {
+  switch (a.dtype) {
+    case kF32:
+      return run8<float>(a);
+    case kF16:
+      return run8<__half>(a);
+    default:
+      return run8<__nv_bfloat16>(a);
+  }
+}
+
+}  // namespace fpscan

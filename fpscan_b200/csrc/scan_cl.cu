@@ -25,6 +25,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "quant8.cuh"
 
 namespace fpscan {
 
@@ -89,6 +90,9 @@ struct StreamParams {
   int64_t n_map; // seg_map entries (bounds checks of debug builds)
   float2* seg_map;          // SPLIT 1: per (column, segment, vector, channel) map (A, B)
   const float* seg_carry;   // SPLIT 2: state entering each segment (same indexing)
+  int8_t* codes;            // Q8: the output in 8 bits, rows of code_stride bytes
+  float* steps;             // Q8: (batch, ceil(L / 8), dv)
+  int64_t code_stride;
 };
 
 // SPLIT (few columns: the time axis is cut into nseg segments, one CTA each):
@@ -98,7 +102,11 @@ struct StreamParams {
 //        seg_map;
 //   2 -- scan: as 0 within the segment, entering with seg_carry (segments
 //        after the first; cl_seg_carry_kernel composes the maps in between).
-template <typename T, int MODE, int TW, int S, int NTH, int SPLIT = 0>
+// Q8: the forward also writes its (rounded) output in 8 bits, and the
+// backward reads that in place of y (tm_c covers the codes).  A block of the
+// format is what one thread holds in a chunk, 8 timesteps x one 16-byte
+// channel vector, so its magnitude needs no exchange between threads.
+template <typename T, int MODE, int TW, int S, int NTH, int SPLIT = 0, bool Q8 = false>
 __global__ void __launch_bounds__(NTH, 1)
     scan_cl_stream_kernel(const __grid_constant__ StreamParams p) {
   using Cfg = StreamCfg<T, MODE, TW, S, NTH>;
@@ -107,6 +115,9 @@ __global__ void __launch_bounds__(NTH, 1)
   constexpr int R = Cfg::R;
   constexpr bool DESC = MODE != kClFwd;
   constexpr bool BWD = MODE == kClBwd;
+  static_assert(!Q8 || TW == 8, "a thread's timesteps are a block of the 8-bit format");
+  constexpr int kStageTx =  // bytes that land in a stage
+      BWD && Q8 ? 2 * Cfg::kTileBytes + R * kStreamVecs * V : Cfg::kStageBytes;
 
   extern __shared__ __align__(128) unsigned char csm_raw[];
   unsigned char* csm = reinterpret_cast<unsigned char*>(
@@ -153,7 +164,7 @@ __global__ void __launch_bounds__(NTH, 1)
     const int s = (int)(j % S);
     unsigned char* dst = csm + s * Cfg::kStageBytes;
     const int r0 = (int)(m * R);
-    mbar_expect_tx(&s_bar[s], (uint32_t)Cfg::kStageBytes);
+    mbar_expect_tx(&s_bar[s], (uint32_t)kStageTx);
     if (BWD) {
       tma_load_3d(dst, &p.tm_a, x, r0 + 1, (int)b, &s_bar[s]);
       tma_load_3d(dst + Cfg::kTileBytes, &p.tm_b, x, r0, (int)b, &s_bar[s]);
@@ -183,6 +194,15 @@ __global__ void __launch_bounds__(NTH, 1)
     const int64_t k = k0 + j;
     const int64_t m = DESC ? nck - 1 - k : k;
     const int64_t r0 = m * R;
+    // Q8: the steps of y at the thread's timesteps - 1: this block's, and
+    // the one's before it for the first
+    const int64_t blk0 = r0 + (DESC ? R - TW - tg * TW : tg * TW);
+    float y_step = 0.f, y_step_prev = 0.f;
+    if (BWD && Q8 && SPLIT != 1 && lane_ok && blk0 < L) {
+      const float* sp = p.steps + (b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv;
+      y_step = sp[0];
+      if (blk0 > 0) y_step_prev = sp[-p.dv];
+    }
     const bool ok = mbar_wait_bounded(&s_bar[s], phase);
     const uint4* s_a = reinterpret_cast<const uint4*>(csm + s * Cfg::kStageBytes);
     const uint4* s_b = reinterpret_cast<const uint4*>(csm + s * Cfg::kStageBytes + Cfg::kTileBytes);
@@ -284,6 +304,7 @@ __global__ void __launch_bounds__(NTH, 1)
       for (int c = 0; c < V; ++c) st[c] = zero ? EB[c] : fmaf(EA[c], st[c], EB[c]);
 
     // pass 2: rerun the recurrence from the entering state, store
+    uint4 kept[Q8 && MODE == kClFwd ? TW : 1];
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
       const int lr = DESC ? R - 1 - (tg * TW + i) : tg * TW + i;
@@ -299,11 +320,50 @@ __global__ void __launch_bounds__(NTH, 1)
         *reinterpret_cast<uint4*>(out + base + t * row_elems) = pack_vec<T>(st);
         if (BWD) {
           float yp[V], dg[V];
-          unpack<T>(s_c[lr * kStreamVecs + vec], yp);
+          if constexpr (Q8) {
+            const uint32_t* cp = reinterpret_cast<const uint32_t*>(s_c) + (lr * kStreamVecs + vec) * (V / 4);
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+              yp[c] = quant8_value(cp[c / 4], c % 4, i == TW - 1 ? y_step_prev : y_step);
+          } else {
+            unpack<T>(s_c[lr * kStreamVecs + vec], yp);
+          }
 #pragma unroll
           for (int c = 0; c < V; ++c) dg[c] = st[c] * yp[c];
           FPSCAN_DEBUG_ONLY(if (in_bounds(out2 + base + t * row_elems, 16, out2, out2 + p.n_el)))
           *reinterpret_cast<uint4*>(out2 + base + t * row_elems) = pack_vec<T>(dg);
+        }
+      }
+      if constexpr (Q8 && MODE == kClFwd) kept[i] = pack_vec<T>(st);
+    }
+    if constexpr (Q8 && MODE == kClFwd && SPLIT != 1) {
+      // rows past L and vectors past dim were read as zeros and hold zeros
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        float y[V];
+        unpack<T>(kept[i], y);
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+          most = max(most, __float_as_uint(y[c]) & (blk0 + i < L ? 0x7fffffffu : 0u));
+      }
+      const Quant8 q8 = quant8_block(most);
+      if (lane_ok && blk0 < L) p.steps[(b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv] = q8.step;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        float y[V];
+        unpack<T>(kept[i], y);
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int c = 0; c < V; c += 4)
+          w[c / 4] = quant8_pack4(quant8_code(q8, y[c]), quant8_code(q8, y[c + 1]),
+                                  quant8_code(q8, y[c + 2]), quant8_code(q8, y[c + 3]));
+        if (lane_ok && blk0 + i < L) {
+          int8_t* o = p.codes + (b * L + blk0 + i) * p.code_stride + cv * V;
+          if constexpr (V == 8)
+            *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+          else
+            *reinterpret_cast<uint32_t*>(o) = w[0];
         }
       }
     }
@@ -389,6 +449,20 @@ cudaError_t make_map(CUtensorMap* m, const void* ptr, int dtype, int64_t batch, 
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// The 8-bit codes: bytes, rows of code_stride.
+cudaError_t make_code_map(CUtensorMap* m, const ClArgs& a, int ts) {
+  auto fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.dim, (cuuint64_t)a.seqlen, (cuuint64_t)a.batch};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.code_stride, (cuuint64_t)(a.seqlen * a.code_stride)};
+  const cuuint32_t box[3] = {(cuuint32_t)(kStreamVecs * (16 / dtype_size(a.dtype))), (cuuint32_t)ts, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.codes, dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // Few-column plan: time segments per column so that columns x segments is
 // about two CTAs per SM, each segment at least two chunks.  FPSCAN_B200_CL_PATH
 // =stream / =split forces one CTA per column / the segmented path.
@@ -448,7 +522,7 @@ cudaError_t configure(Kern kern, int smem, int* configured) {
   return cudaSuccess;
 }
 
-template <typename T, int MODE, int TW, int S, int NTH = kThreads>
+template <typename T, int MODE, int TW, int S, int NTH = kThreads, bool Q8 = false>
 cudaError_t launch_stream_t(const ClArgs& a) {
   using Cfg = StreamCfg<T, MODE, TW, S, NTH>;
   constexpr int V = Elem<T>::kVec;
@@ -472,7 +546,9 @@ cudaError_t launch_stream_t(const ClArgs& a) {
     e = make_map(&p.tm_a, a.gates, a.dtype, a.batch, a.seqlen, a.dim, R, kStreamRowBytes);
     if (e == cudaSuccess)
       e = make_map(&p.tm_b, a.grad_out, a.dtype, a.batch, a.seqlen, a.dim, R, kStreamRowBytes);
-    if (e == cudaSuccess) e = make_map(&p.tm_c, a.y, a.dtype, a.batch, a.seqlen, a.dim, R, kStreamRowBytes);
+    if (e == cudaSuccess)
+      e = Q8 ? make_code_map(&p.tm_c, a, (int)R)
+             : make_map(&p.tm_c, a.y, a.dtype, a.batch, a.seqlen, a.dim, R, kStreamRowBytes);
     p.out = a.dtokens;
     p.out2 = a.dgates;
   } else {
@@ -487,8 +563,11 @@ cudaError_t launch_stream_t(const ClArgs& a) {
   p.nseg = plan.nseg;
   p.cps = plan.cps;
   p.n_el = a.batch * a.seqlen * a.dim;
+  p.codes = a.codes;
+  p.steps = a.steps;
+  p.code_stride = a.code_stride;
   if (plan.nseg == 1) {
-    auto kern = scan_cl_stream_kernel<T, MODE, TW, S, NTH, 0>;
+    auto kern = scan_cl_stream_kernel<T, MODE, TW, S, NTH, 0, Q8>;
     if ((e = configure(kern, smem, conf0)) != cudaSuccess) return e;
     return launch_pdl(kern, (unsigned)cols, NTH, smem, a.stream, p);
   }
@@ -501,8 +580,8 @@ cudaError_t launch_stream_t(const ClArgs& a) {
   p.n_map = n;
   p.seg_carry = reinterpret_cast<const float*>(static_cast<char*>(a.workspace) + map_bytes);
   const unsigned grid = (unsigned)(cols * plan.nseg);
-  auto k1 = scan_cl_stream_kernel<T, MODE, TW, S, NTH, 1>;
-  auto k2 = scan_cl_stream_kernel<T, MODE, TW, S, NTH, 2>;
+  auto k1 = scan_cl_stream_kernel<T, MODE, TW, S, NTH, 1, Q8>;
+  auto k2 = scan_cl_stream_kernel<T, MODE, TW, S, NTH, 2, Q8>;
   if ((e = configure(k1, smem, conf1)) != cudaSuccess) return e;
   if ((e = configure(k2, smem, conf2)) != cudaSuccess) return e;
   if ((e = launch_pdl(k1, grid, NTH, smem, a.stream, p)) != cudaSuccess) return e;
@@ -553,6 +632,9 @@ cudaError_t launch_stream_mode(const ClArgs& a) {
 
 template <typename T>
 cudaError_t launch_cl_dtype(const ClArgs& a) {
+  if (a.codes != nullptr)  // 8-bit checkpoint: blocks of 8 timesteps fix the shape
+    return a.backward ? launch_stream_t<T, kClBwd, 8, 2, kThreads, true>(a)
+                      : launch_stream_t<T, kClFwd, 8, 3, kThreads, true>(a);
   if (a.backward) return launch_stream_mode<T, kClBwd>(a);
   return a.reverse ? launch_stream_mode<T, kClRev>(a) : launch_stream_mode<T, kClFwd>(a);
 }

@@ -541,6 +541,57 @@ class PScanChannelsLast(torch.autograd.Function):
         return scan_backward_channels_last(gates, out, grad_output.contiguous())
 
 
-def pscan_channels_last(gates: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
-    """Differentiable scan along dim 1 of (batch, seqlen, dim) tensors."""
+def _cl8_workspace(t: torch.Tensor, backward: bool) -> torch.Tensor:
+    # not the shared per-stream one: from torch's allocator at every call, so
+    # that captured graphs that may run at the same time never share one
+    b, l, d = t.shape
+    nbytes = _fn("fpscan_cl_workspace_bytes")(b, l, d, DTYPE_CODES[t.dtype], 1 if backward else 0)
+    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=t.device)
+
+
+class PScanChannelsLast8(torch.autograd.Function):
+    """``PScanChannelsLast`` that keeps its output for the backward pass in 8 bits, written and read inside
+    the scan kernels: one step per block of 8 timesteps x one 16-byte channel vector."""
+
+    @staticmethod
+    def forward(ctx, gates, tokens):
+        _lib.load()
+        validate_channels_last(gates, tokens)
+        out = torch.empty_like(tokens)
+        b, l, d = tokens.shape
+        # rows of codes start on 16-byte boundaries, as the kernels' tile copies need
+        codes = torch.empty(b, l, (d + 15) // 16 * 16, dtype=torch.int8, device=tokens.device)
+        steps = torch.empty(b, (l + 7) // 8, d * tokens.element_size() // 16, dtype=torch.float32,
+                            device=tokens.device)
+        if b and d:
+            ws = _cl8_workspace(tokens, False)
+            _launch(tokens.get_device(), "fpscan_scan_fwd_cl8", gates.data_ptr(), tokens.data_ptr(),
+                    out.data_ptr(), codes.data_ptr(), steps.data_ptr(), b, l, d,
+                    DTYPE_CODES[tokens.dtype], ws.data_ptr(), ws.numel())
+        ctx.save_for_backward(gates, codes, steps)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        gates, codes, steps = ctx.saved_tensors
+        grad_output = grad_output.contiguous()
+        validate_channels_last(gates, grad_output)
+        dgates = torch.empty_like(grad_output)
+        dtokens = torch.empty_like(grad_output)
+        b, l, d = grad_output.shape
+        if b and d:
+            ws = _cl8_workspace(grad_output, True)
+            _launch(grad_output.get_device(), "fpscan_scan_bwd_cl8", gates.data_ptr(),
+                    codes.data_ptr(), steps.data_ptr(), grad_output.data_ptr(), dgates.data_ptr(),
+                    dtokens.data_ptr(), b, l, d, DTYPE_CODES[grad_output.dtype], ws.data_ptr(),
+                    ws.numel())
+        return dgates, dtokens
+
+
+def pscan_channels_last(gates: torch.Tensor, tokens: torch.Tensor,
+                        checkpoint8: bool = False) -> torch.Tensor:
+    """Differentiable scan along dim 1 of (batch, seqlen, dim) tensors.  ``checkpoint8=True`` keeps the
+    output for the backward pass in 8 bits: grad_gates is then that of the values these stand for."""
+    if checkpoint8:
+        return PScanChannelsLast8.apply(gates, tokens)
     return PScanChannelsLast.apply(gates, tokens)

@@ -170,6 +170,91 @@ FPSCAN_API int fpscan_scan_bwd_cl(const void* gates, const void* y, const void* 
                                   int64_t workspace_bytes, void* stream);
 
 /*
+ * Channel-last scan that keeps its output for the backward pass in 8 bits
+ * (no reference counterpart: its autograd saves the output as it is,
+ * fpscan/ops.py:64-67).  fpscan_scan_fwd_cl8 is fpscan_scan_fwd_cl (forward
+ * order) and also writes `codes`, int8 (batch, seqlen, dim rounded up to a
+ * multiple of 16), and `steps`, fp32 (batch, ceil(seqlen / 8), dim vectors of
+ * 16 bytes): a block of 8 timesteps (from a multiple of 8) x one channel
+ * vector has the step max|out| / 127, and a code is the nearest multiple of
+ * it, ties to even.  A block that holds an infinity or a NaN reads back as
+ * NaN.  fpscan_scan_bwd_cl8 is fpscan_scan_bwd_cl with
+ * y[t] = code * step.  Operands must not overlap.
+ */
+FPSCAN_API int fpscan_scan_fwd_cl8(const void* gates, const void* tokens, void* out, void* codes,
+                                   float* steps, int64_t batch, int64_t seqlen, int64_t dim,
+                                   int dtype, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+FPSCAN_API int fpscan_scan_bwd_cl8(const void* gates, const void* codes, const float* steps,
+                                   const void* grad_out, void* dgates, void* dtokens,
+                                   int64_t batch, int64_t seqlen, int64_t dim, int dtype,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * n values in 8 bits: blocks of 64 consecutive values (the last may be
+ * shorter) with one fp32 step each, in the format above.  codes: n bytes;
+ * steps: ceil(n / 64).  No reference counterpart.
+ */
+FPSCAN_API int fpscan_quantize8(const void* x, void* codes, float* steps, int64_t n, int dtype,
+                                void* stream);
+FPSCAN_API int fpscan_dequantize8(const void* codes, const float* steps, void* out, int64_t n,
+                                  int dtype, void* stream);
+
+/*
+ * Gated delta rule: the recurrence of a matrix-valued state.  Per head, with
+ * a state S of (dv, dk) and a[t] = exp(log_decay[t]),
+ *     S[t]   = a[t] S[t-1] + beta[t] (v[t] - a[t] S[t-1] k[t]) k[t]^T,
+ *     out[t] = scale S[t] q[t].
+ * q, k: (batch, seqlen, key_heads, dk); v, out: (batch, seqlen, heads, dv);
+ * log_decay, beta: (batch, seqlen, heads); all of `dtype`, contiguous.
+ * heads is a multiple of key_heads: value head h uses key head
+ * h / (heads / key_heads).  States (initial, final_state and their
+ * gradients) are fp32 (batch, heads, dv, dk); NULL: zero / not wanted.
+ * dk: a multiple of 8 in [8, 128]; dv: a multiple of 8 in [8, 65536]; seqlen
+ * >= 1.  log_decay may be -inf: the state before that token counts no more
+ * (a sequence packed behind another begins there); its gradient there is 0.
+ * No reference counterpart (its state is one number per channel).
+ *
+ * `wide` != 0: products carry fp32's relative error (2^-24) for 16-bit data
+ * too; 0: 2^-16, enough for 16-bit outputs.  Set it where an fp32 state goes
+ * in or out.  fp32 data is always wide.
+ * workspace: fpscan_delta_workspace_bytes() bytes, 16-byte aligned, needs no
+ * initialisation; calls that may overlap on the GPU need separate ones.  Long
+ * batches are processed a few sequences at a time to bound it.
+ * No operand that is written may overlap another.
+ */
+FPSCAN_API int64_t fpscan_delta_workspace_bytes(int64_t batch, int64_t seqlen, int64_t key_heads,
+                                                int64_t heads, int64_t dk, int64_t dv, int dtype,
+                                                int wide, int backward);
+FPSCAN_API int fpscan_delta_fwd(const void* q, const void* k, const void* v, const void* log_decay,
+                                const void* beta, const float* initial, void* out,
+                                float* final_state, int64_t batch, int64_t seqlen,
+                                int64_t key_heads, int64_t heads, int64_t dk, int64_t dv,
+                                float scale, int dtype, int wide, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/* Gradients of fpscan_delta_fwd from the gradients of out (grad_out) and of
+ * the final state (grad_final, may be NULL).  dinitial may be NULL.  dq and
+ * dk are summed over the heads that share a key head, in a fixed order. */
+FPSCAN_API int fpscan_delta_bwd(const void* q, const void* k, const void* v, const void* log_decay,
+                                const void* beta, const float* initial, const void* grad_out,
+                                const float* grad_final, void* dq, void* dk_out, void* dv_out,
+                                void* dlog_decay, void* dbeta, float* dinitial, int64_t batch,
+                                int64_t seqlen, int64_t key_heads, int64_t heads, int64_t dk,
+                                int64_t dv, float scale, int dtype, int wide, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/* fpscan_delta_fwd token by token, for one or a few tokens (a serving step):
+ * fp32 arithmetic, no workspace.  final_state may be `initial` itself (the
+ * state is updated in place); otherwise no written operand may overlap
+ * another. */
+FPSCAN_API int fpscan_delta_step(const void* q, const void* k, const void* v,
+                                 const void* log_decay, const void* beta, const float* initial,
+                                 void* out, float* final_state, int64_t batch, int64_t seqlen,
+                                 int64_t key_heads, int64_t heads, int64_t dk, int64_t dv,
+                                 float scale, int dtype, void* stream);
+
+/*
  * Scan with a per-row initial state `init` (fp32, batch*dim values):
  * y[0] = gates[0]*init + tokens[0] (reverse: y[L-1] = gates[L-1]*init +
  * tokens[L-1]).  The final state is the last element of out in scan order.
