@@ -1,5 +1,7 @@
 // Thin torch binding over the C ABI (include/fpscan_b200.h): the fast path of
-// fpscan_b200.ops for the reference's own entry points.  It plays the role of
+// fpscan_b200.ops for the reference's own entry points, and of the calls of
+// delta.py and checkpoint8.py, where a serving step's kernel takes less time
+// than a Python + ctypes call.  It plays the role of
 // the reference's pybind module (csrc/main.cpp:10, fullscan_forward) -- tensor
 // checks, output allocation, the caller's current stream -- in C++, so a
 // call costs what the reference's does instead of a Python + ctypes round
@@ -120,6 +122,165 @@ std::tuple<at::Tensor, at::Tensor> scan_backward(const at::Tensor& gates, const 
   return {dgates, dtokens};
 }
 
+// ---------------------------------------------------------------- gated delta rule
+// Same conditions and wording as delta.validate_delta.
+struct DeltaSizes {
+  int64_t b, l, hk, h, dk, dv;
+  int code;
+};
+
+DeltaSizes check_delta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                       const at::Tensor& log_decay, const at::Tensor& beta,
+                       const c10::optional<at::Tensor>& state,
+                       const c10::optional<at::Tensor>& out) {
+  const at::Tensor* all[5] = {&q, &k, &v, &log_decay, &beta};
+  static const char* const names[5] = {"q", "k", "v", "log_decay", "beta"};
+  for (int i = 0; i < 5; ++i) {
+    TORCH_CHECK(all[i]->is_cuda(), names[i], " must be a CUDA tensor");
+    TORCH_CHECK(all[i]->is_contiguous(), names[i], " must be contiguous");
+    TORCH_CHECK(all[i]->scalar_type() == at::kFloat || all[i]->scalar_type() == at::kHalf ||
+                    all[i]->scalar_type() == at::kBFloat16,
+                names[i], " must be float16 or bfloat16 or float32");
+  }
+  for (int i = 0; i < 3; ++i)
+    TORCH_CHECK(all[i]->dim() == 4, names[i], " must be 4-D (batch, seqlen, heads, channels), got ",
+                all[i]->sizes());
+  DeltaSizes s{v.size(0), v.size(1), q.size(2), v.size(2), q.size(3), v.size(3), dtype_code(v)};
+  TORCH_CHECK(q.sizes() == k.sizes(), "q ", q.sizes(), " and k ", k.sizes(),
+              " must have the same shape");
+  TORCH_CHECK(q.size(0) == s.b && q.size(1) == s.l, "q ", q.sizes(), " and v ", v.sizes(),
+              " must agree in batch and seqlen");
+  TORCH_CHECK(s.hk >= 1 && s.h >= 1 && s.h % s.hk == 0, "heads of v (", s.h,
+              ") must be a positive multiple of the heads of q and k (", s.hk, ")");
+  TORCH_CHECK(s.l >= 1, "seqlen must be >= 1 (got ", s.l, ")");
+  TORCH_CHECK(s.dk % 8 == 0 && s.dk >= 8 && s.dk <= 128,
+              "dk must be a multiple of 8 in [8, 128] (got ", s.dk, ")");
+  TORCH_CHECK(s.dv % 8 == 0 && s.dv >= 8 && s.dv <= 65536,
+              "dv must be a multiple of 8 in [8, 65536] (got ", s.dv, ")");
+  for (int i = 3; i < 5; ++i)
+    TORCH_CHECK(all[i]->dim() == 3 && all[i]->size(0) == s.b && all[i]->size(1) == s.l &&
+                    all[i]->size(2) == s.h,
+                names[i], " must have shape (", s.b, ", ", s.l, ", ", s.h,
+                ") (batch, seqlen, heads), got ", all[i]->sizes());
+  for (int i = 0; i < 5; ++i) {
+    TORCH_CHECK(all[i]->scalar_type() == v.scalar_type(), names[i], " dtype ",
+                all[i]->scalar_type(), " must equal v dtype ", v.scalar_type());
+    TORCH_CHECK(all[i]->device() == v.device(), names[i], " and v must be on the same device");
+  }
+  if (state) {
+    TORCH_CHECK(state->dim() == 4 && state->size(0) == s.b && state->size(1) == s.h &&
+                    state->size(2) == s.dv && state->size(3) == s.dk,
+                "the state must have shape (", s.b, ", ", s.h, ", ", s.dv, ", ", s.dk,
+                ") (batch, heads, dv, dk), got ", state->sizes());
+    TORCH_CHECK(state->device() == v.device(), "the state must be on the device of v");
+    TORCH_CHECK(state->scalar_type() == at::kFloat && state->is_contiguous(),
+                "the state must be float32 and contiguous");
+  }
+  if (out) {
+    TORCH_CHECK(out->sizes() == v.sizes() && out->scalar_type() == v.scalar_type() &&
+                    out->device() == v.device(),
+                "out must match v in shape, dtype and device");
+    TORCH_CHECK(out->is_contiguous(), "out must be contiguous");
+  }
+  return s;
+}
+
+at::Tensor delta_workspace(const at::Tensor& v, const DeltaSizes& s, bool wide, bool backward) {
+  const int64_t n = fpscan_delta_workspace_bytes(s.b, s.l, s.hk, s.h, s.dk, s.dv, s.code, wide, backward);
+  return at::empty({std::max<int64_t>(n, 16)}, v.options().dtype(at::kByte));
+}
+
+float* state_ptr(const c10::optional<at::Tensor>& t) {
+  return t && t->numel() ? t->data_ptr<float>() : nullptr;
+}
+
+at::Tensor delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                      const at::Tensor& log_decay, const at::Tensor& beta, at::Tensor state,
+                      double scale, const c10::optional<at::Tensor>& out_) {
+  const DeltaSizes s = check_delta(q, k, v, log_decay, beta, state, out_);
+  const c10::cuda::CUDAGuard guard(v.device());
+  at::Tensor out = out_ ? *out_ : at::empty_like(v);
+  raise_on(fpscan_delta_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                             beta.data_ptr(), state_ptr(state), out.data_ptr(), state_ptr(state),
+                             s.b, s.l, s.hk, s.h, s.dk, s.dv, (float)scale, s.code,
+                             at::cuda::getCurrentCUDAStream().stream()),
+           "fpscan_delta_step");
+  return out;
+}
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> delta_forward(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+    const at::Tensor& beta, const c10::optional<at::Tensor>& initial, double scale,
+    bool return_state, const c10::optional<at::Tensor>& out_) {
+  const DeltaSizes s = check_delta(q, k, v, log_decay, beta, initial, out_);
+  const c10::cuda::CUDAGuard guard(v.device());
+  const bool wide = initial || return_state;
+  at::Tensor out = out_ ? *out_ : at::empty_like(v);
+  c10::optional<at::Tensor> last;
+  if (return_state) last = at::empty({s.b, s.h, s.dv, s.dk}, v.options().dtype(at::kFloat));
+  const at::Tensor ws = delta_workspace(v, s, wide, false);
+  raise_on(fpscan_delta_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                            beta.data_ptr(), state_ptr(initial), out.data_ptr(), state_ptr(last),
+                            s.b, s.l, s.hk, s.h, s.dk, s.dv, (float)scale, s.code, wide,
+                            ws.data_ptr(), ws.numel(), at::cuda::getCurrentCUDAStream().stream()),
+           "fpscan_delta_fwd");
+  return {out, last};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>>
+delta_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+               const at::Tensor& log_decay, const at::Tensor& beta, const at::Tensor& grad_out,
+               const c10::optional<at::Tensor>& initial,
+               const c10::optional<at::Tensor>& grad_final, double scale, bool need_initial) {
+  const DeltaSizes s = check_delta(q, k, v, log_decay, beta, initial, grad_out);
+  if (grad_final) check_delta(q, k, v, log_decay, beta, grad_final, c10::nullopt);
+  const c10::cuda::CUDAGuard guard(v.device());
+  const bool wide = initial || grad_final || need_initial;
+  at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v),
+             dg = at::empty_like(log_decay), db = at::empty_like(beta);
+  c10::optional<at::Tensor> di;
+  if (need_initial) di = at::empty({s.b, s.h, s.dv, s.dk}, v.options().dtype(at::kFloat));
+  const at::Tensor ws = delta_workspace(v, s, wide, true);
+  raise_on(fpscan_delta_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                            beta.data_ptr(), state_ptr(initial), grad_out.data_ptr(),
+                            state_ptr(grad_final), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                            dg.data_ptr(), db.data_ptr(), state_ptr(di), s.b, s.l, s.hk, s.h, s.dk,
+                            s.dv, (float)scale, s.code, wide, ws.data_ptr(), ws.numel(),
+                            at::cuda::getCurrentCUDAStream().stream()),
+           "fpscan_delta_bwd");
+  return {dq, dk, dv, dg, db, di};
+}
+
+// ---------------------------------------------------------------- 8-bit checkpoints
+std::tuple<at::Tensor, at::Tensor> quantize8(const at::Tensor& x) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK(x.is_contiguous(), "x must be contiguous");
+  TORCH_CHECK(x.scalar_type() == at::kFloat || x.scalar_type() == at::kHalf ||
+                  x.scalar_type() == at::kBFloat16,
+              "x must be float16 or bfloat16 or float32");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t n = x.numel();
+  at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar).requires_grad(false));
+  at::Tensor steps = at::empty({(n + 63) / 64}, x.options().dtype(at::kFloat).requires_grad(false));
+  if (n)
+    raise_on(fpscan_quantize8(x.data_ptr(), codes.data_ptr(), steps.data_ptr<float>(), n,
+                              dtype_code(x), at::cuda::getCurrentCUDAStream().stream()),
+             "fpscan_quantize8");
+  return {codes, steps};
+}
+
+// Called with checked codes and steps (checkpoint8.dequantize8).
+at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& steps, at::ScalarType dtype) {
+  const c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  if (codes.numel())
+    raise_on(fpscan_dequantize8(codes.data_ptr(), steps.data_ptr<float>(), out.data_ptr(),
+                                codes.numel(), dtype_code(out),
+                                at::cuda::getCurrentCUDAStream().stream()),
+             "fpscan_dequantize8");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -128,5 +289,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scan_forward", &scan_forward, "scan_forward(gates, tokens, reverse) -> out");
   m.def("scan_backward", &scan_backward,
         "scan_backward(gates, y, grad_out) -> (dgates, dtokens), the fused PScan backward");
+  m.def("delta_step", &delta_step, "delta_step(q, k, v, log_decay, beta, state, scale, out) -> out");
+  m.def("delta_forward", &delta_forward,
+        "delta_forward(q, k, v, log_decay, beta, initial, scale, return_state, out) -> (out, final)");
+  m.def("delta_backward", &delta_backward,
+        "delta_backward(q, k, v, log_decay, beta, grad_out, initial, grad_final, scale, need_initial)"
+        " -> (dq, dk, dv, dlog_decay, dbeta, dinitial)");
+  m.def("quantize8", &quantize8, "quantize8(x) -> (codes, steps)");
+  m.def("dequantize8", [](const at::Tensor& codes, const at::Tensor& steps, py::object dtype) {
+    return dequantize8(codes, steps, torch::python::detail::py_object_to_dtype(dtype));
+  });
   m.def("abi_version", []() { return fpscan_abi_version(); });
 }

@@ -17,7 +17,7 @@ from typing import Tuple
 
 import torch
 
-from .ops import DTYPE_CODES, _check_input, _launch
+from .ops import _EXT, DTYPE_CODES, _check_input, _launch
 
 __all__ = ["quantize8", "dequantize8"]
 
@@ -27,6 +27,8 @@ BLOCK = 64
 def quantize8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x`` (contiguous, float32 / float16 / bfloat16, any shape) in 8 bits: int8 codes of x's shape and
     fp32 steps, one per 64 consecutive values.  No autograd."""
+    if _EXT is not None and isinstance(x, torch.Tensor):
+        return _EXT.quantize8(x)
     _check_input(x, "x")
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     steps = torch.empty((x.numel() + BLOCK - 1) // BLOCK, dtype=torch.float32, device=x.device)
@@ -56,6 +58,8 @@ def dequantize8(codes: torch.Tensor, steps: torch.Tensor,
     if steps.numel() != (n + BLOCK - 1) // BLOCK:
         raise RuntimeError(f"steps must hold one value per {BLOCK} codes: {(n + BLOCK - 1) // BLOCK}, "
                            f"got {steps.numel()}")
+    if _EXT is not None:
+        return _EXT.dequantize8(codes, steps, dtype)
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     if n:
         _launch(codes.get_device(), "fpscan_dequantize8", codes.data_ptr(), steps.data_ptr(),

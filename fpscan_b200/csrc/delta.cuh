@@ -137,6 +137,56 @@ __device__ __forceinline__ uint32_t at_at(uint32_t base, int lane, int m0, int k
   return tile_at<ROWB>(base, kk * 16 + (m >> 1) * 8 + r, m0 / 8 + (m & 1));
 }
 
+// Strips: 64 tokens x 16 values, rows of 16 values (32 bytes; fp32 64).  A
+// warp's 16 rows of the transposed state meet one strip of v, E, dO or dV.
+// Units are exchanged so that 8 rows of one unit column again fall on 8
+// different bank groups.
+constexpr int kStrip = kChunk * 32;  // bytes of a bf16 strip
+__device__ __forceinline__ uint32_t strip_at(uint32_t base, int row, int unit) {
+  return base + row * 32 + ((unit ^ ((row >> 2) & 1)) << 4);
+}
+__device__ __forceinline__ uint32_t strip32_at(uint32_t base, int row, int unit) {
+  return base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+}
+// A operand with the tokens as its rows (m0..m0+15).
+__device__ __forceinline__ uint32_t strip_a(uint32_t base, int lane, int m0) {
+  const int m = lane >> 3, r = lane & 7;
+  return strip_at(base, m0 + (m & 1) * 8 + r, m >> 1);
+}
+// A operand with the values as its rows, tokens 16 kk.. (transposing load or store).
+__device__ __forceinline__ uint32_t strip_at_t(uint32_t base, int lane, int kk) {
+  const int m = lane >> 3, r = lane & 7;
+  return strip_at(base, kk * 16 + (m >> 1) * 8 + r, m & 1);
+}
+// B operand with the tokens as its columns n0..n0+15.
+__device__ __forceinline__ uint32_t strip_b(uint32_t base, int lane, int n0) {
+  const int m = lane >> 3, r = lane & 7;
+  return strip_at(base, n0 + (m >> 1) * 8 + r, m & 1);
+}
+__device__ __forceinline__ void stsm4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void stsm4_t(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+
 // ---------------------------------------------------------------- bf16 parts
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -203,6 +253,59 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const void* src, int64_t
     const int r = i / U, u = i % U;
     const bool in = r < rows && u < units;
     cp16(tile_at<ROWB>(dst, r, u), in ? s + r * stride + u * 16 : s, in);
+  }
+}
+
+// The kept tiles move between global and shared memory as they lie there, by
+// bulk copies.  Stores: what the warp wrote is made visible to the copy
+// engine, then one lane stores and commits; before the bytes are written
+// again the lane waits until at most N later groups are unread.
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// Non-multicast bulk copy to a shared-memory address, completing on `bar`.
+__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes,
+                                        uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(smem_addr(bar))
+      : "memory");
+}
+// One arrival for a warp whose lanes are done with (or have written) what
+// the barrier guards.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+// A strip of T from token rows: rows [0, rows) and `units` 16-byte units of
+// each from src + r * stride (bytes), zeros elsewhere.  One warp.
+template <typename T>
+__device__ __forceinline__ void load_strip(uint32_t dst, const void* src, int64_t stride, int rows,
+                                           int units, int lane) {
+  constexpr int U = (int)sizeof(T);  // 16 values: 2 or 4 units
+  const char* s = static_cast<const char*>(src);
+#pragma unroll
+  for (int i = 0; i < kChunk * U / 32; ++i) {
+    const int r = (i * 32 + lane) / U, u = (i * 32 + lane) % U;
+    const bool in = r < rows && u < units;
+    cp16(U == 2 ? strip_at(dst, r, u) : strip32_at(dst, r, u), in ? s + r * stride + u * 16 : s, in);
   }
 }
 

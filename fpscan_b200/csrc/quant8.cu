@@ -63,15 +63,12 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const Quant8Params p) {
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) most = max(most, __shfl_xor_sync(mask, most, d));
     const Quant8 q = quant8_block(most);
-    int code[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) code[c] = quant8_code(q, x[c]);
+    const uint2 code = make_uint2(quant8_codes(q, x[0], x[1], x[2], x[3]),
+                                  quant8_codes(q, x[4], x[5], x[6], x[7]));
     if (left >= 8)
-      *reinterpret_cast<uint2*>(p.codes + i) =
-          make_uint2(quant8_pack4(code[0], code[1], code[2], code[3]),
-                     quant8_pack4(code[4], code[5], code[6], code[7]));
+      *reinterpret_cast<uint2*>(p.codes + i) = code;
     else
-      for (int c = 0; c < left; ++c) p.codes[i + c] = (int8_t)code[c];
+      for (int c = 0; c < left; ++c) p.codes[i + c] = (int8_t)((c < 4 ? code.x : code.y) >> (8 * (c & 3)));
     if ((u & 7) == 0) p.steps[u / 8] = q.step;
   }
 }

@@ -2,14 +2,21 @@
 // fp32 step, its largest magnitude over 127, and each value is kept as the
 // nearest multiple -127..127 of it (ties to even).
 //
-// The code is the rounding of x * 127 / most, one product and one quotient,
-// each rounded as IEEE 754 says: for fp16 and bf16 the product is exact and
-// the quotient can only be a tie where it is one exactly, so the codes are
-// those of real arithmetic.  (x times a rounded reciprocal is not: half of
-// a block's largest value, common in bf16, is a tie.)  Magnitudes near the
-// ends of fp32 are brought to its middle by a power of two first.  A block
-// that holds an infinity or a NaN has a step that is not finite and codes of
-// 0: all of it reads back as NaN.
+// The code is the rounding of the quotient x * 127 / most.  Times a rounded
+// reciprocal alone it would not be: half of a block's largest value, common
+// in bf16, is a tie, and the product may land on either side of it.  So the
+// quotient is corrected once by its residual (Markstein, 1990: with the
+// correctly rounded reciprocal y of b and q near a / b, q + (a - q b) y
+// rounds to the quotient), three multiply-adds in place of a division: the
+// kernels below read and write about 3 bytes for a value and have some 20
+// instructions for it before they are bound by them.  For fp16 and bf16
+// x * 127 is exact and a quotient that is not a tie is at least 2^-19 of
+// itself away from one, so the codes are those of real arithmetic; for fp32
+// they are those of fp32 arithmetic.
+//
+// Magnitudes near the ends of fp32 are brought to its middle by a power of
+// two.  A block that holds an infinity or a NaN has a step that is not finite
+// and codes of 0: all of it reads back as NaN.
 #pragma once
 
 #include "common.cuh"
@@ -17,28 +24,42 @@
 namespace fpscan {
 
 struct Quant8 {
-  float step, up, most;  // codes are rint(x * up * 127 / most)
+  float step;       // most / 127
+  float mul;        // 127 times the power of two
+  float most, inv;  // the largest magnitude times the power of two, its reciprocal
+  uint32_t keep;    // all ones; 0: every code is 0
 };
 
 // `bits`: the largest magnitude of the block, as the bits of its absolute
 // value (compared as integers, a NaN is above everything).
 __device__ __forceinline__ Quant8 quant8_block(uint32_t bits) {
   Quant8 q;
-  q.most = __uint_as_float(bits);
-  q.step = q.most / 127.f;
-  q.up = q.most > 0x1p100f ? 0x1p-40f : q.most < 0x1p-80f ? 0x1p40f : 1.f;
-  q.most *= q.up;
+  const float most = __uint_as_float(bits);
+  q.step = most / 127.f;
+  q.keep = bits != 0 && bits < 0x7f800000u ? ~0u : 0u;
+  const float up = most > 0x1p100f ? 0x1p-60f : most < 0x1p-80f ? 0x1p80f : 1.f;
+  q.mul = 127.f * up;
+  q.most = q.keep ? most * up : 1.f;
+  q.inv = __frcp_rn(q.most);
   return q;
 }
 
-__device__ __forceinline__ int quant8_code(const Quant8& q, float x) {
-  const float r = __fdiv_rn(x * q.up * 127.f, q.most);
-  // 127 may come out an ulp larger; NaN (0 / 0 of a block of zeros, too) and infinity give 0
-  return fabsf(r) < 127.5f ? __float2int_rn(r) : 0;
-}
-
-__device__ __forceinline__ uint32_t quant8_pack4(int a, int b, int c, int d) {
-  return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | ((uint32_t)d << 24);
+// Codes of four values, one byte each.
+__device__ __forceinline__ uint32_t quant8_codes(const Quant8& q, float a, float b, float c,
+                                                 float d) {
+  const float x[4] = {a, b, c, d};
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = x[i] * q.mul;
+    float r = t * q.inv;
+    r = fmaf(fmaf(-r, q.most, t), q.inv, r);
+    // adding 1.5 * 2^23 rounds to an integer, ties to even, whose low byte
+    // in two's complement is the sum's
+    w[i] = __float_as_uint(r + 12582912.f);
+  }
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410) &
+         q.keep;
 }
 
 // Value of byte j of w.

@@ -356,8 +356,7 @@ __global__ void __launch_bounds__(NTH, 1)
         uint32_t w[V / 4];
 #pragma unroll
         for (int c = 0; c < V; c += 4)
-          w[c / 4] = quant8_pack4(quant8_code(q8, y[c]), quant8_code(q8, y[c + 1]),
-                                  quant8_code(q8, y[c + 2]), quant8_code(q8, y[c + 3]));
+          w[c / 4] = quant8_codes(q8, y[c], y[c + 1], y[c + 2], y[c + 3]);
         if (lane_ok && blk0 + i < L) {
           int8_t* o = p.codes + (b * L + blk0 + i) * p.code_stride + cv * V;
           if constexpr (V == 8)

@@ -31,7 +31,7 @@ import torch
 
 from . import _lib
 from .checkpoint8 import dequantize8, quantize8
-from .ops import DTYPE_CODES, _check_input, _fn, _launch, nvtx_range
+from .ops import _EXT, DTYPE_CODES, _check_input, _fn, _launch, nvtx_range
 
 __all__ = ["gated_delta", "gated_delta_forward", "gated_delta_step"]
 
@@ -99,7 +99,9 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 
 def _scale(scale: Optional[float], q: torch.Tensor) -> float:
-    return q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if scale is not None:
+        return float(scale)
+    return q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
 
 
 def _delta_workspace(q, v, wide: bool, backward: bool) -> torch.Tensor:
@@ -110,7 +112,18 @@ def _delta_workspace(q, v, wide: bool, backward: bool) -> torch.Tensor:
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=v.device)
 
 
-def _run_forward(q, k, v, log_decay, beta, state, scale, return_state, wide, out=None):
+def _tensors(*ts) -> bool:
+    # what the compiled binding takes; anything else gets its error from validate_delta
+    return _EXT is not None and all(t is None or isinstance(t, torch.Tensor) for t in ts)
+
+
+def _run_forward(q, k, v, log_decay, beta, state, scale, return_state, out=None):
+    if _tensors(q, k, v, log_decay, beta, state, out):
+        return _EXT.delta_forward(q, k, v, log_decay, beta, _state_in(state), scale, return_state, out)
+    _lib.load()
+    validate_delta(q, k, v, log_decay, beta, state, out)
+    state = _state_in(state)
+    wide = state is not None or return_state
     if out is None:
         out = torch.empty_like(v)
     b, l, hk, h, dk, dv = _sizes(q, v)
@@ -129,11 +142,7 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
                         ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """The gated delta rule over a sequence (no autograd): ``out``, or ``(out, final_state)`` with
     ``return_state``.  ``scale`` defaults to ``dk ** -0.5``; ``initial_state`` to zero."""
-    _lib.load()
-    validate_delta(q, k, v, log_decay, beta, initial_state, out)
-    state = _state_in(initial_state)
-    wide = state is not None or return_state
-    out, final = _run_forward(q, k, v, log_decay, beta, state, _scale(scale, q), return_state, wide, out)
+    out, final = _run_forward(q, k, v, log_decay, beta, initial_state, _scale(scale, q), bool(return_state), out)
     return (out, final) if return_state else out
 
 
@@ -145,6 +154,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     if not (isinstance(state, torch.Tensor) and state.is_cuda and state.dtype == torch.float32
             and state.is_contiguous()):
         raise RuntimeError("state must be a contiguous float32 CUDA tensor")
+    if _tensors(q, k, v, log_decay, beta, out):
+        return _EXT.delta_step(q, k, v, log_decay, beta, state, _scale(scale, q), out)
     validate_delta(q, k, v, log_decay, beta, state, out)
     if out is None:
         out = torch.empty_like(v)
@@ -158,8 +169,13 @@ def gated_delta_backward(q, k, v, log_decay, beta, grad_out, initial_state=None,
                          scale: Optional[float] = None, need_initial: bool = False):
     """Gradients of ``gated_delta_forward``: (dq, dk, dv, dlog_decay, dbeta, dinitial); ``grad_final`` is
     the gradient of the final state, ``dinitial`` is None unless ``need_initial``."""
+    if _tensors(q, k, v, log_decay, beta, grad_out, initial_state, grad_final):
+        return _EXT.delta_backward(q, k, v, log_decay, beta, grad_out, _state_in(initial_state),
+                                   _state_in(grad_final), _scale(scale, q), need_initial)
     validate_delta(q, k, v, log_decay, beta, initial_state, grad_out)
     _check_input(grad_out, "grad_out")
+    if grad_final is not None:
+        validate_delta_layout(q, k, v, log_decay, beta, grad_final)
     state, grad_final = _state_in(initial_state), _state_in(grad_final)
     b, l, hk, h, dk, dv = _sizes(q, v)
     wide = state is not None or grad_final is not None or need_initial
@@ -179,12 +195,10 @@ class GatedDelta(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, beta, state, scale, return_state, checkpoint8):
-        validate_delta(q, k, v, log_decay, beta, state)
+        with nvtx_range("fpscan.delta.forward"):
+            out, final = _run_forward(q, k, v, log_decay, beta, state, scale, return_state)
         ctx.state_dtype = None if state is None else state.dtype
         state = _state_in(state)
-        wide = state is not None or return_state
-        with nvtx_range("fpscan.delta.forward"):
-            out, final = _run_forward(q, k, v, log_decay, beta, state, scale, return_state, wide)
         kept = [t for x in (q, k, v) for t in quantize8(x)] if checkpoint8 else [q, k, v]
         ctx.save_for_backward(*kept, log_decay, beta, state)
         ctx.scale, ctx.checkpoint8, ctx.dtype = scale, checkpoint8, v.dtype
