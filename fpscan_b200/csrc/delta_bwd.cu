@@ -14,6 +14,7 @@
 // decay scales what is read after it like q and k do: no quotient of a
 // gradient by beta or by a decay appears, so zeros of both are harmless.
 //
+//   delta_split_kernel  fp16 / fp32 only: cuts dO into bf16 parts.
 //   delta_rev_kernel    from the last chunk to the first, dS^T in registers
 //                       as delta_scan_kernel keeps S^T; writes dV, dS per chunk.
 //   delta_grad_kernel   one CTA per (chunk, head), all in parallel.
@@ -32,18 +33,51 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
 
 namespace {
 
+// ------------------------------------------------------------------ parts of dO
+struct SplitParams {
+  const void* src;
+  __nv_bfloat16* dst;  // part p at + p * n
+  int64_t n;           // elements (a multiple of 8)
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) delta_split_kernel(const SplitParams p) {
+  constexpr int NP = kParts<T>, V = Elem<T>::kVec;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t step = (int64_t)gridDim.x * blockDim.x * 8;
+  const T* src = static_cast<const T*>(p.src);
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < p.n; i += step) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8 / V; ++j) {
+      Vec16<T> v;
+      v.raw = *reinterpret_cast<const uint4*>(src + i + j * V);
+#pragma unroll
+      for (int c = 0; c < V; ++c) x[j * V + c] = Elem<T>::load(v.e[c]);
+    }
+    uint32_t w[4][NP];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split_pair<NP>(x[2 * j], x[2 * j + 1], w[j]);
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+      *reinterpret_cast<uint4*>(p.dst + q * p.n + i) = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
+  }
+}
+
 // ------------------------------------------------------------------ along the chunks, backwards
 struct RevParams {
-  const __nv_bfloat16* q;
-  const __nv_bfloat16* k;
-  const __nv_bfloat16* grad;  // dO parts
-  int64_t part_stride, grad_stride;
+  const __nv_bfloat16* q_tiles;
+  const __nv_bfloat16* k_tiles;
+  const __nv_bfloat16* grad;  // dO parts in token rows, part p at + p * grad_stride
+  int64_t grad_stride;
   const __nv_bfloat16* n_mat;
   const __nv_bfloat16* p_mat;
   const float* vecs;
   const float* grad_final;
   float* dinitial;
   void* dv_out;
+  __nv_bfloat16* do_parts;    // strips, as e_parts
   __nv_bfloat16* dv_parts;
   __nv_bfloat16* ds_parts;
   int64_t L, chunks;
@@ -51,32 +85,45 @@ struct RevParams {
   float scale;
 };
 
+// As in delta_scan_kernel a warp owns 16 rows of dS^T, and its work is shared
+// by two: the helper warp computes what does not need dS -- Z = P^T dO and
+// the sum (scale exp(G) dO)^T Q that joins the state -- and leaves both in
+// shared memory; the chain warp does the rest.  K, N are loaded by the first
+// chain warp, Q, P by the first helper.
 template <int NP, int LV, int DKP, int NW>
 struct RevCfg {
   static constexpr int NS = LV + 1;
   static constexpr int kTileK = kChunk * DKP * 2;
-  static constexpr int kRowG = NW * 32;
-  static constexpr int kTileG = kChunk * kRowG;
   static constexpr int kMat = kChunk * kChunk * 2;
-  static constexpr int oQ = NP * kTileK;
-  static constexpr int oG = oQ + NP * kTileK;
-  static constexpr int oN = oG + NP * kTileG;
-  static constexpr int oP = oN + NS * kMat;
-  static constexpr int oVec = oP + NS * kMat;
-  static constexpr int kStage = oVec + 3 * kChunk * 4 + 256;
-  static constexpr int kStages = 2 * kStage + 128 <= 227 * 1024 ? 2 : 1;
-  static constexpr int kSmem = kStages * kStage + 128;
-  static_assert(kStage % 128 == 0 && kSmem <= 227 * 1024);
+  static constexpr int oN = NP * kTileK, oVec = oN + NS * kMat;
+  static constexpr int kStageK = oVec + 1024;
+  static constexpr int oP = NP * kTileK, oEnter = oP + NS * kMat;
+  static constexpr int kStageQ = oEnter + 256;
+  static constexpr int kG = NP * kStrip;
+  static constexpr int kXS = NS * 16 * DKP * 2, kXV = NS * kStrip;
+  static constexpr int kZ = 8 * 512, kSum = DKP / 8 * 512;
+  static constexpr int kRoom = 227 * 1024 - 1536;
+  static constexpr int kBase = kXS + kXV + kZ + kSum;
+  static constexpr int kBufG = NW * (kBase + 2 * kG) + kStageK + kStageQ <= kRoom ? 2 : 1;
+  static constexpr int kWarp = kBufG * kG + kBase;
+  static constexpr int kStK = NW * kWarp + 2 * kStageK + kStageQ <= kRoom ? 2 : 1;
+  static constexpr int kStQ = NW * kWarp + kStK * kStageK + 2 * kStageQ <= kRoom ? 2 : 1;
+  static constexpr int oQ = kStK * kStageK, oWarp = oQ + kStQ * kStageQ;
+  static constexpr int kSmem = oWarp + NW * kWarp + 128;
+  static constexpr bool kFits = kSmem + 1024 <= 227 * 1024;
 };
 
 template <typename T, int NP, int LV, int DKP, int NW>
-__global__ void __launch_bounds__(NW * 32) delta_rev_kernel(const RevParams p) {
+__global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p) {
   using Cfg = RevCfg<NP, LV, DKP, NW>;
-  constexpr int NS = Cfg::NS, NTH = NW * 32, ROWB = DKP * 2, NT = DKP / 8, MROW = kChunk * 2;
+  static_assert(Cfg::kFits);
+  constexpr int NS = Cfg::NS, ROWB = DKP * 2, NT = DKP / 8, MROW = kChunk * 2;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
   const uint32_t sm0 = smem_addr(dsm);
+  __shared__ __align__(8) uint64_t full_k[2], free_k[2], full_q[2], free_q[2];
+  __shared__ __align__(8) uint64_t full_z[NW], free_z[NW], full_g[NW], free_g[NW];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, t4 = lane & 3;
@@ -84,108 +131,122 @@ __global__ void __launch_bounds__(NW * 32) delta_rev_kernel(const RevParams p) {
   const int slice = (int)(blockIdx.x - bh * p.slices);
   const int64_t b = bh / p.heads;
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
-  const int dv_cta = slice * NW * 16, dv0 = dv_cta + warp * 16;
-  const int nval = p.dv - dv0;
-  const int64_t kstride = (int64_t)p.key_heads * p.dk, vstride = (int64_t)p.heads * p.dv;
-  const int vunits = min(NW * 16, p.dv - dv_cta) / 8;
-
-  auto load = [&](int64_t c, int s) {
-    const uint32_t st = sm0 + s * Cfg::kStage;
-    const int64_t t0 = c * kChunk;
-    const int rows = (int)min((int64_t)kChunk, p.L - t0);
-    const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
-    const int64_t vf = (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv_cta;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      load_tile<kChunk, ROWB, NTH>(st + i * Cfg::kTileK, p.k + i * p.part_stride + kf, kstride * 2,
-                                   rows, p.dk / 8, tid);
-      load_tile<kChunk, ROWB, NTH>(st + Cfg::oQ + i * Cfg::kTileK, p.q + i * p.part_stride + kf,
-                                   kstride * 2, rows, p.dk / 8, tid);
-      load_tile<kChunk, Cfg::kRowG, NTH>(st + Cfg::oG + i * Cfg::kTileG,
-                                         p.grad + i * p.grad_stride + vf, vstride * 2, rows, vunits,
-                                         tid);
+  const int dv_cta = slice * NW * 16;
+  const int nact = min(NW, (p.dv - dv_cta + 15) / 16);
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full_k[i], 1);
+      mbar_init(&free_k[i], nact);
+      mbar_init(&full_q[i], 1);
+      mbar_init(&free_q[i], nact);
     }
-    const int64_t mat = (bh * p.chunks + c) * NS * (kChunk * kChunk);
-    load_tile<NS * kChunk, MROW, NTH>(st + Cfg::oN, p.n_mat + mat, MROW, NS * kChunk, 8, tid);
-    load_tile<NS * kChunk, MROW, NTH>(st + Cfg::oP, p.p_mat + mat, MROW, NS * kChunk, 8, tid);
-    const char* vec = reinterpret_cast<const char*>(p.vecs + (bh * p.chunks + c) * (kVecCount * kChunk));
-    for (int i = tid; i < 3 * kChunk * 4 / 16; i += NTH) cp16(st + Cfg::oVec + i * 16, vec + i * 16, true);
-    cp_commit();
-  };
-
+    for (int i = 0; i < NW; ++i) {
+      mbar_init(&full_z[i], 1);
+      mbar_init(&free_z[i], 1);
+      mbar_init(&full_g[i], 1);
+      mbar_init(&free_g[i], 1);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
 
-  float S[NT][4];  // dS^T
+  const int w = warp < NW ? warp : warp - NW;
+  const int dv0 = dv_cta + w * 16, nval = p.dv - dv0;
+  const int strips = (p.dv + 15) / 16, dvp = strips * 16;
+  const int64_t unit0 = bh * p.chunks, tile = (b * p.key_heads + hk) * p.chunks;
+  const int64_t vstride = (int64_t)p.heads * p.dv;
+  const uint32_t own = sm0 + Cfg::oWarp + w * Cfg::kWarp;
+  const uint32_t x_s = own + Cfg::kBufG * Cfg::kG, x_v = x_s + Cfg::kXS, x_z = x_v + Cfg::kXV,
+                 x_g = x_z + Cfg::kZ;
+  // step d handles chunk chunks - 1 - d
+  int64_t next = 0;  // steps issued by this loading lane
+  auto issue_k = [&]() {
+    const int64_t c = p.chunks - 1 - next;
+    const int s = (int)(next % Cfg::kStK);
+    if (next >= Cfg::kStK && !mbar_wait_bounded(&free_k[s], (uint32_t)((next / Cfg::kStK - 1) & 1)))
+      return false;
+    const uint32_t st = sm0 + s * Cfg::kStageK;
+    mbar_expect_tx(&full_k[s], Cfg::oVec + 3 * kChunk * 4);
+    bulk_in(st, p.k_tiles + (tile + c) * NP * (kChunk * DKP), NP * Cfg::kTileK, &full_k[s]);
+    bulk_in(st + Cfg::oN, p.n_mat + (unit0 + c) * NS * (kChunk * kChunk), NS * Cfg::kMat, &full_k[s]);
+    bulk_in(st + Cfg::oVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), 3 * kChunk * 4, &full_k[s]);
+    ++next;
+    return true;
+  };
+  auto issue_q = [&]() {
+    const int64_t c = p.chunks - 1 - next;
+    const int s = (int)(next % Cfg::kStQ);
+    if (next >= Cfg::kStQ && !mbar_wait_bounded(&free_q[s], (uint32_t)((next / Cfg::kStQ - 1) & 1)))
+      return false;
+    const uint32_t st = sm0 + Cfg::oQ + s * Cfg::kStageQ;
+    mbar_expect_tx(&full_q[s], Cfg::oEnter + kChunk * 4);
+    bulk_in(st, p.q_tiles + (tile + c) * NP * (kChunk * DKP), NP * Cfg::kTileK, &full_q[s]);
+    bulk_in(st + Cfg::oP, p.p_mat + (unit0 + c) * NS * (kChunk * kChunk), NS * Cfg::kMat, &full_q[s]);
+    bulk_in(st + Cfg::oEnter, p.vecs + (unit0 + c) * (kVecCount * kChunk), kChunk * 4, &full_q[s]);
+    ++next;
+    return true;
+  };
+
+  if (warp < NW && nval > 0) {
+    // ---------------------------------------------------------- chain
+    const bool loads = w == 0 && lane == 0;
+    if (loads)
+      while (next < min((int64_t)Cfg::kStK, p.chunks)) issue_k();
+    __syncwarp();
+    float S[NT][4];  // dS^T
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
-    if (p.grad_final != nullptr) {
-      const int dk = n * 8 + 2 * t4;
-      const float* src = p.grad_final + (bh * p.dv + dv0 + g4) * p.dk + dk;
-      if (dk < p.dk) {
-        if (g4 < nval) {
+      for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
+      if (p.grad_final != nullptr) {
+        const int dk = n * 8 + 2 * t4;
+        const float* src = p.grad_final + (bh * p.dv + dv0 + g4) * p.dk + dk;
+        if (dk < p.dk) {
           const float2 v = *reinterpret_cast<const float2*>(src);
           S[n][0] = v.x;
           S[n][1] = v.y;
-        }
-        if (g4 + 8 < nval) {
-          const float2 v = *reinterpret_cast<const float2*>(src + 8 * p.dk);
-          S[n][2] = v.x;
-          S[n][3] = v.y;
+          if (nval > 8) {
+            const float2 y = *reinterpret_cast<const float2*>(src + 8 * p.dk);
+            S[n][2] = y.x;
+            S[n][3] = y.y;
+          }
         }
       }
     }
-  }
-
-  if (Cfg::kStages == 2) load(p.chunks - 1, 0);
-  for (int64_t done = 0; done < p.chunks; ++done) {
-    const int64_t c = p.chunks - 1 - done;
-    const int s = Cfg::kStages == 2 ? (int)(done & 1) : 0;
-    if (Cfg::kStages == 1) {
-      load(c, 0);
-      cp_wait<0>();
-    } else if (c > 0) {
-      load(c - 1, s ^ 1);
-      cp_wait<1>();
-    } else {
-      cp_wait<0>();
-    }
-    __syncthreads();
-    if (nval > 0) {
-      const uint32_t st = sm0 + s * Cfg::kStage;
-      const float* vec = reinterpret_cast<const float*>(dsm + s * Cfg::kStage + Cfg::oVec);
+    bool ok = true;
+    for (int64_t d = 0; d < p.chunks; ++d) {
+      const int64_t c = p.chunks - 1 - d;
+      const int sk = (int)(d % Cfg::kStK);
+      const uint32_t st = sm0 + sk * Cfg::kStageK;
+      const float* vec = reinterpret_cast<const float*>(dsm + sk * Cfg::kStageK + Cfg::oVec);
       const float* enter = vec + kVecEnter * kChunk;
       const float* leave = vec + kVecLeave * kChunk;
       const float* beta = vec + kVecBeta * kChunk;
+      if (Cfg::kStK == 1 && d > 0) {  // one stage: the load waits for every chain warp
+        if (loads) ok = issue_k();
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_k[sk], (uint32_t)((d / Cfg::kStK) & 1)));
+      if (!ok) break;
+      if (d > 0 && lane == 0) bulk_wait_read<1>();
+      __syncwarp();
       const float total = enter[kChunk - 1];
-      const int64_t t0 = c * kChunk;
 
-      __nv_bfloat16* sp = p.ds_parts + (bh * p.chunks + c) * NS * p.dv * DKP;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint32_t w[NS];
-          split_pair<NS>(S[n][2 * r], S[n][2 * r + 1], w);
-          if (g4 + 8 * r < nval)
-#pragma unroll
-            for (int q = 0; q < NS; ++q)
-              *reinterpret_cast<uint32_t*>(sp + ((int64_t)q * p.dv + dv0 + g4 + 8 * r) * DKP +
-                                           n * 8 + 2 * t4) = w[q];
-        }
-
-      // Y = (K dS^T)^T, Z = (P^T dO)^T: 16 values x 64 tokens
-      float Y[8][4], Z[8][4];
+      // Y = (K dS^T)^T: 16 values x 64 tokens.  dS's parts are kept.
+      float Y[8][4];
 #pragma unroll
       for (int n = 0; n < 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Y[n][e] = Z[n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) Y[n][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < DKP / 16; ++kk) {
         uint32_t a[NS][4];
         split_frag<NS>(S[2 * kk], S[2 * kk + 1], a);
+#pragma unroll
+        for (int q = 0; q < NS; ++q) stsm4(at_a<ROWB>(x_s + q * 16 * ROWB, lane, 0, kk), a[q]);
 #pragma unroll
         for (int n2 = 0; n2 < 4; ++n2) {
           Step<LV == 2, 2> s;
@@ -203,12 +264,222 @@ __global__ void __launch_bounds__(NW * 32) delta_rev_kernel(const RevParams p) {
           s.add(1, Y[2 * n2 + 1]);
         }
       }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) {
+        __nv_bfloat16* sp = p.ds_parts + ((unit0 + c) * NS * dvp + dv0) * DKP;
+#pragma unroll
+        for (int q = 0; q < NS; ++q)
+          bulk_s2g(sp + (int64_t)q * dvp * DKP, x_s + q * 16 * ROWB, 16 * ROWB);
+        bulk_commit();
+      }
+      // the stage of the chunk before is free by now
+      if (Cfg::kStK == 2 && loads && d > 0 && next < p.chunks) ok = issue_k();
+      ok = ok && mbar_wait_bounded(&full_z[w], (uint32_t)(d & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+
+      // F = Z + beta exp(G_C - G) Y, in place
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int tok = n * 8 + 2 * t4;
+        const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
+        const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
+        const uint4 z = lds128(x_z + n * 512 + lane * 16);
+        const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
+        Y[n][0] = fmaf(w0, Y[n][0], __uint_as_float(z.x));
+        Y[n][1] = fmaf(w1, Y[n][1], __uint_as_float(z.y));
+        Y[n][2] = fmaf(w0, Y[n][2], __uint_as_float(z.z));
+        Y[n][3] = fmaf(w1, Y[n][3], __uint_as_float(z.w));
+      }
+      warp_arrive(&free_z[w], lane);
+
+      // dV = N^T F
+      float V[8][4];
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) V[n][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t a[NS][4];
+        split_frag<NS>(Y[2 * kk], Y[2 * kk + 1], a);
+#pragma unroll
+        for (int n2 = 0; n2 <= kk; ++n2) {
+          Step<LV == 2, 2> s;
+#pragma unroll
+          for (int i = LV; i >= 0; --i) {
+            uint32_t nb[4];
+            ldsm4_t(nb, at_bt<MROW>(st + Cfg::oN + i * Cfg::kMat, lane, n2 * 16, kk));
+#pragma unroll
+            for (int j = LV - i; j >= 0; --j) {
+              s.mma(0, V[2 * n2], a[j], nb[0], nb[1]);
+              s.mma(1, V[2 * n2 + 1], a[j], nb[2], nb[3]);
+            }
+          }
+          s.add(0, V[2 * n2]);
+          s.add(1, V[2 * n2 + 1]);
+        }
+      }
+      if (lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t a[NS][4];
+        split_frag<NS>(V[2 * kk], V[2 * kk + 1], a);
+#pragma unroll
+        for (int q = 0; q < NS; ++q) stsm4_t(strip_at_t(x_v + q * kStrip, lane, kk), a[q]);
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) {
+        bulk_s2g(p.dv_parts + ((unit0 + c) * strips + dv0 / 16) * NS * (kStrip / 2), x_v, NS * kStrip);
+        bulk_commit();
+      }
+      {
+        const int64_t t0 = c * kChunk;
+        const int rows = (int)min((int64_t)kChunk, p.L - t0);
+        T* out = static_cast<T*>(p.dv_out) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0;
+        if constexpr (NP == 1) {  // the first bf16 part is the rounded value
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 16 + (lane >> 1), un = lane & 1;
+            if (r < rows && un * 8 < nval)
+              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_v, r, un));
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            store_t<T>(out + (int64_t)n * 8 * vstride, vstride, V[n], lane, rows - n * 8, nval);
+        }
+      }
+
+      // dS <- exp(G_C) dS + (scale exp(G) dO)^T Q - (exp(G) dV)^T K
+      uint32_t uv[4][NS][4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int n = 2 * kk + half;
+          const float2 ge = *reinterpret_cast<const float2*>(enter + n * 8 + 2 * t4);
+          V[n][0] *= -ge.x;
+          V[n][1] *= -ge.y;
+          V[n][2] *= -ge.x;
+          V[n][3] *= -ge.y;
+        }
+        split_frag<NS>(V[2 * kk], V[2 * kk + 1], uv[kk]);
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_g[w], (uint32_t)(d & 1)));
+      if (!ok) break;
+#pragma unroll
+      for (int n4 = 0; n4 < NT / 4; ++n4) {
+        float x[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint4 g = lds128(x_g + (n4 * 4 + n) * 512 + lane * 16);
+          x[n][0] = __uint_as_float(g.x);
+          x[n][1] = __uint_as_float(g.y);
+          x[n][2] = __uint_as_float(g.z);
+          x[n][3] = __uint_as_float(g.w);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          Step<LV == 2, 4> s;
+#pragma unroll
+          for (int i = NP - 1; i >= 0; --i) {
+            uint32_t b0[4], b1[4];
+            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
+            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
+#pragma unroll
+            for (int j = LV - i; j >= 0; --j) {
+              s.mma(0, x[0], uv[kk][j], b0[0], b0[1]);
+              s.mma(1, x[1], uv[kk][j], b0[2], b0[3]);
+              s.mma(2, x[2], uv[kk][j], b1[0], b1[1]);
+              s.mma(3, x[3], uv[kk][j], b1[2], b1[3]);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n) s.add(n, x[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[n4 * 4 + n][e] = fmaf(total, S[n4 * 4 + n][e], x[n][e]);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&free_g[w]);
+        mbar_arrive(&free_k[sk]);
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    if (!ok && loads)  // no copy may land after the CTA is gone
+      for (int64_t j = max((int64_t)0, next - Cfg::kStK); j < next; ++j)
+        mbar_wait_bounded(&full_k[j % Cfg::kStK], (uint32_t)((j / Cfg::kStK) & 1));
+    if (ok && p.dinitial != nullptr) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int dk = n * 8 + 2 * t4;
+        float* dst = p.dinitial + (bh * p.dv + dv0 + g4) * p.dk + dk;
+        if (dk < p.dk) {
+          *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
+          if (nval > 8) *reinterpret_cast<float2*>(dst + 8 * p.dk) = make_float2(S[n][2], S[n][3]);
+        }
+      }
+    }
+  } else if (warp >= NW && nval > 0) {
+    // ---------------------------------------------------------- helper
+    const bool loads = w == 0 && lane == 0;
+    if (loads)
+      while (next < min((int64_t)Cfg::kStQ, p.chunks)) issue_q();
+    __syncwarp();
+    auto load_g = [&](int64_t d) {
+      const int64_t t0 = (p.chunks - 1 - d) * kChunk;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        load_strip<__nv_bfloat16>(
+            own + (int)(d % Cfg::kBufG) * Cfg::kG + i * kStrip,
+            p.grad + i * p.grad_stride + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0,
+            vstride * 2, (int)min((int64_t)kChunk, p.L - t0), min(16, nval) / 8, lane);
+      cp_commit();
+    };
+    if (Cfg::kBufG == 2) load_g(0);
+    bool ok = true;
+    for (int64_t d = 0; d < p.chunks; ++d) {
+      const int64_t c = p.chunks - 1 - d;
+      const int sq = (int)(d % Cfg::kStQ);
+      const uint32_t st = sm0 + Cfg::oQ + sq * Cfg::kStageQ, gst = own + (int)(d % Cfg::kBufG) * Cfg::kG;
+      const float* enter = reinterpret_cast<const float*>(dsm + Cfg::oQ + sq * Cfg::kStageQ + Cfg::oEnter);
+      if (lane == 0) bulk_wait_read<0>();  // the strip of the step before has been kept
+      __syncwarp();
+      if (Cfg::kBufG == 1) load_g(d);
+      if (Cfg::kBufG == 2 && d + 1 < p.chunks) {
+        load_g(d + 1);
+        cp_wait<1>();
+      } else {
+        cp_wait<0>();
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) {
+        bulk_s2g(p.do_parts + ((unit0 + c) * strips + dv0 / 16) * NP * (kStrip / 2), gst, NP * kStrip);
+        bulk_commit();
+      }
+      ok = mbar_wait_bounded(&full_q[sq], (uint32_t)((d / Cfg::kStQ) & 1));
+      if (d > 0) ok = ok && mbar_wait_bounded(&free_z[w], (uint32_t)((d - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      float Z[8][4];
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Z[n][e] = 0.f;
+      uint32_t ug[4][NS][4];  // parts of scale exp(G) dO
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         uint32_t a[NP][4];
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
-          ldsm4_t(a[i], at_at<Cfg::kRowG>(st + Cfg::oG + i * Cfg::kTileG, lane, warp * 16, kk));
+        for (int i = 0; i < NP; ++i) ldsm4_t(a[i], strip_at_t(gst + i * kStrip, lane, kk));
 #pragma unroll
         for (int n2 = 0; n2 <= kk; ++n2) {
           Step<LV == 2, 2> s;
@@ -226,157 +497,85 @@ __global__ void __launch_bounds__(NW * 32) delta_rev_kernel(const RevParams p) {
           s.add(0, Z[2 * n2]);
           s.add(1, Z[2 * n2 + 1]);
         }
-      }
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int tok = n * 8 + 2 * t4;
-        const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
-        const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
-        const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
-        Z[n][0] = fmaf(w0, Y[n][0], Z[n][0]);
-        Z[n][1] = fmaf(w1, Y[n][1], Z[n][1]);
-        Z[n][2] = fmaf(w0, Y[n][2], Z[n][2]);
-        Z[n][3] = fmaf(w1, Y[n][3], Z[n][3]);
+        for (int r = 0; r < 4; ++r) {
+          const float2 ge = *reinterpret_cast<const float2*>(enter + kk * 16 + (r >> 1) * 8 + 2 * t4);
+          float x = 0.f, y = 0.f;
+#pragma unroll
+          for (int i = NP - 1; i >= 0; --i) {
+            x += bf16_lo(a[i][r]);
+            y += bf16_hi(a[i][r]);
+          }
+          uint32_t parts[NS];
+          split_pair<NS>(x * (ge.x * p.scale), y * (ge.y * p.scale), parts);
+#pragma unroll
+          for (int q = 0; q < NS; ++q) ug[kk][q][r] = parts[q];
+        }
       }
-
-      // dV = N^T F (in Y)
 #pragma unroll
       for (int n = 0; n < 8; ++n)
+        sts128(x_z + n * 512 + lane * 16,
+               make_uint4(__float_as_uint(Z[n][0]), __float_as_uint(Z[n][1]),
+                          __float_as_uint(Z[n][2]), __float_as_uint(Z[n][3])));
+      warp_arrive(&full_z[w], lane);
+      if (d > 0) ok = mbar_wait_bounded(&free_g[w], (uint32_t)((d - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll 2
+      for (int n4 = 0; n4 < NT / 4; ++n4) {
+        float x[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Y[n][e] = 0.f;
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t a[NS][4];
-        split_frag<NS>(Z[2 * kk], Z[2 * kk + 1], a);
-#pragma unroll
-        for (int n2 = 0; n2 <= kk; ++n2) {
-          Step<LV == 2, 2> s;
-#pragma unroll
-          for (int i = LV; i >= 0; --i) {
-            uint32_t nb[4];
-            ldsm4_t(nb, at_bt<MROW>(st + Cfg::oN + i * Cfg::kMat, lane, n2 * 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, Y[2 * n2], a[j], nb[0], nb[1]);
-              s.mma(1, Y[2 * n2 + 1], a[j], nb[2], nb[3]);
-            }
-          }
-          s.add(0, Y[2 * n2]);
-          s.add(1, Y[2 * n2 + 1]);
-        }
-      }
-      {
-        T* out = static_cast<T*>(p.dv_out) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0;
-        const int rows = (int)min((int64_t)kChunk, p.L - t0);
-        __nv_bfloat16* vp = p.dv_parts + (bh * p.chunks + c) * NS * kChunk * p.dv + dv0;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          store_t<T>(out + (int64_t)n * 8 * vstride, vstride, Y[n], lane, rows - n * 8, nval);
-          uint32_t lo[NS], hi[NS];
-          split_pair<NS>(Y[n][0], Y[n][1], lo);
-          split_pair<NS>(Y[n][2], Y[n][3], hi);
-#pragma unroll
-          for (int q = 0; q < NS; ++q) {
-            const uint32_t x = movmatrix_t(lo[q]), y = movmatrix_t(hi[q]);
-            __nv_bfloat16* o = vp + ((int64_t)q * kChunk + n * 8 + g4) * p.dv + 2 * t4;
-            *reinterpret_cast<uint32_t*>(o) = x;
-            if (nval > 8) *reinterpret_cast<uint32_t*>(o + 8) = y;
-          }
-        }
-      }
-
-      // dS <- exp(G_C) dS + (scale exp(G) dO)^T Q - (exp(G) dV)^T K
-      uint32_t ug[4][NS][4], uv[4][NS][4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        float x[4][2];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r][0] = x[r][1] = 0.f;
-#pragma unroll
-        for (int i = NP - 1; i >= 0; --i) {
-          uint32_t a[4];
-          ldsm4_t(a, at_at<Cfg::kRowG>(st + Cfg::oG + i * Cfg::kTileG, lane, warp * 16, kk));
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[r][0] += bf16_lo(a[r]);
-            x[r][1] += bf16_hi(a[r]);
-          }
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float2 ge = *reinterpret_cast<const float2*>(enter + kk * 16 + half * 8 + 2 * t4);
-          const int n = 2 * kk + half;
-          Y[n][0] *= -ge.x;
-          Y[n][1] *= -ge.y;
-          Y[n][2] *= -ge.x;
-          Y[n][3] *= -ge.y;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            x[2 * half + r][0] *= ge.x * p.scale;
-            x[2 * half + r][1] *= ge.y * p.scale;
-            uint32_t w[NS];
-            split_pair<NS>(x[2 * half + r][0], x[2 * half + r][1], w);
-#pragma unroll
-            for (int q = 0; q < NS; ++q) ug[kk][q][2 * half + r] = w[q];
-          }
-        }
-        split_frag<NS>(Y[2 * kk], Y[2 * kk + 1], uv[kk]);
-      }
-#pragma unroll
-      for (int n2 = 0; n2 < NT / 2; ++n2) {
-        float d[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           Step<LV == 2, 4> s;
 #pragma unroll
           for (int i = NP - 1; i >= 0; --i) {
-            uint32_t qb[4], kb[4];
-            ldsm4_t(qb, at_bt<ROWB>(st + Cfg::oQ + i * Cfg::kTileK, lane, n2 * 16, kk));
-            ldsm4_t(kb, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n2 * 16, kk));
+            uint32_t b0[4], b1[4];
+            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
+            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
 #pragma unroll
             for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, d[0], ug[kk][j], qb[0], qb[1]);
-              s.mma(1, d[1], ug[kk][j], qb[2], qb[3]);
-              s.mma(2, d[0], uv[kk][j], kb[0], kb[1]);
-              s.mma(3, d[1], uv[kk][j], kb[2], kb[3]);
+              s.mma(0, x[0], ug[kk][j], b0[0], b0[1]);
+              s.mma(1, x[1], ug[kk][j], b0[2], b0[3]);
+              s.mma(2, x[2], ug[kk][j], b1[0], b1[1]);
+              s.mma(3, x[3], ug[kk][j], b1[2], b1[3]);
             }
           }
 #pragma unroll
-          for (int n = 0; n < 4; ++n) s.add(n, d[n & 1]);
+          for (int n = 0; n < 4; ++n) s.add(n, x[n]);
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[n2 * 2 + n][e] = fmaf(total, S[n2 * 2 + n][e], d[n][e]);
+        for (int n = 0; n < 4; ++n)
+          sts128(x_g + (n4 * 4 + n) * 512 + lane * 16,
+                 make_uint4(__float_as_uint(x[n][0]), __float_as_uint(x[n][1]),
+                            __float_as_uint(x[n][2]), __float_as_uint(x[n][3])));
       }
-    }
-    __syncthreads();
-  }
-
-  if (p.dinitial != nullptr && nval > 0) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int dk = n * 8 + 2 * t4;
-      float* dst = p.dinitial + (bh * p.dv + dv0 + g4) * p.dk + dk;
-      if (dk < p.dk) {
-        if (g4 < nval) *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
-        if (g4 + 8 < nval)
-          *reinterpret_cast<float2*>(dst + 8 * p.dk) = make_float2(S[n][2], S[n][3]);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full_g[w]);
+        mbar_arrive(&free_q[sq]);
       }
+      if (loads && next < p.chunks) ok = issue_q();
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
     }
+    cp_wait<0>();
+    if (lane == 0) bulk_wait_all();
+    if (!ok && loads)
+      for (int64_t j = max((int64_t)0, next - Cfg::kStQ); j < next; ++j)
+        mbar_wait_bounded(&full_q[j % Cfg::kStQ], (uint32_t)((j / Cfg::kStQ) & 1));
   }
+  __syncthreads();  // shared memory outlives every copy into it and out of it
 }
 
 // ------------------------------------------------------------------ gradients of a chunk
 struct GradParams {
-  const __nv_bfloat16* q;
-  const __nv_bfloat16* k;
-  const __nv_bfloat16* grad;
-  int64_t part_stride, grad_stride;
+  const __nv_bfloat16* q_tiles;
+  const __nv_bfloat16* k_tiles;
+  const __nv_bfloat16* do_parts;
   const __nv_bfloat16* e_parts;
   const __nv_bfloat16* dv_parts;
   const __nv_bfloat16* s_parts;
@@ -395,36 +594,42 @@ struct GradParams {
 };
 
 constexpr int kGradThreads = 256;
-constexpr int kSlice = 64;  // values (dv) per step of the first phase
 
+// A CTA of 8 warps: H and X as 2 x 4 tiles of 32 x 16, the three 64 x dk sums
+// as 2 x 4 tiles of 32 x dk / 4, all in registers (128 a thread at dk = 128)
+// while dO, dV, E, S0 and dS pass once through a ring of bulk copies, KS
+// strips of 16 values at a time.
 template <int NP, int LV, int DKP>
 struct GradCfg {
   static constexpr int NS = LV + 1;
   static constexpr int kTileK = kChunk * DKP * 2;
-  static constexpr int kTileV = kChunk * kSlice * 2;
   static constexpr int kMat = kChunk * kChunk * 2;
-  // first phase: dO, dV, E, S0, dS of one slice
-  static constexpr int oV = NP * kTileV;
-  static constexpr int oE = oV + NS * kTileV;
-  static constexpr int oS = oE + NS * kTileV;
-  static constexpr int oD = oS + NS * kSlice * DKP * 2;
-  static constexpr int kFirst = oD + NS * kSlice * DKP * 2;
-  // second phase, over the first's: K, Q, and four matrices
+  static constexpr int kRows = 16 * DKP * 2;  // 16 rows of a part of S0 or dS
+  static constexpr int kOne = (NP + 2 * NS) * kStrip + 2 * NS * kRows;  // one strip's share
+  static constexpr int KS = LV == 1 ? 2 : 1;
+  // a stage
+  static constexpr int oV = KS * NP * kStrip;
+  static constexpr int oE = oV + KS * NS * kStrip;
+  static constexpr int oS = oE + KS * NS * kStrip;
+  static constexpr int oD = oS + NS * KS * kRows;
+  static constexpr int kStage = oD + NS * KS * kRows;
+  static_assert(kStage == KS * kOne);
+  // K and Q stay; the four matrices take the place of the ring
   static constexpr int oQ = NP * kTileK;
-  static constexpr int oHs = 2 * NP * kTileK;
-  static constexpr int oHb = oHs + NS * kMat;
-  static constexpr int oXd = oHb + NS * kMat;
-  static constexpr int oXb = oXd + NS * kMat;
-  static constexpr int kSecond = oXb + NS * kMat;
-  static constexpr int kBody = kFirst > kSecond ? kFirst : kSecond;
-  static constexpr int kSmem = kBody + 128;
-  static_assert(kSmem + 8192 <= 227 * 1024);
+  static constexpr int oRing = 2 * NP * kTileK;
+  static constexpr int oHs = oRing, oHb = oHs + NS * kMat, oXd = oHb + NS * kMat, oXb = oXd + NS * kMat;
+  static constexpr int kMats = 4 * NS * kMat;
+  static constexpr int kRoom = 227 * 1024 - 6144 - 128 - oRing;
+  static constexpr int kStages = kRoom / kStage < 4 ? kRoom / kStage : 4;
+  static constexpr int kRing = kStages * kStage > kMats ? kStages * kStage : kMats;
+  static constexpr int kSmem = oRing + kRing + 128;
+  static_assert(kStages >= 2 && kSmem + 6144 <= 227 * 1024);
 };
 
 template <typename T, int NP, int LV, int DKP>
 __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradParams p) {
   using Cfg = GradCfg<NP, LV, DKP>;
-  constexpr int NS = Cfg::NS, NTH = kGradThreads, ROWB = DKP * 2, VROW = kSlice * 2, MROW = kChunk * 2;
+  constexpr int NS = Cfg::NS, NTH = kGradThreads, ROWB = DKP * 2, MROW = kChunk * 2, KS = Cfg::KS;
   constexpr int NT = DKP / 32;  // n tiles of a warp's DKP / 4 columns
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
@@ -433,6 +638,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   __shared__ __align__(16) float s_vec[kVecCount * kChunk];
   __shared__ float s_red[3][4][kChunk];
   __shared__ float s_dot[NTH / 32];
+  __shared__ __align__(8) uint64_t full[Cfg::kStages], freed[Cfg::kStages], full_kq;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, t4 = lane & 3;
@@ -442,16 +648,53 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
   const int64_t t0 = chunk * kChunk;
   const int rows = (int)min((int64_t)kChunk, p.L - t0);
-  const int64_t kstride = (int64_t)p.key_heads * p.dk, vstride = (int64_t)p.heads * p.dv;
+  const int64_t kstride = (int64_t)p.key_heads * p.dk;
   const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
   const int64_t unit = bh * p.chunks + chunk;
-
+  const int strips = (p.dv + 15) / 16, dvp = strips * 16, slices = (strips + KS - 1) / KS;
+  if (tid == 0) {
+    for (int i = 0; i < Cfg::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&freed[i], NTH / 32);
+    }
+    mbar_init(&full_kq, 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
+
+  // thread 0 issues the copies
+  int next = 0;
+  auto issue = [&]() {
+    const int s = next % Cfg::kStages;
+    if (next >= Cfg::kStages && !mbar_wait_bounded(&freed[s], (uint32_t)((next / Cfg::kStages - 1) & 1)))
+      return false;
+    const int v0 = next * KS, n = min(KS, strips - v0);
+    const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
+    mbar_expect_tx(&full[s], n * Cfg::kOne);
+    bulk_in(at, p.do_parts + (unit * strips + v0) * NP * (kStrip / 2), n * NP * kStrip, &full[s]);
+    bulk_in(at + Cfg::oV, p.dv_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
+    bulk_in(at + Cfg::oE, p.e_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int64_t sv = ((unit * NS + i) * dvp + v0 * 16) * DKP;
+      bulk_in(at + Cfg::oS + i * KS * Cfg::kRows, p.s_parts + sv, n * Cfg::kRows, &full[s]);
+      bulk_in(at + Cfg::oD + i * KS * Cfg::kRows, p.ds_parts + sv, n * Cfg::kRows, &full[s]);
+    }
+    ++next;
+    return true;
+  };
+  if (tid == 0) {
+    while (next < min(Cfg::kStages, slices)) issue();
+    const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kChunk * DKP);
+    mbar_expect_tx(&full_kq, 2 * NP * Cfg::kTileK);
+    bulk_in(st, p.k_tiles + tile, NP * Cfg::kTileK, &full_kq);
+    bulk_in(st + Cfg::oQ, p.q_tiles + tile, NP * Cfg::kTileK, &full_kq);
+  }
   {
-    const char* vec = reinterpret_cast<const char*>(p.vecs + unit * (kVecCount * kChunk));
-    const uint32_t dst = smem_addr(s_vec);
-    for (int i = tid; i < kVecCount * kChunk * 4 / 16; i += NTH) cp16(dst + i * 16, vec + i * 16, true);
+    const float* vec = p.vecs + unit * (kVecCount * kChunk);
+    for (int i = tid; i < kVecCount * kChunk; i += NTH) s_vec[i] = vec[i];
   }
 
   float aq[2][NT][4], ar[2][NT][4], aw[2][NT][4], ah[2][2][4], ax[2][2][4];
@@ -470,42 +713,24 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   const int col0 = wc * (DKP / 4);
   float dot = 0.f;  // this thread's share of <S0, dS>
 
-  for (int v0 = 0; v0 < p.dv; v0 += kSlice) {
-    const int vals = min(kSlice, p.dv - v0);
-    const int64_t vf = (b * p.L + t0) * vstride + (int64_t)h * p.dv + v0;
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-      load_tile<kChunk, VROW, NTH>(st + i * Cfg::kTileV, p.grad + i * p.grad_stride + vf,
-                                   vstride * 2, rows, vals / 8, tid);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int64_t ev = (unit * NS + i) * kChunk * p.dv + v0;
-      const int64_t sv = ((unit * NS + i) * p.dv + v0) * DKP;
-      load_tile<kChunk, VROW, NTH>(st + Cfg::oV + i * Cfg::kTileV, p.dv_parts + ev, (int64_t)p.dv * 2,
-                                   kChunk, vals / 8, tid);
-      load_tile<kChunk, VROW, NTH>(st + Cfg::oE + i * Cfg::kTileV, p.e_parts + ev, (int64_t)p.dv * 2,
-                                   kChunk, vals / 8, tid);
-      load_tile<kSlice, ROWB, NTH>(st + Cfg::oS + i * kSlice * ROWB, p.s_parts + sv, ROWB, vals,
-                                   ROWB / 16, tid);
-      load_tile<kSlice, ROWB, NTH>(st + Cfg::oD + i * kSlice * ROWB, p.ds_parts + sv, ROWB, vals,
-                                   ROWB / 16, tid);
-    }
-    cp_commit();
-    cp_wait<0>();
-    __syncthreads();
-
-#pragma unroll
-    for (int kk = 0; kk < kSlice / 16; ++kk) {
+  bool ok = true;
+  for (int it = 0; it < slices; ++it) {
+    const int s_id = it % Cfg::kStages, n = min(KS, strips - it * KS);
+    const uint32_t at = st + Cfg::oRing + s_id * Cfg::kStage;
+    ok = mbar_wait_bounded(&full[s_id], (uint32_t)((it / Cfg::kStages) & 1));
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    for (int kk = 0; kk < n; ++kk) {
       {
         uint32_t ag[NP][2][4], av[NS][2][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
           for (int i = 0; i < NP; ++i)
-            ldsm4(ag[i][m], at_a<VROW>(st + i * Cfg::kTileV, lane, wr * 32 + m * 16, kk));
+            ldsm4(ag[i][m], strip_a(at + (kk * NP + i) * kStrip, lane, wr * 32 + m * 16));
 #pragma unroll
           for (int i = 0; i < NS; ++i)
-            ldsm4(av[i][m], at_a<VROW>(st + Cfg::oV + i * Cfg::kTileV, lane, wr * 32 + m * 16, kk));
+            ldsm4(av[i][m], strip_a(at + Cfg::oV + (kk * NS + i) * kStrip, lane, wr * 32 + m * 16));
         }
         if (lower) {
 #pragma unroll
@@ -514,7 +739,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 #pragma unroll
             for (int j = LV; j >= 0; --j) {
               uint32_t eb[4];
-              ldsm4(eb, at_b<VROW>(st + Cfg::oE + j * Cfg::kTileV, lane, wc * 16, kk));
+              ldsm4(eb, strip_b(at + Cfg::oE + (kk * NS + j) * kStrip, lane, wc * 16));
 #pragma unroll
               for (int i = LV - j; i >= 0; --i) {
                 if (i < NP) {
@@ -537,7 +762,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 #pragma unroll
           for (int j = LV; j >= 0; --j) {
             uint32_t sb[4];
-            ldsm4_t(sb, at_bt<ROWB>(st + Cfg::oS + j * kSlice * ROWB, lane, col0 + n2 * 16, kk));
+            ldsm4_t(sb, at_bt<ROWB>(at + Cfg::oS + j * KS * Cfg::kRows, lane, col0 + n2 * 16, kk));
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -564,14 +789,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-          ldsm4(ae[i][m], at_a<VROW>(st + Cfg::oE + i * Cfg::kTileV, lane, wr * 32 + m * 16, kk));
+          ldsm4(ae[i][m], strip_a(at + Cfg::oE + (kk * NS + i) * kStrip, lane, wr * 32 + m * 16));
 #pragma unroll
       for (int n2 = 0; n2 < NT / 2; ++n2) {
         Step<LV == 2, 4> s;
 #pragma unroll
         for (int j = LV; j >= 0; --j) {
           uint32_t db[4];
-          ldsm4_t(db, at_bt<ROWB>(st + Cfg::oD + j * kSlice * ROWB, lane, col0 + n2 * 16, kk));
+          ldsm4_t(db, at_bt<ROWB>(at + Cfg::oD + j * KS * Cfg::kRows, lane, col0 + n2 * 16, kk));
 #pragma unroll
           for (int i = LV - j; i >= 0; --i)
 #pragma unroll
@@ -588,34 +813,41 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       }
     }
     // <S0, dS> over this slice (the same place of every part: swizzle does not matter)
-    for (int i = tid; i < kSlice * DKP / 2; i += NTH) {
-      float x0 = 0.f, x1 = 0.f, y0 = 0.f, y1 = 0.f;
+    for (int i = tid; i < n * Cfg::kRows / 16; i += NTH) {
+      float x[8] = {}, y[8] = {};
 #pragma unroll
       for (int q = NS - 1; q >= 0; --q) {
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(dsm + Cfg::oS + q * kSlice * ROWB + i * 4);
-        const uint32_t y = *reinterpret_cast<const uint32_t*>(dsm + Cfg::oD + q * kSlice * ROWB + i * 4);
-        x0 += bf16_lo(x);
-        x1 += bf16_hi(x);
-        y0 += bf16_lo(y);
-        y1 += bf16_hi(y);
+        const uint4 u = lds128(at + Cfg::oS + q * KS * Cfg::kRows + i * 16);
+        const uint4 v = lds128(at + Cfg::oD + q * KS * Cfg::kRows + i * 16);
+        const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] += bf16_lo(uw[e]);
+          x[2 * e + 1] += bf16_hi(uw[e]);
+          y[2 * e] += bf16_lo(vw[e]);
+          y[2 * e + 1] += bf16_hi(vw[e]);
+        }
       }
-      dot = fmaf(x0, y0, fmaf(x1, y1, dot));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
     }
-    __syncthreads();
+    warp_arrive(&freed[s_id], lane);
+    // refill the stage of the slice before: every warp is done with it by now
+    if (tid == 0 && it > 0 && next < slices) ok = issue();
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
   if (lane == 0) s_dot[warp] = dot;
-
-  // second phase: K and Q take the place of the slices
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    load_tile<kChunk, ROWB, NTH>(st + i * Cfg::kTileK, p.k + i * p.part_stride + kf, kstride * 2, rows,
-                                 p.dk / 8, tid);
-    load_tile<kChunk, ROWB, NTH>(st + Cfg::oQ + i * Cfg::kTileK, p.q + i * p.part_stride + kf,
-                                 kstride * 2, rows, p.dk / 8, tid);
+  if (tid == 0) {
+    // no copy may land later: what was issued is waited for, also after a
+    // wait that gave up
+    for (int j = max(0, next - Cfg::kStages); j < next; ++j)
+      ok = mbar_wait_bounded(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1)) && ok;
+    ok = mbar_wait_bounded(&full_kq, 0) && ok;
   }
-  cp_commit();
+  if (__syncthreads_or(!ok)) return;  // also: the ring is read, s_vec written
+
+  // second phase: the matrices take the place of the ring
   const float* enter = s_vec + kVecEnter * kChunk;
   const float* leave = s_vec + kVecLeave * kChunk;
   const float* beta = s_vec + kVecBeta * kChunk;
@@ -654,7 +886,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
         put(xd, Cfg::oXd);
         put(xb, Cfg::oXb);
       }
-  cp_wait<0>();
+  mbar_wait_bounded(&full_kq, 0);  // landed: thread 0 has seen it
   __syncthreads();
 
   // an element pair of K or Q as fp32 (the sum of its parts)
@@ -867,7 +1099,7 @@ cudaError_t rev_nw(const DeltaArgs& a, RevParams& p, int64_t bh) {
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
   p.slices = (int)((a.dv + NW * 16 - 1) / (NW * 16));
-  return launch_pdl(kern, (unsigned)(bh * p.slices), NW * 32, Cfg::kSmem, a.stream, p);
+  return launch_pdl(kern, (unsigned)(bh * p.slices), NW * 64, Cfg::kSmem, a.stream, p);
 }
 
 template <typename T, int LV, int DKP>
@@ -882,23 +1114,25 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   const int64_t tok = nb * a.seqlen, bh = nb * a.heads;
 
   RevParams r{};
-  if (NP > 1) {
-    r.q = bf(pl.q_parts);
-    r.k = bf(pl.k_parts);
-    r.grad = bf(pl.do_parts);
-    r.part_stride = tok * a.key_heads * a.dk;
-    r.grad_stride = tok * a.heads * a.dv;
+  if constexpr (NP > 1) {
+    SplitParams sp{static_cast<const T*>(a.grad_out) + v0, bf(pl.grad_rows), tok * a.heads * a.dv};
+    const unsigned grid = (unsigned)std::min<int64_t>((sp.n + 2047) / 2048, 16 * a.num_sms);
+    e = launch_pdl(delta_split_kernel<T>, grid, 256, 0, a.stream, sp);
+    if (e != cudaSuccess) return e;
+    r.grad = sp.dst;
+    r.grad_stride = sp.n;
   } else {
-    r.q = static_cast<const __nv_bfloat16*>(a.q) + k0;
-    r.k = static_cast<const __nv_bfloat16*>(a.k) + k0;
     r.grad = static_cast<const __nv_bfloat16*>(a.grad_out) + v0;
   }
+  r.q_tiles = bf(pl.q_tiles);
+  r.k_tiles = bf(pl.k_tiles);
   r.n_mat = bf(pl.n_mat);
   r.p_mat = bf(pl.p_mat);
   r.vecs = reinterpret_cast<const float*>(ws + pl.vecs);
   r.grad_final = a.grad_final ? a.grad_final + s0 : nullptr;
   r.dinitial = a.dinitial ? a.dinitial + s0 : nullptr;
   r.dv_out = static_cast<T*>(a.dv_out) + v0;
+  r.do_parts = bf(pl.do_parts);
   r.dv_parts = bf(pl.dv_parts);
   r.ds_parts = bf(pl.ds_parts);
   r.L = a.seqlen;
@@ -908,16 +1142,18 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   r.dk = (int)a.dk;
   r.dv = (int)a.dv;
   r.scale = a.scale;
-  const bool narrow = bh * ((a.dv + 127) / 128) < a.num_sms || a.dv <= 64;
-  e = narrow ? rev_nw<T, LV, DKP, 4>(a, r, bh) : rev_nw<T, LV, DKP, 8>(a, r, bh);
+  // chain warps per CTA as in the forward; where four do not fit, two
+  const bool two = !RevCfg<NP, LV, DKP, 4>::kFits || bh * ((a.dv + 31) / 32) <= a.num_sms;
+  if constexpr (RevCfg<NP, LV, DKP, 4>::kFits)
+    e = two ? rev_nw<T, LV, DKP, 2>(a, r, bh) : rev_nw<T, LV, DKP, 4>(a, r, bh);
+  else
+    e = rev_nw<T, LV, DKP, 2>(a, r, bh);
   if (e != cudaSuccess) return e;
 
   GradParams g{};
-  g.q = r.q;
-  g.k = r.k;
-  g.grad = r.grad;
-  g.part_stride = r.part_stride;
-  g.grad_stride = r.grad_stride;
+  g.q_tiles = r.q_tiles;
+  g.k_tiles = r.k_tiles;
+  g.do_parts = r.do_parts;
   g.e_parts = bf(pl.e_parts);
   g.dv_parts = r.dv_parts;
   g.s_parts = bf(pl.s_parts);

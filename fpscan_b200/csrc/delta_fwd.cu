@@ -1,21 +1,33 @@
 // Gated delta rule, forward over a sequence in chunks of 64 tokens (sm_100a).
 // The mathematics and the number format of the products are in delta.cuh.
 //
-//   delta_split_kernel  fp16 / fp32 inputs only: cuts q, k into bf16 parts.
 //   delta_prep_kernel   one CTA per (chunk, head), all in parallel: the
-//                       64 x 64 matrices N and P and the decay vectors.
+//                       64 x 64 matrices N and P, the decay vectors, and K
+//                       and Q as bf16 parts in the layout of the tiles in
+//                       shared memory.
 //   delta_scan_kernel   runs along the chunks of a head with the state in
 //                       registers: the only sequential part.
 //
 // The scan keeps the state transposed, S^T tiles as accumulators: a warp
 // owns 16 rows of values (dv) and all of dk (64 registers a thread at
 // dk = 128).  Every product of the chain then has the warp's own rows as its
-// A operand -- K S0^T, N R, P E, the state's update -- and an accumulator
-// turns into the next product's A operand by packing registers, so the
-// chain of a chunk runs without shared memory or a barrier between its
-// products; K, Q, N and P are the B operands and come from shared memory
-// once for all warps.  Columns of the state never mix, so a head may be cut
-// along dv over as many CTAs as the GPU has room for.
+// A operand -- K S0^T, N R, the state's update -- and an accumulator turns
+// into the next product's A operand by packing registers, so the chain of a
+// chunk needs no barrier between its products.  Columns of the state never
+// mix, so a head is cut along dv over as many CTAs as the GPU has room for.
+//
+// One warp alone issues about every third cycle (its products wait for one
+// another), so the work of a chunk is shared by two kinds of warps:
+//   chain warps   R, E and the state;
+//   output warps  one for each chain warp: O = scale exp(G) Q S0^T + P E,
+//                 from the parts of S0 and E that the chain warp leaves in
+//                 shared memory, while that goes on to the update and the
+//                 next chunk.
+// K, N (chain) and Q, P (output) come by bulk copies through a ring of one or
+// two stages each, issued by the first output warp after each of its chunks
+// (a ninth warp for it would cost every thread a third of its registers).
+// Where the states and E are kept for the backward pass there is no output,
+// and one more warp loads.
 #include <algorithm>
 
 #include "delta.cuh"
@@ -25,46 +37,12 @@ namespace fpscan {
 
 namespace {
 
-// ------------------------------------------------------------------ input parts
-struct SplitParams {
-  const void* src[3];
-  __nv_bfloat16* dst[3];
-  int64_t n[3];       // elements (multiples of 8)
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) delta_split_kernel(const SplitParams p) {
-  constexpr int NP = kParts<T>;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int which = blockIdx.x % 3;
-  const int64_t n = p.n[which], step = (int64_t)(gridDim.x / 3) * blockDim.x * 8;
-  const T* src = static_cast<const T*>(p.src[which]);
-  __nv_bfloat16* dst = p.dst[which];
-  for (int64_t i = ((int64_t)(blockIdx.x / 3) * blockDim.x + threadIdx.x) * 8; i < n; i += step) {
-    float x[8];
-    constexpr int V = Elem<T>::kVec;
-#pragma unroll
-    for (int j = 0; j < 8 / V; ++j) {
-      Vec16<T> v;
-      v.raw = *reinterpret_cast<const uint4*>(src + i + j * V);
-#pragma unroll
-      for (int c = 0; c < V; ++c) x[j * V + c] = Elem<T>::load(v.e[c]);
-    }
-    uint32_t w[4][NP];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) split_pair<NP>(x[2 * j], x[2 * j + 1], w[j]);
-#pragma unroll
-    for (int q = 0; q < NP; ++q)
-      *reinterpret_cast<uint4*>(dst + q * n + i) = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
-  }
-}
-
 // ------------------------------------------------------------------ per-chunk matrices
 struct PrepParams {
-  const __nv_bfloat16* q;   // parts, part p at + p * part_stride
-  const __nv_bfloat16* k;
-  int64_t part_stride;
+  const void* q;
+  const void* k;
+  __nv_bfloat16* q_tiles;   // [key head][chunk][NP][64][DKP], as in shared memory
+  __nv_bfloat16* k_tiles;
   const void* log_decay;
   const void* beta;
   __nv_bfloat16* n_mat;
@@ -76,11 +54,52 @@ struct PrepParams {
 };
 
 constexpr int kPrepThreads = 128;
+constexpr int kMatBytes = kChunk * kChunk * 2;  // one part of N or P
 constexpr int kPad = kChunk + 1;  // fp32 rows in shared memory: columns on distinct banks
 
 template <int NP, int DKP>
 constexpr int prep_smem() {
   return 2 * NP * kChunk * DKP * 2 + 2 * kChunk * kPad * 4 + kVecCount * kChunk * 4 + 128;
+}
+
+// The chunk's rows of x as parts in a tile: 16-byte units of 8 values.
+template <typename T, int NP, int DKP>
+__device__ __forceinline__ void split_tile(uint32_t dst, const T* x, int64_t stride, int rows,
+                                           int units, int tid) {
+  constexpr int ROWB = DKP * 2, U = DKP / 8, N = kChunk * U / kPrepThreads, V = Elem<T>::kVec;
+  if constexpr (NP == 1) {
+    load_tile<kChunk, ROWB, kPrepThreads>(dst, x, stride * 2, rows, units, tid);
+  } else {
+    uint4 raw[N][8 / V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (tid + i * kPrepThreads) / U, u = (tid + i * kPrepThreads) % U;
+#pragma unroll
+      for (int j = 0; j < 8 / V; ++j)
+        raw[i][j] = r < rows && u < units
+                        ? *reinterpret_cast<const uint4*>(x + r * stride + u * 8 + j * V)
+                        : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = (tid + i * kPrepThreads) / U, u = (tid + i * kPrepThreads) % U;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8 / V; ++j) {
+        Vec16<T> w;
+        w.raw = raw[i][j];
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[j * V + c] = Elem<T>::load(w.e[c]);
+      }
+      uint32_t w[4][NP];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) split_pair<NP>(v[2 * c], v[2 * c + 1], w[c]);
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+        sts128(tile_at<ROWB>(dst + q * kChunk * ROWB, r, u),
+               make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]));
+    }
+  }
 }
 
 template <typename T, int NP, int LV, int DKP>
@@ -106,13 +125,8 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const PrepPara
   pdl_launch_dependents();
   const int64_t tok_stride = (int64_t)p.key_heads * p.dk;
   const int64_t first = (b * p.L + t0) * tok_stride + (int64_t)hk * p.dk;
-#pragma unroll
-  for (int q = 0; q < NP; ++q) {
-    load_tile<kChunk, ROWB, kPrepThreads>(s_k + q * TILE, p.k + q * p.part_stride + first,
-                                          tok_stride * 2, rows, p.dk / 8, tid);
-    load_tile<kChunk, ROWB, kPrepThreads>(s_q + q * TILE, p.q + q * p.part_stride + first,
-                                          tok_stride * 2, rows, p.dk / 8, tid);
-  }
+  split_tile<T, NP, DKP>(s_k, static_cast<const T*>(p.k) + first, tok_stride, rows, p.dk / 8, tid);
+  split_tile<T, NP, DKP>(s_q, static_cast<const T*>(p.q) + first, tok_stride, rows, p.dk / 8, tid);
   cp_commit();
 
   // decay vectors: one warp, two tokens a lane; the running sum in 64 bits
@@ -152,7 +166,16 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const PrepPara
     }
   }
   cp_wait<0>();
+  fence_async();
   __syncthreads();
+  // the first of the heads that share them keeps the tiles
+  const bool keeper = tid == 0 && h % (p.heads / p.key_heads) == 0;
+  if (keeper) {
+    const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kChunk * DKP);
+    bulk_s2g(p.k_tiles + tile, s_k, NP * TILE);
+    bulk_s2g(p.q_tiles + tile, s_q, NP * TILE);
+    bulk_commit();
+  }
 
   // K K^T and Q K^T, 16 rows a warp; tiles above the diagonal are not needed
   const int g4 = lane >> 2, t4 = lane & 3;
@@ -219,7 +242,8 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const PrepPara
       split_pair<NS>(pv[0], pv[1], w);
 #pragma unroll
       for (int q = 0; q < NS; ++q)
-        *reinterpret_cast<uint32_t*>(p.p_mat + mat + q * (kChunk * kChunk) + i * kChunk + j0) = w[q];
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(p.p_mat + mat) +
+                                     tile_at<kChunk * 2>(q * kMatBytes, i, n) + 4 * t4) = w[q];
     }
   }
   __syncthreads();
@@ -287,16 +311,17 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const PrepPara
       split_pair<NS>(s_n[i * kPad + j0 + 2 * c], s_n[i * kPad + j0 + 2 * c + 1], w[c]);
 #pragma unroll
     for (int q = 0; q < NS; ++q)
-      *reinterpret_cast<uint4*>(p.n_mat + mat + q * (kChunk * kChunk) + i * kChunk + j0) =
+      *reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.n_mat + mat) +
+                                tile_at<kChunk * 2>(q * kMatBytes, i, j0 / 8)) =
           make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
   }
+  if (keeper) bulk_wait_all();
 }
 
 // ------------------------------------------------------------------ along the chunks
 struct ScanParams {
-  const __nv_bfloat16* q;
-  const __nv_bfloat16* k;
-  int64_t part_stride;
+  const __nv_bfloat16* q_tiles;
+  const __nv_bfloat16* k_tiles;
   const void* v;
   const __nv_bfloat16* n_mat;
   const __nv_bfloat16* p_mat;
@@ -304,8 +329,8 @@ struct ScanParams {
   const float* initial;
   float* final_state;
   void* out;                  // KEEP false
-  __nv_bfloat16* e_parts;     // KEEP true
-  __nv_bfloat16* s_parts;
+  __nv_bfloat16* e_parts;     // KEEP true: strips [head][chunk][dv / 16][NS], as in shared memory
+  __nv_bfloat16* s_parts;     //            [head][chunk][NS][dv padded to 16][DKP], too
   int64_t L, chunks;
   int key_heads, heads, dk, dv, slices;
   float scale;
@@ -316,30 +341,41 @@ struct ScanParams {
 template <typename T, int NP, int LV, int DKP, int NW, bool KEEP>
 struct ScanCfg {
   static constexpr int NS = LV + 1;
+  // parts of S0 and E that leave the chain warps: outputs of 16 bits need two
+  static constexpr int NO = KEEP ? NS : sizeof(T) == 4 ? 3 : 2;
+  static constexpr int kThreads = (KEEP ? NW + 1 : 2 * NW) * 32;
   static constexpr int kTileK = kChunk * DKP * 2;
-  static constexpr int kRowV = NW * 16 * (int)sizeof(T);
-  static constexpr int kTileV = kChunk * kRowV;
-  static constexpr int kMat = kChunk * kChunk * 2;
-  static constexpr int oQ = NP * kTileK;
-  static constexpr int oV = oQ + (KEEP ? 0 : NP * kTileK);
-  static constexpr int oN = oV + kTileV;
-  static constexpr int oP = oN + NS * kMat;
-  static constexpr int oVec = oP + (KEEP ? 0 : NS * kMat);
-  static constexpr int kStage = oVec + 3 * kChunk * 4 + 256;  // enter, leave, beta
-  static constexpr int kStages = 2 * kStage + 128 <= 227 * 1024 ? 2 : 1;
-  static constexpr int kSmem = kStages * kStage + 128;
-  static_assert(kStage % 128 == 0 && kSmem <= 227 * 1024);
+  static constexpr int oN = NP * kTileK, oVec = oN + NS * kMatBytes;
+  static constexpr int kStageK = oVec + 1024;            // enter, leave, beta: 768 bytes
+  static constexpr int oP = NP * kTileK, oEnter = oP + NO * kMatBytes;
+  static constexpr int kStageQ = KEEP ? 0 : oEnter + 256;
+  static constexpr int kV = kChunk * 16 * (int)sizeof(T);
+  static constexpr int kXS = NO * 16 * DKP * 2, kXE = NO * kStrip;
+  static constexpr int kWarp = 2 * kV + kXS + kXE;       // a chain warp's own
+  static constexpr int kRoom = 227 * 1024 - 1536;        // barriers, alignment
+  static constexpr int kStK = NW * kWarp + 2 * kStageK + kStageQ <= kRoom ? 2 : 1;
+  static constexpr int kStQ = KEEP ? 1 : NW * kWarp + kStK * kStageK + 2 * kStageQ <= kRoom ? 2 : 1;
+  static constexpr int oQ = kStK * kStageK, oWarp = oQ + kStQ * kStageQ;
+  static constexpr int kSmem = oWarp + NW * kWarp + 128;
+  static_assert(kStageK % 128 == 0 && kStageQ % 128 == 0 && kSmem + 1024 <= 227 * 1024);
 };
 
 template <typename T, int NP, int LV, int DKP, int NW, bool KEEP>
-__global__ void __launch_bounds__(NW * 32) delta_scan_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1)
+    delta_scan_kernel(const ScanParams p) {
   using Cfg = ScanCfg<T, NP, LV, DKP, NW, KEEP>;
-  constexpr int NS = Cfg::NS, NTH = NW * 32, ROWB = DKP * 2, NT = DKP / 8;
+  constexpr int NS = Cfg::NS, NO = Cfg::NO, LO = NO - 1, ROWB = DKP * 2, NT = DKP / 8;
   constexpr int MROW = kChunk * 2;  // bytes of a row of N and P
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
   const uint32_t sm0 = smem_addr(dsm);
+  // full: the copies of a stage have landed / the chain warp has written;
+  // free: whoever reads a stage or a buffer is done with it
+  __shared__ __align__(8) uint64_t full_k[2], free_k[2], full_q[2], free_q[2];
+  __shared__ __align__(8) uint64_t full_s[NW], free_s[NW], full_e[NW], free_e[NW];
+  __shared__ int s_bad[NW];
+  __shared__ int s_spoilt[NW][16];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, t4 = lane & 3;
@@ -347,269 +383,453 @@ __global__ void __launch_bounds__(NW * 32) delta_scan_kernel(const ScanParams p)
   const int slice = (int)(blockIdx.x - bh * p.slices);
   const int64_t b = bh / p.heads;
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
-  const int dv_cta = slice * NW * 16, dv0 = dv_cta + warp * 16;
-  const int nval = p.dv - dv0;  // values of this warp's 16 rows that exist (may be <= 0)
-  const int64_t kstride = (int64_t)p.key_heads * p.dk, vstride = (int64_t)p.heads * p.dv;
-  const int vunits = min(NW * 16, p.dv - dv_cta) * (int)sizeof(T) / 16;
-
-  auto load = [&](int64_t c, int s) {
-    const uint32_t st = sm0 + s * Cfg::kStage;
-    const int64_t t0 = c * kChunk;
-    const int rows = (int)min((int64_t)kChunk, p.L - t0);
-    const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      load_tile<kChunk, ROWB, NTH>(st + i * Cfg::kTileK, p.k + i * p.part_stride + kf, kstride * 2,
-                                   rows, p.dk / 8, tid);
-      if (!KEEP)
-        load_tile<kChunk, ROWB, NTH>(st + Cfg::oQ + i * Cfg::kTileK, p.q + i * p.part_stride + kf,
-                                     kstride * 2, rows, p.dk / 8, tid);
+  const int dv_cta = slice * NW * 16;
+  const int nact = min(NW, (p.dv - dv_cta + 15) / 16);  // chain warps with values
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full_k[i], 1);
+      mbar_init(&free_k[i], nact);
+      mbar_init(&full_q[i], 1);
+      mbar_init(&free_q[i], nact);
     }
-    load_tile<kChunk, Cfg::kRowV, NTH>(
-        st + Cfg::oV, static_cast<const T*>(p.v) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv_cta,
-        vstride * (int)sizeof(T), rows, vunits, tid);
-    const int64_t mat = (bh * p.chunks + c) * NS * (kChunk * kChunk);
-    load_tile<NS * kChunk, MROW, NTH>(st + Cfg::oN, p.n_mat + mat, MROW, NS * kChunk, 8, tid);
-    if (!KEEP) load_tile<NS * kChunk, MROW, NTH>(st + Cfg::oP, p.p_mat + mat, MROW, NS * kChunk, 8, tid);
-    const char* vec = reinterpret_cast<const char*>(p.vecs + (bh * p.chunks + c) * (kVecCount * kChunk));
-    for (int i = tid; i < 3 * kChunk * 4 / 16; i += NTH) cp16(st + Cfg::oVec + i * 16, vec + i * 16, true);
-    cp_commit();
-  };
-
+    for (int i = 0; i < NW; ++i) {
+      mbar_init(&full_s[i], 1);
+      mbar_init(&free_s[i], 1);
+      mbar_init(&full_e[i], 1);
+      mbar_init(&free_e[i], 1);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
 
-  float S[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
-    if (p.initial != nullptr) {
-      const int dk = n * 8 + 2 * t4;
-      const float* src = p.initial + (bh * p.dv + dv0 + g4) * p.dk + dk;
-      if (dk < p.dk) {
-        if (g4 < nval) {
-          const float2 v = *reinterpret_cast<const float2*>(src);
-          S[n][0] = v.x;
-          S[n][1] = v.y;
-        }
-        if (g4 + 8 < nval) {
-          const float2 v = *reinterpret_cast<const float2*>(src + 8 * p.dk);
-          S[n][2] = v.x;
-          S[n][3] = v.y;
-        }
-      }
+  const int64_t unit0 = bh * p.chunks;
+  // loads of a chunk's stages; `free` waits until the stage's last reader is done
+  const int64_t tile = (b * p.key_heads + hk) * p.chunks;
+  int64_t next_k = 0, next_q = 0;  // chunks issued (by the one lane that loads)
+  auto issue_k = [&]() {
+    const int64_t c = next_k;
+    const int s = (int)(c % Cfg::kStK);
+    if (c >= Cfg::kStK && !mbar_wait_bounded(&free_k[s], (uint32_t)((c / Cfg::kStK - 1) & 1)))
+      return false;
+    const uint32_t st = sm0 + s * Cfg::kStageK;
+    mbar_expect_tx(&full_k[s], Cfg::oVec + 3 * kChunk * 4);
+    bulk_in(st, p.k_tiles + (tile + c) * NP * (kChunk * DKP), NP * Cfg::kTileK, &full_k[s]);
+    bulk_in(st + Cfg::oN, p.n_mat + (unit0 + c) * NS * (kChunk * kChunk), NS * kMatBytes, &full_k[s]);
+    bulk_in(st + Cfg::oVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), 3 * kChunk * 4, &full_k[s]);
+    ++next_k;
+    return true;
+  };
+  auto issue_q = [&]() {
+    const int64_t c = next_q;
+    const int s = (int)(c % Cfg::kStQ);
+    if (c >= Cfg::kStQ && !mbar_wait_bounded(&free_q[s], (uint32_t)((c / Cfg::kStQ - 1) & 1)))
+      return false;
+    const uint32_t st = sm0 + Cfg::oQ + s * Cfg::kStageQ;
+    mbar_expect_tx(&full_q[s], Cfg::oEnter + kChunk * 4);
+    bulk_in(st, p.q_tiles + (tile + c) * NP * (kChunk * DKP), NP * Cfg::kTileK, &full_q[s]);
+    bulk_in(st + Cfg::oP, p.p_mat + (unit0 + c) * NS * (kChunk * kChunk), NO * kMatBytes, &full_q[s]);
+    bulk_in(st + Cfg::oEnter, p.vecs + (unit0 + c) * (kVecCount * kChunk), kChunk * 4, &full_q[s]);
+    ++next_q;
+    return true;
+  };
+  // After a wait that gave up: no copy may land after the CTA is gone.
+  auto drain = [&]() {
+    for (int64_t j = max((int64_t)0, next_k - Cfg::kStK); j < next_k; ++j)
+      mbar_wait_bounded(&full_k[j % Cfg::kStK], (uint32_t)((j / Cfg::kStK) & 1));
+    for (int64_t j = max((int64_t)0, next_q - Cfg::kStQ); j < next_q; ++j)
+      mbar_wait_bounded(&full_q[j % Cfg::kStQ], (uint32_t)((j / Cfg::kStQ) & 1));
+  };
+  if (KEEP && warp == NW) {
+    // ---------------------------------------------------------- loader
+    if (lane == 0) {
+      bool ok = true;
+      while (ok && next_k < p.chunks) ok = issue_k();
+      if (!ok) drain();
     }
-  }
-
-  if (Cfg::kStages == 2) load(0, 0);
-  for (int64_t c = 0; c < p.chunks; ++c) {
-    const int s = Cfg::kStages == 2 ? (int)(c & 1) : 0;
-    if (Cfg::kStages == 1) {
-      load(c, 0);
-      cp_wait<0>();
-    } else if (c + 1 < p.chunks) {
-      load(c + 1, s ^ 1);
-      cp_wait<1>();
-    } else {
-      cp_wait<0>();
-    }
-    __syncthreads();
+  } else if (warp < NW) {
+    // ---------------------------------------------------------- chain
+    const int dv0 = dv_cta + warp * 16;
+    const int nval = p.dv - dv0;  // values of this warp's 16 rows that exist (may be <= 0)
     if (nval > 0) {
-      const uint32_t st = sm0 + s * Cfg::kStage;
-      const float* vec = reinterpret_cast<const float*>(dsm + s * Cfg::kStage + Cfg::oVec);
-      const float* enter = vec + kVecEnter * kChunk;
-      const float* leave = vec + kVecLeave * kChunk;
-      const float* beta = vec + kVecBeta * kChunk;
-      const float total = enter[kChunk - 1];
-      const int64_t t0 = c * kChunk;
+      const int64_t vstride = (int64_t)p.heads * p.dv;
+      const uint32_t own = sm0 + Cfg::oWarp + warp * Cfg::kWarp;
+      const uint32_t x_s = own + 2 * Cfg::kV, x_e = x_s + Cfg::kXS;
+      auto load_v = [&](int64_t c) {
+        const int64_t t0 = c * kChunk;
+        load_strip<T>(own + (int)(c & 1) * Cfg::kV,
+                      static_cast<const T*>(p.v) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0,
+                      vstride * (int)sizeof(T), (int)min((int64_t)kChunk, p.L - t0),
+                      min(16, nval) * (int)sizeof(T) / 16, lane);
+        cp_commit();
+      };
+      load_v(0);
 
-      if (KEEP) {
-        __nv_bfloat16* sp = p.s_parts + (bh * p.chunks + c) * NS * p.dv * DKP;
+      float S[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            uint32_t w[NS];
-            split_pair<NS>(S[n][2 * r], S[n][2 * r + 1], w);
-            if (g4 + 8 * r < nval)
-#pragma unroll
-              for (int q = 0; q < NS; ++q)
-                *reinterpret_cast<uint32_t*>(sp + ((int64_t)q * p.dv + dv0 + g4 + 8 * r) * DKP +
-                                             n * 8 + 2 * t4) = w[q];
+        for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
+        if (p.initial != nullptr) {
+          const int dk = n * 8 + 2 * t4;
+          const float* src = p.initial + (bh * p.dv + dv0 + g4) * p.dk + dk;
+          if (dk < p.dk) {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            S[n][0] = v.x;
+            S[n][1] = v.y;
+            if (nval > 8) {
+              const float2 w = *reinterpret_cast<const float2*>(src + 8 * p.dk);
+              S[n][2] = w.x;
+              S[n][3] = w.y;
+            }
           }
+        }
       }
 
-      // X = (K S0^T)^T, O = (Q S0^T)^T: 16 values x 64 tokens
-      float X[8][4], O[8][4];
+      bool ok = true;
+      for (int64_t c = 0; c < p.chunks; ++c) {
+        const int sk = (int)(c % Cfg::kStK);
+        const uint32_t st = sm0 + sk * Cfg::kStageK;
+        const float* vec = reinterpret_cast<const float*>(dsm + sk * Cfg::kStageK + Cfg::oVec);
+        const float* enter = vec + kVecEnter * kChunk;
+        const float* leave = vec + kVecLeave * kChunk;
+        const float* beta = vec + kVecBeta * kChunk;
+        if (c + 1 < p.chunks) {
+          load_v(c + 1);
+          cp_wait<1>();
+        } else {
+          cp_wait<0>();
+        }
+        ok = mbar_wait_bounded(&full_k[sk], (uint32_t)((c / Cfg::kStK) & 1));
+        if (!KEEP && c > 0) ok = ok && mbar_wait_bounded(&free_s[warp], (uint32_t)((c - 1) & 1));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (KEEP && c > 0 && lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+        const float total = enter[kChunk - 1];
+
+        // X = (K S0^T)^T: 16 values x 64 tokens.  S0's parts go to shared memory.
+        float X[8][4];
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) X[n][e] = O[n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) X[n][e] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < DKP / 16; ++kk) {
-        uint32_t a[NS][4];
-        split_frag<NS>(S[2 * kk], S[2 * kk + 1], a);
+        for (int kk = 0; kk < DKP / 16; ++kk) {
+          uint32_t a[NS][4];
+          split_frag<NS>(S[2 * kk], S[2 * kk + 1], a);
 #pragma unroll
-        for (int n2 = 0; n2 < 4; ++n2) {
-          Step<LV == 2, 4> s;
+          for (int q = 0; q < NO; ++q)
+            stsm4(at_a<ROWB>(x_s + q * 16 * ROWB, lane, 0, kk), a[q]);
 #pragma unroll
-          for (int i = NP - 1; i >= 0; --i) {
-            uint32_t kb[4], qb[4];
-            ldsm4(kb, at_b<ROWB>(st + i * Cfg::kTileK, lane, n2 * 16, kk));
-            if (!KEEP) ldsm4(qb, at_b<ROWB>(st + Cfg::oQ + i * Cfg::kTileK, lane, n2 * 16, kk));
+          for (int n2 = 0; n2 < 4; ++n2) {
+            Step<LV == 2, 2> s;
 #pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, X[2 * n2], a[j], kb[0], kb[1]);
-              s.mma(1, X[2 * n2 + 1], a[j], kb[2], kb[3]);
-              if (!KEEP) {
-                s.mma(2, O[2 * n2], a[j], qb[0], qb[1]);
-                s.mma(3, O[2 * n2 + 1], a[j], qb[2], qb[3]);
+            for (int i = NP - 1; i >= 0; --i) {
+              uint32_t kb[4];
+              ldsm4(kb, at_b<ROWB>(st + i * Cfg::kTileK, lane, n2 * 16, kk));
+#pragma unroll
+              for (int j = LV - i; j >= 0; --j) {
+                s.mma(0, X[2 * n2], a[j], kb[0], kb[1]);
+                s.mma(1, X[2 * n2 + 1], a[j], kb[2], kb[3]);
               }
             }
-          }
-          s.add(0, X[2 * n2]);
-          s.add(1, X[2 * n2 + 1]);
-          if (!KEEP) {
-            s.add(2, O[2 * n2]);
-            s.add(3, O[2 * n2 + 1]);
+            s.add(0, X[2 * n2]);
+            s.add(1, X[2 * n2 + 1]);
           }
         }
-      }
+        if (KEEP) {
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            const int64_t dvp = (p.dv + 15) / 16 * 16;
+            __nv_bfloat16* sp = p.s_parts + ((unit0 + c) * NS * dvp + dv0) * DKP;
+#pragma unroll
+            for (int q = 0; q < NS; ++q)
+              bulk_s2g(sp + q * dvp * DKP, x_s + q * 16 * ROWB, 16 * ROWB);
+            bulk_commit();
+          }
+        } else {
+          warp_arrive(&full_s[warp], lane);
+        }
 
-      // R = V - exp(G) X, in place; O *= scale exp(G)
+        // R = V - exp(G) X, in place
+        const uint32_t vst = own + (int)(c & 1) * Cfg::kV;
 #pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        uint32_t vb[4];
-        if constexpr (sizeof(T) == 2) {
-          const int m = lane >> 3, r = lane & 7;
-          ldsm4_t(vb, tile_at<Cfg::kRowV>(st + Cfg::oV, n2 * 16 + (m >> 1) * 8 + r,
-                                          warp * 2 + (m & 1)));
-        }
+        for (int n2 = 0; n2 < 4; ++n2) {
+          uint32_t vb[4];
+          if constexpr (sizeof(T) == 2) ldsm4_t(vb, strip_at_t(vst, lane, n2));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int n = 2 * n2 + half, tok = n * 8 + 2 * t4;
-          const float2 ge = *reinterpret_cast<const float2*>(enter + tok);
-          float v[4];
-          if constexpr (sizeof(T) == 2) {
-            const float2 x = unpack2<T>(vb[2 * half]), y = unpack2<T>(vb[2 * half + 1]);
-            v[0] = x.x;
-            v[1] = x.y;
-            v[2] = y.x;
-            v[3] = y.y;
-          } else {
+          for (int half = 0; half < 2; ++half) {
+            const int n = 2 * n2 + half, tok = n * 8 + 2 * t4;
+            const float2 ge = *reinterpret_cast<const float2*>(enter + tok);
+            float v[4];
+            if constexpr (sizeof(T) == 2) {
+              const float2 x = unpack2<T>(vb[2 * half]), y = unpack2<T>(vb[2 * half + 1]);
+              v[0] = x.x;
+              v[1] = x.y;
+              v[2] = y.x;
+              v[3] = y.y;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int row = tok + (e & 1), col = warp * 16 + g4 + (e >> 1) * 8;
-              const uint32_t at = tile_at<Cfg::kRowV>(st + Cfg::oV, row, col / 4) + (col % 4) * 4;
-              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[e]) : "r"(at) : "memory");
+              for (int e = 0; e < 4; ++e) {
+                const int col = g4 + (e >> 1) * 8;
+                const uint32_t at = strip32_at(vst, tok + (e & 1), col / 4) + (col % 4) * 4;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[e]) : "r"(at) : "memory");
+              }
             }
-          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float w = (e & 1) ? ge.y : ge.x;
-            X[n][e] = fmaf(-w, X[n][e], v[e]);
-            if (!KEEP) O[n][e] *= w * p.scale;
+            for (int e = 0; e < 4; ++e) X[n][e] = fmaf(-((e & 1) ? ge.y : ge.x), X[n][e], v[e]);
           }
         }
-      }
 
-      // An infinity or a NaN in R (of v, k, or the state) spoils its row of
-      // values from that token on, but the zeros above the diagonals of N
-      // and P would carry it to earlier tokens: it is taken out here and
-      // put back into E, O and the state below.
-      int spoilt[2] = {kChunk, kChunk};  // first such token of the thread's two rows
-      float probe = 0.f;
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) probe = fmaf(X[n][e], 0.f, probe);
-      const bool bad = __any_sync(0xffffffffu, probe != 0.f);
-      if (bad) {
+        // An infinity or a NaN in R (of v, k, or the state) spoils its row of
+        // values from that token on, but the zeros above the diagonals of N
+        // and P would carry it to earlier tokens: it is taken out here and
+        // put back into E, O and the state afterwards.
+        int spoilt[2] = {kChunk, kChunk};  // first such token of the thread's two rows
+        float probe = 0.f;
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(fabsf(X[n][e]) <= 3.4e38f))
-              spoilt[e >> 1] = min(spoilt[e >> 1], n * 8 + 2 * t4 + (e & 1));
+          for (int e = 0; e < 4; ++e) probe = fmaf(X[n][e], 0.f, probe);
+        const bool bad = __any_sync(0xffffffffu, probe != 0.f);
+        if (bad) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          spoilt[r] = min(spoilt[r], __shfl_xor_sync(0xffffffffu, spoilt[r], 1));
-          spoilt[r] = min(spoilt[r], __shfl_xor_sync(0xffffffffu, spoilt[r], 2));
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(fabsf(X[n][e]) <= 3.4e38f))
+                spoilt[e >> 1] = min(spoilt[e >> 1], n * 8 + 2 * t4 + (e & 1));
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            spoilt[r] = min(spoilt[r], __shfl_xor_sync(0xffffffffu, spoilt[r], 1));
+            spoilt[r] = min(spoilt[r], __shfl_xor_sync(0xffffffffu, spoilt[r], 2));
+          }
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1]) X[n][e] = 0.f;
         }
+
+        // E = N R
+        float E[8][4];
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1]) X[n][e] = 0.f;
-      }
-      auto spoil = [&](float (&y)[8][4]) {
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1]) y[n][e] = __int_as_float(0x7fc00000);
-      };
-
-      // E = N R
-      float E[8][4];
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) E[n][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t a[NS][4];
-        split_frag<NS>(X[2 * kk], X[2 * kk + 1], a);
-#pragma unroll
-        for (int n2 = kk; n2 < 4; ++n2) {
-          Step<LV == 2, 2> s;
-#pragma unroll
-          for (int i = LV; i >= 0; --i) {
-            uint32_t nb[4];
-            ldsm4(nb, at_b<MROW>(st + Cfg::oN + i * Cfg::kMat, lane, n2 * 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, E[2 * n2], a[j], nb[0], nb[1]);
-              s.mma(1, E[2 * n2 + 1], a[j], nb[2], nb[3]);
-            }
-          }
-          s.add(0, E[2 * n2]);
-          s.add(1, E[2 * n2 + 1]);
-        }
-      }
-
-      if (KEEP) {
-        if (bad) spoil(E);
-        __nv_bfloat16* ep = p.e_parts + (bh * p.chunks + c) * NS * kChunk * p.dv + dv0;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          uint32_t lo[NS], hi[NS];
-          split_pair<NS>(E[n][0], E[n][1], lo);
-          split_pair<NS>(E[n][2], E[n][3], hi);
-#pragma unroll
-          for (int q = 0; q < NS; ++q) {
-            const uint32_t x = movmatrix_t(lo[q]), y = movmatrix_t(hi[q]);
-            __nv_bfloat16* o = ep + ((int64_t)q * kChunk + n * 8 + g4) * p.dv + 2 * t4;
-            *reinterpret_cast<uint32_t*>(o) = x;
-            if (nval > 8) *reinterpret_cast<uint32_t*>(o + 8) = y;
-          }
-        }
-      } else {
-        // O += P E
+          for (int e = 0; e < 4; ++e) E[n][e] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t a[NS][4];
-          split_frag<NS>(E[2 * kk], E[2 * kk + 1], a);
+          split_frag<NS>(X[2 * kk], X[2 * kk + 1], a);
 #pragma unroll
           for (int n2 = kk; n2 < 4; ++n2) {
             Step<LV == 2, 2> s;
 #pragma unroll
             for (int i = LV; i >= 0; --i) {
-              uint32_t pb[4];
-              ldsm4(pb, at_b<MROW>(st + Cfg::oP + i * Cfg::kMat, lane, n2 * 16, kk));
+              uint32_t nb[4];
+              ldsm4(nb, at_b<MROW>(st + Cfg::oN + i * kMatBytes, lane, n2 * 16, kk));
 #pragma unroll
               for (int j = LV - i; j >= 0; --j) {
+                s.mma(0, E[2 * n2], a[j], nb[0], nb[1]);
+                s.mma(1, E[2 * n2 + 1], a[j], nb[2], nb[3]);
+              }
+            }
+            s.add(0, E[2 * n2]);
+            s.add(1, E[2 * n2 + 1]);
+          }
+        }
+
+        // E's parts go to shared memory, and on: to the output warp, or kept
+        if (KEEP) {
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+          if (bad) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1]) E[n][e] = __int_as_float(0x7fc00000);
+          }
+        } else {
+          if (c > 0) ok = mbar_wait_bounded(&free_e[warp], (uint32_t)((c - 1) & 1));
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) s_bad[warp] = bad;
+          if (bad && t4 == 0) {
+            s_spoilt[warp][g4] = spoilt[0];
+            s_spoilt[warp][g4 + 8] = spoilt[1];
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          uint32_t a[NO][4];
+          split_frag<NO>(E[2 * kk], E[2 * kk + 1], a);
+#pragma unroll
+          for (int q = 0; q < NO; ++q) stsm4_t(strip_at_t(x_e + q * kStrip, lane, kk), a[q]);
+        }
+        if (KEEP) {
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            bulk_s2g(p.e_parts + ((unit0 + c) * ((p.dv + 15) / 16) + dv0 / 16) * NS * (kStrip / 2),
+                     x_e, NS * kStrip);
+            bulk_commit();
+          }
+        } else {
+          warp_arrive(&full_e[warp], lane);
+        }
+
+        // S = exp(G_C) S + (beta exp(G_C - G) E)^T K.  The chunk's sum starts
+        // at zero and joins the state in one rounded multiply-add.
+        uint32_t u[4][NS][4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int tok = (2 * kk + half) * 8 + 2 * t4;
+            const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
+            const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
+            const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
+            E[2 * kk + half][0] *= w0;
+            E[2 * kk + half][1] *= w1;
+            E[2 * kk + half][2] *= w0;
+            E[2 * kk + half][3] *= w1;
+          }
+          split_frag<NS>(E[2 * kk], E[2 * kk + 1], u[kk]);
+        }
+#pragma unroll
+        for (int n4 = 0; n4 < NT / 4; ++n4) {
+          float d[4][4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            Step<LV == 2, 4> s;
+#pragma unroll
+            for (int i = NP - 1; i >= 0; --i) {
+              uint32_t b0[4], b1[4];
+              ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
+              ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
+#pragma unroll
+              for (int j = LV - i; j >= 0; --j) {
+                s.mma(0, d[0], u[kk][j], b0[0], b0[1]);
+                s.mma(1, d[1], u[kk][j], b0[2], b0[3]);
+                s.mma(2, d[2], u[kk][j], b1[0], b1[1]);
+                s.mma(3, d[3], u[kk][j], b1[2], b1[3]);
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) s.add(n, d[n]);
+          }
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[n4 * 4 + n][e] = fmaf(total, S[n4 * 4 + n][e], d[n][e]);
+        }
+        if (bad)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (spoilt[e >> 1] < kChunk) S[n][e] = __int_as_float(0x7fc00000);
+        warp_arrive(&free_k[sk], lane);
+      }
+
+      if (KEEP) {
+        if (lane == 0) bulk_wait_all();
+      } else if (ok && p.final_state != nullptr) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int dk = n * 8 + 2 * t4;
+          float* dst = p.final_state + (bh * p.dv + dv0 + g4) * p.dk + dk;
+          if (dk < p.dk) {
+            *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
+            if (nval > 8) *reinterpret_cast<float2*>(dst + 8 * p.dk) = make_float2(S[n][2], S[n][3]);
+          }
+        }
+      }
+    }
+  } else if (!KEEP) {
+    // ---------------------------------------------------------- output
+    const int w = warp - NW;
+    const int dv0 = dv_cta + w * 16;
+    const int nval = p.dv - dv0;
+    if (nval > 0) {
+      const int64_t vstride = (int64_t)p.heads * p.dv;
+      const uint32_t x_s = sm0 + Cfg::oWarp + w * Cfg::kWarp + 2 * Cfg::kV, x_e = x_s + Cfg::kXS;
+      const bool loads = w == 0 && lane == 0;
+      if (loads) {
+        while (next_k < min((int64_t)Cfg::kStK, p.chunks)) issue_k();
+        while (next_q < min((int64_t)Cfg::kStQ, p.chunks)) issue_q();
+      }
+      __syncwarp();
+      bool ok = true;
+      for (int64_t c = 0; c < p.chunks; ++c) {
+        const int sq = (int)(c % Cfg::kStQ);
+        const uint32_t st = sm0 + Cfg::oQ + sq * Cfg::kStageQ;
+        const float* enter = reinterpret_cast<const float*>(dsm + Cfg::oQ + sq * Cfg::kStageQ + Cfg::oEnter);
+        ok = mbar_wait_bounded(&full_q[sq], (uint32_t)((c / Cfg::kStQ) & 1));
+        ok = ok && mbar_wait_bounded(&full_s[w], (uint32_t)(c & 1));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float O[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[n][e] = 0.f;
+#pragma unroll 2
+        for (int kk = 0; kk < DKP / 16; ++kk) {
+          uint32_t a[NO][4];
+#pragma unroll
+          for (int q = 0; q < NO; ++q) ldsm4(a[q], at_a<ROWB>(x_s + q * 16 * ROWB, lane, 0, kk));
+#pragma unroll
+          for (int n2 = 0; n2 < 4; ++n2) {
+            Step<LO == 2, 2> s;
+#pragma unroll
+            for (int i = NP - 1; i >= 0; --i) {
+              if (i > LO) continue;
+              uint32_t qb[4];
+              ldsm4(qb, at_b<ROWB>(st + i * Cfg::kTileK, lane, n2 * 16, kk));
+#pragma unroll
+              for (int j = LO - i; j >= 0; --j) {
+                s.mma(0, O[2 * n2], a[j], qb[0], qb[1]);
+                s.mma(1, O[2 * n2 + 1], a[j], qb[2], qb[3]);
+              }
+            }
+            s.add(0, O[2 * n2]);
+            s.add(1, O[2 * n2 + 1]);
+          }
+        }
+        warp_arrive(&free_s[w], lane);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const float2 ge = *reinterpret_cast<const float2*>(enter + n * 8 + 2 * t4);
+          O[n][0] *= ge.x * p.scale;
+          O[n][1] *= ge.y * p.scale;
+          O[n][2] *= ge.x * p.scale;
+          O[n][3] *= ge.y * p.scale;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_e[w], (uint32_t)(c & 1)));
+        if (!ok) break;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          uint32_t a[NO][4];
+#pragma unroll
+          for (int q = 0; q < NO; ++q) ldsm4_t(a[q], strip_at_t(x_e + q * kStrip, lane, kk));
+#pragma unroll
+          for (int n2 = kk; n2 < 4; ++n2) {
+            Step<LO == 2, 2> s;
+#pragma unroll
+            for (int i = LO; i >= 0; --i) {
+              uint32_t pb[4];
+              ldsm4(pb, at_b<MROW>(st + Cfg::oP + i * kMatBytes, lane, n2 * 16, kk));
+#pragma unroll
+              for (int j = LO - i; j >= 0; --j) {
                 s.mma(0, O[2 * n2], a[j], pb[0], pb[1]);
                 s.mma(1, O[2 * n2 + 1], a[j], pb[2], pb[3]);
               }
@@ -618,85 +838,52 @@ __global__ void __launch_bounds__(NW * 32) delta_scan_kernel(const ScanParams p)
             s.add(1, O[2 * n2 + 1]);
           }
         }
+        warp_arrive(&free_q[sq], lane);
+        if (s_bad[w]) {
+          const int first[2] = {s_spoilt[w][g4], s_spoilt[w][g4 + 8]};
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n * 8 + 2 * t4 + (e & 1) >= first[e >> 1]) O[n][e] = __int_as_float(0x7fc00000);
+        }
+        const int64_t t0 = c * kChunk;
         T* out = static_cast<T*>(p.out) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0;
         const int rows = (int)min((int64_t)kChunk, p.L - t0);
-        if (bad) spoil(O);
+        if constexpr (sizeof(T) == 2) {
+          // through E's strip, transposed, for stores of 16 bytes
+          __syncwarp();
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-          store_t<T>(out + (int64_t)n * 8 * vstride, vstride, O[n], lane, rows - n * 8, nval);
-      }
-
-      // S = exp(G_C) S + (beta exp(G_C - G) E)^T K.  The chunk's sum starts
-      // at zero and joins the state in one rounded multiply-add.
-      uint32_t u[4][NS][4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int tok = (2 * kk + half) * 8 + 2 * t4;
-          const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
-          const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
-          const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
-          E[2 * kk + half][0] *= w0;
-          E[2 * kk + half][1] *= w1;
-          E[2 * kk + half][2] *= w0;
-          E[2 * kk + half][3] *= w1;
-        }
-        split_frag<NS>(E[2 * kk], E[2 * kk + 1], u[kk]);
-      }
-#pragma unroll
-      for (int n4 = 0; n4 < NT / 4; ++n4) {
-        float d[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          Step<LV == 2, 4> s;
-#pragma unroll
-          for (int i = NP - 1; i >= 0; --i) {
-            uint32_t b0[4], b1[4];
-            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
-            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, d[0], u[kk][j], b0[0], b0[1]);
-              s.mma(1, d[1], u[kk][j], b0[2], b0[3]);
-              s.mma(2, d[2], u[kk][j], b1[0], b1[1]);
-              s.mma(3, d[3], u[kk][j], b1[2], b1[3]);
-            }
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t a[4] = {pack2<T>(O[2 * kk][0], O[2 * kk][1]), pack2<T>(O[2 * kk][2], O[2 * kk][3]),
+                                   pack2<T>(O[2 * kk + 1][0], O[2 * kk + 1][1]),
+                                   pack2<T>(O[2 * kk + 1][2], O[2 * kk + 1][3])};
+            stsm4_t(strip_at_t(x_e, lane, kk), a);
           }
+          __syncwarp();
 #pragma unroll
-          for (int n = 0; n < 4; ++n) s.add(n, d[n]);
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 16 + (lane >> 1), un = lane & 1;
+            if (r < rows && un * 8 < nval)
+              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_e, r, un));
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            store_t<T>(out + (int64_t)n * 8 * vstride, vstride, O[n], lane, rows - n * 8, nval);
         }
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[n4 * 4 + n][e] = fmaf(total, S[n4 * 4 + n][e], d[n][e]);
+        warp_arrive(&free_e[w], lane);
+        if (loads) {
+          if (next_k < p.chunks) ok = issue_k();
+          if (ok && next_q < p.chunks) ok = issue_q();
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
-      if (bad)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (spoilt[e >> 1] < kChunk) S[n][e] = __int_as_float(0x7fc00000);
-    }
-    __syncthreads();
-  }
-
-  if (p.final_state != nullptr && nval > 0) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int dk = n * 8 + 2 * t4;
-      float* dst = p.final_state + (bh * p.dv + dv0 + g4) * p.dk + dk;
-      if (dk < p.dk) {
-        if (g4 < nval) *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
-        if (g4 + 8 < nval)
-          *reinterpret_cast<float2*>(dst + 8 * p.dk) = make_float2(S[n][2], S[n][3]);
-      }
+      if (loads && !ok) drain();
     }
   }
+  __syncthreads();  // shared memory outlives every copy into it
 }
 
 // ------------------------------------------------------------------ host side
@@ -712,7 +899,7 @@ cudaError_t scan_nw(const DeltaArgs& a, ScanParams& p, int64_t bh) {
   const cudaError_t e = configure(kern, Cfg::kSmem);
   if (e != cudaSuccess) return e;
   p.slices = (int)((a.dv + NW * 16 - 1) / (NW * 16));
-  return launch_pdl(kern, (unsigned)(bh * p.slices), NW * 32, Cfg::kSmem, a.stream, p);
+  return launch_pdl(kern, (unsigned)(bh * p.slices), Cfg::kThreads, Cfg::kSmem, a.stream, p);
 }
 
 }  // namespace
@@ -724,39 +911,19 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
                            bool keep) {
   constexpr int NP = kParts<T>;
   char* ws = static_cast<char*>(a.workspace);
-  const int64_t nk = nb * a.seqlen * a.key_heads * a.dk, nv = nb * a.seqlen * a.heads * a.dv;
+  auto bf = [&](int64_t off) { return reinterpret_cast<__nv_bfloat16*>(ws + off); };
   const int64_t k0 = b0 * a.seqlen * a.key_heads * a.dk, v0 = b0 * a.seqlen * a.heads * a.dv;
   const int64_t g0 = b0 * a.seqlen * a.heads, s0 = b0 * a.heads * a.dv * a.dk;
-  const T* q = static_cast<const T*>(a.q) + k0;
-  const T* k = static_cast<const T*>(a.k) + k0;
+  const int64_t bh = nb * a.heads;
   PrepParams pp{};
-  if constexpr (NP > 1) {
-    SplitParams sp{};
-    sp.src[0] = q;
-    sp.src[1] = k;
-    sp.dst[0] = reinterpret_cast<__nv_bfloat16*>(ws + pl.q_parts);
-    sp.dst[1] = reinterpret_cast<__nv_bfloat16*>(ws + pl.k_parts);
-    sp.n[0] = sp.n[1] = nk;
-    if (keep) {
-      sp.src[2] = static_cast<const T*>(a.grad_out) + v0;
-      sp.dst[2] = reinterpret_cast<__nv_bfloat16*>(ws + pl.do_parts);
-      sp.n[2] = nv;
-    }
-    const int64_t per = (std::max(nk, keep ? nv : 0) + 2047) / 2048;
-    const unsigned grid = 3 * (unsigned)std::min<int64_t>(per, 4 * a.num_sms);
-    const cudaError_t e = launch_pdl(delta_split_kernel<T>, grid, 256, 0, a.stream, sp);
-    if (e != cudaSuccess) return e;
-    pp.q = sp.dst[0];
-    pp.k = sp.dst[1];
-    pp.part_stride = nk;
-  } else {
-    pp.q = reinterpret_cast<const __nv_bfloat16*>(q);
-    pp.k = reinterpret_cast<const __nv_bfloat16*>(k);
-  }
+  pp.q = static_cast<const T*>(a.q) + k0;
+  pp.k = static_cast<const T*>(a.k) + k0;
+  pp.q_tiles = bf(pl.q_tiles);
+  pp.k_tiles = bf(pl.k_tiles);
   pp.log_decay = static_cast<const T*>(a.log_decay) + g0;
   pp.beta = static_cast<const T*>(a.beta) + g0;
-  pp.n_mat = reinterpret_cast<__nv_bfloat16*>(ws + pl.n_mat);
-  pp.p_mat = reinterpret_cast<__nv_bfloat16*>(ws + pl.p_mat);
+  pp.n_mat = bf(pl.n_mat);
+  pp.p_mat = bf(pl.p_mat);
   pp.vecs = reinterpret_cast<float*>(ws + pl.vecs);
   pp.L = a.seqlen;
   pp.chunks = pl.chunks;
@@ -764,7 +931,6 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   pp.heads = (int)a.heads;
   pp.dk = (int)a.dk;
   pp.scale = a.scale;
-  const int64_t bh = nb * a.heads;
   auto prep = delta_prep_kernel<T, NP, LV, DKP>;
   cudaError_t e = configure(prep, prep_smem<NP, DKP>());
   if (e != cudaSuccess) return e;
@@ -772,9 +938,8 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   if (e != cudaSuccess) return e;
 
   ScanParams p{};
-  p.q = pp.q;
-  p.k = pp.k;
-  p.part_stride = pp.part_stride;
+  p.q_tiles = pp.q_tiles;
+  p.k_tiles = pp.k_tiles;
   p.v = static_cast<const T*>(a.v) + v0;
   p.n_mat = pp.n_mat;
   p.p_mat = pp.p_mat;
@@ -782,8 +947,8 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   p.initial = a.initial ? a.initial + s0 : nullptr;
   p.final_state = !keep && a.final_state ? a.final_state + s0 : nullptr;
   p.out = keep ? nullptr : static_cast<T*>(a.out) + v0;
-  p.e_parts = reinterpret_cast<__nv_bfloat16*>(ws + pl.e_parts);
-  p.s_parts = reinterpret_cast<__nv_bfloat16*>(ws + pl.s_parts);
+  p.e_parts = bf(pl.e_parts);
+  p.s_parts = bf(pl.s_parts);
   p.L = a.seqlen;
   p.chunks = pl.chunks;
   p.key_heads = (int)a.key_heads;
@@ -791,10 +956,16 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   p.dk = (int)a.dk;
   p.dv = (int)a.dv;
   p.scale = a.scale;
-  const bool narrow = bh * ((a.dv + 127) / 128) < a.num_sms || a.dv <= 64;
-  if (keep)
-    return narrow ? scan_nw<T, LV, DKP, 4, true>(a, p, bh) : scan_nw<T, LV, DKP, 8, true>(a, p, bh);
-  return narrow ? scan_nw<T, LV, DKP, 4, false>(a, p, bh) : scan_nw<T, LV, DKP, 8, false>(a, p, bh);
+  // Chain warps per CTA: 4, or 2 where that still leaves an SM to every CTA
+  // (and for fp32, whose tiles leave room for no more).
+  const bool two = sizeof(T) == 4 || bh * ((a.dv + 31) / 32) <= a.num_sms;
+  if constexpr (sizeof(T) == 4) {
+    return keep ? scan_nw<T, LV, DKP, 2, true>(a, p, bh) : scan_nw<T, LV, DKP, 2, false>(a, p, bh);
+  } else {
+    if (keep)
+      return two ? scan_nw<T, LV, DKP, 2, true>(a, p, bh) : scan_nw<T, LV, DKP, 4, true>(a, p, bh);
+    return two ? scan_nw<T, LV, DKP, 2, false>(a, p, bh) : scan_nw<T, LV, DKP, 4, false>(a, p, bh);
+  }
 }
 
 template cudaError_t delta_fwd_pass<__nv_bfloat16, 1, 64>(const DeltaArgs&, const DeltaPlan&, int64_t, int64_t, bool);
@@ -825,19 +996,20 @@ DeltaPlan delta_plan(int64_t batch, int64_t seqlen, int64_t key_heads, int64_t h
       return o;
     };
     const int64_t nb = pl.batch, c = nb * heads * pl.chunks, tok = nb * seqlen;
-    if (pl.np > 1) {
-      pl.q_parts = take(pl.np * tok * key_heads * dk * 2);
-      pl.k_parts = take(pl.np * tok * key_heads * dk * 2);
-    }
+    const int64_t tiles = nb * key_heads * pl.chunks * pl.np * kChunk * pl.dkp * 2;
+    pl.q_tiles = take(tiles);
+    pl.k_tiles = take(tiles);
     pl.n_mat = take(c * pl.ns * kChunk * kChunk * 2);
     pl.p_mat = take(c * pl.ns * kChunk * kChunk * 2);
     pl.vecs = take(c * kVecCount * kChunk * 4);
     if (backward) {
-      if (pl.np > 1) pl.do_parts = take(pl.np * tok * heads * dv * 2);
-      pl.e_parts = take(c * pl.ns * kChunk * dv * 2);
-      pl.dv_parts = take(c * pl.ns * kChunk * dv * 2);
-      pl.s_parts = take(c * pl.ns * dv * pl.dkp * 2);
-      pl.ds_parts = take(c * pl.ns * dv * pl.dkp * 2);
+      const int64_t strips = (dv + 15) / 16;
+      if (pl.np > 1) pl.grad_rows = take(pl.np * tok * heads * dv * 2);
+      pl.do_parts = take(c * pl.np * kStrip * strips);
+      pl.e_parts = take(c * pl.ns * kStrip * strips);
+      pl.dv_parts = take(c * pl.ns * kStrip * strips);
+      pl.s_parts = take(c * pl.ns * strips * 16 * pl.dkp * 2);
+      pl.ds_parts = take(c * pl.ns * strips * 16 * pl.dkp * 2);
       if (heads != key_heads) {
         pl.dq_part = take(tok * heads * dk * 4);
         pl.dk_part = take(tok * heads * dk * 4);
