@@ -17,7 +17,7 @@
 //   delta_split_kernel  fp16 / fp32 only: cuts dO into bf16 parts.
 //   delta_rev_kernel    from the last chunk to the first, dS^T in registers
 //                       as delta_scan_kernel keeps S^T; writes dV, dS per chunk.
-//   delta_grad_kernel   one CTA per (chunk, head), all in parallel.
+//   delta_grad_kernel   the rest, every (chunk, head) by itself.
 //   delta_group_kernel  sums dQ, dK over the heads that share a key head, in
 //                       a fixed order.
 #include <algorithm>
@@ -588,72 +588,76 @@ struct GradParams {
   float* dk_part;
   void* dlog_decay;
   void* dbeta;
-  int64_t L, chunks;
+  int64_t L, chunks, units;  // units: chunks of all heads
   int key_heads, heads, dk, dv;
   float scale;
 };
 
-constexpr int kGradThreads = 256;
+constexpr int kGradThreads = 512;
 
-// A CTA of 8 warps: H and X as 2 x 4 tiles of 32 x 16, the three 64 x dk sums
-// as 2 x 4 tiles of 32 x dk / 4, all in registers (128 a thread at dk = 128)
+// 16 warps.  The three 64 x dk sums (dQ, R, W) are cut into tiles of 16 MT
+// rows x 16 columns, H and X into tiles of 16 x 16; all stay in registers
 // while dO, dV, E, S0 and dS pass once through a ring of bulk copies, KS
-// strips of 16 values at a time.
+// strips of 16 values at a time.  One CTA per SM takes chunk after chunk, and
+// the ring runs on into the next chunk during the second phase: with a CTA
+// per chunk the copies of a chunk and its products took turns.
 template <int NP, int LV, int DKP>
 struct GradCfg {
   static constexpr int NS = LV + 1;
+  static constexpr int MT = DKP / 64;           // m tiles of a warp in the 64 x dk sums
+  static constexpr int kColW = DKP / 16;        // warps side by side there
   static constexpr int kTileK = kChunk * DKP * 2;
   static constexpr int kMat = kChunk * kChunk * 2;
   static constexpr int kRows = 16 * DKP * 2;  // 16 rows of a part of S0 or dS
   static constexpr int kOne = (NP + 2 * NS) * kStrip + 2 * NS * kRows;  // one strip's share
-  static constexpr int KS = LV == 1 ? 2 : 1;
-  // a stage
+  static constexpr int KS = 1;
+  // a stage of the ring
   static constexpr int oV = KS * NP * kStrip;
   static constexpr int oE = oV + KS * NS * kStrip;
   static constexpr int oS = oE + KS * NS * kStrip;
   static constexpr int oD = oS + NS * KS * kRows;
   static constexpr int kStage = oD + NS * KS * kRows;
   static_assert(kStage == KS * kOne);
-  // K and Q stay; the four matrices take the place of the ring
+  // K, Q and the decay vectors; the matrices of the second phase (two at a
+  // time where four do not fit); the ring
   static constexpr int oQ = NP * kTileK;
-  static constexpr int oRing = 2 * NP * kTileK;
-  static constexpr int oHs = oRing, oHb = oHs + NS * kMat, oXd = oHb + NS * kMat, oXb = oXd + NS * kMat;
-  static constexpr int kMats = 4 * NS * kMat;
-  static constexpr int kRoom = 227 * 1024 - 6144 - 128 - oRing;
+  static constexpr int oVec = 2 * NP * kTileK;
+  static constexpr int kVecBytes = kVecCount * kChunk * 4;
+  static constexpr int oMats = oVec + (kVecBytes + 127) / 128 * 128;
+  static constexpr int kSets = LV == 1 ? 2 : 1;  // of two matrices
+  static constexpr int oRing = oMats + kSets * 2 * NS * kMat;
+  static constexpr int kRoom = 227 * 1024 - 8192 - 128 - oRing;
   static constexpr int kStages = kRoom / kStage < 4 ? kRoom / kStage : 4;
-  static constexpr int kRing = kStages * kStage > kMats ? kStages * kStage : kMats;
-  static constexpr int kSmem = oRing + kRing + 128;
-  static_assert(kStages >= 2 && kSmem + 6144 <= 227 * 1024);
+  static constexpr int kSmem = oRing + kStages * kStage + 128;
+  static_assert(kStages >= 1 && kSmem + 8192 <= 227 * 1024);
 };
 
 template <typename T, int NP, int LV, int DKP>
 __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradParams p) {
   using Cfg = GradCfg<NP, LV, DKP>;
   constexpr int NS = Cfg::NS, NTH = kGradThreads, ROWB = DKP * 2, MROW = kChunk * 2, KS = Cfg::KS;
-  constexpr int NT = DKP / 32;  // n tiles of a warp's DKP / 4 columns
+  constexpr int MT = Cfg::MT, ST = Cfg::kStages, CW = Cfg::kColW;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
   const uint32_t st = smem_addr(dsm);
-  __shared__ __align__(16) float s_vec[kVecCount * kChunk];
-  __shared__ float s_red[3][4][kChunk];
+  __shared__ float s_red[3][CW][kChunk];
   __shared__ float s_dot[NTH / 32];
-  __shared__ __align__(8) uint64_t full[Cfg::kStages], freed[Cfg::kStages], full_kq;
+  __shared__ __align__(8) uint64_t full[ST], freed[ST], full_kq;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, t4 = lane & 3;
-  const int wr = warp >> 2, wc = warp & 3;
-  const int64_t bh = blockIdx.x / p.chunks, chunk = blockIdx.x - bh * p.chunks;
-  const int64_t b = bh / p.heads;
-  const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
-  const int64_t t0 = chunk * kChunk;
-  const int rows = (int)min((int64_t)kChunk, p.L - t0);
+  const int row0 = warp / CW * 16 * MT, col0 = warp % CW * 16;  // in the 64 x dk sums
+  const int hr = (warp >> 2) * 16, hc = (warp & 3) * 16;        // in H and X
+  // The tiles of H and X above the diagonal are not needed: their 6 warps
+  // take <S0, dS> instead, and one of them (thread kLoader) issues the copies.
+  const bool lower = hc <= hr;
+  constexpr int kLoader = 3 * 32;
+  const int above = warp < 4 ? warp - 1 : warp < 8 ? warp - 3 : 5;  // 0..5 among those
   const int64_t kstride = (int64_t)p.key_heads * p.dk;
-  const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
-  const int64_t unit = bh * p.chunks + chunk;
   const int strips = (p.dv + 15) / 16, dvp = strips * 16, slices = (strips + KS - 1) / KS;
   if (tid == 0) {
-    for (int i = 0; i < Cfg::kStages; ++i) {
+    for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&freed[i], NTH / 32);
     }
@@ -664,13 +668,17 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   pdl_wait();
   pdl_launch_dependents();
 
-  // thread 0 issues the copies
-  int next = 0;
+  // the copies: slice by slice, over this CTA's chunks
+  const int64_t mine = (p.units - blockIdx.x + gridDim.x - 1) / gridDim.x;  // chunks of this CTA
+  const int64_t total = mine * slices;
+  int64_t next = 0;      // slices issued
+  int64_t next_unit = blockIdx.x;
+  int next_slice = 0;
   auto issue = [&]() {
-    const int s = next % Cfg::kStages;
-    if (next >= Cfg::kStages && !mbar_wait_bounded(&freed[s], (uint32_t)((next / Cfg::kStages - 1) & 1)))
-      return false;
-    const int v0 = next * KS, n = min(KS, strips - v0);
+    const int s = (int)(next % ST);
+    if (next >= ST && !mbar_wait_bounded(&freed[s], (uint32_t)((next / ST - 1) & 1))) return false;
+    const int64_t unit = next_unit;
+    const int v0 = next_slice * KS, n = min(KS, strips - v0);
     const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
     mbar_expect_tx(&full[s], n * Cfg::kOne);
     bulk_in(at, p.do_parts + (unit * strips + v0) * NP * (kStrip / 2), n * NP * kStrip, &full[s]);
@@ -683,376 +691,413 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       bulk_in(at + Cfg::oD + i * KS * Cfg::kRows, p.ds_parts + sv, n * Cfg::kRows, &full[s]);
     }
     ++next;
+    if (++next_slice == slices) {
+      next_slice = 0;
+      next_unit += gridDim.x;
+    }
     return true;
   };
-  if (tid == 0) {
-    while (next < min(Cfg::kStages, slices)) issue();
+  auto issue_kq = [&](int64_t unit) {
+    const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
+    const int hk = (int)(bh - b * p.heads) / (p.heads / p.key_heads);
     const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kChunk * DKP);
-    mbar_expect_tx(&full_kq, 2 * NP * Cfg::kTileK);
+    mbar_expect_tx(&full_kq, 2 * NP * Cfg::kTileK + Cfg::kVecBytes);
     bulk_in(st, p.k_tiles + tile, NP * Cfg::kTileK, &full_kq);
     bulk_in(st + Cfg::oQ, p.q_tiles + tile, NP * Cfg::kTileK, &full_kq);
+    bulk_in(st + Cfg::oVec, p.vecs + unit * (kVecCount * kChunk), Cfg::kVecBytes, &full_kq);
+  };
+  if (tid == kLoader) {
+    while (next < min((int64_t)ST, total)) issue();
+    issue_kq(blockIdx.x);
   }
-  {
-    const float* vec = p.vecs + unit * (kVecCount * kChunk);
-    for (int i = tid; i < kVecCount * kChunk; i += NTH) s_vec[i] = vec[i];
-  }
-
-  float aq[2][NT][4], ar[2][NT][4], aw[2][NT][4], ah[2][2][4], ax[2][2][4];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) aq[m][n][e] = ar[m][n][e] = aw[m][n][e] = 0.f;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ah[m][n][e] = ax[m][n][e] = 0.f;
-  }
-  const bool lower = wc * 16 <= wr * 32 + 31;  // this warp's tile of H and X reaches the lower triangle
-  const int col0 = wc * (DKP / 4);
-  float dot = 0.f;  // this thread's share of <S0, dS>
 
   bool ok = true;
-  for (int it = 0; it < slices; ++it) {
-    const int s_id = it % Cfg::kStages, n = min(KS, strips - it * KS);
-    const uint32_t at = st + Cfg::oRing + s_id * Cfg::kStage;
-    ok = mbar_wait_bounded(&full[s_id], (uint32_t)((it / Cfg::kStages) & 1));
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
-    for (int kk = 0; kk < n; ++kk) {
-      {
-        uint32_t ag[NP][2][4], av[NS][2][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-#pragma unroll
-          for (int i = 0; i < NP; ++i)
-            ldsm4(ag[i][m], strip_a(at + (kk * NP + i) * kStrip, lane, wr * 32 + m * 16));
-#pragma unroll
-          for (int i = 0; i < NS; ++i)
-            ldsm4(av[i][m], strip_a(at + Cfg::oV + (kk * NS + i) * kStrip, lane, wr * 32 + m * 16));
-        }
-        if (lower) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            Step<LV == 2, 4> s;
-#pragma unroll
-            for (int j = LV; j >= 0; --j) {
-              uint32_t eb[4];
-              ldsm4(eb, strip_b(at + Cfg::oE + (kk * NS + j) * kStrip, lane, wc * 16));
-#pragma unroll
-              for (int i = LV - j; i >= 0; --i) {
-                if (i < NP) {
-                  s.mma(0, ah[m][0], ag[i < NP ? i : 0][m], eb[0], eb[1]);
-                  s.mma(1, ah[m][1], ag[i < NP ? i : 0][m], eb[2], eb[3]);
-                }
-                s.mma(2, ax[m][0], av[i][m], eb[0], eb[1]);
-                s.mma(3, ax[m][1], av[i][m], eb[2], eb[3]);
-              }
-            }
-            s.add(0, ah[m][0]);
-            s.add(1, ah[m][1]);
-            s.add(2, ax[m][0]);
-            s.add(3, ax[m][1]);
-          }
-        }
-#pragma unroll
-        for (int n2 = 0; n2 < NT / 2; ++n2) {
-          Step<LV == 2, 8> s;
-#pragma unroll
-          for (int j = LV; j >= 0; --j) {
-            uint32_t sb[4];
-            ldsm4_t(sb, at_bt<ROWB>(at + Cfg::oS + j * KS * Cfg::kRows, lane, col0 + n2 * 16, kk));
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-              for (int i = LV - j; i >= 0; --i) {
-                if (i < NP) {
-                  s.mma(4 * m, aq[m][2 * n2], ag[i < NP ? i : 0][m], sb[0], sb[1]);
-                  s.mma(4 * m + 1, aq[m][2 * n2 + 1], ag[i < NP ? i : 0][m], sb[2], sb[3]);
-                }
-                s.mma(4 * m + 2, ar[m][2 * n2], av[i][m], sb[0], sb[1]);
-                s.mma(4 * m + 3, ar[m][2 * n2 + 1], av[i][m], sb[2], sb[3]);
-              }
-          }
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            s.add(4 * m, aq[m][2 * n2]);
-            s.add(4 * m + 1, aq[m][2 * n2 + 1]);
-            s.add(4 * m + 2, ar[m][2 * n2]);
-            s.add(4 * m + 3, ar[m][2 * n2 + 1]);
-          }
-        }
-      }
-      uint32_t ae[NS][2][4];
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-          ldsm4(ae[i][m], strip_a(at + Cfg::oE + (kk * NS + i) * kStrip, lane, wr * 32 + m * 16));
-#pragma unroll
-      for (int n2 = 0; n2 < NT / 2; ++n2) {
-        Step<LV == 2, 4> s;
-#pragma unroll
-        for (int j = LV; j >= 0; --j) {
-          uint32_t db[4];
-          ldsm4_t(db, at_bt<ROWB>(at + Cfg::oD + j * KS * Cfg::kRows, lane, col0 + n2 * 16, kk));
-#pragma unroll
-          for (int i = LV - j; i >= 0; --i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              s.mma(2 * m, aw[m][2 * n2], ae[i][m], db[0], db[1]);
-              s.mma(2 * m + 1, aw[m][2 * n2 + 1], ae[i][m], db[2], db[3]);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          s.add(2 * m, aw[m][2 * n2]);
-          s.add(2 * m + 1, aw[m][2 * n2 + 1]);
-        }
-      }
-    }
-    // <S0, dS> over this slice (the same place of every part: swizzle does not matter)
-    for (int i = tid; i < n * Cfg::kRows / 16; i += NTH) {
-      float x[8] = {}, y[8] = {};
-#pragma unroll
-      for (int q = NS - 1; q >= 0; --q) {
-        const uint4 u = lds128(at + Cfg::oS + q * KS * Cfg::kRows + i * 16);
-        const uint4 v = lds128(at + Cfg::oD + q * KS * Cfg::kRows + i * 16);
-        const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] += bf16_lo(uw[e]);
-          x[2 * e + 1] += bf16_hi(uw[e]);
-          y[2 * e] += bf16_lo(vw[e]);
-          y[2 * e + 1] += bf16_hi(vw[e]);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
-    }
-    warp_arrive(&freed[s_id], lane);
-    // refill the stage of the slice before: every warp is done with it by now
-    if (tid == 0 && it > 0 && next < slices) ok = issue();
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-  if (lane == 0) s_dot[warp] = dot;
-  if (tid == 0) {
-    // no copy may land later: what was issued is waited for, also after a
-    // wait that gave up
-    for (int j = max(0, next - Cfg::kStages); j < next; ++j)
-      ok = mbar_wait_bounded(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1)) && ok;
-    ok = mbar_wait_bounded(&full_kq, 0) && ok;
-  }
-  if (__syncthreads_or(!ok)) return;  // also: the ring is read, s_vec written
+  int64_t it = 0;  // slices consumed
+  for (int64_t done = 0; done < mine; ++done) {
+    const int64_t unit = blockIdx.x + done * gridDim.x;
+    const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
+    const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
+    const int64_t t0 = chunk * kChunk;
+    const int rows = (int)min((int64_t)kChunk, p.L - t0);
 
-  // second phase: the matrices take the place of the ring
-  const float* enter = s_vec + kVecEnter * kChunk;
-  const float* leave = s_vec + kVecLeave * kChunk;
-  const float* beta = s_vec + kVecBeta * kChunk;
-  const float* hi = s_vec + kVecCumHi * kChunk;
-  const float* lo = s_vec + kVecCumLo * kChunk;
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
+    float aq[MT][2][4], ar[MT][2][4], aw[MT][2][4], ah[2][4], ax[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = wr * 32 + m * 16 + r * 8 + g4, j0 = wc * 16 + n * 8 + 2 * t4;
-        float hs[2], hb[2], xd[2], xb[2];
+      for (int e = 0; e < 4; ++e) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int j = j0 + c;
-          hs[c] = xd[c] = 0.f;
-          if (i >= j) {
-            const float d = i == j ? 1.f : expf((hi[i] - hi[j]) + (lo[i] - lo[j]));
-            hs[c] = ah[m][n][2 * r + c] * d * p.scale;
-            if (i > j) xd[c] = -ax[m][n][2 * r + c] * d;
-          }
-          hb[c] = hs[c] * beta[j];
-          xb[c] = xd[c] * beta[j];
-        }
-        const uint32_t at = tile_at<MROW>(0, i, j0 / 8) + (j0 % 8) * 2;
-        uint32_t w[NS];
-        auto put = [&](const float* x, int off) {
-          split_pair<NS>(x[0], x[1], w);
-#pragma unroll
-          for (int q = 0; q < NS; ++q)
-            *reinterpret_cast<uint32_t*>(dsm + off + q * Cfg::kMat + at) = w[q];
-        };
-        put(hs, Cfg::oHs);
-        put(hb, Cfg::oHb);
-        put(xd, Cfg::oXd);
-        put(xb, Cfg::oXb);
+        for (int m = 0; m < MT; ++m) aq[m][n][e] = ar[m][n][e] = aw[m][n][e] = 0.f;
+        ah[n][e] = ax[n][e] = 0.f;
       }
-  mbar_wait_bounded(&full_kq, 0);  // landed: thread 0 has seen it
-  __syncthreads();
+    float dot = 0.f;  // this thread's share of <S0, dS>
 
-  // an element pair of K or Q as fp32 (the sum of its parts)
-  auto kq_pair = [&](int off, int row, int col) {
-    float2 v = make_float2(0.f, 0.f);
+    for (int sl = 0; sl < slices; ++sl, ++it) {
+      const int s_id = (int)(it % ST), n = min(KS, strips - sl * KS);
+      const uint32_t at = st + Cfg::oRing + s_id * Cfg::kStage;
+      // refill the stage of the slice before: every warp is done with it, or nearly
+      if (tid == kLoader && ST > 1 && it > 0 && next < total) issue();
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s_id], (uint32_t)((it / ST) & 1)));
+      if (!ok) break;
+      for (int kk = 0; kk < n; ++kk) {
+        const uint32_t a_g = at + kk * NP * kStrip, a_v = at + Cfg::oV + kk * NS * kStrip,
+                       a_e = at + Cfg::oE + kk * NS * kStrip;
+        if (lower) {
+          uint32_t ag[NP][4], av[NS][4];
 #pragma unroll
-    for (int i = NP - 1; i >= 0; --i) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(
-          dsm + off + i * Cfg::kTileK + tile_at<ROWB>(0, row, col / 8) + (col % 8) * 2);
-      v.x += bf16_lo(w);
-      v.y += bf16_hi(w);
-    }
-    return v;
-  };
-  // sums over a warp's columns of a row, one value per row and warp column
-  auto put_row = [&](int which, int row, float v) {
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    v += __shfl_xor_sync(0xffffffffu, v, 2);
-    if (t4 == 0) s_red[which][wc][row] = v;
-  };
+          for (int i = 0; i < NP; ++i) ldsm4(ag[i], strip_a(a_g + i * kStrip, lane, hr));
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+          for (int i = 0; i < NS; ++i) ldsm4(av[i], strip_a(a_v + i * kStrip, lane, hr));
+          Step<LV == 2, 4> s;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = wr * 32 + m * 16 + r * 8 + g4;
-      const float ge = enter[i], gl = leave[i];
-      float sum = 0.f;
+          for (int j = LV; j >= 0; --j) {
+            uint32_t eb[4];
+            ldsm4(eb, strip_b(a_e + j * kStrip, lane, hc));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float2 kv = kq_pair(0, i, col0 + n * 8 + 2 * t4);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          aq[m][n][2 * r + c] *= ge * p.scale;
-          ar[m][n][2 * r + c] *= -ge;
-          aw[m][n][2 * r + c] *= gl;
-          sum = fmaf(aw[m][n][2 * r + c], c ? kv.y : kv.x, sum);
-        }
-      }
-      put_row(2, i, sum);
-    }
-
-#pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
-    const bool left = kk <= 2 * wr + 1;   // columns j = 16 kk.. of rows i: j <= i somewhere
-    const bool right = kk >= 2 * wr;      // rows i = 16 kk.. of columns j: i >= j somewhere
-    // the matrices' parts i and K's or Q's parts j, smallest first
-    auto product = [&](int hs, int xs, bool trans, int hb_off, float (&h_acc)[2][NT][4],
-                       float (&x_acc)[2][NT][4]) {
-#pragma unroll
-      for (int n2 = 0; n2 < NT / 2; ++n2) {
-        Step<LV == 2, 8> s;
-#pragma unroll
-        for (int j = NP - 1; j >= 0; --j) {
-          uint32_t kb[4], hb[4];
-          ldsm4_t(kb, at_bt<ROWB>(st + j * Cfg::kTileK, lane, col0 + n2 * 16, kk));
-          if (hb_off != 0)
-            ldsm4_t(hb, at_bt<ROWB>(st + hb_off + j * Cfg::kTileK, lane, col0 + n2 * 16, kk));
-#pragma unroll
-          for (int i = LV - j; i >= 0; --i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              uint32_t fh[4], fx[4];
-              if (trans) {
-                ldsm4_t(fh, at_at<MROW>(st + hs + i * Cfg::kMat, lane, wr * 32 + m * 16, kk));
-                ldsm4_t(fx, at_at<MROW>(st + xs + i * Cfg::kMat, lane, wr * 32 + m * 16, kk));
-              } else {
-                ldsm4(fh, at_a<MROW>(st + hs + i * Cfg::kMat, lane, wr * 32 + m * 16, kk));
-                ldsm4(fx, at_a<MROW>(st + xs + i * Cfg::kMat, lane, wr * 32 + m * 16, kk));
+            for (int i = LV - j; i >= 0; --i) {
+              if (i < NP) {
+                s.mma(0, ah[0], ag[i < NP ? i : 0], eb[0], eb[1]);
+                s.mma(1, ah[1], ag[i < NP ? i : 0], eb[2], eb[3]);
               }
-              const uint32_t(&b)[4] = hb_off != 0 ? hb : kb;
-              s.mma(4 * m, h_acc[m][2 * n2], fh, b[0], b[1]);
-              s.mma(4 * m + 1, h_acc[m][2 * n2 + 1], fh, b[2], b[3]);
-              s.mma(4 * m + 2, x_acc[m][2 * n2], fx, kb[0], kb[1]);
-              s.mma(4 * m + 3, x_acc[m][2 * n2 + 1], fx, kb[2], kb[3]);
+              s.mma(2, ax[0], av[i], eb[0], eb[1]);
+              s.mma(3, ax[1], av[i], eb[2], eb[3]);
             }
+          }
+          s.add(0, ah[0]);
+          s.add(1, ah[1]);
+          s.add(2, ax[0]);
+          s.add(3, ax[1]);
+        }
+        {
+          uint32_t sb[NS][4];
+#pragma unroll
+          for (int j = 0; j < NS; ++j)
+            ldsm4_t(sb[j], at_bt<ROWB>(at + Cfg::oS + j * KS * Cfg::kRows, lane, col0, kk));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            uint32_t ag[NP][4], av[NS][4];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) ldsm4(ag[i], strip_a(a_g + i * kStrip, lane, row0 + m * 16));
+#pragma unroll
+            for (int i = 0; i < NS; ++i) ldsm4(av[i], strip_a(a_v + i * kStrip, lane, row0 + m * 16));
+            Step<LV == 2, 4> s;
+#pragma unroll
+            for (int j = LV; j >= 0; --j)
+#pragma unroll
+              for (int i = LV - j; i >= 0; --i) {
+                if (i < NP) {
+                  s.mma(0, aq[m][0], ag[i < NP ? i : 0], sb[j][0], sb[j][1]);
+                  s.mma(1, aq[m][1], ag[i < NP ? i : 0], sb[j][2], sb[j][3]);
+                }
+                s.mma(2, ar[m][0], av[i], sb[j][0], sb[j][1]);
+                s.mma(3, ar[m][1], av[i], sb[j][2], sb[j][3]);
+              }
+            s.add(0, aq[m][0]);
+            s.add(1, aq[m][1]);
+            s.add(2, ar[m][0]);
+            s.add(3, ar[m][1]);
+          }
+        }
+        {
+          uint32_t db[NS][4];
+#pragma unroll
+          for (int j = 0; j < NS; ++j)
+            ldsm4_t(db[j], at_bt<ROWB>(at + Cfg::oD + j * KS * Cfg::kRows, lane, col0, kk));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            uint32_t ae[NS][4];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) ldsm4(ae[i], strip_a(a_e + i * kStrip, lane, row0 + m * 16));
+            Step<LV == 2, 2> s;
+#pragma unroll
+            for (int j = LV; j >= 0; --j)
+#pragma unroll
+              for (int i = LV - j; i >= 0; --i) {
+                s.mma(0, aw[m][0], ae[i], db[j][0], db[j][1]);
+                s.mma(1, aw[m][1], ae[i], db[j][2], db[j][3]);
+              }
+            s.add(0, aw[m][0]);
+            s.add(1, aw[m][1]);
+          }
+        }
+      }
+      // <S0, dS> over this slice (the same place of every part: swizzle does not matter)
+      for (int i = above * 32 + lane; !lower && i < n * Cfg::kRows / 16; i += 6 * 32) {
+        float x[8] = {}, y[8] = {};
+#pragma unroll
+        for (int q = NS - 1; q >= 0; --q) {
+          const uint4 u = lds128(at + Cfg::oS + q * KS * Cfg::kRows + i * 16);
+          const uint4 v = lds128(at + Cfg::oD + q * KS * Cfg::kRows + i * 16);
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[2 * e] += bf16_lo(uw[e]);
+            x[2 * e + 1] += bf16_hi(uw[e]);
+            y[2 * e] += bf16_lo(vw[e]);
+            y[2 * e + 1] += bf16_hi(vw[e]);
+          }
         }
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          s.add(4 * m, h_acc[m][2 * n2]);
-          s.add(4 * m + 1, h_acc[m][2 * n2 + 1]);
-          s.add(4 * m + 2, x_acc[m][2 * n2]);
-          s.add(4 * m + 3, x_acc[m][2 * n2 + 1]);
-        }
+        for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
+      }
+      warp_arrive(&freed[s_id], lane);
+      if (tid == kLoader && ST == 1 && next < total) issue();
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if (lane == 0) s_dot[warp] = dot;
+    ok = ok && mbar_wait_bounded(&full_kq, (uint32_t)(done & 1));
+    if (__syncthreads_or(!ok)) {
+      ok = false;
+      break;
+    }
+
+    // second phase
+    const float* s_vec = reinterpret_cast<const float*>(dsm + Cfg::oVec);
+    const float* enter = s_vec + kVecEnter * kChunk;
+    const float* leave = s_vec + kVecLeave * kChunk;
+    const float* beta = s_vec + kVecBeta * kChunk;
+    const float* hi = s_vec + kVecCumHi * kChunk;
+    const float* lo = s_vec + kVecCumLo * kChunk;
+    // H and X times D: rows i, columns j, in the order of an A operand's
+    // registers.  As parts in shared memory with each column times beta (set
+    // 0, row operands of dQ and R) or without (set 1, column operands of W).
+    float2 hd[4], xd[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = q >> 1, r = q & 1;
+      const int i = hr + r * 8 + g4, j0 = hc + n * 8 + 2 * t4;
+      hd[q] = xd[q] = make_float2(0.f, 0.f);
+      if (lower) {
+        const float2 hj = *reinterpret_cast<const float2*>(hi + j0);
+        const float2 lj = *reinterpret_cast<const float2*>(lo + j0);
+        const float d0 = i > j0 ? expf((hi[i] - hj.x) + (lo[i] - lj.x)) : 1.f;
+        const float d1 = i > j0 + 1 ? expf((hi[i] - hj.y) + (lo[i] - lj.y)) : 1.f;
+        if (i >= j0) hd[q].x = ah[n][2 * r] * d0 * p.scale;
+        if (i >= j0 + 1) hd[q].y = ah[n][2 * r + 1] * d1 * p.scale;
+        if (i > j0) xd[q].x = -ax[n][2 * r] * d0;
+        if (i > j0 + 1) xd[q].y = -ax[n][2 * r + 1] * d1;
+      }
+    }
+    auto put_mats = [&](int set) {
+      const uint32_t base = st + Cfg::oMats + (Cfg::kSets == 2 ? set : 0) * 2 * NS * Cfg::kMat;
+      uint32_t wh[4][NS], wx[4][NS];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float2 w = make_float2(1.f, 1.f);
+        if (set == 0) w = *reinterpret_cast<const float2*>(beta + hc + (q >> 1) * 8 + 2 * t4);
+        split_pair<NS>(hd[q].x * w.x, hd[q].y * w.y, wh[q]);
+        split_pair<NS>(xd[q].x * w.x, xd[q].y * w.y, wx[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < NS; ++q) {
+        const uint32_t a[4] = {wh[0][q], wh[1][q], wh[2][q], wh[3][q]};
+        const uint32_t x[4] = {wx[0][q], wx[1][q], wx[2][q], wx[3][q]};
+        stsm4(at_a<MROW>(base + q * Cfg::kMat, lane, hr, hc / 16), a);
+        stsm4(at_a<MROW>(base + (NS + q) * Cfg::kMat, lane, hr, hc / 16), x);
       }
     };
-    if (left) product(Cfg::oHb, Cfg::oXb, false, 0, aq, ar);
-    if (right) product(Cfg::oHs, Cfg::oXd, true, Cfg::oQ, aw, aw);
-  }
+    put_mats(0);
+    if (Cfg::kSets == 2) put_mats(1);
+    // an element pair of K or Q as fp32 (the sum of its parts)
+    auto kq_pair = [&](int off, int row, int col) {
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = NP - 1; i >= 0; --i) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(
+            dsm + off + i * Cfg::kTileK + tile_at<ROWB>(0, row, col / 8) + (col % 8) * 2);
+        v.x += bf16_lo(w);
+        v.y += bf16_hi(w);
+      }
+      return v;
+    };
+    // sums over a warp's columns of a row, one value per row and warp column
+    auto put_row = [&](int which, int row, float v) {
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (t4 == 0) s_red[which][warp % CW][row] = v;
+    };
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = row0 + m * 16 + r * 8 + g4;
+        const float ge = enter[i], gl = leave[i];
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float2 kv = kq_pair(0, i, col0 + n * 8 + 2 * t4);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            aq[m][n][2 * r + c] *= ge * p.scale;
+            ar[m][n][2 * r + c] *= -ge;
+            aw[m][n][2 * r + c] *= gl;
+            sum = fmaf(aw[m][n][2 * r + c], c ? kv.y : kv.x, sum);
+          }
+        }
+        put_row(2, i, sum);
+      }
+    __syncthreads();
 
+    // dQ += Hb K, R += Xb K: rows i, columns j <= i
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk * 16 > row0 + 16 * MT - 1) break;
+      uint32_t kb[NP][4];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = wr * 32 + m * 16 + r * 8 + g4;
-      const float be = beta[i];
-      float reads = 0.f, writes = 0.f;
+      for (int j = 0; j < NP; ++j) ldsm4_t(kb[j], at_bt<ROWB>(st + j * Cfg::kTileK, lane, col0, kk));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int col = col0 + n * 8 + 2 * t4;
-        const float2 kv = kq_pair(0, i, col), qv = kq_pair(Cfg::oQ, i, col);
-        const float q0 = aq[m][n][2 * r], q1 = aq[m][n][2 * r + 1];
-        const float r0 = ar[m][n][2 * r], r1 = ar[m][n][2 * r + 1];
-        const float w0 = aw[m][n][2 * r], w1 = aw[m][n][2 * r + 1];
-        reads = fmaf(qv.x, q0, fmaf(qv.y, q1, fmaf(kv.x, r0, fmaf(kv.y, r1, reads))));
-        writes = fmaf(kv.x, w0, fmaf(kv.y, w1, writes));
-        const float k0 = fmaf(be, w0, r0), k1 = fmaf(be, w1, r1);
-        if (i < rows && col < p.dk) {
-          if (p.dq_part != nullptr) {
-            const int64_t o = ((b * p.L + t0 + i) * p.heads + h) * p.dk + col;
-            *reinterpret_cast<float2*>(p.dq_part + o) = make_float2(q0, q1);
-            *reinterpret_cast<float2*>(p.dk_part + o) = make_float2(k0, k1);
-          } else {
-            const int64_t o = kf + (int64_t)i * kstride + col;
-            T* dq = static_cast<T*>(p.dq) + o;
-            T* dk = static_cast<T*>(p.dk_out) + o;
-            if constexpr (sizeof(T) == 4) {
-              *reinterpret_cast<float2*>(dq) = make_float2(q0, q1);
-              *reinterpret_cast<float2*>(dk) = make_float2(k0, k1);
+      for (int m = 0; m < MT; ++m) {
+        Step<LV == 2, 4> s;
+#pragma unroll
+        for (int i = LV; i >= 0; --i) {
+          uint32_t fh[4], fx[4];
+          const uint32_t base = st + Cfg::oMats + i * Cfg::kMat;
+          ldsm4(fh, at_a<MROW>(base, lane, row0 + m * 16, kk));
+          ldsm4(fx, at_a<MROW>(base + NS * Cfg::kMat, lane, row0 + m * 16, kk));
+#pragma unroll
+          for (int j = NP - 1; j >= 0; --j) {
+            if (i + j > LV) continue;
+            s.mma(0, aq[m][0], fh, kb[j][0], kb[j][1]);
+            s.mma(1, aq[m][1], fh, kb[j][2], kb[j][3]);
+            s.mma(2, ar[m][0], fx, kb[j][0], kb[j][1]);
+            s.mma(3, ar[m][1], fx, kb[j][2], kb[j][3]);
+          }
+        }
+        s.add(0, aq[m][0]);
+        s.add(1, aq[m][1]);
+        s.add(2, ar[m][0]);
+        s.add(3, ar[m][1]);
+      }
+    }
+    if (Cfg::kSets == 1) {
+      __syncthreads();
+      put_mats(1);
+      __syncthreads();
+    }
+    // W += Hs^T Q + Xd^T K: rows j, columns i >= j
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk * 16 + 15 < row0) continue;
+      uint32_t kb[NP][4], qb[NP][4];
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        ldsm4_t(kb[j], at_bt<ROWB>(st + j * Cfg::kTileK, lane, col0, kk));
+        ldsm4_t(qb[j], at_bt<ROWB>(st + Cfg::oQ + j * Cfg::kTileK, lane, col0, kk));
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        Step<LV == 2, 4> s;
+#pragma unroll
+        for (int i = LV; i >= 0; --i) {
+          uint32_t fh[4], fx[4];
+          const uint32_t base =
+              st + Cfg::oMats + (Cfg::kSets == 2 ? 2 * NS * Cfg::kMat : 0) + i * Cfg::kMat;
+          ldsm4_t(fh, at_at<MROW>(base, lane, row0 + m * 16, kk));
+          ldsm4_t(fx, at_at<MROW>(base + NS * Cfg::kMat, lane, row0 + m * 16, kk));
+#pragma unroll
+          for (int j = NP - 1; j >= 0; --j) {
+            if (i + j > LV) continue;
+            s.mma(0, aw[m][0], fh, qb[j][0], qb[j][1]);
+            s.mma(1, aw[m][1], fh, qb[j][2], qb[j][3]);
+            s.mma(2, aw[m][0], fx, kb[j][0], kb[j][1]);
+            s.mma(3, aw[m][1], fx, kb[j][2], kb[j][3]);
+          }
+        }
+        s.add(0, aw[m][0]);
+        s.add(1, aw[m][1]);
+        s.add(2, aw[m][0]);
+        s.add(3, aw[m][1]);
+      }
+    }
+
+    const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = row0 + m * 16 + r * 8 + g4;
+        const float be = beta[i];
+        float reads = 0.f, writes = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int col = col0 + n * 8 + 2 * t4;
+          const float2 kv = kq_pair(0, i, col), qv = kq_pair(Cfg::oQ, i, col);
+          const float q0 = aq[m][n][2 * r], q1 = aq[m][n][2 * r + 1];
+          const float r0 = ar[m][n][2 * r], r1 = ar[m][n][2 * r + 1];
+          const float w0 = aw[m][n][2 * r], w1 = aw[m][n][2 * r + 1];
+          reads = fmaf(qv.x, q0, fmaf(qv.y, q1, fmaf(kv.x, r0, fmaf(kv.y, r1, reads))));
+          writes = fmaf(kv.x, w0, fmaf(kv.y, w1, writes));
+          const float k0 = fmaf(be, w0, r0), k1 = fmaf(be, w1, r1);
+          if (i < rows && col < p.dk) {
+            if (p.dq_part != nullptr) {
+              const int64_t o = ((b * p.L + t0 + i) * p.heads + h) * p.dk + col;
+              *reinterpret_cast<float2*>(p.dq_part + o) = make_float2(q0, q1);
+              *reinterpret_cast<float2*>(p.dk_part + o) = make_float2(k0, k1);
             } else {
-              *reinterpret_cast<uint32_t*>(dq) = pack2<T>(q0, q1);
-              *reinterpret_cast<uint32_t*>(dk) = pack2<T>(k0, k1);
+              const int64_t o = kf + (int64_t)i * kstride + col;
+              T* dq = static_cast<T*>(p.dq) + o;
+              T* dk = static_cast<T*>(p.dk_out) + o;
+              if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float2*>(dq) = make_float2(q0, q1);
+                *reinterpret_cast<float2*>(dk) = make_float2(k0, k1);
+              } else {
+                *reinterpret_cast<uint32_t*>(dq) = pack2<T>(q0, q1);
+                *reinterpret_cast<uint32_t*>(dk) = pack2<T>(k0, k1);
+              }
             }
           }
         }
+        put_row(0, i, reads);
+        put_row(1, i, writes);
       }
-      put_row(0, i, reads);
-      put_row(1, i, writes);
-    }
-  __syncthreads();
+    __syncthreads();
 
-  // dbeta, and the suffix sums of dlog_decay: one warp, two tokens a lane, in 64 bits
-  if (warp == 0) {
-    double dg[2], state = 0.0;
-    float db[2];
+    // dbeta, and the suffix sums of dlog_decay: one warp, two tokens a lane, in 64 bits
+    if (warp == 0) {
+      double dg[2], state = 0.0;
+      float db[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int i = 2 * lane + c;
-      auto sum4 = [&](int which) {
-        return (s_red[which][0][i] + s_red[which][1][i]) + (s_red[which][2][i] + s_red[which][3][i]);
-      };
-      db[c] = sum4(1);
-      dg[c] = (double)sum4(0) - (double)beta[i] * (double)db[c];
-      state += (double)beta[i] * (double)sum4(2);
-    }
+      for (int c = 0; c < 2; ++c) {
+        const int i = 2 * lane + c;
+        float sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < NTH / 32; ++w)
-      if (lane == 0) state += (double)enter[kChunk - 1] * (double)s_dot[w];
-    double suffix = dg[0] + dg[1];
+        for (int w = 0; w < CW; ++w)
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double o = __shfl_down_sync(0xffffffffu, suffix, d);
-      if (lane + d < 32) suffix += o;
-      state += __shfl_xor_sync(0xffffffffu, state, d);
-    }
-    const double out[2] = {suffix + state, suffix - dg[0] + state};
+          for (int q = 0; q < 3; ++q) sum[q] += s_red[q][w][i];
+        db[c] = sum[1];
+        dg[c] = (double)sum[0] - (double)beta[i] * (double)sum[1];
+        state += (double)beta[i] * (double)sum[2];
+      }
+      if (lane < NTH / 32) state += (double)enter[kChunk - 1] * (double)s_dot[lane];
+      double suffix = dg[0] + dg[1];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int i = 2 * lane + c;
-      if (i < rows) {
-        const int64_t o = (b * p.L + t0 + i) * p.heads + h;
-        // a decay of exactly 0 has no slope in its logarithm
-        const bool reset = Elem<T>::load(static_cast<const T*>(p.log_decay)[o]) < kDecayFloor;
-        static_cast<T*>(p.dlog_decay)[o] = Elem<T>::store(reset ? 0.f : (float)out[c]);
-        static_cast<T*>(p.dbeta)[o] = Elem<T>::store(db[c]);
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_down_sync(0xffffffffu, suffix, d);
+        if (lane + d < 32) suffix += o;
+        state += __shfl_xor_sync(0xffffffffu, state, d);
+      }
+      const double out[2] = {suffix + state, suffix - dg[0] + state};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = 2 * lane + c;
+        if (i < rows) {
+          const int64_t o = (b * p.L + t0 + i) * p.heads + h;
+          // a decay of exactly 0 has no slope in its logarithm
+          const bool reset = Elem<T>::load(static_cast<const T*>(p.log_decay)[o]) < kDecayFloor;
+          static_cast<T*>(p.dlog_decay)[o] = Elem<T>::store(reset ? 0.f : (float)out[c]);
+          static_cast<T*>(p.dbeta)[o] = Elem<T>::store(db[c]);
+        }
       }
     }
+    __syncthreads();  // K, Q, the vectors and the sums are used up
+    if (tid == kLoader && done + 1 < mine) issue_kq(unit + gridDim.x);
+  }
+  // After a wait that gave up: no copy may land after the CTA is gone.
+  if (!ok && tid == kLoader) {
+    for (int64_t j = max((int64_t)0, next - ST); j < next; ++j)
+      mbar_wait_bounded(&full[j % ST], (uint32_t)((j / ST) & 1));
+    mbar_wait_bounded(&full_kq, 0);
+    mbar_wait_bounded(&full_kq, 1);
   }
 }
 
@@ -1171,6 +1216,7 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   g.dbeta = static_cast<T*>(a.dbeta) + g0;
   g.L = a.seqlen;
   g.chunks = pl.chunks;
+  g.units = bh * pl.chunks;
   g.key_heads = (int)a.key_heads;
   g.heads = (int)a.heads;
   g.dk = (int)a.dk;
@@ -1180,7 +1226,8 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   auto kern = delta_grad_kernel<T, NP, LV, DKP>;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC::kSmem);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, (unsigned)(bh * pl.chunks), kGradThreads, GC::kSmem, a.stream, g);
+  e = launch_pdl(kern, (unsigned)std::min<int64_t>(g.units, a.num_sms), kGradThreads, GC::kSmem,
+                 a.stream, g);
   if (e != cudaSuccess || !shared) return e;
 
   GroupParams s{};

@@ -55,12 +55,19 @@ struct PrepParams {
 
 constexpr int kPrepThreads = 128;
 constexpr int kMatBytes = kChunk * kChunk * 2;  // one part of N or P
-constexpr int kPad = kChunk + 1;  // fp32 rows in shared memory: columns on distinct banks
+constexpr int kPad = kChunk + 4;  // fp32 rows in shared memory: 16-byte vectors on distinct banks
 
-template <int NP, int DKP>
-constexpr int prep_smem() {
-  return 2 * NP * kChunk * DKP * 2 + 2 * kChunk * kPad * 4 + kVecCount * kChunk * 4 + 128;
-}
+// K and Q; over them, once they are used up, the image of P and the inverse.
+template <int NP, int NS, int DKP>
+struct PrepCfg {
+  static constexpr int kTile = kChunk * DKP * 2;
+  static constexpr int kF32 = kChunk * kPad * 4;
+  static constexpr int kTiles = 2 * NP * kTile;
+  static constexpr int oN = NS * kMatBytes;  // the image of P lies at 0
+  static constexpr int kBody = kTiles > oN + kF32 ? kTiles : oN + kF32;
+  static constexpr int oA = kBody, oVec = oA + kF32;
+  static constexpr int kSmem = oVec + kVecCount * kChunk * 4 + 128;
+};
 
 // The chunk's rows of x as parts in a tile: 16-byte units of 8 values.
 template <typename T, int NP, int DKP>
@@ -103,16 +110,17 @@ __device__ __forceinline__ void split_tile(uint32_t dst, const T* x, int64_t str
 }
 
 template <typename T, int NP, int LV, int DKP>
-__global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const PrepParams p) {
+__global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepParams p) {
   constexpr int NS = LV + 1;
-  constexpr int ROWB = DKP * 2, TILE = kChunk * ROWB;
+  constexpr int ROWB = DKP * 2, TILE = kChunk * ROWB, MROW = kChunk * 2;
+  using Cfg = PrepCfg<NP, NS, DKP>;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
   const uint32_t s_k = smem_addr(dsm), s_q = s_k + NP * TILE;
-  float* s_a = reinterpret_cast<float*>(dsm + 2 * NP * TILE);  // M diag(beta), strictly lower
-  float* s_n = s_a + kChunk * kPad;                            // its unit-triangle inverse
-  float* s_vec = s_n + kChunk * kPad;
+  float* s_n = reinterpret_cast<float*>(dsm + Cfg::oN);  // the inverse
+  float* s_a = reinterpret_cast<float*>(dsm + Cfg::oA);  // M diag(beta), strictly lower
+  float* s_vec = reinterpret_cast<float*>(dsm + Cfg::oVec);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t bh = blockIdx.x / p.chunks, chunk = blockIdx.x - bh * p.chunks;
@@ -177,145 +185,183 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const PrepPara
     bulk_commit();
   }
 
-  // K K^T and Q K^T, 16 rows a warp; tiles above the diagonal are not needed
+  // K K^T, then Q K^T, 16 rows a warp; tiles above the diagonal are not needed
   const int g4 = lane >> 2, t4 = lane & 3;
-  float kk_acc[8][4], qk_acc[8][4];
-#pragma unroll
-  for (int n = 0; n < 8; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) kk_acc[n][c] = qk_acc[n][c] = 0.f;
-#pragma unroll 2
-  for (int kk = 0; kk < DKP / 16; ++kk) {
-    uint32_t ka[NP][4], qa[NP][4];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      ldsm4(ka[i], at_a<ROWB>(s_k + i * TILE, lane, warp * 16, kk));
-      ldsm4(qa[i], at_a<ROWB>(s_q + i * TILE, lane, warp * 16, kk));
-    }
-#pragma unroll
-    for (int np2 = 0; np2 < 4; ++np2) {
-      if (np2 > warp) break;
-      Step<LV == 2, 4> s;
-#pragma unroll
-      for (int j = NP - 1; j >= 0; --j) {
-        uint32_t bf[4];
-        ldsm4(bf, at_b<ROWB>(s_k + j * TILE, lane, np2 * 16, kk));
-#pragma unroll
-        for (int i = NP - 1; i >= 0; --i) {
-          if (i + j > LV) continue;
-          s.mma(0, kk_acc[2 * np2], ka[i], bf[0], bf[1]);
-          s.mma(1, kk_acc[2 * np2 + 1], ka[i], bf[2], bf[3]);
-          s.mma(2, qk_acc[2 * np2], qa[i], bf[0], bf[1]);
-          s.mma(3, qk_acc[2 * np2 + 1], qa[i], bf[2], bf[3]);
-        }
-      }
-      s.add(0, kk_acc[2 * np2]);
-      s.add(1, kk_acc[2 * np2 + 1]);
-      s.add(2, qk_acc[2 * np2]);
-      s.add(3, qk_acc[2 * np2 + 1]);
-    }
-  }
   const float* hi = s_vec + kVecCumHi * kChunk;
   const float* lo = s_vec + kVecCumLo * kChunk;
   const float* be = s_vec + kVecBeta * kChunk;
-  const int64_t mat = (bh * p.chunks + chunk) * NS * (kChunk * kChunk);
+  auto with_k = [&](uint32_t rows_at, float (&acc)[8][4]) {
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[n][c] = 0.f;
+#pragma unroll 2
+    for (int kk = 0; kk < DKP / 16; ++kk) {
+      uint32_t af[NP][4];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) ldsm4(af[i], at_a<ROWB>(rows_at + i * TILE, lane, warp * 16, kk));
+#pragma unroll
+      for (int np2 = 0; np2 < 4; ++np2) {
+        if (np2 > warp) break;
+        Step<LV == 2, 2> s;
+#pragma unroll
+        for (int j = NP - 1; j >= 0; --j) {
+          uint32_t bf[4];
+          ldsm4(bf, at_b<ROWB>(s_k + j * TILE, lane, np2 * 16, kk));
+#pragma unroll
+          for (int i = NP - 1; i >= 0; --i) {
+            if (i + j > LV) continue;
+            s.mma(0, acc[2 * np2], af[i], bf[0], bf[1]);
+            s.mma(1, acc[2 * np2 + 1], af[i], bf[2], bf[3]);
+          }
+        }
+        s.add(0, acc[2 * np2]);
+        s.add(1, acc[2 * np2 + 1]);
+      }
+    }
+  };
+  float acc[8][4];
+  with_k(s_k, acc);
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int i = warp * 16 + g4 + r * 8, j0 = n * 8 + 2 * t4;
-      float pv[2];
+      float a[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int j = j0 + c;
-        float d = 0.f, a = 0.f;
-        if (i >= j) {
-          d = i == j ? 1.f : expf((hi[i] - hi[j]) + (lo[i] - lo[j]));
-          if (i > j) a = kk_acc[n][2 * r + c] * d * be[j];
-          d = qk_acc[n][2 * r + c] * d * p.scale * be[j];
-        }
-        s_a[i * kPad + j] = a;
-        s_n[i * kPad + j] = 0.f;
-        pv[c] = d;
+        a[c] = i > j ? acc[n][2 * r + c] * expf((hi[i] - hi[j]) + (lo[i] - lo[j])) * be[j] : 0.f;
       }
-      uint32_t w[NS];
-      split_pair<NS>(pv[0], pv[1], w);
+      *reinterpret_cast<float2*>(&s_a[i * kPad + j0]) = make_float2(a[0], a[1]);
+    }
+  with_k(s_q, acc);
+  if (keeper) bulk_wait_read<0>();
+  __syncthreads();  // K and Q are used up
 #pragma unroll
-      for (int q = 0; q < NS; ++q)
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(p.p_mat + mat) +
-                                     tile_at<kChunk * 2>(q * kMatBytes, i, n) + 4 * t4) = w[q];
+  for (int kk = 0; kk < 4; ++kk) {
+    uint32_t w[4][NS];  // P's 16 x 16 tile, in the order of an A operand
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = 2 * kk + (q >> 1), r = q & 1;
+      const int i = warp * 16 + g4 + r * 8, j0 = n * 8 + 2 * t4;
+      float v[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int j = j0 + c;
+        const float d = i == j ? 1.f : i > j ? expf((hi[i] - hi[j]) + (lo[i] - lo[j])) : 0.f;
+        v[c] = i >= j ? acc[n][2 * r + c] * d * p.scale * be[j] : 0.f;
+      }
+      split_pair<NS>(v[0], v[1], w[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < NS; ++q) {
+      const uint32_t a[4] = {w[0][q], w[1][q], w[2][q], w[3][q]};
+      stsm4(at_a<MROW>(s_k + q * kMatBytes, lane, warp * 16, kk), a);
     }
   }
-  __syncthreads();
+  fence_async();
 
   // N = (I + A)^-1.  16 x 16 blocks on the diagonal by substitution, a column
   // a lane; then [[B, 0], [C, D]]^-1 = [[B', 0], [-D' C B', D']] twice.
-  if (lane < 16) {
+  {
+    const int o = warp * 16;
     float x[16];
-    const float* a = s_a + (warp * 16) * kPad + warp * 16;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = i == lane ? 1.f : 0.f;
+      float v = i == (lane & 15) ? 1.f : 0.f;
+      const float4* a = reinterpret_cast<const float4*>(&s_a[(o + i) * kPad + o]);
 #pragma unroll
-      for (int l = 0; l < i; ++l) v = fmaf(-a[i * kPad + l], x[l], v);
+      for (int l4 = 0; l4 < (i + 3) / 4; ++l4) {
+        const float4 q = a[l4];
+        if (4 * l4 < i) v = fmaf(-q.x, x[4 * l4], v);
+        if (4 * l4 + 1 < i) v = fmaf(-q.y, x[4 * l4 + 1], v);
+        if (4 * l4 + 2 < i) v = fmaf(-q.z, x[4 * l4 + 2], v);
+        if (4 * l4 + 3 < i) v = fmaf(-q.w, x[4 * l4 + 3], v);
+      }
       x[i] = v;
     }
+    // lanes 0..15 store the block; 16..31 clear the block to its right
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s_n[(warp * 16 + i) * kPad + warp * 16 + lane] = x[i];
+    for (int i = 0; i < 16; ++i) {
+      const int col = o + lane;
+      if (col < kChunk) s_n[(o + i) * kPad + col] = lane < 16 ? x[i] : 0.f;
+    }
+    for (int i = 0; i < 16; ++i)  // and the blocks beyond
+      for (int col = o + 32 + lane; col < kChunk; col += 32) s_n[(o + i) * kPad + col] = 0.f;
   }
   __syncthreads();
-  float* s_t = s_a;  // the products C B' overwrite the blocks C that they use up
+  if (tid == 0) {  // every warp has written its rows of P
+    bulk_s2g(p.p_mat + (bh * p.chunks + chunk) * NS * (kChunk * kChunk), s_k, NS * kMatBytes);
+    bulk_commit();
+  }
 #pragma unroll
   for (int half = 16; half <= 32; half <<= 1) {
-    // per 2*half block: rows half..2*half, columns 0..half.  A thread takes
-    // one column and `per` rows.
-    const int per = half * half * (32 / half) / kPrepThreads;  // 4, 8
-    const int item = tid * per;
-    const int blk = item / (half * half), in = item - blk * half * half;
-    const int col = (in / per) % half, row = (in / per) / half * per;
+    // per 2*half block: rows half..2*half, columns 0..half.  A thread takes 2
+    // rows x 4 columns; 16-byte vectors along both.
+    const int per = half * half / 8;  // threads of a block: 32, 128
+    const int blk = tid / per, in = tid % per;
+    const bool on = blk < 32 / half;
+    const int col = in % (half / 4) * 4, row = in / (half / 4) * 2;
     const int o = blk * 2 * half;
-    float acc[8];
+    float4 r0, r1;
+    auto product = [&](const float* left, const float* right, int lo_, int ro) {
+      // rows row, row + 1 of left (columns lo_..) x rows of right (columns ro + col..)
+      r0 = r1 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int l = 0; l < half; l += 4) {
+        const float4 a0 = *reinterpret_cast<const float4*>(&left[(o + half + row) * kPad + lo_ + l]);
+        const float4 a1 = *reinterpret_cast<const float4*>(&left[(o + half + row + 1) * kPad + lo_ + l]);
+        const float x0[4] = {a0.x, a0.y, a0.z, a0.w}, x1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-    for (int r = 0; r < 8; ++r) acc[r] = 0.f;
-    for (int l = 0; l < half; ++l) {
-      const float nv = s_n[(o + l) * kPad + o + col];
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < per) acc[r] = fmaf(s_a[(o + half + row + r) * kPad + o + l], nv, acc[r]);
+        for (int q = 0; q < 4; ++q) {
+          const float4 y = *reinterpret_cast<const float4*>(&right[(ro + l + q) * kPad + o + col]);
+          r0.x = fmaf(x0[q], y.x, r0.x);
+          r0.y = fmaf(x0[q], y.y, r0.y);
+          r0.z = fmaf(x0[q], y.z, r0.z);
+          r0.w = fmaf(x0[q], y.w, r0.w);
+          r1.x = fmaf(x1[q], y.x, r1.x);
+          r1.y = fmaf(x1[q], y.y, r1.y);
+          r1.z = fmaf(x1[q], y.z, r1.z);
+          r1.w = fmaf(x1[q], y.w, r1.w);
+        }
+      }
+    };
+    // C B' over C, then -D' (C B') into the inverse
+    if (on) product(s_a, s_n, o, o);
+    __syncthreads();
+    if (on) {
+      *reinterpret_cast<float4*>(&s_a[(o + half + row) * kPad + o + col]) = r0;
+      *reinterpret_cast<float4*>(&s_a[(o + half + row + 1) * kPad + o + col]) = r1;
     }
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < per) s_t[(o + half + row + r) * kPad + o + col] = acc[r];
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 8; ++r) acc[r] = 0.f;
-    for (int l = 0; l < half; ++l) {
-      const float tv = s_t[(o + half + l) * kPad + o + col];
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < per) acc[r] = fmaf(-s_n[(o + half + row + r) * kPad + o + half + l], tv, acc[r]);
+    if (on) {
+      product(s_n, s_a, o + half, o + half);
+      *reinterpret_cast<float4*>(&s_n[(o + half + row) * kPad + o + col]) =
+          make_float4(-r0.x, -r0.y, -r0.z, -r0.w);
+      *reinterpret_cast<float4*>(&s_n[(o + half + row + 1) * kPad + o + col]) =
+          make_float4(-r1.x, -r1.y, -r1.z, -r1.w);
     }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < per) s_n[(o + half + row + r) * kPad + o + col] = acc[r];
     __syncthreads();
   }
 
+  const int64_t mat = (bh * p.chunks + chunk) * NS * (kChunk * kChunk);
   for (int s = tid; s < kChunk * kChunk / 8; s += kPrepThreads) {
     const int i = s / (kChunk / 8), j0 = (s % (kChunk / 8)) * 8;
+    const float4 x = *reinterpret_cast<const float4*>(&s_n[i * kPad + j0]);
+    const float4 y = *reinterpret_cast<const float4*>(&s_n[i * kPad + j0 + 4]);
     uint32_t w[4][NS];
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      split_pair<NS>(s_n[i * kPad + j0 + 2 * c], s_n[i * kPad + j0 + 2 * c + 1], w[c]);
+    split_pair<NS>(x.x, x.y, w[0]);
+    split_pair<NS>(x.z, x.w, w[1]);
+    split_pair<NS>(y.x, y.y, w[2]);
+    split_pair<NS>(y.z, y.w, w[3]);
 #pragma unroll
     for (int q = 0; q < NS; ++q)
       *reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.n_mat + mat) +
-                                tile_at<kChunk * 2>(q * kMatBytes, i, j0 / 8)) =
+                                tile_at<MROW>(q * kMatBytes, i, j0 / 8)) =
           make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
   }
-  if (keeper) bulk_wait_all();
+  if (tid == 0) bulk_wait_all();
 }
 
 // ------------------------------------------------------------------ along the chunks
@@ -589,12 +635,13 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
         // and P would carry it to earlier tokens: it is taken out here and
         // put back into E, O and the state afterwards.
         int spoilt[2] = {kChunk, kChunk};  // first such token of the thread's two rows
-        float probe = 0.f;
+        float probe[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) probe = fmaf(X[n][e], 0.f, probe);
-        const bool bad = __any_sync(0xffffffffu, probe != 0.f);
+          for (int e = 0; e < 4; ++e) probe[e] = fmaf(X[n][e], 0.f, probe[e]);
+        const bool bad =
+            __any_sync(0xffffffffu, (probe[0] + probe[1]) + (probe[2] + probe[3]) != 0.f);
         if (bad) {
 #pragma unroll
           for (int n = 0; n < 8; ++n)
@@ -932,9 +979,10 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   pp.dk = (int)a.dk;
   pp.scale = a.scale;
   auto prep = delta_prep_kernel<T, NP, LV, DKP>;
-  cudaError_t e = configure(prep, prep_smem<NP, DKP>());
+  constexpr int prep_smem = PrepCfg<NP, LV + 1, DKP>::kSmem;
+  cudaError_t e = configure(prep, prep_smem);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(prep, (unsigned)(bh * pl.chunks), kPrepThreads, prep_smem<NP, DKP>(), a.stream, pp);
+  e = launch_pdl(prep, (unsigned)(bh * pl.chunks), kPrepThreads, prep_smem, a.stream, pp);
   if (e != cudaSuccess) return e;
 
   ScanParams p{};
