@@ -137,6 +137,26 @@ __device__ __forceinline__ uint32_t at_at(uint32_t base, int lane, int m0, int k
   return tile_at<ROWB>(base, kk * 16 + (m >> 1) * 8 + r, m0 / 8 + (m & 1));
 }
 
+// The parts of the state are kept as two half tiles of dk / 2 columns, one
+// for each chain warp of a strip: rows of DKP bytes (128 or 64).
+template <int DKP>
+__device__ __forceinline__ uint32_t half_at(uint32_t base, int row, int unit) {
+  return DKP == 128 ? base + row * 128 + ((unit ^ (row & 7)) << 4)
+                    : base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+}
+// A operand, 16 rows, columns 16 kk.. of the half.
+template <int DKP>
+__device__ __forceinline__ uint32_t half_a(uint32_t base, int lane, int kk) {
+  const int m = lane >> 3, r = lane & 7;
+  return half_at<DKP>(base, (m & 1) * 8 + r, kk * 2 + (m >> 1));
+}
+// B operand (transposing load): k = rows 0..15, columns n0..n0+15 of the half.
+template <int DKP>
+__device__ __forceinline__ uint32_t half_bt(uint32_t base, int lane, int n0) {
+  const int m = lane >> 3, r = lane & 7;
+  return half_at<DKP>(base, (m & 1) * 8 + r, n0 / 8 + (m >> 1));
+}
+
 // Strips: 64 tokens x 16 values, rows of 16 values (32 bytes; fp32 64).  A
 // warp's 16 rows of the transposed state meet one strip of v, E, dO or dV.
 // Units are exchanged so that 8 rows of one unit column again fall on 8
@@ -185,6 +205,19 @@ __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
                : "memory");
+}
+
+// An accumulator tile, a 16-byte vector per lane.
+__device__ __forceinline__ void sts_acc(uint32_t addr, const float (&c)[4]) {
+  sts128(addr, make_uint4(__float_as_uint(c[0]), __float_as_uint(c[1]), __float_as_uint(c[2]),
+                          __float_as_uint(c[3])));
+}
+__device__ __forceinline__ void lds_acc(uint32_t addr, float (&c)[4]) {
+  const uint4 v = lds128(addr);
+  c[0] = __uint_as_float(v.x);
+  c[1] = __uint_as_float(v.y);
+  c[2] = __uint_as_float(v.z);
+  c[3] = __uint_as_float(v.w);
 }
 
 // ---------------------------------------------------------------- bf16 parts

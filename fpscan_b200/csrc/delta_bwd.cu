@@ -85,10 +85,10 @@ struct RevParams {
   float scale;
 };
 
-// As in delta_scan_kernel a warp owns 16 rows of dS^T, and its work is shared
-// by two: the helper warp computes what does not need dS -- Z = P^T dO and
-// the sum (scale exp(G) dO)^T Q that joins the state -- and leaves both in
-// shared memory; the chain warp does the rest.  K, N are loaded by the first
+// As in delta_scan_kernel 16 rows of dS^T are shared by three warps: two
+// chain warps with half of dk each, and a helper that computes what does not
+// need dS -- Z = P^T dO and the sum (scale exp(G) dO)^T Q that joins the
+// state -- and leaves both in shared memory.  K, N are loaded by the first
 // chain warp, Q, P by the first helper.
 template <int NP, int LV, int DKP, int NW>
 struct RevCfg {
@@ -96,25 +96,27 @@ struct RevCfg {
   static constexpr int kTileK = kChunk * DKP * 2;
   static constexpr int kMat = kChunk * kChunk * 2;
   static constexpr int oN = NP * kTileK, oVec = oN + NS * kMat;
-  static constexpr int kStageK = oVec + 1024;
+  static constexpr int kStageK = oVec + 3 * kChunk * 4;
   static constexpr int oP = NP * kTileK, oEnter = oP + NS * kMat;
   static constexpr int kStageQ = oEnter + 256;
-  static constexpr int kG = NP * kStrip;
-  static constexpr int kXS = NS * 16 * DKP * 2, kXV = NS * kStrip;
-  static constexpr int kZ = 8 * 512, kSum = DKP / 8 * 512;
-  static constexpr int kRoom = 227 * 1024 - 1536;
-  static constexpr int kBase = kXS + kXV + kZ + kSum;
-  static constexpr int kBufG = NW * (kBase + 2 * kG) + kStageK + kStageQ <= kRoom ? 2 : 1;
+  // of a strip: dO once or twice; dS's parts; two halves of K dS^T, later dV;
+  // Z, later dV's parts; the sum that joins the state
+  static constexpr int kG = NP * kStrip, kXS = NS * 16 * DKP * 2, kHalf = 8 * 512;
+  static constexpr int kZ = NS * kStrip > 8 * 512 ? NS * kStrip : 8 * 512, kSum = DKP / 8 * 512;
+  static constexpr int kRoom = 227 * 1024 - 1280;
+  static constexpr int kBase = kXS + 2 * kHalf + kZ + kSum;
+  // two stages of K, N come first, then two of dO, then two of Q, P
+  static constexpr int kStK = NW * (kBase + kG) + 2 * kStageK + kStageQ <= kRoom ? 2 : 1;
+  static constexpr int kBufG = NW * (kBase + 2 * kG) + kStK * kStageK + kStageQ <= kRoom ? 2 : 1;
   static constexpr int kWarp = kBufG * kG + kBase;
-  static constexpr int kStK = NW * kWarp + 2 * kStageK + kStageQ <= kRoom ? 2 : 1;
   static constexpr int kStQ = NW * kWarp + kStK * kStageK + 2 * kStageQ <= kRoom ? 2 : 1;
   static constexpr int oQ = kStK * kStageK, oWarp = oQ + kStQ * kStageQ;
   static constexpr int kSmem = oWarp + NW * kWarp + 128;
-  static constexpr bool kFits = kSmem + 1024 <= 227 * 1024;
+  static constexpr bool kFits = kSmem + 1152 <= 227 * 1024;
 };
 
 template <typename T, int NP, int LV, int DKP, int NW>
-__global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p) {
+__global__ void __launch_bounds__(NW * 96, 1) delta_rev_kernel(const RevParams p) {
   using Cfg = RevCfg<NP, LV, DKP, NW>;
   static_assert(Cfg::kFits);
   constexpr int NS = Cfg::NS, ROWB = DKP * 2, NT = DKP / 8, MROW = kChunk * 2;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
       (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
   const uint32_t sm0 = smem_addr(dsm);
   __shared__ __align__(8) uint64_t full_k[2], free_k[2], full_q[2], free_q[2];
-  __shared__ __align__(8) uint64_t full_z[NW], free_z[NW], full_g[NW], free_g[NW];
+  __shared__ __align__(8) uint64_t full_z[NW], free_z[NW], full_g[NW], free_g[NW], pair[NW];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g4 = lane >> 2, t4 = lane & 3;
@@ -136,15 +138,16 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&full_k[i], 1);
-      mbar_init(&free_k[i], nact);
+      mbar_init(&free_k[i], 2 * nact);
       mbar_init(&full_q[i], 1);
       mbar_init(&free_q[i], nact);
     }
     for (int i = 0; i < NW; ++i) {
       mbar_init(&full_z[i], 1);
-      mbar_init(&free_z[i], 1);
+      mbar_init(&free_z[i], 2);
       mbar_init(&full_g[i], 1);
-      mbar_init(&free_g[i], 1);
+      mbar_init(&free_g[i], 2);
+      mbar_init(&pair[i], 2);
     }
     fence_mbar_init();
   }
@@ -152,13 +155,14 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
   pdl_wait();
   pdl_launch_dependents();
 
-  const int w = warp < NW ? warp : warp - NW;
+  const int w = warp < 2 * NW ? warp >> 1 : warp - 2 * NW;  // strip
+  const int side = warp & 1;                                // chain: half of dk
   const int dv0 = dv_cta + w * 16, nval = p.dv - dv0;
-  const int strips = (p.dv + 15) / 16, dvp = strips * 16;
+  const int strips = (p.dv + 15) / 16;
   const int64_t unit0 = bh * p.chunks, tile = (b * p.key_heads + hk) * p.chunks;
   const int64_t vstride = (int64_t)p.heads * p.dv;
   const uint32_t own = sm0 + Cfg::oWarp + w * Cfg::kWarp;
-  const uint32_t x_s = own + Cfg::kBufG * Cfg::kG, x_v = x_s + Cfg::kXS, x_z = x_v + Cfg::kXV,
+  const uint32_t x_s = own + Cfg::kBufG * Cfg::kG, x_h = x_s + Cfg::kXS, x_z = x_h + 2 * Cfg::kHalf,
                  x_g = x_z + Cfg::kZ;
   // step d handles chunk chunks - 1 - d
   int64_t next = 0;  // steps issued by this loading lane
@@ -189,19 +193,26 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
     return true;
   };
 
-  if (warp < NW && nval > 0) {
+  if (warp < 2 * NW && nval > 0) {
     // ---------------------------------------------------------- chain
-    const bool loads = w == 0 && lane == 0;
+    constexpr int HT = NT / 2;  // tiles of this half
+    const int d0 = side * (DKP / 2);
+    const bool loads = warp == 0 && lane == 0;
+    // dV's tiles, as E's in delta_scan_kernel
+    auto e_at = [&](int n) {
+      const int blk = n >> 1, of = blk == 0 || blk == 3 ? 0 : 1;
+      return x_h + (1 - of) * Cfg::kHalf + ((blk >> 1) * 2 + (n & 1)) * 512 + lane * 16;
+    };
     if (loads)
       while (next < min((int64_t)Cfg::kStK, p.chunks)) issue_k();
     __syncwarp();
-    float S[NT][4];  // dS^T
+    float S[HT][4];  // dS^T
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < HT; ++n) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
       if (p.grad_final != nullptr) {
-        const int dk = n * 8 + 2 * t4;
+        const int dk = d0 + n * 8 + 2 * t4;
         const float* src = p.grad_final + (bh * p.dv + dv0 + g4) * p.dk + dk;
         if (dk < p.dk) {
           const float2 v = *reinterpret_cast<const float2*>(src);
@@ -224,29 +235,28 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
       const float* enter = vec + kVecEnter * kChunk;
       const float* leave = vec + kVecLeave * kChunk;
       const float* beta = vec + kVecBeta * kChunk;
-      if (Cfg::kStK == 1 && d > 0) {  // one stage: the load waits for every chain warp
-        if (loads) ok = issue_k();
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_k[sk], (uint32_t)((d / Cfg::kStK) & 1)));
+      // one stage: the load waits for every chain warp
+      if (Cfg::kStK == 1 && d > 0 && loads) ok = issue_k();
+      ok = ok && mbar_wait_bounded(&full_k[sk], (uint32_t)((d / Cfg::kStK) & 1));
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      if (d > 0 && lane == 0) bulk_wait_read<1>();
-      __syncwarp();
       const float total = enter[kChunk - 1];
 
-      // Y = (K dS^T)^T: 16 values x 64 tokens.  dS's parts are kept.
+      // Y = (K dS^T)^T: 16 values x 64 tokens, this half of dk.  dS's parts
+      // are kept.
       float Y[8][4];
 #pragma unroll
       for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) Y[n][e] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < DKP / 16; ++kk) {
+      for (int k2 = 0; k2 < HT / 2; ++k2) {
+        const int kk = side * (HT / 2) + k2;
         uint32_t a[NS][4];
-        split_frag<NS>(S[2 * kk], S[2 * kk + 1], a);
+        split_frag<NS>(S[2 * k2], S[2 * k2 + 1], a);
 #pragma unroll
-        for (int q = 0; q < NS; ++q) stsm4(at_a<ROWB>(x_s + q * 16 * ROWB, lane, 0, kk), a[q]);
+        for (int q = 0; q < NS; ++q)
+          stsm4(half_a<DKP>(x_s + (side * NS + q) * 16 * DKP, lane, k2), a[q]);
 #pragma unroll
         for (int n2 = 0; n2 < 4; ++n2) {
           Step<LV == 2, 2> s;
@@ -264,17 +274,19 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
           s.add(1, Y[2 * n2 + 1]);
         }
       }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) sts_acc(x_h + side * Cfg::kHalf + n * 512 + lane * 16, Y[n]);
       fence_async();
       __syncwarp();
       if (lane == 0) {
-        __nv_bfloat16* sp = p.ds_parts + ((unit0 + c) * NS * dvp + dv0) * DKP;
-#pragma unroll
-        for (int q = 0; q < NS; ++q)
-          bulk_s2g(sp + (int64_t)q * dvp * DKP, x_s + q * 16 * ROWB, 16 * ROWB);
+        bulk_s2g(p.ds_parts + (((unit0 + c) * strips + dv0 / 16) * 2 + side) * NS * 8 * DKP,
+                 x_s + side * NS * 16 * DKP, NS * 16 * DKP);
         bulk_commit();
+        mbar_arrive(&pair[w]);
       }
       // the stage of the chunk before is free by now
       if (Cfg::kStK == 2 && loads && d > 0 && next < p.chunks) ok = issue_k();
+      ok = ok && mbar_wait_bounded(&pair[w], 0);
       ok = ok && mbar_wait_bounded(&full_z[w], (uint32_t)(d & 1));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -285,27 +297,27 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
         const int tok = n * 8 + 2 * t4;
         const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
         const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
-        const uint4 z = lds128(x_z + n * 512 + lane * 16);
+        float z[4], y[4];
+        lds_acc(x_z + n * 512 + lane * 16, z);
+        lds_acc(x_h + (1 - side) * Cfg::kHalf + n * 512 + lane * 16, y);
         const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
-        Y[n][0] = fmaf(w0, Y[n][0], __uint_as_float(z.x));
-        Y[n][1] = fmaf(w1, Y[n][1], __uint_as_float(z.y));
-        Y[n][2] = fmaf(w0, Y[n][2], __uint_as_float(z.z));
-        Y[n][3] = fmaf(w1, Y[n][3], __uint_as_float(z.w));
+        Y[n][0] = fmaf(w0, Y[n][0] + y[0], z[0]);
+        Y[n][1] = fmaf(w1, Y[n][1] + y[1], z[1]);
+        Y[n][2] = fmaf(w0, Y[n][2] + y[2], z[2]);
+        Y[n][3] = fmaf(w1, Y[n][3] + y[3], z[3]);
       }
-      warp_arrive(&free_z[w], lane);
 
-      // dV = N^T F
-      float V[8][4];
+      // dV = N^T F, this side's blocks of tokens: 0, 3 or 1, 2
+      float V[4][4];
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) V[n][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         uint32_t a[NS][4];
         split_frag<NS>(Y[2 * kk], Y[2 * kk + 1], a);
-#pragma unroll
-        for (int n2 = 0; n2 <= kk; ++n2) {
+        auto block = [&](int n2, float (&v0)[4], float (&v1)[4]) {
           Step<LV == 2, 2> s;
 #pragma unroll
           for (int i = LV; i >= 0; --i) {
@@ -313,83 +325,105 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
             ldsm4_t(nb, at_bt<MROW>(st + Cfg::oN + i * Cfg::kMat, lane, n2 * 16, kk));
 #pragma unroll
             for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, V[2 * n2], a[j], nb[0], nb[1]);
-              s.mma(1, V[2 * n2 + 1], a[j], nb[2], nb[3]);
+              s.mma(0, v0, a[j], nb[0], nb[1]);
+              s.mma(1, v1, a[j], nb[2], nb[3]);
             }
           }
-          s.add(0, V[2 * n2]);
-          s.add(1, V[2 * n2 + 1]);
-        }
+          s.add(0, v0);
+          s.add(1, v1);
+        };
+        if (kk >= side) block(side, V[0], V[1]);
+        if (kk >= 3 - side) block(3 - side, V[2], V[3]);
       }
-      if (lane == 0) bulk_wait_read<1>();
-      __syncwarp();
+      // dV's tiles go to the other side; its parts, over Z once both sides
+      // have read that, are kept
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
+      for (int i = 0; i < 2; ++i) {
+        const int n2 = i == 0 ? side : 3 - side;
+        sts_acc(e_at(2 * n2), V[2 * i]);
+        sts_acc(e_at(2 * n2 + 1), V[2 * i + 1]);
+      }
+      warp_arrive(&pair[w], lane);
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pair[w], 1));
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n2 = i == 0 ? side : 3 - side;
         uint32_t a[NS][4];
-        split_frag<NS>(V[2 * kk], V[2 * kk + 1], a);
+        split_frag<NS>(V[2 * i], V[2 * i + 1], a);
 #pragma unroll
-        for (int q = 0; q < NS; ++q) stsm4_t(strip_at_t(x_v + q * kStrip, lane, kk), a[q]);
+        for (int q = 0; q < NS; ++q) stsm4_t(strip_at_t(x_z + q * kStrip, lane, n2), a[q]);
       }
       fence_async();
       __syncwarp();
       if (lane == 0) {
-        bulk_s2g(p.dv_parts + ((unit0 + c) * strips + dv0 / 16) * NS * (kStrip / 2), x_v, NS * kStrip);
+        __nv_bfloat16* vp = p.dv_parts + ((unit0 + c) * strips + dv0 / 16) * NS * (kStrip / 2);
+#pragma unroll
+        for (int q = 0; q < NS; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n2 = i == 0 ? side : 3 - side;  // 16 rows of 32 bytes
+            bulk_s2g(vp + q * (kStrip / 2) + n2 * 256, x_z + q * kStrip + n2 * 512, 512);
+          }
         bulk_commit();
       }
       {
         const int64_t t0 = c * kChunk;
         const int rows = (int)min((int64_t)kChunk, p.L - t0);
         T* out = static_cast<T*>(p.dv_out) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0;
-        if constexpr (NP == 1) {  // the first bf16 part is the rounded value
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = i * 16 + (lane >> 1), un = lane & 1;
+        for (int i = 0; i < 2; ++i) {
+          const int n2 = i == 0 ? side : 3 - side;
+          if constexpr (NP == 1) {  // the first bf16 part is the rounded value
+            const int r = n2 * 16 + (lane >> 1), un = lane & 1;
             if (r < rows && un * 8 < nval)
-              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_v, r, un));
-          }
-        } else {
+              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_z, r, un));
+          } else {
 #pragma unroll
-          for (int n = 0; n < 8; ++n)
-            store_t<T>(out + (int64_t)n * 8 * vstride, vstride, V[n], lane, rows - n * 8, nval);
+            for (int n = 0; n < 2; ++n)
+              store_t<T>(out + (int64_t)(n2 * 16 + n * 8) * vstride, vstride, V[2 * i + n], lane,
+                         rows - n2 * 16 - n * 8, nval);
+          }
         }
       }
 
-      // dS <- exp(G_C) dS + (scale exp(G) dO)^T Q - (exp(G) dV)^T K
+      // dS <- exp(G_C) dS + (scale exp(G) dO)^T Q - (exp(G) dV)^T K, this half
       uint32_t uv[4][NS][4];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
+        float f[2][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int n = 2 * kk + half;
           const float2 ge = *reinterpret_cast<const float2*>(enter + n * 8 + 2 * t4);
-          V[n][0] *= -ge.x;
-          V[n][1] *= -ge.y;
-          V[n][2] *= -ge.x;
-          V[n][3] *= -ge.y;
+          if ((kk == side) | (kk == 3 - side)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[half][e] = V[(kk >> 1) * 2 + half][e];
+          } else {
+            lds_acc(e_at(n), f[half]);
+          }
+          f[half][0] *= -ge.x;
+          f[half][1] *= -ge.y;
+          f[half][2] *= -ge.x;
+          f[half][3] *= -ge.y;
         }
-        split_frag<NS>(V[2 * kk], V[2 * kk + 1], uv[kk]);
+        split_frag<NS>(f[0], f[1], uv[kk]);
       }
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_g[w], (uint32_t)(d & 1)));
       if (!ok) break;
 #pragma unroll
-      for (int n4 = 0; n4 < NT / 4; ++n4) {
+      for (int n4 = 0; n4 < HT / 4; ++n4) {
         float x[4][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint4 g = lds128(x_g + (n4 * 4 + n) * 512 + lane * 16);
-          x[n][0] = __uint_as_float(g.x);
-          x[n][1] = __uint_as_float(g.y);
-          x[n][2] = __uint_as_float(g.z);
-          x[n][3] = __uint_as_float(g.w);
-        }
+        for (int n = 0; n < 4; ++n) lds_acc(x_g + (side * HT + n4 * 4 + n) * 512 + lane * 16, x[n]);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           Step<LV == 2, 4> s;
 #pragma unroll
           for (int i = NP - 1; i >= 0; --i) {
             uint32_t b0[4], b1[4];
-            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
-            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
+            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, d0 + n4 * 32, kk));
+            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, d0 + n4 * 32 + 16, kk));
 #pragma unroll
             for (int j = LV - i; j >= 0; --j) {
               s.mma(0, x[0], uv[kk][j], b0[0], b0[1]);
@@ -406,8 +440,10 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
 #pragma unroll
           for (int e = 0; e < 4; ++e) S[n4 * 4 + n][e] = fmaf(total, S[n4 * 4 + n][e], x[n][e]);
       }
+      if (lane == 0) bulk_wait_read<0>();  // dS's and dV's parts: Z may come again
       __syncwarp();
       if (lane == 0) {
+        mbar_arrive(&free_z[w]);
         mbar_arrive(&free_g[w]);
         mbar_arrive(&free_k[sk]);
       }
@@ -418,8 +454,8 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
         mbar_wait_bounded(&full_k[j % Cfg::kStK], (uint32_t)((j / Cfg::kStK) & 1));
     if (ok && p.dinitial != nullptr) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int dk = n * 8 + 2 * t4;
+      for (int n = 0; n < HT; ++n) {
+        const int dk = d0 + n * 8 + 2 * t4;
         float* dst = p.dinitial + (bh * p.dv + dv0 + g4) * p.dk + dk;
         if (dk < p.dk) {
           *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
@@ -427,7 +463,7 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
         }
       }
     }
-  } else if (warp >= NW && nval > 0) {
+  } else if (warp >= 2 * NW && nval > 0) {
     // ---------------------------------------------------------- helper
     const bool loads = w == 0 && lane == 0;
     if (loads)
@@ -465,9 +501,7 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
         bulk_s2g(p.do_parts + ((unit0 + c) * strips + dv0 / 16) * NP * (kStrip / 2), gst, NP * kStrip);
         bulk_commit();
       }
-      ok = mbar_wait_bounded(&full_q[sq], (uint32_t)((d / Cfg::kStQ) & 1));
-      if (d > 0) ok = ok && mbar_wait_bounded(&free_z[w], (uint32_t)((d - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_q[sq], (uint32_t)((d / Cfg::kStQ) & 1)));
       if (!ok) break;
       float Z[8][4];
 #pragma unroll
@@ -512,11 +546,11 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
           for (int q = 0; q < NS; ++q) ug[kk][q][r] = parts[q];
         }
       }
+      if (d > 0) ok = mbar_wait_bounded(&free_z[w], (uint32_t)((d - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
-        sts128(x_z + n * 512 + lane * 16,
-               make_uint4(__float_as_uint(Z[n][0]), __float_as_uint(Z[n][1]),
-                          __float_as_uint(Z[n][2]), __float_as_uint(Z[n][3])));
+      for (int n = 0; n < 8; ++n) sts_acc(x_z + n * 512 + lane * 16, Z[n]);
       warp_arrive(&full_z[w], lane);
       if (d > 0) ok = mbar_wait_bounded(&free_g[w], (uint32_t)((d - 1) & 1));
       ok = __all_sync(0xffffffffu, ok);
@@ -548,10 +582,7 @@ __global__ void __launch_bounds__(NW * 64, 1) delta_rev_kernel(const RevParams p
           for (int n = 0; n < 4; ++n) s.add(n, x[n]);
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-          sts128(x_g + (n4 * 4 + n) * 512 + lane * 16,
-                 make_uint4(__float_as_uint(x[n][0]), __float_as_uint(x[n][1]),
-                            __float_as_uint(x[n][2]), __float_as_uint(x[n][3])));
+        for (int n = 0; n < 4; ++n) sts_acc(x_g + (n4 * 4 + n) * 512 + lane * 16, x[n]);
       }
       __syncwarp();
       if (lane == 0) {
@@ -655,7 +686,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   constexpr int kLoader = 3 * 32;
   const int above = warp < 4 ? warp - 1 : warp < 8 ? warp - 3 : 5;  // 0..5 among those
   const int64_t kstride = (int64_t)p.key_heads * p.dk;
-  const int strips = (p.dv + 15) / 16, dvp = strips * 16, slices = (strips + KS - 1) / KS;
+  const int strips = (p.dv + 15) / 16, slices = (strips + KS - 1) / KS;
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
@@ -684,12 +715,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     bulk_in(at, p.do_parts + (unit * strips + v0) * NP * (kStrip / 2), n * NP * kStrip, &full[s]);
     bulk_in(at + Cfg::oV, p.dv_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
     bulk_in(at + Cfg::oE, p.e_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int64_t sv = ((unit * NS + i) * dvp + v0 * 16) * DKP;
-      bulk_in(at + Cfg::oS + i * KS * Cfg::kRows, p.s_parts + sv, n * Cfg::kRows, &full[s]);
-      bulk_in(at + Cfg::oD + i * KS * Cfg::kRows, p.ds_parts + sv, n * Cfg::kRows, &full[s]);
-    }
+    const int64_t sv = (unit * strips + v0) * NS * 16 * DKP;
+    bulk_in(at + Cfg::oS, p.s_parts + sv, n * NS * Cfg::kRows, &full[s]);
+    bulk_in(at + Cfg::oD, p.ds_parts + sv, n * NS * Cfg::kRows, &full[s]);
     ++next;
     if (++next_slice == slices) {
       next_slice = 0;
@@ -741,6 +769,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       for (int kk = 0; kk < n; ++kk) {
         const uint32_t a_g = at + kk * NP * kStrip, a_v = at + Cfg::oV + kk * NS * kStrip,
                        a_e = at + Cfg::oE + kk * NS * kStrip;
+        // this warp's half of dk in the strip's S0 and dS (plus oS, oD)
+        const uint32_t s_half = at + (kk * 2 + col0 / (DKP / 2)) * NS * 16 * DKP;
         if (lower) {
           uint32_t ag[NP][4], av[NS][4];
 #pragma unroll
@@ -771,7 +801,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           uint32_t sb[NS][4];
 #pragma unroll
           for (int j = 0; j < NS; ++j)
-            ldsm4_t(sb[j], at_bt<ROWB>(at + Cfg::oS + j * KS * Cfg::kRows, lane, col0, kk));
+            ldsm4_t(sb[j], half_bt<DKP>(s_half + Cfg::oS + j * 16 * DKP, lane, col0 % (DKP / 2)));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             uint32_t ag[NP][4], av[NS][4];
@@ -801,7 +831,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           uint32_t db[NS][4];
 #pragma unroll
           for (int j = 0; j < NS; ++j)
-            ldsm4_t(db[j], at_bt<ROWB>(at + Cfg::oD + j * KS * Cfg::kRows, lane, col0, kk));
+            ldsm4_t(db[j], half_bt<DKP>(s_half + Cfg::oD + j * 16 * DKP, lane, col0 % (DKP / 2)));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             uint32_t ae[NS][4];
@@ -823,10 +853,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       // <S0, dS> over this slice (the same place of every part: swizzle does not matter)
       for (int i = above * 32 + lane; !lower && i < n * Cfg::kRows / 16; i += 6 * 32) {
         float x[8] = {}, y[8] = {};
+        // 16-byte piece i % DKP of half i / DKP (16 rows of DKP bytes)
+        const uint32_t at_i = at + i / DKP * NS * 16 * DKP + i % DKP * 16;
 #pragma unroll
         for (int q = NS - 1; q >= 0; --q) {
-          const uint4 u = lds128(at + Cfg::oS + q * KS * Cfg::kRows + i * 16);
-          const uint4 v = lds128(at + Cfg::oD + q * KS * Cfg::kRows + i * 16);
+          const uint4 u = lds128(at_i + Cfg::oS + q * 16 * DKP);
+          const uint4 v = lds128(at_i + Cfg::oD + q * 16 * DKP);
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -1144,7 +1176,7 @@ cudaError_t rev_nw(const DeltaArgs& a, RevParams& p, int64_t bh) {
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
   p.slices = (int)((a.dv + NW * 16 - 1) / (NW * 16));
-  return launch_pdl(kern, (unsigned)(bh * p.slices), NW * 64, Cfg::kSmem, a.stream, p);
+  return launch_pdl(kern, (unsigned)(bh * p.slices), NW * 96, Cfg::kSmem, a.stream, p);
 }
 
 template <typename T, int LV, int DKP>

@@ -16,16 +16,16 @@
 // chunk needs no barrier between its products.  Columns of the state never
 // mix, so a head is cut along dv over as many CTAs as the GPU has room for.
 //
-// One warp alone issues about every third cycle (its products wait for one
-// another), so the work of a chunk is shared by two kinds of warps:
-//   chain warps   R, E and the state;
-//   output warps  one for each chain warp: O = scale exp(G) Q S0^T + P E,
-//                 from the parts of S0 and E that the chain warp leaves in
-//                 shared memory, while that goes on to the update and the
-//                 next chunk.
+// A chunk's products wait for one another, and one warp alone issues only
+// about every sixth cycle, so the 16 rows are shared by three warps:
+//   two chain warps  each with half of dk: their parts of K S0^T are summed
+//                    through shared memory, each computes E for half of the
+//                    tokens, and each updates its half of the state;
+//   an output warp   O = scale exp(G) Q S0^T + P E, from the parts of S0 and
+//                    from E in shared memory, while the chain goes on to the
+//                    update and the next chunk.
 // K, N (chain) and Q, P (output) come by bulk copies through a ring of one or
-// two stages each, issued by the first output warp after each of its chunks
-// (a ninth warp for it would cost every thread a third of its registers).
+// two stages each, issued by the first chain and the first output warp.
 // Where the states and E are kept for the backward pass there is no output,
 // and one more warp loads.
 #include <algorithm>
@@ -376,7 +376,7 @@ struct ScanParams {
   float* final_state;
   void* out;                  // KEEP false
   __nv_bfloat16* e_parts;     // KEEP true: strips [head][chunk][dv / 16][NS], as in shared memory
-  __nv_bfloat16* s_parts;     //            [head][chunk][NS][dv padded to 16][DKP], too
+  __nv_bfloat16* s_parts;     // [head][chunk][dv / 16][half of dk][NS][16][DKP / 2]
   int64_t L, chunks;
   int key_heads, heads, dk, dv, slices;
   float scale;
@@ -389,21 +389,23 @@ struct ScanCfg {
   static constexpr int NS = LV + 1;
   // parts of S0 and E that leave the chain warps: outputs of 16 bits need two
   static constexpr int NO = KEEP ? NS : sizeof(T) == 4 ? 3 : 2;
-  static constexpr int kThreads = (KEEP ? NW + 1 : 2 * NW) * 32;
+  static constexpr int kThreads = (KEEP ? 2 * NW + 1 : 3 * NW) * 32;
   static constexpr int kTileK = kChunk * DKP * 2;
   static constexpr int oN = NP * kTileK, oVec = oN + NS * kMatBytes;
-  static constexpr int kStageK = oVec + 1024;            // enter, leave, beta: 768 bytes
+  static constexpr int kStageK = oVec + 3 * kChunk * 4;  // enter, leave, beta
   static constexpr int oP = NP * kTileK, oEnter = oP + NO * kMatBytes;
   static constexpr int kStageQ = KEEP ? 0 : oEnter + 256;
   static constexpr int kV = kChunk * 16 * (int)sizeof(T);
-  static constexpr int kXS = NO * 16 * DKP * 2, kXE = NO * kStrip;
-  static constexpr int kWarp = 2 * kV + kXS + kXE;       // a chain warp's own
-  static constexpr int kRoom = 227 * 1024 - 1536;        // barriers, alignment
+  // of a strip: v twice; S0's parts; two halves of K S0^T, later E; E's parts or O
+  static constexpr int kXS = NO * 16 * DKP * 2, kHalf = 8 * 512;
+  static constexpr int kXE = KEEP ? NS * kStrip : sizeof(T) == 2 ? kStrip : 0;  // else: O's
+  static constexpr int kWarp = 2 * kV + kXS + 2 * kHalf + kXE;
+  static constexpr int kRoom = 227 * 1024 - 1280;        // barriers, alignment
   static constexpr int kStK = NW * kWarp + 2 * kStageK + kStageQ <= kRoom ? 2 : 1;
   static constexpr int kStQ = KEEP ? 1 : NW * kWarp + kStK * kStageK + 2 * kStageQ <= kRoom ? 2 : 1;
   static constexpr int oQ = kStK * kStageK, oWarp = oQ + kStQ * kStageQ;
   static constexpr int kSmem = oWarp + NW * kWarp + 128;
-  static_assert(kStageK % 128 == 0 && kStageQ % 128 == 0 && kSmem + 1024 <= 227 * 1024);
+  static_assert(kStageK % 128 == 0 && kStageQ % 128 == 0 && kSmem + 1152 <= 227 * 1024);
 };
 
 template <typename T, int NP, int LV, int DKP, int NW, bool KEEP>
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
   // full: the copies of a stage have landed / the chain warp has written;
   // free: whoever reads a stage or a buffer is done with it
   __shared__ __align__(8) uint64_t full_k[2], free_k[2], full_q[2], free_q[2];
-  __shared__ __align__(8) uint64_t full_s[NW], free_s[NW], full_e[NW], free_e[NW];
+  __shared__ __align__(8) uint64_t full_s[NW], free_s[NW], full_e[NW], free_e[NW], pair[NW];
   __shared__ int s_bad[NW];
   __shared__ int s_spoilt[NW][16];
 
@@ -430,19 +432,20 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
   const int64_t b = bh / p.heads;
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
   const int dv_cta = slice * NW * 16;
-  const int nact = min(NW, (p.dv - dv_cta + 15) / 16);  // chain warps with values
+  const int nact = min(NW, (p.dv - dv_cta + 15) / 16);  // strips with values
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&full_k[i], 1);
-      mbar_init(&free_k[i], nact);
+      mbar_init(&free_k[i], 2 * nact);
       mbar_init(&full_q[i], 1);
       mbar_init(&free_q[i], nact);
     }
     for (int i = 0; i < NW; ++i) {
-      mbar_init(&full_s[i], 1);
+      mbar_init(&full_s[i], 2);
       mbar_init(&free_s[i], 1);
-      mbar_init(&full_e[i], 1);
+      mbar_init(&full_e[i], 2);
       mbar_init(&free_e[i], 1);
+      mbar_init(&pair[i], 2);
     }
     fence_mbar_init();
   }
@@ -487,47 +490,71 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
     for (int64_t j = max((int64_t)0, next_q - Cfg::kStQ); j < next_q; ++j)
       mbar_wait_bounded(&full_q[j % Cfg::kStQ], (uint32_t)((j / Cfg::kStQ) & 1));
   };
-  if (KEEP && warp == NW) {
+  if (KEEP && warp == 2 * NW) {
     // ---------------------------------------------------------- loader
     if (lane == 0) {
       bool ok = true;
       while (ok && next_k < p.chunks) ok = issue_k();
       if (!ok) drain();
     }
-  } else if (warp < NW) {
+  } else if (warp < 2 * NW) {
     // ---------------------------------------------------------- chain
-    const int dv0 = dv_cta + warp * 16;
-    const int nval = p.dv - dv0;  // values of this warp's 16 rows that exist (may be <= 0)
+    const int w = warp >> 1, side = warp & 1;  // strip, half of dk
+    const int dv0 = dv_cta + w * 16;
+    const int nval = p.dv - dv0;  // values of the strip's 16 rows that exist (may be <= 0)
     if (nval > 0) {
+      constexpr int HT = NT / 2;  // tiles of this half
+      const int d0 = side * (DKP / 2);
       const int64_t vstride = (int64_t)p.heads * p.dv;
-      const uint32_t own = sm0 + Cfg::oWarp + warp * Cfg::kWarp;
-      const uint32_t x_s = own + 2 * Cfg::kV, x_e = x_s + Cfg::kXS;
-      auto load_v = [&](int64_t c) {
-        const int64_t t0 = c * kChunk;
-        load_strip<T>(own + (int)(c & 1) * Cfg::kV,
-                      static_cast<const T*>(p.v) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0,
-                      vstride * (int)sizeof(T), (int)min((int64_t)kChunk, p.L - t0),
-                      min(16, nval) * (int)sizeof(T) / 16, lane);
+      const uint32_t own = sm0 + Cfg::oWarp + w * Cfg::kWarp;
+      const uint32_t x_s = own + 2 * Cfg::kV, x_h = x_s + Cfg::kXS, x_e = x_h + 2 * Cfg::kHalf;
+      // E's tiles: blocks of 16 tokens 0, 3 are side 0's, 1, 2 side 1's (five
+      // products of 16 x 16 blocks each).  A side leaves them where the other's
+      // half of K S0^T was, which only it has read; of the two sides only the
+      // other reads them (and writes there next).
+      auto e_at = [&](int n) {
+        const int blk = n >> 1, of = blk == 0 || blk == 3 ? 0 : 1;
+        return x_h + (1 - of) * Cfg::kHalf + ((blk >> 1) * 2 + (n & 1)) * 512 + lane * 16;
+      };
+      const char* v_next = reinterpret_cast<const char*>(static_cast<const T*>(p.v) +
+                                                         b * p.L * vstride + (int64_t)h * p.dv + dv0);
+      const int vunits = min(16, nval) * (int)sizeof(T) / 16;
+      const bool loads = warp == 0 && lane == 0;
+      if (!KEEP && loads)
+        while (next_k < min((int64_t)Cfg::kStK, p.chunks)) issue_k();
+      __syncwarp();
+      auto load_v = [&](int64_t c) {  // side s loads rows 32 s..
+        constexpr int U = (int)sizeof(T);
+        const int rows = (int)min((int64_t)kChunk, p.L - c * kChunk);
+        const uint32_t dst = own + (int)(c & 1) * Cfg::kV;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int r = side * 32 + (i * 32 + lane) / U, u = (i * 32 + lane) % U;
+          const bool in = r < rows && u < vunits;
+          cp16(U == 2 ? strip_at(dst, r, u) : strip32_at(dst, r, u),
+               in ? v_next + r * (vstride * (int)sizeof(T)) + u * 16 : v_next, in);
+        }
+        v_next += kChunk * vstride * (int)sizeof(T);
         cp_commit();
       };
       load_v(0);
 
-      float S[NT][4];
+      float S[HT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < HT; ++n) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
         if (p.initial != nullptr) {
-          const int dk = n * 8 + 2 * t4;
+          const int dk = d0 + n * 8 + 2 * t4;
           const float* src = p.initial + (bh * p.dv + dv0 + g4) * p.dk + dk;
           if (dk < p.dk) {
             const float2 v = *reinterpret_cast<const float2*>(src);
             S[n][0] = v.x;
             S[n][1] = v.y;
             if (nval > 8) {
-              const float2 w = *reinterpret_cast<const float2*>(src + 8 * p.dk);
-              S[n][2] = w.x;
-              S[n][3] = w.y;
+              const float2 y = *reinterpret_cast<const float2*>(src + 8 * p.dk);
+              S[n][2] = y.x;
+              S[n][3] = y.y;
             }
           }
         }
@@ -541,33 +568,36 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
         const float* enter = vec + kVecEnter * kChunk;
         const float* leave = vec + kVecLeave * kChunk;
         const float* beta = vec + kVecBeta * kChunk;
-        if (c + 1 < p.chunks) {
-          load_v(c + 1);
-          cp_wait<1>();
-        } else {
-          cp_wait<0>();
+        // one stage: the load waits for every chain warp
+        if (!KEEP && Cfg::kStK == 1 && c > 0 && loads) ok = issue_k();
+        ok = ok && mbar_wait_bounded(&full_k[sk], (uint32_t)((c / Cfg::kStK) & 1));
+        if (!KEEP && c > 0) {
+          ok = ok && mbar_wait_bounded(&free_s[w], (uint32_t)((c - 1) & 1));
+          ok = ok && mbar_wait_bounded(&free_e[w], (uint32_t)((c - 1) & 1));
         }
-        ok = mbar_wait_bounded(&full_k[sk], (uint32_t)((c / Cfg::kStK) & 1));
-        if (!KEEP && c > 0) ok = ok && mbar_wait_bounded(&free_s[warp], (uint32_t)((c - 1) & 1));
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (KEEP && c > 0 && lane == 0) bulk_wait_read<1>();
-        __syncwarp();
         const float total = enter[kChunk - 1];
+        if (KEEP) {  // S0's parts of the chunk before have been read
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+        }
 
-        // X = (K S0^T)^T: 16 values x 64 tokens.  S0's parts go to shared memory.
+        // X = (K S0^T)^T: 16 values x 64 tokens, this half of dk.  S0's parts
+        // go to shared memory.
         float X[8][4];
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) X[n][e] = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < DKP / 16; ++kk) {
+        for (int k2 = 0; k2 < HT / 2; ++k2) {
+          const int kk = side * (HT / 2) + k2;
           uint32_t a[NS][4];
-          split_frag<NS>(S[2 * kk], S[2 * kk + 1], a);
+          split_frag<NS>(S[2 * k2], S[2 * k2 + 1], a);
 #pragma unroll
           for (int q = 0; q < NO; ++q)
-            stsm4(at_a<ROWB>(x_s + q * 16 * ROWB, lane, 0, kk), a[q]);
+            stsm4(half_a<DKP>(x_s + (side * NO + q) * 16 * DKP, lane, k2), a[q]);
 #pragma unroll
           for (int n2 = 0; n2 < 4; ++n2) {
             Step<LV == 2, 2> s;
@@ -585,22 +615,27 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
             s.add(1, X[2 * n2 + 1]);
           }
         }
-        if (KEEP) {
-          fence_async();
-          __syncwarp();
-          if (lane == 0) {
-            const int64_t dvp = (p.dv + 15) / 16 * 16;
-            __nv_bfloat16* sp = p.s_parts + ((unit0 + c) * NS * dvp + dv0) * DKP;
 #pragma unroll
-            for (int q = 0; q < NS; ++q)
-              bulk_s2g(sp + q * dvp * DKP, x_s + q * 16 * ROWB, 16 * ROWB);
-            bulk_commit();
-          }
-        } else {
-          warp_arrive(&full_s[warp], lane);
+        for (int n = 0; n < 8; ++n) sts_acc(x_h + side * Cfg::kHalf + n * 512 + lane * 16, X[n]);
+        if (KEEP) fence_async();
+        cp_wait<0>();  // this side's rows of v
+        __syncwarp();
+        if (KEEP && lane == 0) {
+          bulk_s2g(p.s_parts + (((unit0 + c) * ((p.dv + 15) / 16) + dv0 / 16) * 2 + side) * NS * 8 * DKP,
+                   x_s + side * NS * 16 * DKP, NS * 16 * DKP);
+          bulk_commit();
         }
+        if (lane == 0) {
+          mbar_arrive(&pair[w]);
+          if (!KEEP) mbar_arrive(&full_s[w]);
+        }
+        // the stage of the chunk before is free by now, or nearly
+        if (!KEEP && Cfg::kStK == 2 && loads && c > 0 && next_k < p.chunks) ok = issue_k();
+        ok = ok && mbar_wait_bounded(&pair[w], 0);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
 
-        // R = V - exp(G) X, in place
+        // R = V - exp(G) X, in place; both sides add the halves in the same order
         const uint32_t vst = own + (int)(c & 1) * Cfg::kV;
 #pragma unroll
         for (int n2 = 0; n2 < 4; ++n2) {
@@ -610,13 +645,14 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
           for (int half = 0; half < 2; ++half) {
             const int n = 2 * n2 + half, tok = n * 8 + 2 * t4;
             const float2 ge = *reinterpret_cast<const float2*>(enter + tok);
-            float v[4];
+            float v[4], y[4];
+            lds_acc(x_h + (1 - side) * Cfg::kHalf + n * 512 + lane * 16, y);
             if constexpr (sizeof(T) == 2) {
-              const float2 x = unpack2<T>(vb[2 * half]), y = unpack2<T>(vb[2 * half + 1]);
-              v[0] = x.x;
-              v[1] = x.y;
-              v[2] = y.x;
-              v[3] = y.y;
+              const float2 lo = unpack2<T>(vb[2 * half]), hi = unpack2<T>(vb[2 * half + 1]);
+              v[0] = lo.x;
+              v[1] = lo.y;
+              v[2] = hi.x;
+              v[3] = hi.y;
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -626,9 +662,10 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
               }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) X[n][e] = fmaf(-((e & 1) ? ge.y : ge.x), X[n][e], v[e]);
+            for (int e = 0; e < 4; ++e) X[n][e] = fmaf(-((e & 1) ? ge.y : ge.x), X[n][e] + y[e], v[e]);
           }
         }
+        if (c + 1 < p.chunks) load_v(c + 1);  // the buffer of the chunk before
 
         // An infinity or a NaN in R (of v, k, or the state) spoils its row of
         // values from that token on, but the zeros above the diagonals of N
@@ -661,18 +698,17 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
               if (n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1]) X[n][e] = 0.f;
         }
 
-        // E = N R
-        float E[8][4];
+        // E = N R, this side's blocks of tokens: 0, 3 or 1, 2
+        float E[4][4];
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) E[n][e] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t a[NS][4];
           split_frag<NS>(X[2 * kk], X[2 * kk + 1], a);
-#pragma unroll
-          for (int n2 = kk; n2 < 4; ++n2) {
+          auto block = [&](int n2, float (&e0)[4], float (&e1)[4]) {
             Step<LV == 2, 2> s;
 #pragma unroll
             for (int i = LV; i >= 0; --i) {
@@ -680,75 +716,99 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
               ldsm4(nb, at_b<MROW>(st + Cfg::oN + i * kMatBytes, lane, n2 * 16, kk));
 #pragma unroll
               for (int j = LV - i; j >= 0; --j) {
-                s.mma(0, E[2 * n2], a[j], nb[0], nb[1]);
-                s.mma(1, E[2 * n2 + 1], a[j], nb[2], nb[3]);
+                s.mma(0, e0, a[j], nb[0], nb[1]);
+                s.mma(1, e1, a[j], nb[2], nb[3]);
               }
             }
-            s.add(0, E[2 * n2]);
-            s.add(1, E[2 * n2 + 1]);
-          }
+            s.add(0, e0);
+            s.add(1, e1);
+          };
+          if (kk <= side) block(side, E[0], E[1]);
+          if (kk <= 3 - side) block(3 - side, E[2], E[3]);
         }
-
-        // E's parts go to shared memory, and on: to the output warp, or kept
-        if (KEEP) {
+        // E's tiles go to the other side and the output warp
+        if (KEEP) {  // E's parts of the chunk before have been read
           if (lane == 0) bulk_wait_read<1>();
           __syncwarp();
-          if (bad) {
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1]) E[n][e] = __int_as_float(0x7fc00000);
-          }
-        } else {
-          if (c > 0) ok = mbar_wait_bounded(&free_e[warp], (uint32_t)((c - 1) & 1));
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) s_bad[warp] = bad;
-          if (bad && t4 == 0) {
-            s_spoilt[warp][g4] = spoilt[0];
-            s_spoilt[warp][g4 + 8] = spoilt[1];
-          }
         }
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t a[NO][4];
-          split_frag<NO>(E[2 * kk], E[2 * kk + 1], a);
+        for (int i = 0; i < 2; ++i) {
+          const int n2 = i == 0 ? side : 3 - side;
+          sts_acc(e_at(2 * n2), E[2 * i]);
+          sts_acc(e_at(2 * n2 + 1), E[2 * i + 1]);
+          if (KEEP) {
+            if (bad) {
 #pragma unroll
-          for (int q = 0; q < NO; ++q) stsm4_t(strip_at_t(x_e + q * kStrip, lane, kk), a[q]);
+              for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (n2 * 16 + n * 8 + 2 * t4 + (e & 1) >= spoilt[e >> 1])
+                    E[2 * i + n][e] = __int_as_float(0x7fc00000);
+            }
+            uint32_t a[NS][4];
+            split_frag<NS>(E[2 * i], E[2 * i + 1], a);
+#pragma unroll
+            for (int q = 0; q < NS; ++q) stsm4_t(strip_at_t(x_e + q * kStrip, lane, n2), a[q]);
+          }
         }
         if (KEEP) {
           fence_async();
           __syncwarp();
           if (lane == 0) {
-            bulk_s2g(p.e_parts + ((unit0 + c) * ((p.dv + 15) / 16) + dv0 / 16) * NS * (kStrip / 2),
-                     x_e, NS * kStrip);
+            __nv_bfloat16* ep =
+                p.e_parts + ((unit0 + c) * ((p.dv + 15) / 16) + dv0 / 16) * NS * (kStrip / 2);
+#pragma unroll
+            for (int q = 0; q < NS; ++q)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int n2 = i == 0 ? side : 3 - side;  // 16 rows of 32 bytes
+                bulk_s2g(ep + q * (kStrip / 2) + n2 * 256, x_e + q * kStrip + n2 * 512, 512);
+              }
             bulk_commit();
           }
         } else {
-          warp_arrive(&full_e[warp], lane);
+          if (side == 0 && lane == 0) s_bad[w] = bad;
+          if (side == 0 && bad && t4 == 0) {
+            s_spoilt[w][g4] = spoilt[0];
+            s_spoilt[w][g4 + 8] = spoilt[1];
+          }
         }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&pair[w]);
+          if (!KEEP) mbar_arrive(&full_e[w]);
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pair[w], 1));
+        if (!ok) break;
 
-        // S = exp(G_C) S + (beta exp(G_C - G) E)^T K.  The chunk's sum starts
-        // at zero and joins the state in one rounded multiply-add.
+        // S = exp(G_C) S + (beta exp(G_C - G) E)^T K, this half of dk.  The
+        // chunk's sum starts at zero and joins the state in one rounded
+        // multiply-add.
         uint32_t u[4][NS][4];
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
+          float f[2][4];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int tok = (2 * kk + half) * 8 + 2 * t4;
+            const int n = 2 * kk + half, tok = n * 8 + 2 * t4;
             const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
             const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
             const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
-            E[2 * kk + half][0] *= w0;
-            E[2 * kk + half][1] *= w1;
-            E[2 * kk + half][2] *= w0;
-            E[2 * kk + half][3] *= w1;
+            if ((kk == side) | (kk == 3 - side)) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[half][e] = E[(kk >> 1) * 2 + half][e];
+            } else {
+              lds_acc(e_at(n), f[half]);
+            }
+            f[half][0] *= w0;
+            f[half][1] *= w1;
+            f[half][2] *= w0;
+            f[half][3] *= w1;
           }
-          split_frag<NS>(E[2 * kk], E[2 * kk + 1], u[kk]);
+          split_frag<NS>(f[0], f[1], u[kk]);
         }
 #pragma unroll
-        for (int n4 = 0; n4 < NT / 4; ++n4) {
+        for (int n4 = 0; n4 < HT / 4; ++n4) {
           float d[4][4];
 #pragma unroll
           for (int n = 0; n < 4; ++n)
@@ -760,8 +820,8 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
 #pragma unroll
             for (int i = NP - 1; i >= 0; --i) {
               uint32_t b0[4], b1[4];
-              ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
-              ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
+              ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, d0 + n4 * 32, kk));
+              ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, d0 + n4 * 32 + 16, kk));
 #pragma unroll
               for (int j = LV - i; j >= 0; --j) {
                 s.mma(0, d[0], u[kk][j], b0[0], b0[1]);
@@ -780,19 +840,21 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
         }
         if (bad)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < HT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (spoilt[e >> 1] < kChunk) S[n][e] = __int_as_float(0x7fc00000);
         warp_arrive(&free_k[sk], lane);
       }
 
+      cp_wait<0>();
+      if (!ok && loads) drain();
       if (KEEP) {
         if (lane == 0) bulk_wait_all();
       } else if (ok && p.final_state != nullptr) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int dk = n * 8 + 2 * t4;
+        for (int n = 0; n < HT; ++n) {
+          const int dk = d0 + n * 8 + 2 * t4;
           float* dst = p.final_state + (bh * p.dv + dv0 + g4) * p.dk + dk;
           if (dk < p.dk) {
             *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
@@ -803,15 +865,15 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
     }
   } else if (!KEEP) {
     // ---------------------------------------------------------- output
-    const int w = warp - NW;
+    const int w = warp - 2 * NW;
     const int dv0 = dv_cta + w * 16;
     const int nval = p.dv - dv0;
     if (nval > 0) {
       const int64_t vstride = (int64_t)p.heads * p.dv;
-      const uint32_t x_s = sm0 + Cfg::oWarp + w * Cfg::kWarp + 2 * Cfg::kV, x_e = x_s + Cfg::kXS;
+      const uint32_t x_s = sm0 + Cfg::oWarp + w * Cfg::kWarp + 2 * Cfg::kV, x_h = x_s + Cfg::kXS,
+                     x_o = x_h + 2 * Cfg::kHalf;
       const bool loads = w == 0 && lane == 0;
       if (loads) {
-        while (next_k < min((int64_t)Cfg::kStK, p.chunks)) issue_k();
         while (next_q < min((int64_t)Cfg::kStQ, p.chunks)) issue_q();
       }
       __syncwarp();
@@ -829,11 +891,12 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
         for (int n = 0; n < 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) O[n][e] = 0.f;
-#pragma unroll 2
+#pragma unroll
         for (int kk = 0; kk < DKP / 16; ++kk) {
           uint32_t a[NO][4];
 #pragma unroll
-          for (int q = 0; q < NO; ++q) ldsm4(a[q], at_a<ROWB>(x_s + q * 16 * ROWB, lane, 0, kk));
+          for (int q = 0; q < NO; ++q)
+            ldsm4(a[q], half_a<DKP>(x_s + (kk / (DKP / 32) * NO + q) * 16 * DKP, lane, kk % (DKP / 32)));
 #pragma unroll
           for (int n2 = 0; n2 < 4; ++n2) {
             Step<LO == 2, 2> s;
@@ -865,9 +928,12 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
         if (!ok) break;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
+          float e0[4], e1[4];  // where the chain's e_at puts them
+          const uint32_t e_blk = x_h + (kk == 0 || kk == 3 ? Cfg::kHalf : 0) + (kk >> 1) * 1024 + lane * 16;
+          lds_acc(e_blk, e0);
+          lds_acc(e_blk + 512, e1);
           uint32_t a[NO][4];
-#pragma unroll
-          for (int q = 0; q < NO; ++q) ldsm4_t(a[q], strip_at_t(x_e + q * kStrip, lane, kk));
+          split_frag<NO>(e0, e1, a);
 #pragma unroll
           for (int n2 = kk; n2 < 4; ++n2) {
             Step<LO == 2, 2> s;
@@ -885,9 +951,14 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
             s.add(1, O[2 * n2 + 1]);
           }
         }
-        warp_arrive(&free_q[sq], lane);
-        if (s_bad[w]) {
-          const int first[2] = {s_spoilt[w][g4], s_spoilt[w][g4 + 8]};
+        const bool bad = s_bad[w] != 0;
+        const int first[2] = {s_spoilt[w][g4], s_spoilt[w][g4 + 8]};
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&free_q[sq]);
+          mbar_arrive(&free_e[w]);
+        }
+        if (bad) {
 #pragma unroll
           for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -898,32 +969,28 @@ __global__ void __launch_bounds__(ScanCfg<T, NP, LV, DKP, NW, KEEP>::kThreads, 1
         T* out = static_cast<T*>(p.out) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0;
         const int rows = (int)min((int64_t)kChunk, p.L - t0);
         if constexpr (sizeof(T) == 2) {
-          // through E's strip, transposed, for stores of 16 bytes
+          // through shared memory, transposed, for stores of 16 bytes
           __syncwarp();
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             const uint32_t a[4] = {pack2<T>(O[2 * kk][0], O[2 * kk][1]), pack2<T>(O[2 * kk][2], O[2 * kk][3]),
                                    pack2<T>(O[2 * kk + 1][0], O[2 * kk + 1][1]),
                                    pack2<T>(O[2 * kk + 1][2], O[2 * kk + 1][3])};
-            stsm4_t(strip_at_t(x_e, lane, kk), a);
+            stsm4_t(strip_at_t(x_o, lane, kk), a);
           }
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = i * 16 + (lane >> 1), un = lane & 1;
             if (r < rows && un * 8 < nval)
-              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_e, r, un));
+              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_o, r, un));
           }
         } else {
 #pragma unroll
           for (int n = 0; n < 8; ++n)
             store_t<T>(out + (int64_t)n * 8 * vstride, vstride, O[n], lane, rows - n * 8, nval);
         }
-        warp_arrive(&free_e[w], lane);
-        if (loads) {
-          if (next_k < p.chunks) ok = issue_k();
-          if (ok && next_q < p.chunks) ok = issue_q();
-        }
+        if (loads && next_q < p.chunks) ok = issue_q();
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
@@ -1004,7 +1071,7 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   p.dk = (int)a.dk;
   p.dv = (int)a.dv;
   p.scale = a.scale;
-  // Chain warps per CTA: 4, or 2 where that still leaves an SM to every CTA
+  // Strips per CTA: 4, or 2 where that still leaves an SM to every CTA
   // (and for fp32, whose tiles leave room for no more).
   const bool two = sizeof(T) == 4 || bh * ((a.dv + 31) / 32) <= a.num_sms;
   if constexpr (sizeof(T) == 4) {

@@ -261,7 +261,7 @@ struct DeltaPlan {
   int64_t grad_rows;                   // [np][batch x seqlen x heads x dv], np > 1
   int64_t do_parts;                    // [head][chunk][dvp / 16][np][64][16]
   int64_t e_parts, dv_parts;           // [head][chunk][dvp / 16][ns][64][16]
-  int64_t s_parts, ds_parts;           // [head][chunk][ns][dvp][dkp]
+  int64_t s_parts, ds_parts;           // [head][chunk][dvp / 16][half][ns][16][dkp / 2]
   int64_t dq_part, dk_part;            // [batch x seqlen][heads][dk] fp32 (backward, shared heads)
   int64_t bytes;
 };
