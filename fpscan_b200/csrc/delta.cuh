@@ -220,6 +220,126 @@ __device__ __forceinline__ void lds_acc(uint32_t addr, float (&c)[4]) {
   c[3] = __uint_as_float(v.w);
 }
 
+// ---------------------------------------------------------------- tcgen05
+// Products of the sequential kernels: A and B in shared memory, D (128 rows
+// of 2 C values, fp32) in tensor memory, one thread issues.  A tiles have
+// rows of 128 bytes, B tiles (rows are k, 2 C values each) rows of 4 C; 16-byte
+// units are exchanged by the bits of the row that the descriptors' 128- and
+// 64-byte swizzles take (tile_at, val_at); tiles start on 1024-byte
+// boundaries.  An A tile serves as K-major operand (rows are the operand's
+// rows, 64 values of k in 128 bytes) or, with the transpose bit, as MN-major
+// operand (rows are k).
+template <int C>
+__device__ __forceinline__ uint32_t val_at(uint32_t base, int row, int unit) {
+  return C == 32 ? base + row * 128 + ((unit ^ (row & 7)) << 4)
+                 : base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+}
+// leading: bytes from 64 rows of an MN-major operand to its next 64.
+__device__ __forceinline__ uint64_t umma_desc_a(uint32_t addr, uint32_t leading) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)((leading >> 4) & 0x3fff) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+template <int C>
+__device__ __forceinline__ uint64_t umma_desc_b(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(8 * 4 * C >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(C == 32 ? 2 : 4) << 61);
+}
+// fp32 D, bf16 A and B, M = 128, N = 2 C, B MN-major, A MN-major where `ta`.
+template <int C>
+__host__ __device__ constexpr uint32_t umma_idesc(bool ta) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((ta ? 1u : 0u) << 15) | (1u << 16) |
+         ((2 * C >> 3) << 17) | ((128u >> 4) << 24);
+}
+// A wait that is short as a rule: tries for a while before it reads the clock
+// and the limit (a load from global memory), which take longer than the wait.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity);
+}
+
+// One lane of a whole warp, the same one every time.  The issuing warp takes
+// its branch as a warp, so that descriptors stay in uniform registers: issued
+// by a lone thread of a divergent branch a product took 100 cycles, twice its
+// own time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                     bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0)
+      : "memory");
+}
+// The barrier's phase completes when all products issued so far have.
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void umma_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void umma_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// D = sum over parts i of A and j of B, i < NA, i + j <= LV, smallest first,
+// and over KS steps of 16 values of k: a_step / b_step are bytes of one step,
+// a_part / b_part of one part.  SPLIT: A's steps from the fifth on lie a_half
+// further (K-major tiles of 128 columns).
+template <int NA, int LV, int KS, bool SPLIT>
+__device__ __forceinline__ void umma_parts(uint32_t d, uint64_t a, uint64_t b, uint32_t a_part,
+                                           uint32_t b_part, uint32_t a_step, uint32_t b_step,
+                                           uint32_t a_half, uint32_t idesc, int ksteps) {
+#pragma unroll
+  for (int lv = LV; lv >= 0; --lv)
+#pragma unroll
+    for (int i = 0; i <= lv && i < NA; ++i)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if (ks < ksteps) {
+          const uint32_t ao = i * a_part + (SPLIT ? (ks >> 2) * a_half + (ks & 3) * a_step : ks * a_step);
+          const uint32_t bo = (lv - i) * b_part + ks * b_step;
+          umma(d, a + (ao >> 4), b + (bo >> 4), idesc, lv != LV || i != 0 || ks != 0);
+        }
+}
+
+// 16 or 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // ---------------------------------------------------------------- bf16 parts
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -260,6 +380,28 @@ __device__ __forceinline__ void split_frag(const float (&lo)[4], const float (&h
   for (int p = 0; p < P; ++p) a[p][3] = t[p];
 }
 
+// The parts of C values of a row as 16-byte units 0.., handed to
+// put(part, unit, value).
+template <int P, int C, typename F>
+__device__ __forceinline__ void split_row(const float (&x)[C], F put) {
+#pragma unroll
+  for (int u = 0; u < C / 8; ++u) {
+    uint32_t w[4][P];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) split_pair<P>(x[u * 8 + 2 * c], x[u * 8 + 2 * c + 1], w[c]);
+#pragma unroll
+    for (int q = 0; q < P; ++q) put(q, u, make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]));
+  }
+}
+
+template <typename T, int C>
+__device__ __forceinline__ void store_row(T* p, int n, const float (&x)[C]) {
+#pragma unroll
+  for (int i = 0; i < C / Elem<T>::kVec; ++i)
+    if (i * Elem<T>::kVec < n)
+      *reinterpret_cast<uint4*>(p + i * Elem<T>::kVec) = pack_vec<T>(x + i * Elem<T>::kVec);
+}
+
 // ---------------------------------------------------------------- asynchronous copies
 // 16 bytes global -> shared; zeros when `in` is false (then src is not read).
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
@@ -272,6 +414,45 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+
+// A thread's next row of C values of T, fetched a chunk ahead.  16-bit
+// rows wait in shared memory (units of the 128 fetching threads side by
+// side), copied asynchronously: loads into registers would be waited for at
+// the next loop, which the waits on barriers are.  fp32 rows have no room
+// there and are loaded.
+template <typename T, int C>
+struct NextRow {
+  static constexpr int V = Elem<T>::kVec, N = C / V;
+  static constexpr int kBytes = sizeof(T) == 2 ? 128 * C * 2 : 0;  // of shared memory
+  uint4 raw[sizeof(T) == 2 ? 1 : N];
+  uint32_t at;
+  __device__ __forceinline__ NextRow(uint32_t room, int thread) : at(room + thread * 16) {}
+  // the first `n` values (a multiple of 8, may be <= 0) from p, zeros behind them
+  __device__ __forceinline__ void fetch(const T* p, int n, const T* valid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = i * V < n;
+      if constexpr (sizeof(T) == 2)
+        cp16(at + i * 128 * 16, in ? p + i * V : valid, in);
+      else
+        raw[i] = in ? *reinterpret_cast<const uint4*>(p + i * V) : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (sizeof(T) == 2) cp_commit();
+  }
+  __device__ __forceinline__ void take(float (&x)[C]) {
+    if constexpr (sizeof(T) == 2) cp_wait<0>();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      Vec16<T> v;
+      if constexpr (sizeof(T) == 2)
+        v.raw = lds128(at + i * 128 * 16);
+      else
+        v.raw = raw[i];
+#pragma unroll
+      for (int c = 0; c < V; ++c) x[i * V + c] = Elem<T>::load(v.e[c]);
+    }
+  }
+};
 
 // Tile of ROWS rows of ROWB bytes: row r from src + r * stride (bytes), the
 // first `rows` rows and `units` units of each; the rest is zeros.  src must

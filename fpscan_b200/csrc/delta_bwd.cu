@@ -14,9 +14,8 @@
 // decay scales what is read after it like q and k do: no quotient of a
 // gradient by beta or by a decay appears, so zeros of both are harmless.
 //
-//   delta_split_kernel  fp16 / fp32 only: cuts dO into bf16 parts.
-//   delta_rev_kernel    from the last chunk to the first, dS^T in registers
-//                       as delta_scan_kernel keeps S^T; writes dV, dS per chunk.
+//   delta_rev_kernel    from the last chunk to the first, as
+//                       delta_scan_kernel; writes dV, and dV, dO, dS as parts.
 //   delta_grad_kernel   the rest, every (chunk, head) by itself.
 //   delta_group_kernel  sums dQ, dK over the heads that share a key head, in
 //                       a fixed order.
@@ -27,585 +26,307 @@
 
 namespace fpscan {
 
-template <typename T, int LV, int DKP>
+template <typename T, int LV>
 cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_t nb,
                            bool keep);
 
 namespace {
 
-// ------------------------------------------------------------------ parts of dO
-struct SplitParams {
-  const void* src;
-  __nv_bfloat16* dst;  // part p at + p * n
-  int64_t n;           // elements (a multiple of 8)
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) delta_split_kernel(const SplitParams p) {
-  constexpr int NP = kParts<T>, V = Elem<T>::kVec;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int64_t step = (int64_t)gridDim.x * blockDim.x * 8;
-  const T* src = static_cast<const T*>(p.src);
-  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < p.n; i += step) {
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8 / V; ++j) {
-      Vec16<T> v;
-      v.raw = *reinterpret_cast<const uint4*>(src + i + j * V);
-#pragma unroll
-      for (int c = 0; c < V; ++c) x[j * V + c] = Elem<T>::load(v.e[c]);
-    }
-    uint32_t w[4][NP];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) split_pair<NP>(x[2 * j], x[2 * j + 1], w[j]);
-#pragma unroll
-    for (int q = 0; q < NP; ++q)
-      *reinterpret_cast<uint4*>(p.dst + q * p.n + i) = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
-  }
-}
+constexpr int kHalfTile = 2 * kChunk * 128;    // 64 columns of K's, then Q's rows
+constexpr int kTileKQ = 2 * kHalfTile;         // one part of K and Q
+constexpr int kMatBytes = kChunk * kChunk * 2; // one part of N or PN
 
 // ------------------------------------------------------------------ along the chunks, backwards
 struct RevParams {
-  const __nv_bfloat16* q_tiles;
-  const __nv_bfloat16* k_tiles;
-  const __nv_bfloat16* grad;  // dO parts in token rows, part p at + p * grad_stride
-  int64_t grad_stride;
-  const __nv_bfloat16* n_mat;
-  const __nv_bfloat16* p_mat;
+  const __nv_bfloat16* kq_tiles;
+  const void* grad;           // dO
+  const __nv_bfloat16* npn;
   const float* vecs;
   const float* grad_final;
   float* dinitial;
   void* dv_out;
-  __nv_bfloat16* do_parts;    // strips, as e_parts
-  __nv_bfloat16* dv_parts;
-  __nv_bfloat16* ds_parts;
+  __nv_bfloat16* do_parts;    // strips [head][chunk][dv / 16][NP][64][16]
+  __nv_bfloat16* dv_parts;    //        [head][chunk][dv / 16][NS][64][16]
+  __nv_bfloat16* ds_parts;    //        [head][chunk][dv / 16][NS][128][16]
   int64_t L, chunks;
   int key_heads, heads, dk, dv, slices;
   float scale;
 };
 
-// As in delta_scan_kernel 16 rows of dS^T are shared by three warps: two
-// chain warps with half of dk each, and a helper that computes what does not
-// need dS -- Z = P^T dO and the sum (scale exp(G) dO)^T Q that joins the
-// state -- and leaves both in shared memory.  K, N are loaded by the first
-// chain warp, Q, P by the first helper.
-template <int NP, int LV, int DKP, int NW>
+constexpr int kRevThreads = 256;
+
+// As delta_scan_kernel, three products per chunk for 2 C values:
+//     K dS                                    -> Y,
+//     [N; PN]^T [beta exp(G_C - G) Y; dO]     -> dV, since P^T dO enters F and
+//                                                N^T P^T = (P N)^T,
+//     [K; Q]^T [-exp(G) dV; scale exp(G) dO]  -> the sum that joins dS.
+// Both operands of the last two are stacked to 128 rows of k.  The warps of
+// tensor memory lanes 0..63 work on Y and dV, those of 64..127 on dO; the
+// second product's 64 rows are computed twice over (an operand whose next 64
+// rows are the same ones), so that the latter find dV in their lanes too and
+// write it out.
+template <typename T, int LV, int C>
 struct RevCfg {
+  static constexpr int NP = kParts<T>;
   static constexpr int NS = LV + 1;
-  static constexpr int kTileK = kChunk * DKP * 2;
-  static constexpr int kMat = kChunk * kChunk * 2;
-  static constexpr int oN = NP * kTileK, oVec = oN + NS * kMat;
-  static constexpr int kStageK = oVec + 3 * kChunk * 4;
-  static constexpr int oP = NP * kTileK, oEnter = oP + NS * kMat;
-  static constexpr int kStageQ = oEnter + 256;
-  // of a strip: dO once or twice; dS's parts; two halves of K dS^T, later dV;
-  // Z, later dV's parts; the sum that joins the state
-  static constexpr int kG = NP * kStrip, kXS = NS * 16 * DKP * 2, kHalf = 8 * 512;
-  static constexpr int kZ = NS * kStrip > 8 * 512 ? NS * kStrip : 8 * 512, kSum = DKP / 8 * 512;
-  static constexpr int kRoom = 227 * 1024 - 1280;
-  static constexpr int kBase = kXS + 2 * kHalf + kZ + kSum;
-  // two stages of K, N come first, then two of dO, then two of Q, P
-  static constexpr int kStK = NW * (kBase + kG) + 2 * kStageK + kStageQ <= kRoom ? 2 : 1;
-  static constexpr int kBufG = NW * (kBase + 2 * kG) + kStK * kStageK + kStageQ <= kRoom ? 2 : 1;
-  static constexpr int kWarp = kBufG * kG + kBase;
-  static constexpr int kStQ = NW * kWarp + kStK * kStageK + 2 * kStageQ <= kRoom ? 2 : 1;
-  static constexpr int oQ = kStK * kStageK, oWarp = oQ + kStQ * kStageQ;
-  static constexpr int kSmem = oWarp + NW * kWarp + 128;
-  static constexpr bool kFits = kSmem + 1152 <= 227 * 1024;
+  static constexpr int kKQ = NP * kTileKQ;
+  static constexpr int kNPN = NS * 2 * kMatBytes;
+  static constexpr int kPart = 128 * 4 * C;    // of dS; of the stacked operands
+  static constexpr int kVec = 3 * kChunk * 4;  // enter, leave, beta
+  // The stacked operand may lie over dS's parts: they are used up by the
+  // first product.  It does where the room is short.
+  static constexpr int kRoom = 227 * 1024 - 2 * 1024;
+  static constexpr int kFixed = kNPN + 2 * NS * kPart + NextRow<T, C>::kBytes;
+  static constexpr bool kOver = kFixed + kKQ + kVec > kRoom;
+  static constexpr int kBody = kOver ? kFixed - NS * kPart : kFixed;
+  static constexpr int kSt = kBody + 2 * (kKQ + kVec) <= kRoom ? 2 : 1;  // stages of K, Q
+  static constexpr int oNPN = kSt * kKQ, oS = oNPN + kNPN, oE = kOver ? oS : oS + NS * kPart;
+  static constexpr int oRow = oE + NS * kPart, oVec = oRow + NextRow<T, C>::kBytes;
+  static constexpr int kSmem = oVec + kSt * kVec + 1024;
+  static_assert(kSmem + 1024 <= 227 * 1024);
 };
 
-template <typename T, int NP, int LV, int DKP, int NW>
-__global__ void __launch_bounds__(NW * 96, 1) delta_rev_kernel(const RevParams p) {
-  using Cfg = RevCfg<NP, LV, DKP, NW>;
-  static_assert(Cfg::kFits);
-  constexpr int NS = Cfg::NS, ROWB = DKP * 2, NT = DKP / 8, MROW = kChunk * 2;
+template <typename T, int LV, int C>
+__global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevParams p) {
+  using Cfg = RevCfg<T, LV, C>;
+  constexpr int kTmem = C == 32 ? 256 : 128;
+  constexpr int NP = Cfg::NP, NS = Cfg::NS;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
+      (reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sm0 = smem_addr(dsm);
-  __shared__ __align__(8) uint64_t full_k[2], free_k[2], full_q[2], free_q[2];
-  __shared__ __align__(8) uint64_t full_z[NW], free_z[NW], full_g[NW], free_g[NW], pair[NW];
+  const uint32_t s_npn = sm0 + Cfg::oNPN, s_s = sm0 + Cfg::oS, s_e = sm0 + Cfg::oE;
+  __shared__ __align__(8) uint64_t full_kq[2], full_n, done[3];
+  __shared__ uint32_t s_tmem;
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g4 = lane >> 2, t4 = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
+  const int quad = warp & 3, col0 = (warp >> 2) * C;  // tensor memory lanes 32 quad.., columns
+  const bool is_y = quad < 2;                          // Y and dV; else dO
+  const int tok = (quad & 1) * 32 + lane;              // this thread's token
+  const int dk = quad * 32 + lane;                     // and row of the state
   const int64_t bh = blockIdx.x / p.slices;
   const int slice = (int)(blockIdx.x - bh * p.slices);
   const int64_t b = bh / p.heads;
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
-  const int dv_cta = slice * NW * 16;
-  const int nact = min(NW, (p.dv - dv_cta + 15) / 16);
+  const int dv0 = slice * 2 * C + col0;
+  const int nval = min(C, p.dv - dv0);  // values of this thread's C that exist (may be <= 0)
+  const int strips = (p.dv + 15) / 16;
+  const int64_t vstride = (int64_t)p.heads * p.dv;
+  const int64_t tile = (b * p.key_heads + hk) * p.chunks, unit0 = bh * p.chunks;
+
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&full_k[i], 1);
-      mbar_init(&free_k[i], 2 * nact);
-      mbar_init(&full_q[i], 1);
-      mbar_init(&free_q[i], nact);
-    }
-    for (int i = 0; i < NW; ++i) {
-      mbar_init(&full_z[i], 1);
-      mbar_init(&free_z[i], 2);
-      mbar_init(&full_g[i], 1);
-      mbar_init(&free_g[i], 2);
-      mbar_init(&pair[i], 2);
-    }
+    mbar_init(&full_kq[0], 1);
+    mbar_init(&full_kq[1], 1);
+    mbar_init(&full_n, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&done[i], 1);
     fence_mbar_init();
   }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&s_tmem)), "n"(kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  umma_fence_before();
   __syncthreads();
+  umma_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint32_t my_tmem = tmem + ((uint32_t)(quad * 32) << 16) + col0;
   pdl_wait();
   pdl_launch_dependents();
 
-  const int w = warp < 2 * NW ? warp >> 1 : warp - 2 * NW;  // strip
-  const int side = warp & 1;                                // chain: half of dk
-  const int dv0 = dv_cta + w * 16, nval = p.dv - dv0;
-  const int strips = (p.dv + 15) / 16;
-  const int64_t unit0 = bh * p.chunks, tile = (b * p.key_heads + hk) * p.chunks;
-  const int64_t vstride = (int64_t)p.heads * p.dv;
-  const uint32_t own = sm0 + Cfg::oWarp + w * Cfg::kWarp;
-  const uint32_t x_s = own + Cfg::kBufG * Cfg::kG, x_h = x_s + Cfg::kXS, x_z = x_h + 2 * Cfg::kHalf,
-                 x_g = x_z + Cfg::kZ;
   // step d handles chunk chunks - 1 - d
-  int64_t next = 0;  // steps issued by this loading lane
-  auto issue_k = [&]() {
-    const int64_t c = p.chunks - 1 - next;
-    const int s = (int)(next % Cfg::kStK);
-    if (next >= Cfg::kStK && !mbar_wait_bounded(&free_k[s], (uint32_t)((next / Cfg::kStK - 1) & 1)))
-      return false;
-    const uint32_t st = sm0 + s * Cfg::kStageK;
-    mbar_expect_tx(&full_k[s], Cfg::oVec + 3 * kChunk * 4);
-    bulk_in(st, p.k_tiles + (tile + c) * NP * (kChunk * DKP), NP * Cfg::kTileK, &full_k[s]);
-    bulk_in(st + Cfg::oN, p.n_mat + (unit0 + c) * NS * (kChunk * kChunk), NS * Cfg::kMat, &full_k[s]);
-    bulk_in(st + Cfg::oVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), 3 * kChunk * 4, &full_k[s]);
-    ++next;
-    return true;
+  const bool loads = tid == kRevThreads - 32;
+  auto load_kq = [&](int64_t d) {
+    const int64_t c = p.chunks - 1 - d;
+    const int s = (int)(d % Cfg::kSt);
+    mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
+    bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
+    bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
+            &full_kq[s]);
   };
-  auto issue_q = [&]() {
-    const int64_t c = p.chunks - 1 - next;
-    const int s = (int)(next % Cfg::kStQ);
-    if (next >= Cfg::kStQ && !mbar_wait_bounded(&free_q[s], (uint32_t)((next / Cfg::kStQ - 1) & 1)))
-      return false;
-    const uint32_t st = sm0 + Cfg::oQ + s * Cfg::kStageQ;
-    mbar_expect_tx(&full_q[s], Cfg::oEnter + kChunk * 4);
-    bulk_in(st, p.q_tiles + (tile + c) * NP * (kChunk * DKP), NP * Cfg::kTileK, &full_q[s]);
-    bulk_in(st + Cfg::oP, p.p_mat + (unit0 + c) * NS * (kChunk * kChunk), NS * Cfg::kMat, &full_q[s]);
-    bulk_in(st + Cfg::oEnter, p.vecs + (unit0 + c) * (kVecCount * kChunk), kChunk * 4, &full_q[s]);
-    ++next;
-    return true;
+  auto load_n = [&](int64_t d) {
+    mbar_expect_tx(&full_n, Cfg::kNPN);
+    bulk_in(s_npn, p.npn + (unit0 + p.chunks - 1 - d) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
   };
-
-  if (warp < 2 * NW && nval > 0) {
-    // ---------------------------------------------------------- chain
-    constexpr int HT = NT / 2;  // tiles of this half
-    const int d0 = side * (DKP / 2);
-    const bool loads = warp == 0 && lane == 0;
-    // dV's tiles, as E's in delta_scan_kernel
-    auto e_at = [&](int n) {
-      const int blk = n >> 1, of = blk == 0 || blk == 3 ? 0 : 1;
-      return x_h + (1 - of) * Cfg::kHalf + ((blk >> 1) * 2 + (n & 1)) * 512 + lane * 16;
-    };
-    if (loads)
-      while (next < min((int64_t)Cfg::kStK, p.chunks)) issue_k();
-    __syncwarp();
-    float S[HT][4];  // dS^T
-#pragma unroll
-    for (int n = 0; n < HT; ++n) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) S[n][c] = 0.f;
-      if (p.grad_final != nullptr) {
-        const int dk = d0 + n * 8 + 2 * t4;
-        const float* src = p.grad_final + (bh * p.dv + dv0 + g4) * p.dk + dk;
-        if (dk < p.dk) {
-          const float2 v = *reinterpret_cast<const float2*>(src);
-          S[n][0] = v.x;
-          S[n][1] = v.y;
-          if (nval > 8) {
-            const float2 y = *reinterpret_cast<const float2*>(src + 8 * p.dk);
-            S[n][2] = y.x;
-            S[n][3] = y.y;
-          }
-        }
-      }
-    }
-    bool ok = true;
-    for (int64_t d = 0; d < p.chunks; ++d) {
-      const int64_t c = p.chunks - 1 - d;
-      const int sk = (int)(d % Cfg::kStK);
-      const uint32_t st = sm0 + sk * Cfg::kStageK;
-      const float* vec = reinterpret_cast<const float*>(dsm + sk * Cfg::kStageK + Cfg::oVec);
-      const float* enter = vec + kVecEnter * kChunk;
-      const float* leave = vec + kVecLeave * kChunk;
-      const float* beta = vec + kVecBeta * kChunk;
-      // one stage: the load waits for every chain warp
-      if (Cfg::kStK == 1 && d > 0 && loads) ok = issue_k();
-      ok = ok && mbar_wait_bounded(&full_k[sk], (uint32_t)((d / Cfg::kStK) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const float total = enter[kChunk - 1];
-
-      // Y = (K dS^T)^T: 16 values x 64 tokens, this half of dk.  dS's parts
-      // are kept.
-      float Y[8][4];
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) Y[n][e] = 0.f;
-#pragma unroll
-      for (int k2 = 0; k2 < HT / 2; ++k2) {
-        const int kk = side * (HT / 2) + k2;
-        uint32_t a[NS][4];
-        split_frag<NS>(S[2 * k2], S[2 * k2 + 1], a);
-#pragma unroll
-        for (int q = 0; q < NS; ++q)
-          stsm4(half_a<DKP>(x_s + (side * NS + q) * 16 * DKP, lane, k2), a[q]);
-#pragma unroll
-        for (int n2 = 0; n2 < 4; ++n2) {
-          Step<LV == 2, 2> s;
-#pragma unroll
-          for (int i = NP - 1; i >= 0; --i) {
-            uint32_t kb[4];
-            ldsm4(kb, at_b<ROWB>(st + i * Cfg::kTileK, lane, n2 * 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, Y[2 * n2], a[j], kb[0], kb[1]);
-              s.mma(1, Y[2 * n2 + 1], a[j], kb[2], kb[3]);
-            }
-          }
-          s.add(0, Y[2 * n2]);
-          s.add(1, Y[2 * n2 + 1]);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) sts_acc(x_h + side * Cfg::kHalf + n * 512 + lane * 16, Y[n]);
-      fence_async();
-      __syncwarp();
-      if (lane == 0) {
-        bulk_s2g(p.ds_parts + (((unit0 + c) * strips + dv0 / 16) * 2 + side) * NS * 8 * DKP,
-                 x_s + side * NS * 16 * DKP, NS * 16 * DKP);
-        bulk_commit();
-        mbar_arrive(&pair[w]);
-      }
-      // the stage of the chunk before is free by now
-      if (Cfg::kStK == 2 && loads && d > 0 && next < p.chunks) ok = issue_k();
-      ok = ok && mbar_wait_bounded(&pair[w], 0);
-      ok = ok && mbar_wait_bounded(&full_z[w], (uint32_t)(d & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-
-      // F = Z + beta exp(G_C - G) Y, in place
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int tok = n * 8 + 2 * t4;
-        const float2 lv = *reinterpret_cast<const float2*>(leave + tok);
-        const float2 bt = *reinterpret_cast<const float2*>(beta + tok);
-        float z[4], y[4];
-        lds_acc(x_z + n * 512 + lane * 16, z);
-        lds_acc(x_h + (1 - side) * Cfg::kHalf + n * 512 + lane * 16, y);
-        const float w0 = lv.x * bt.x, w1 = lv.y * bt.y;
-        Y[n][0] = fmaf(w0, Y[n][0] + y[0], z[0]);
-        Y[n][1] = fmaf(w1, Y[n][1] + y[1], z[1]);
-        Y[n][2] = fmaf(w0, Y[n][2] + y[2], z[2]);
-        Y[n][3] = fmaf(w1, Y[n][3] + y[3], z[3]);
-      }
-
-      // dV = N^T F, this side's blocks of tokens: 0, 3 or 1, 2
-      float V[4][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) V[n][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t a[NS][4];
-        split_frag<NS>(Y[2 * kk], Y[2 * kk + 1], a);
-        auto block = [&](int n2, float (&v0)[4], float (&v1)[4]) {
-          Step<LV == 2, 2> s;
-#pragma unroll
-          for (int i = LV; i >= 0; --i) {
-            uint32_t nb[4];
-            ldsm4_t(nb, at_bt<MROW>(st + Cfg::oN + i * Cfg::kMat, lane, n2 * 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, v0, a[j], nb[0], nb[1]);
-              s.mma(1, v1, a[j], nb[2], nb[3]);
-            }
-          }
-          s.add(0, v0);
-          s.add(1, v1);
-        };
-        if (kk >= side) block(side, V[0], V[1]);
-        if (kk >= 3 - side) block(3 - side, V[2], V[3]);
-      }
-      // dV's tiles go to the other side; its parts, over Z once both sides
-      // have read that, are kept
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n2 = i == 0 ? side : 3 - side;
-        sts_acc(e_at(2 * n2), V[2 * i]);
-        sts_acc(e_at(2 * n2 + 1), V[2 * i + 1]);
-      }
-      warp_arrive(&pair[w], lane);
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pair[w], 1));
-      if (!ok) break;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n2 = i == 0 ? side : 3 - side;
-        uint32_t a[NS][4];
-        split_frag<NS>(V[2 * i], V[2 * i + 1], a);
-#pragma unroll
-        for (int q = 0; q < NS; ++q) stsm4_t(strip_at_t(x_z + q * kStrip, lane, n2), a[q]);
-      }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) {
-        __nv_bfloat16* vp = p.dv_parts + ((unit0 + c) * strips + dv0 / 16) * NS * (kStrip / 2);
-#pragma unroll
-        for (int q = 0; q < NS; ++q)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int n2 = i == 0 ? side : 3 - side;  // 16 rows of 32 bytes
-            bulk_s2g(vp + q * (kStrip / 2) + n2 * 256, x_z + q * kStrip + n2 * 512, 512);
-          }
-        bulk_commit();
-      }
-      {
-        const int64_t t0 = c * kChunk;
-        const int rows = (int)min((int64_t)kChunk, p.L - t0);
-        T* out = static_cast<T*>(p.dv_out) + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n2 = i == 0 ? side : 3 - side;
-          if constexpr (NP == 1) {  // the first bf16 part is the rounded value
-            const int r = n2 * 16 + (lane >> 1), un = lane & 1;
-            if (r < rows && un * 8 < nval)
-              *reinterpret_cast<uint4*>(out + r * vstride + un * 8) = lds128(strip_at(x_z, r, un));
-          } else {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-              store_t<T>(out + (int64_t)(n2 * 16 + n * 8) * vstride, vstride, V[2 * i + n], lane,
-                         rows - n2 * 16 - n * 8, nval);
-          }
-        }
-      }
-
-      // dS <- exp(G_C) dS + (scale exp(G) dO)^T Q - (exp(G) dV)^T K, this half
-      uint32_t uv[4][NS][4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        float f[2][4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int n = 2 * kk + half;
-          const float2 ge = *reinterpret_cast<const float2*>(enter + n * 8 + 2 * t4);
-          if ((kk == side) | (kk == 3 - side)) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[half][e] = V[(kk >> 1) * 2 + half][e];
-          } else {
-            lds_acc(e_at(n), f[half]);
-          }
-          f[half][0] *= -ge.x;
-          f[half][1] *= -ge.y;
-          f[half][2] *= -ge.x;
-          f[half][3] *= -ge.y;
-        }
-        split_frag<NS>(f[0], f[1], uv[kk]);
-      }
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_g[w], (uint32_t)(d & 1)));
-      if (!ok) break;
-#pragma unroll
-      for (int n4 = 0; n4 < HT / 4; ++n4) {
-        float x[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) lds_acc(x_g + (side * HT + n4 * 4 + n) * 512 + lane * 16, x[n]);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          Step<LV == 2, 4> s;
-#pragma unroll
-          for (int i = NP - 1; i >= 0; --i) {
-            uint32_t b0[4], b1[4];
-            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, d0 + n4 * 32, kk));
-            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, d0 + n4 * 32 + 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, x[0], uv[kk][j], b0[0], b0[1]);
-              s.mma(1, x[1], uv[kk][j], b0[2], b0[3]);
-              s.mma(2, x[2], uv[kk][j], b1[0], b1[1]);
-              s.mma(3, x[3], uv[kk][j], b1[2], b1[3]);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < 4; ++n) s.add(n, x[n]);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[n4 * 4 + n][e] = fmaf(total, S[n4 * 4 + n][e], x[n][e]);
-      }
-      if (lane == 0) bulk_wait_read<0>();  // dS's and dV's parts: Z may come again
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&free_z[w]);
-        mbar_arrive(&free_g[w]);
-        mbar_arrive(&free_k[sk]);
-      }
-    }
-    if (lane == 0) bulk_wait_all();
-    if (!ok && loads)  // no copy may land after the CTA is gone
-      for (int64_t j = max((int64_t)0, next - Cfg::kStK); j < next; ++j)
-        mbar_wait_bounded(&full_k[j % Cfg::kStK], (uint32_t)((j / Cfg::kStK) & 1));
-    if (ok && p.dinitial != nullptr) {
-#pragma unroll
-      for (int n = 0; n < HT; ++n) {
-        const int dk = d0 + n * 8 + 2 * t4;
-        float* dst = p.dinitial + (bh * p.dv + dv0 + g4) * p.dk + dk;
-        if (dk < p.dk) {
-          *reinterpret_cast<float2*>(dst) = make_float2(S[n][0], S[n][1]);
-          if (nval > 8) *reinterpret_cast<float2*>(dst + 8 * p.dk) = make_float2(S[n][2], S[n][3]);
-        }
-      }
-    }
-  } else if (warp >= 2 * NW && nval > 0) {
-    // ---------------------------------------------------------- helper
-    const bool loads = w == 0 && lane == 0;
-    if (loads)
-      while (next < min((int64_t)Cfg::kStQ, p.chunks)) issue_q();
-    __syncwarp();
-    auto load_g = [&](int64_t d) {
-      const int64_t t0 = (p.chunks - 1 - d) * kChunk;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        load_strip<__nv_bfloat16>(
-            own + (int)(d % Cfg::kBufG) * Cfg::kG + i * kStrip,
-            p.grad + i * p.grad_stride + (b * p.L + t0) * vstride + (int64_t)h * p.dv + dv0,
-            vstride * 2, (int)min((int64_t)kChunk, p.L - t0), min(16, nval) / 8, lane);
-      cp_commit();
-    };
-    if (Cfg::kBufG == 2) load_g(0);
-    bool ok = true;
-    for (int64_t d = 0; d < p.chunks; ++d) {
-      const int64_t c = p.chunks - 1 - d;
-      const int sq = (int)(d % Cfg::kStQ);
-      const uint32_t st = sm0 + Cfg::oQ + sq * Cfg::kStageQ, gst = own + (int)(d % Cfg::kBufG) * Cfg::kG;
-      const float* enter = reinterpret_cast<const float*>(dsm + Cfg::oQ + sq * Cfg::kStageQ + Cfg::oEnter);
-      if (lane == 0) bulk_wait_read<0>();  // the strip of the step before has been kept
-      __syncwarp();
-      if (Cfg::kBufG == 1) load_g(d);
-      if (Cfg::kBufG == 2 && d + 1 < p.chunks) {
-        load_g(d + 1);
-        cp_wait<1>();
-      } else {
-        cp_wait<0>();
-      }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) {
-        bulk_s2g(p.do_parts + ((unit0 + c) * strips + dv0 / 16) * NP * (kStrip / 2), gst, NP * kStrip);
-        bulk_commit();
-      }
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full_q[sq], (uint32_t)((d / Cfg::kStQ) & 1)));
-      if (!ok) break;
-      float Z[8][4];
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) Z[n][e] = 0.f;
-      uint32_t ug[4][NS][4];  // parts of scale exp(G) dO
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t a[NP][4];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) ldsm4_t(a[i], strip_at_t(gst + i * kStrip, lane, kk));
-#pragma unroll
-        for (int n2 = 0; n2 <= kk; ++n2) {
-          Step<LV == 2, 2> s;
-#pragma unroll
-          for (int j = LV; j >= 0; --j) {
-            uint32_t pb[4];
-            ldsm4_t(pb, at_bt<MROW>(st + Cfg::oP + j * Cfg::kMat, lane, n2 * 16, kk));
-#pragma unroll
-            for (int i = NP - 1; i >= 0; --i) {
-              if (i + j > LV) continue;
-              s.mma(0, Z[2 * n2], a[i], pb[0], pb[1]);
-              s.mma(1, Z[2 * n2 + 1], a[i], pb[2], pb[3]);
-            }
-          }
-          s.add(0, Z[2 * n2]);
-          s.add(1, Z[2 * n2 + 1]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float2 ge = *reinterpret_cast<const float2*>(enter + kk * 16 + (r >> 1) * 8 + 2 * t4);
-          float x = 0.f, y = 0.f;
-#pragma unroll
-          for (int i = NP - 1; i >= 0; --i) {
-            x += bf16_lo(a[i][r]);
-            y += bf16_hi(a[i][r]);
-          }
-          uint32_t parts[NS];
-          split_pair<NS>(x * (ge.x * p.scale), y * (ge.y * p.scale), parts);
-#pragma unroll
-          for (int q = 0; q < NS; ++q) ug[kk][q][r] = parts[q];
-        }
-      }
-      if (d > 0) ok = mbar_wait_bounded(&free_z[w], (uint32_t)((d - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) sts_acc(x_z + n * 512 + lane * 16, Z[n]);
-      warp_arrive(&full_z[w], lane);
-      if (d > 0) ok = mbar_wait_bounded(&free_g[w], (uint32_t)((d - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-#pragma unroll 2
-      for (int n4 = 0; n4 < NT / 4; ++n4) {
-        float x[4][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          Step<LV == 2, 4> s;
-#pragma unroll
-          for (int i = NP - 1; i >= 0; --i) {
-            uint32_t b0[4], b1[4];
-            ldsm4_t(b0, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32, kk));
-            ldsm4_t(b1, at_bt<ROWB>(st + i * Cfg::kTileK, lane, n4 * 32 + 16, kk));
-#pragma unroll
-            for (int j = LV - i; j >= 0; --j) {
-              s.mma(0, x[0], ug[kk][j], b0[0], b0[1]);
-              s.mma(1, x[1], ug[kk][j], b0[2], b0[3]);
-              s.mma(2, x[2], ug[kk][j], b1[0], b1[1]);
-              s.mma(3, x[3], ug[kk][j], b1[2], b1[3]);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < 4; ++n) s.add(n, x[n]);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) sts_acc(x_g + (n4 * 4 + n) * 512 + lane * 16, x[n]);
-      }
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&full_g[w]);
-        mbar_arrive(&free_q[sq]);
-      }
-      if (loads && next < p.chunks) ok = issue_q();
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-    }
-    cp_wait<0>();
-    if (lane == 0) bulk_wait_all();
-    if (!ok && loads)
-      for (int64_t j = max((int64_t)0, next - Cfg::kStQ); j < next; ++j)
-        mbar_wait_bounded(&full_q[j % Cfg::kStQ], (uint32_t)((j / Cfg::kStQ) & 1));
+  if (loads) {
+    for (int64_t d = 0; d < min((int64_t)Cfg::kSt, p.chunks); ++d) load_kq(d);
+    load_n(0);
   }
-  __syncthreads();  // shared memory outlives every copy into it and out of it
+
+  const int64_t row0 = (b * p.L + tok) * vstride + (int64_t)h * p.dv + dv0;  // of token 0's chunk
+  NextRow<T, C> next_do(sm0 + Cfg::oRow, (warp >> 2) * 64 + tok);
+  auto load_do = [&](int64_t c) {
+    next_do.fetch(static_cast<const T*>(p.grad) + row0 + c * kChunk * vstride,
+                  c * kChunk + tok < p.L ? nval : 0, static_cast<const T*>(p.grad));
+  };
+  if (!is_y) load_do(p.chunks - 1);
+
+  float S[C];  // dS, one row of dk
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    S[i] = p.grad_final != nullptr && dk < p.dk && i < nval
+               ? p.grad_final[(bh * p.dv + dv0 + i) * p.dk + dk]
+               : 0.f;
+  const int ksteps = (p.dk + 15) / 16;
+
+  // Parts of a row of 32 values: to a stacked operand's row, to strips.
+  auto put_tile = [&](int row, const float (&x)[C]) {
+    split_row<NS>(x, [&](int q, int u, const uint4& w) {
+      sts128(val_at<C>(s_e + q * Cfg::kPart, row, col0 / 8 + u), w);
+    });
+  };
+  auto strip_ptr = [&](__nv_bfloat16* base, int64_t c, int u, int parts, int q, int bytes) {
+    return reinterpret_cast<char*>(base) +
+           (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * parts + q) * (int64_t)bytes;
+  };
+
+  // dS's parts to their strips, by the warps of dO
+  auto keep_ds = [&](int64_t c) {
+    const int have = min(C / 8, strips - slice * (C / 8));
+    char* sp = reinterpret_cast<char*>(p.ds_parts) +
+               ((unit0 + c) * strips + slice * (C / 8)) * (int64_t)(NS * 2 * kStrip);
+    const int t = (warp >> 2) * 64 + (quad - 2) * 32 + lane;  // 0..127
+#pragma unroll 4
+    for (int i = t; i < NS * 128 * (C / 4); i += 128) {
+      const int u = i % (C / 4), r = i / (C / 4) % 128, q = i / (C / 4 * 128);
+      if ((u >> 1) < have)
+        *reinterpret_cast<uint4*>(sp + ((u >> 1) * NS + q) * (2 * kStrip) + strip_at(0, r, u & 1)) =
+            lds128(val_at<C>(s_s + q * Cfg::kPart, r, u));
+    }
+  };
+  bool ok = true;  // as in delta_scan_kernel
+  auto wait = [&](uint64_t* bar, int64_t phase) {
+    if (ok) ok = mbar_wait_soon(bar, (uint32_t)(phase & 1));
+  };
+  for (int64_t d = 0; d < p.chunks; ++d) {
+    const int64_t c = p.chunks - 1 - d;
+    const int s = (int)(d % Cfg::kSt);
+    const uint32_t s_kq = sm0 + s * Cfg::kKQ;
+    const float* vec = reinterpret_cast<const float*>(dsm + Cfg::oVec + s * Cfg::kVec);
+
+    // dS's parts, rows of dk
+    split_row<NS>(S, [&](int q, int u, const uint4& w) {
+      sts128(val_at<C>(s_s + q * Cfg::kPart, dk, col0 / 8 + u), w);
+    });
+    fence_async();
+    umma_fence_before();
+    __syncthreads();
+    if (loads && d > 0 && d + Cfg::kSt - 1 < p.chunks) load_kq(d + Cfg::kSt - 1);
+    if (warp == 0) {
+      umma_fence_after();
+      wait(&full_kq[s], d / Cfg::kSt);
+      if (elect_one()) {
+        umma_parts<NP, LV, 8, true>(tmem, umma_desc_a(s_kq, 16), umma_desc_b<C>(s_s), kTileKQ, Cfg::kPart,
+                                    32, 64 * C, kHalfTile, umma_idesc<C>(false), ksteps);
+        umma_commit(&done[0]);
+      }
+      __syncwarp();
+    }
+    wait(&full_kq[s], d / Cfg::kSt);  // the vectors
+    const float ge = vec[kVecEnter * kChunk + tok], total = vec[kVecEnter * kChunk + kChunk - 1];
+    const float wb = vec[kVecLeave * kChunk + tok] * vec[kVecBeta * kChunk + tok];
+
+    float x[C], g[C];
+    if (Cfg::kOver && !is_y) keep_ds(c);  // before the stacked operand takes its place
+    if (!is_y) {
+      next_do.take(g);
+      split_row<NP>(g, [&](int q, int u, const uint4& w) {
+        if ((u & ~1) * 8 < nval)
+          *reinterpret_cast<uint4*>(strip_ptr(p.do_parts, c, u, NP, q, kStrip) +
+                                    strip_at(0, tok, u & 1)) = w;
+      });
+      if (!Cfg::kOver) put_tile(kChunk + tok, g);
+      if (c > 0) load_do(c - 1);
+    }
+    wait(&done[0], d);
+    if (Cfg::kOver) __syncthreads();  // and has been kept
+    umma_fence_after();
+    if (is_y) {
+      tmem_ld(my_tmem, x);
+#pragma unroll
+      for (int i = 0; i < C; ++i) x[i] *= wb;
+      put_tile(tok, x);
+    } else if (Cfg::kOver) {
+      put_tile(kChunk + tok, g);
+    }
+    fence_async();
+    umma_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+      umma_fence_after();
+      wait(&full_n, d);
+      if (elect_one()) {
+        umma_parts<NS, LV, 8, false>(tmem + 2 * C, umma_desc_a(s_npn, 0), umma_desc_b<C>(s_e), 2 * kMatBytes,
+                                     Cfg::kPart, 2048, 64 * C, 0, umma_idesc<C>(true), 8);
+        umma_commit(&done[1]);
+      }
+      __syncwarp();
+    }
+    if (!Cfg::kOver && !is_y) keep_ds(c);
+    wait(&done[1], d);
+    umma_fence_after();
+    if (loads && d + 1 < p.chunks) load_n(d + 1);  // N and PN are used up
+
+    tmem_ld(my_tmem + 2 * C, x);  // dV, in both halves of the lanes
+    if (is_y) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) g[i] = x[i] * -ge;
+      put_tile(tok, g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) g[i] *= ge * p.scale;
+      put_tile(kChunk + tok, g);
+    }
+    fence_async();
+    umma_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+      umma_fence_after();
+      if (elect_one()) {
+        umma_parts<NP, LV, 8, false>(tmem + 4 * C, umma_desc_a(s_kq, kHalfTile), umma_desc_b<C>(s_e),
+                                     kTileKQ, Cfg::kPart, 2048, 64 * C, 0, umma_idesc<C>(true), 8);
+        umma_commit(&done[2]);
+      }
+      __syncwarp();
+    }
+    // meanwhile: dV to the caller and as parts
+    if (is_y) {
+      split_row<NS>(x, [&](int q, int u, const uint4& w) {
+        if ((u & ~1) * 8 < nval)
+          *reinterpret_cast<uint4*>(strip_ptr(p.dv_parts, c, u, NS, q, kStrip) +
+                                    strip_at(0, tok, u & 1)) = w;
+      });
+    } else if (c * kChunk + tok < p.L) {
+      store_row<T>(static_cast<T*>(p.dv_out) + row0 + c * kChunk * vstride, nval, x);
+    }
+    wait(&done[2], d);
+    umma_fence_after();
+    tmem_ld(my_tmem + 4 * C, x);
+#pragma unroll
+    for (int i = 0; i < C; ++i) S[i] = fmaf(total, S[i], x[i]);
+  }
+
+  if (p.dinitial != nullptr && ok && dk < p.dk)
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (i < nval) p.dinitial[(bh * p.dv + dv0 + i) * p.dk + dk] = S[i];
+  // No copy may land after the CTA is gone: at once, unless a wait gave up.
+  if (loads) {
+    for (int64_t d = max((int64_t)0, p.chunks - Cfg::kSt); d < p.chunks; ++d)
+      mbar_wait_soon(&full_kq[d % Cfg::kSt], (uint32_t)((d / Cfg::kSt) & 1));
+    mbar_wait_soon(&full_n, (uint32_t)((p.chunks - 1) & 1));
+  }
+  umma_fence_before();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem));
 }
 
 // ------------------------------------------------------------------ gradients of a chunk
 struct GradParams {
-  const __nv_bfloat16* q_tiles;
-  const __nv_bfloat16* k_tiles;
+  const __nv_bfloat16* kq_tiles;
   const __nv_bfloat16* do_parts;
   const __nv_bfloat16* e_parts;
   const __nv_bfloat16* dv_parts;
@@ -626,20 +347,19 @@ struct GradParams {
 
 constexpr int kGradThreads = 512;
 
-// 16 warps.  The three 64 x dk sums (dQ, R, W) are cut into tiles of 16 MT
+// 16 warps.  The three 64 x dk sums (dQ, R, W) are cut into tiles of 32
 // rows x 16 columns, H and X into tiles of 16 x 16; all stay in registers
 // while dO, dV, E, S0 and dS pass once through a ring of bulk copies, KS
 // strips of 16 values at a time.  One CTA per SM takes chunk after chunk, and
 // the ring runs on into the next chunk during the second phase: with a CTA
 // per chunk the copies of a chunk and its products took turns.
-template <int NP, int LV, int DKP>
+template <int NP, int LV>
 struct GradCfg {
   static constexpr int NS = LV + 1;
-  static constexpr int MT = DKP / 64;           // m tiles of a warp in the 64 x dk sums
-  static constexpr int kColW = DKP / 16;        // warps side by side there
-  static constexpr int kTileK = kChunk * DKP * 2;
-  static constexpr int kMat = kChunk * kChunk * 2;
-  static constexpr int kRows = 16 * DKP * 2;  // 16 rows of a part of S0 or dS
+  static constexpr int MT = 2;     // m tiles of a warp in the 64 x dk sums
+  static constexpr int kColW = 8;  // warps side by side there
+  static constexpr int kMat = kMatBytes;
+  static constexpr int kRows = 2 * kStrip;  // a strip of a part of S0 or dS
   static constexpr int kOne = (NP + 2 * NS) * kStrip + 2 * NS * kRows;  // one strip's share
   static constexpr int KS = 1;
   // a stage of the ring
@@ -651,8 +371,7 @@ struct GradCfg {
   static_assert(kStage == KS * kOne);
   // K, Q and the decay vectors; the matrices of the second phase (two at a
   // time where four do not fit); the ring
-  static constexpr int oQ = NP * kTileK;
-  static constexpr int oVec = 2 * NP * kTileK;
+  static constexpr int oVec = NP * kTileKQ;
   static constexpr int kVecBytes = kVecCount * kChunk * 4;
   static constexpr int oMats = oVec + (kVecBytes + 127) / 128 * 128;
   static constexpr int kSets = LV == 1 ? 2 : 1;  // of two matrices
@@ -663,10 +382,10 @@ struct GradCfg {
   static_assert(kStages >= 1 && kSmem + 8192 <= 227 * 1024);
 };
 
-template <typename T, int NP, int LV, int DKP>
+template <typename T, int NP, int LV>
 __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradParams p) {
-  using Cfg = GradCfg<NP, LV, DKP>;
-  constexpr int NS = Cfg::NS, NTH = kGradThreads, ROWB = DKP * 2, MROW = kChunk * 2, KS = Cfg::KS;
+  using Cfg = GradCfg<NP, LV>;
+  constexpr int NS = Cfg::NS, NTH = kGradThreads, MROW = kChunk * 2, KS = Cfg::KS;
   constexpr int MT = Cfg::MT, ST = Cfg::kStages, CW = Cfg::kColW;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
@@ -707,7 +426,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   int next_slice = 0;
   auto issue = [&]() {
     const int s = (int)(next % ST);
-    if (next >= ST && !mbar_wait_bounded(&freed[s], (uint32_t)((next / ST - 1) & 1))) return false;
+    if (next >= ST && !mbar_wait_soon(&freed[s], (uint32_t)((next / ST - 1) & 1))) return false;
     const int64_t unit = next_unit;
     const int v0 = next_slice * KS, n = min(KS, strips - v0);
     const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
@@ -715,7 +434,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     bulk_in(at, p.do_parts + (unit * strips + v0) * NP * (kStrip / 2), n * NP * kStrip, &full[s]);
     bulk_in(at + Cfg::oV, p.dv_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
     bulk_in(at + Cfg::oE, p.e_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
-    const int64_t sv = (unit * strips + v0) * NS * 16 * DKP;
+    const int64_t sv = (unit * strips + v0) * NS * (Cfg::kRows / 2);
     bulk_in(at + Cfg::oS, p.s_parts + sv, n * NS * Cfg::kRows, &full[s]);
     bulk_in(at + Cfg::oD, p.ds_parts + sv, n * NS * Cfg::kRows, &full[s]);
     ++next;
@@ -728,10 +447,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   auto issue_kq = [&](int64_t unit) {
     const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
     const int hk = (int)(bh - b * p.heads) / (p.heads / p.key_heads);
-    const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kChunk * DKP);
-    mbar_expect_tx(&full_kq, 2 * NP * Cfg::kTileK + Cfg::kVecBytes);
-    bulk_in(st, p.k_tiles + tile, NP * Cfg::kTileK, &full_kq);
-    bulk_in(st + Cfg::oQ, p.q_tiles + tile, NP * Cfg::kTileK, &full_kq);
+    const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kTileKQ / 2);
+    mbar_expect_tx(&full_kq, NP * kTileKQ + Cfg::kVecBytes);
+    bulk_in(st, p.kq_tiles + tile, NP * kTileKQ, &full_kq);
     bulk_in(st + Cfg::oVec, p.vecs + unit * (kVecCount * kChunk), Cfg::kVecBytes, &full_kq);
   };
   if (tid == kLoader) {
@@ -764,13 +482,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       const uint32_t at = st + Cfg::oRing + s_id * Cfg::kStage;
       // refill the stage of the slice before: every warp is done with it, or nearly
       if (tid == kLoader && ST > 1 && it > 0 && next < total) issue();
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s_id], (uint32_t)((it / ST) & 1)));
+      ok = __all_sync(0xffffffffu, mbar_wait_soon(&full[s_id], (uint32_t)((it / ST) & 1)));
       if (!ok) break;
       for (int kk = 0; kk < n; ++kk) {
         const uint32_t a_g = at + kk * NP * kStrip, a_v = at + Cfg::oV + kk * NS * kStrip,
                        a_e = at + Cfg::oE + kk * NS * kStrip;
-        // this warp's half of dk in the strip's S0 and dS (plus oS, oD)
-        const uint32_t s_half = at + (kk * 2 + col0 / (DKP / 2)) * NS * 16 * DKP;
+        const uint32_t s_strip = at + kk * NS * Cfg::kRows;  // S0's and dS's (plus oS, oD)
         if (lower) {
           uint32_t ag[NP][4], av[NS][4];
 #pragma unroll
@@ -801,7 +518,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           uint32_t sb[NS][4];
 #pragma unroll
           for (int j = 0; j < NS; ++j)
-            ldsm4_t(sb[j], half_bt<DKP>(s_half + Cfg::oS + j * 16 * DKP, lane, col0 % (DKP / 2)));
+            ldsm4(sb[j], strip_b(s_strip + Cfg::oS + j * Cfg::kRows, lane, col0));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             uint32_t ag[NP][4], av[NS][4];
@@ -831,7 +548,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           uint32_t db[NS][4];
 #pragma unroll
           for (int j = 0; j < NS; ++j)
-            ldsm4_t(db[j], half_bt<DKP>(s_half + Cfg::oD + j * 16 * DKP, lane, col0 % (DKP / 2)));
+            ldsm4(db[j], strip_b(s_strip + Cfg::oD + j * Cfg::kRows, lane, col0));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             uint32_t ae[NS][4];
@@ -853,12 +570,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       // <S0, dS> over this slice (the same place of every part: swizzle does not matter)
       for (int i = above * 32 + lane; !lower && i < n * Cfg::kRows / 16; i += 6 * 32) {
         float x[8] = {}, y[8] = {};
-        // 16-byte piece i % DKP of half i / DKP (16 rows of DKP bytes)
-        const uint32_t at_i = at + i / DKP * NS * 16 * DKP + i % DKP * 16;
 #pragma unroll
         for (int q = NS - 1; q >= 0; --q) {
-          const uint4 u = lds128(at_i + Cfg::oS + q * 16 * DKP);
-          const uint4 v = lds128(at_i + Cfg::oD + q * 16 * DKP);
+          const uint4 u = lds128(at + Cfg::oS + q * Cfg::kRows + i * 16);
+          const uint4 v = lds128(at + Cfg::oD + q * Cfg::kRows + i * 16);
           const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -877,7 +592,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
     if (lane == 0) s_dot[warp] = dot;
-    ok = ok && mbar_wait_bounded(&full_kq, (uint32_t)(done & 1));
+    ok = ok && mbar_wait_soon(&full_kq, (uint32_t)(done & 1));
     if (__syncthreads_or(!ok)) {
       ok = false;
       break;
@@ -931,17 +646,20 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     put_mats(0);
     if (Cfg::kSets == 2) put_mats(1);
     // an element pair of K or Q as fp32 (the sum of its parts)
-    auto kq_pair = [&](int off, int row, int col) {
+    auto kq_pair = [&](int row, int col) {  // Q: rows 64..
       float2 v = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = NP - 1; i >= 0; --i) {
         const uint32_t w = *reinterpret_cast<const uint32_t*>(
-            dsm + off + i * Cfg::kTileK + tile_at<ROWB>(0, row, col / 8) + (col % 8) * 2);
+            dsm + i * kTileKQ + (col >> 6) * kHalfTile + tile_at<128>(0, row, (col & 63) / 8) +
+            (col % 8) * 2);
         v.x += bf16_lo(w);
         v.y += bf16_hi(w);
       }
       return v;
     };
+    // this warp's columns of K (and, 64 rows on, Q) as a B operand
+    const uint32_t kq_cols = st + (col0 >> 6) * kHalfTile;
     // sums over a warp's columns of a row, one value per row and warp column
     auto put_row = [&](int which, int row, float v) {
       v += __shfl_xor_sync(0xffffffffu, v, 1);
@@ -957,7 +675,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
         float sum = 0.f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const float2 kv = kq_pair(0, i, col0 + n * 8 + 2 * t4);
+          const float2 kv = kq_pair(i, col0 + n * 8 + 2 * t4);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             aq[m][n][2 * r + c] *= ge * p.scale;
@@ -976,7 +694,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       if (kk * 16 > row0 + 16 * MT - 1) break;
       uint32_t kb[NP][4];
 #pragma unroll
-      for (int j = 0; j < NP; ++j) ldsm4_t(kb[j], at_bt<ROWB>(st + j * Cfg::kTileK, lane, col0, kk));
+      for (int j = 0; j < NP; ++j) ldsm4_t(kb[j], at_bt<128>(kq_cols + j * kTileKQ, lane, col0 & 63, kk));
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         Step<LV == 2, 4> s;
@@ -1013,8 +731,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       uint32_t kb[NP][4], qb[NP][4];
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        ldsm4_t(kb[j], at_bt<ROWB>(st + j * Cfg::kTileK, lane, col0, kk));
-        ldsm4_t(qb[j], at_bt<ROWB>(st + Cfg::oQ + j * Cfg::kTileK, lane, col0, kk));
+        ldsm4_t(kb[j], at_bt<128>(kq_cols + j * kTileKQ, lane, col0 & 63, kk));
+        ldsm4_t(qb[j], at_bt<128>(kq_cols + j * kTileKQ + kChunk * 128, lane, col0 & 63, kk));
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -1053,7 +771,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int col = col0 + n * 8 + 2 * t4;
-          const float2 kv = kq_pair(0, i, col), qv = kq_pair(Cfg::oQ, i, col);
+          const float2 kv = kq_pair(i, col), qv = kq_pair(kChunk + i, col);
           const float q0 = aq[m][n][2 * r], q1 = aq[m][n][2 * r + 1];
           const float r0 = ar[m][n][2 * r], r1 = ar[m][n][2 * r + 1];
           const float w0 = aw[m][n][2 * r], w1 = aw[m][n][2 * r + 1];
@@ -1127,9 +845,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   // After a wait that gave up: no copy may land after the CTA is gone.
   if (!ok && tid == kLoader) {
     for (int64_t j = max((int64_t)0, next - ST); j < next; ++j)
-      mbar_wait_bounded(&full[j % ST], (uint32_t)((j / ST) & 1));
-    mbar_wait_bounded(&full_kq, 0);
-    mbar_wait_bounded(&full_kq, 1);
+      mbar_wait_soon(&full[j % ST], (uint32_t)((j / ST) & 1));
+    mbar_wait_soon(&full_kq, 0);
+    mbar_wait_soon(&full_kq, 1);
   }
 }
 
@@ -1168,21 +886,21 @@ __global__ void __launch_bounds__(256) delta_group_kernel(const GroupParams p) {
 }
 
 // ------------------------------------------------------------------ host side
-template <typename T, int LV, int DKP, int NW>
-cudaError_t rev_nw(const DeltaArgs& a, RevParams& p, int64_t bh) {
-  using Cfg = RevCfg<kParts<T>, LV, DKP, NW>;
-  auto kern = delta_rev_kernel<T, kParts<T>, LV, DKP, NW>;
+template <typename T, int LV, int C>
+cudaError_t launch_rev_as(const DeltaArgs& a, RevParams& r, int64_t bh) {
+  using Cfg = RevCfg<T, LV, C>;
+  auto kern = delta_rev_kernel<T, LV, C>;
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
-  p.slices = (int)((a.dv + NW * 16 - 1) / (NW * 16));
-  return launch_pdl(kern, (unsigned)(bh * p.slices), NW * 96, Cfg::kSmem, a.stream, p);
+  r.slices = (int)((a.dv + 2 * C - 1) / (2 * C));
+  return launch_pdl(kern, (unsigned)(bh * r.slices), kRevThreads, Cfg::kSmem, a.stream, r);
 }
 
-template <typename T, int LV, int DKP>
+template <typename T, int LV>
 cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_t nb) {
   constexpr int NP = kParts<T>;
-  cudaError_t e = delta_fwd_pass<T, LV, DKP>(a, pl, b0, nb, true);
+  cudaError_t e = delta_fwd_pass<T, LV>(a, pl, b0, nb, true);
   if (e != cudaSuccess) return e;
   char* ws = static_cast<char*>(a.workspace);
   auto bf = [&](int64_t off) { return reinterpret_cast<__nv_bfloat16*>(ws + off); };
@@ -1191,20 +909,9 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   const int64_t tok = nb * a.seqlen, bh = nb * a.heads;
 
   RevParams r{};
-  if constexpr (NP > 1) {
-    SplitParams sp{static_cast<const T*>(a.grad_out) + v0, bf(pl.grad_rows), tok * a.heads * a.dv};
-    const unsigned grid = (unsigned)std::min<int64_t>((sp.n + 2047) / 2048, 16 * a.num_sms);
-    e = launch_pdl(delta_split_kernel<T>, grid, 256, 0, a.stream, sp);
-    if (e != cudaSuccess) return e;
-    r.grad = sp.dst;
-    r.grad_stride = sp.n;
-  } else {
-    r.grad = static_cast<const __nv_bfloat16*>(a.grad_out) + v0;
-  }
-  r.q_tiles = bf(pl.q_tiles);
-  r.k_tiles = bf(pl.k_tiles);
-  r.n_mat = bf(pl.n_mat);
-  r.p_mat = bf(pl.p_mat);
+  r.kq_tiles = bf(pl.kq_tiles);
+  r.grad = static_cast<const T*>(a.grad_out) + v0;
+  r.npn = bf(pl.npn);
   r.vecs = reinterpret_cast<const float*>(ws + pl.vecs);
   r.grad_final = a.grad_final ? a.grad_final + s0 : nullptr;
   r.dinitial = a.dinitial ? a.dinitial + s0 : nullptr;
@@ -1219,17 +926,13 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   r.dk = (int)a.dk;
   r.dv = (int)a.dv;
   r.scale = a.scale;
-  // chain warps per CTA as in the forward; where four do not fit, two
-  const bool two = !RevCfg<NP, LV, DKP, 4>::kFits || bh * ((a.dv + 31) / 32) <= a.num_sms;
-  if constexpr (RevCfg<NP, LV, DKP, 4>::kFits)
-    e = two ? rev_nw<T, LV, DKP, 2>(a, r, bh) : rev_nw<T, LV, DKP, 4>(a, r, bh);
-  else
-    e = rev_nw<T, LV, DKP, 2>(a, r, bh);
+  // as launch_scan chooses
+  e = bh * ((a.dv + 31) / 32) <= a.num_sms ? launch_rev_as<T, LV, 16>(a, r, bh)
+                                           : launch_rev_as<T, LV, 32>(a, r, bh);
   if (e != cudaSuccess) return e;
 
   GradParams g{};
-  g.q_tiles = r.q_tiles;
-  g.k_tiles = r.k_tiles;
+  g.kq_tiles = r.kq_tiles;
   g.do_parts = r.do_parts;
   g.e_parts = bf(pl.e_parts);
   g.dv_parts = r.dv_parts;
@@ -1254,8 +957,8 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   g.dk = (int)a.dk;
   g.dv = (int)a.dv;
   g.scale = a.scale;
-  using GC = GradCfg<NP, LV, DKP>;
-  auto kern = delta_grad_kernel<T, NP, LV, DKP>;
+  using GC = GradCfg<NP, LV>;
+  auto kern = delta_grad_kernel<T, NP, LV>;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC::kSmem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kern, (unsigned)std::min<int64_t>(g.units, a.num_sms), kGradThreads, GC::kSmem,
@@ -1278,8 +981,7 @@ template <typename T, int LV>
 cudaError_t bwd_all(const DeltaArgs& a, const DeltaPlan& pl) {
   for (int64_t b0 = 0; b0 < a.batch; b0 += pl.batch) {
     const int64_t nb = std::min(pl.batch, a.batch - b0);
-    const cudaError_t e = pl.dkp == 64 ? bwd_pass<T, LV, 64>(a, pl, b0, nb)
-                                       : bwd_pass<T, LV, 128>(a, pl, b0, nb);
+    const cudaError_t e = bwd_pass<T, LV>(a, pl, b0, nb);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

@@ -252,16 +252,14 @@ struct DeltaPlan {
   int64_t chunks;    // per head and sequence
   int64_t batch;     // sequences per pass (the passes share the workspace)
   int np, ns;        // bf16 parts of the inputs / of fp32 operands
-  int dkp;           // dk padded to 64 or 128
   // as the tiles lie in shared memory (bf16; swizzled rows):
-  int64_t q_tiles, k_tiles;            // [key head][chunk][np][64][dkp]
-  int64_t n_mat, p_mat;                // [head][chunk][ns][64][64]
+  int64_t kq_tiles;                    // [key head][chunk][np][half][K, Q: 128 rows][64]
+  int64_t npn;                         // [head][chunk][ns][N, PN: 128 rows][64]
   int64_t vecs;                        // [head][chunk][kVecCount][64] fp32
-  // backward; dvp: dv padded to 16
-  int64_t grad_rows;                   // [np][batch x seqlen x heads x dv], np > 1
+  // backward, strips of 16 values (dvp: dv padded to 16)
   int64_t do_parts;                    // [head][chunk][dvp / 16][np][64][16]
   int64_t e_parts, dv_parts;           // [head][chunk][dvp / 16][ns][64][16]
-  int64_t s_parts, ds_parts;           // [head][chunk][dvp / 16][half][ns][16][dkp / 2]
+  int64_t s_parts, ds_parts;           // [head][chunk][dvp / 16][ns][128][16]
   int64_t dq_part, dk_part;            // [batch x seqlen][heads][dk] fp32 (backward, shared heads)
   int64_t bytes;
 };
