@@ -251,6 +251,88 @@ delta_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   return {dq, dk, dv, dg, db, di};
 }
 
+// delta.GatedDelta, in C++: a training step's layer is half a dozen kernels,
+// and a Python autograd function costs as much as some of them.
+std::tuple<at::Tensor, at::Tensor> quantize8(const at::Tensor& x);
+at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& steps, at::ScalarType dtype);
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+struct GatedDelta : public torch::autograd::Function<GatedDelta> {
+  static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k,
+                               const Variable& v, const Variable& log_decay, const Variable& beta,
+                               const c10::optional<Variable>& state, double scale,
+                               bool return_state, bool checkpoint8) {
+    c10::optional<at::Tensor> held;
+    if (state) held = state->to(at::kFloat).contiguous();
+    auto [out, last] = delta_forward(q, k, v, log_decay, beta, held, scale, return_state, c10::nullopt);
+    variable_list kept;
+    if (checkpoint8) {
+      for (const Variable* x : {&q, &k, &v}) {
+        auto [codes, steps] = quantize8(*x);
+        kept.push_back(codes);
+        kept.push_back(steps);
+      }
+    } else {
+      kept = {q, k, v};
+    }
+    kept.push_back(log_decay);
+    kept.push_back(beta);
+    kept.push_back(held ? *held : at::Tensor());
+    ctx->save_for_backward(kept);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["checkpoint8"] = checkpoint8;
+    ctx->saved_data["dtype"] = (int64_t)v.scalar_type();
+    ctx->saved_data["state_dtype"] = state ? (int64_t)state->scalar_type() : (int64_t)-1;
+    ctx->set_materialize_grads(false);
+    if (return_state) return {out, *last};
+    return {out};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const at::Tensor none;
+    const at::Tensor grad_final = grads.size() > 1 ? grads[1] : none;
+    if (!grads[0].defined() && !grad_final.defined()) return variable_list(9);
+    variable_list kept = ctx->get_saved_variables();
+    const size_t n = kept.size();
+    at::Tensor q, k, v;
+    if (ctx->saved_data["checkpoint8"].toBool()) {
+      const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+      q = dequantize8(kept[0], kept[1], dtype);
+      k = dequantize8(kept[2], kept[3], dtype);
+      v = dequantize8(kept[4], kept[5], dtype);
+    } else {
+      q = kept[0];
+      k = kept[1];
+      v = kept[2];
+    }
+    const at::Tensor grad_out = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(v);
+    c10::optional<at::Tensor> initial, gf;
+    if (kept[n - 1].defined()) initial = kept[n - 1];
+    if (grad_final.defined()) gf = grad_final.to(at::kFloat).contiguous();
+    const int64_t state_dtype = ctx->saved_data["state_dtype"].toInt();
+    const bool need = state_dtype >= 0 && ctx->needs_input_grad(5);
+    auto [dq, dk, dv, dg, db, di] =
+        delta_backward(q, k, v, kept[n - 3], kept[n - 2], grad_out, initial, gf,
+                       ctx->saved_data["scale"].toDouble(), need);
+    at::Tensor dstate;
+    if (di) dstate = di->to((at::ScalarType)state_dtype);
+    return {dq, dk, dv, dg, db, dstate, none, none, none};
+  }
+};
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> gated_delta(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+    const at::Tensor& beta, const c10::optional<at::Tensor>& state, double scale,
+    bool return_state, bool checkpoint8) {
+  const variable_list r =
+      GatedDelta::apply(q, k, v, log_decay, beta, state, scale, return_state, checkpoint8);
+  if (return_state) return {r[0], r[1]};
+  return {r[0], c10::nullopt};
+}
+
 // ---------------------------------------------------------------- 8-bit checkpoints
 std::tuple<at::Tensor, at::Tensor> quantize8(const at::Tensor& x) {
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
@@ -281,6 +363,73 @@ at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& steps, at::Sca
   return out;
 }
 
+// ops.PScanChannelsLast8, in C++ for the same reason.
+struct Scan8 : public torch::autograd::Function<Scan8> {
+  // Same conditions as ops.validate_channels_last.
+  static void check(const at::Tensor& gates, const at::Tensor& tokens) {
+    const at::Tensor* all[2] = {&gates, &tokens};
+    static const char* const names[2] = {"gates", "tokens"};
+    for (int i = 0; i < 2; ++i) {
+      TORCH_CHECK(all[i]->is_cuda(), names[i], " must be a CUDA tensor");
+      TORCH_CHECK(all[i]->is_contiguous(), names[i], " must be contiguous");
+      TORCH_CHECK(all[i]->scalar_type() == at::kFloat || all[i]->scalar_type() == at::kHalf ||
+                      all[i]->scalar_type() == at::kBFloat16,
+                  names[i], " must be float16 or bfloat16 or float32");
+    }
+    TORCH_CHECK(tokens.dim() == 3, "tokens must be 3-D (batch, seqlen, dim), got ", tokens.sizes());
+    TORCH_CHECK(gates.sizes() == tokens.sizes() && gates.scalar_type() == tokens.scalar_type() &&
+                    gates.device() == tokens.device(),
+                "gates and tokens must have the same shape, dtype and device");
+    TORCH_CHECK(tokens.size(1) >= 1, "seqlen must be >= 1 (got ", tokens.size(1), ")");
+    const int64_t vec = 16 / tokens.element_size();
+    TORCH_CHECK(tokens.size(2) % vec == 0, "dim must be a multiple of ", vec, " for ",
+                tokens.scalar_type(), " (got ", tokens.size(2), ")");
+  }
+
+  static at::Tensor workspace_of(const at::Tensor& t, bool backward) {
+    const int64_t n = fpscan_cl_workspace_bytes(t.size(0), t.size(1), t.size(2), dtype_code(t), backward);
+    return at::empty({std::max<int64_t>(n, 256)}, t.options().dtype(at::kByte).requires_grad(false));
+  }
+
+  static Variable forward(AutogradContext* ctx, const Variable& gates, const Variable& tokens) {
+    check(gates, tokens);
+    const c10::cuda::CUDAGuard guard(tokens.device());
+    const int64_t b = tokens.size(0), l = tokens.size(1), d = tokens.size(2);
+    const auto opts = tokens.options().requires_grad(false);
+    at::Tensor out = at::empty_like(tokens);
+    // rows of codes start on 16-byte boundaries, as the kernels' tile copies need
+    at::Tensor codes = at::empty({b, l, (d + 15) / 16 * 16}, opts.dtype(at::kChar));
+    at::Tensor steps = at::empty({b, (l + 7) / 8, d * tokens.element_size() / 16}, opts.dtype(at::kFloat));
+    if (b && d) {
+      const at::Tensor ws = workspace_of(tokens, false);
+      raise_on(fpscan_scan_fwd_cl8(gates.data_ptr(), tokens.data_ptr(), out.data_ptr(),
+                                   codes.data_ptr(), steps.data_ptr<float>(), b, l, d,
+                                   dtype_code(tokens), ws.data_ptr(), ws.numel(),
+                                   at::cuda::getCurrentCUDAStream().stream()),
+               "fpscan_scan_fwd_cl8");
+    }
+    ctx->save_for_backward({gates, codes, steps});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list kept = ctx->get_saved_variables();
+    const at::Tensor gates = kept[0], go = grads[0].contiguous();
+    check(gates, go);
+    const c10::cuda::CUDAGuard guard(go.device());
+    at::Tensor dgates = at::empty_like(go), dtokens = at::empty_like(go);
+    if (go.size(0) && go.size(2)) {
+      const at::Tensor ws = workspace_of(go, true);
+      raise_on(fpscan_scan_bwd_cl8(gates.data_ptr(), kept[1].data_ptr(), kept[2].data_ptr<float>(),
+                                   go.data_ptr(), dgates.data_ptr(), dtokens.data_ptr(), go.size(0),
+                                   go.size(1), go.size(2), dtype_code(go), ws.data_ptr(), ws.numel(),
+                                   at::cuda::getCurrentCUDAStream().stream()),
+               "fpscan_scan_bwd_cl8");
+    }
+    return {dgates, dtokens};
+  }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -295,6 +444,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("delta_backward", &delta_backward,
         "delta_backward(q, k, v, log_decay, beta, grad_out, initial, grad_final, scale, need_initial)"
         " -> (dq, dk, dv, dlog_decay, dbeta, dinitial)");
+  m.def("gated_delta", &gated_delta,
+        "gated_delta(q, k, v, log_decay, beta, state, scale, return_state, checkpoint8) -> (out, final),"
+        " differentiable");
+  m.def("pscan_channels_last8",
+        [](const at::Tensor& gates, const at::Tensor& tokens) { return Scan8::apply(gates, tokens); },
+        "pscan_channels_last8(gates, tokens) -> out, differentiable, the output kept in 8 bits");
   m.def("quantize8", &quantize8, "quantize8(x) -> (codes, steps)");
   m.def("dequantize8", [](const at::Tensor& codes, const at::Tensor& steps, py::object dtype) {
     return dequantize8(codes, steps, torch::python::detail::py_object_to_dtype(dtype));

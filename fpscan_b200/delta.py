@@ -31,7 +31,7 @@ import torch
 
 from . import _lib
 from .checkpoint8 import dequantize8, quantize8
-from .ops import _EXT, DTYPE_CODES, _check_input, _fn, _launch, nvtx_range
+from .ops import _EXT, DTYPE_CODES, NVTX, _check_input, _fn, _launch, nvtx_range
 
 __all__ = ["gated_delta", "gated_delta_forward", "gated_delta_step"]
 
@@ -190,7 +190,7 @@ def gated_delta_backward(q, k, v, log_decay, beta, grad_out, initial_state=None,
 
 
 class GatedDelta(torch.autograd.Function):
-    """Differentiable gated delta rule.  Saves its inputs (q, k and v in 8 bits with ``checkpoint8``) and
+    """Differentiable gated delta rule (the compiled binding has the same one).  Saves its inputs (q, k and v in 8 bits with ``checkpoint8``) and
     recomputes the chunks' states in the backward pass."""
 
     @staticmethod
@@ -229,5 +229,8 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: to
     ``return_state``; differentiable in all five inputs, the initial and the final state.
     ``checkpoint8=True`` keeps q, k and v for the backward pass in 8 bits (``quantize8``): gradients are
     those of the rule at the values that these stand for."""
-    return GatedDelta.apply(q, k, v, log_decay, beta, initial_state, _scale(scale, q), bool(return_state),
-                            bool(checkpoint8))
+    scale, return_state, checkpoint8 = _scale(scale, q), bool(return_state), bool(checkpoint8)
+    if not NVTX and _tensors(q, k, v, log_decay, beta, initial_state):
+        out, final = _EXT.gated_delta(q, k, v, log_decay, beta, initial_state, scale, return_state, checkpoint8)
+        return (out, final) if return_state else out
+    return GatedDelta.apply(q, k, v, log_decay, beta, initial_state, scale, return_state, checkpoint8)

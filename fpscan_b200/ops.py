@@ -551,7 +551,8 @@ def _cl8_workspace(t: torch.Tensor, backward: bool) -> torch.Tensor:
 
 class PScanChannelsLast8(torch.autograd.Function):
     """``PScanChannelsLast`` that keeps its output for the backward pass in 8 bits, written and read inside
-    the scan kernels: one step per block of 8 timesteps x one 16-byte channel vector."""
+    the scan kernels: one step per block of 8 timesteps x one 16-byte channel vector.  (The compiled binding
+    has the same one.)"""
 
     @staticmethod
     def forward(ctx, gates, tokens):
@@ -593,5 +594,7 @@ def pscan_channels_last(gates: torch.Tensor, tokens: torch.Tensor,
     """Differentiable scan along dim 1 of (batch, seqlen, dim) tensors.  ``checkpoint8=True`` keeps the
     output for the backward pass in 8 bits: grad_gates is then that of the values these stand for."""
     if checkpoint8:
+        if _EXT is not None and not NVTX and isinstance(gates, torch.Tensor) and isinstance(tokens, torch.Tensor):
+            return _EXT.pscan_channels_last8(gates, tokens)
         return PScanChannelsLast8.apply(gates, tokens)
     return PScanChannelsLast.apply(gates, tokens)

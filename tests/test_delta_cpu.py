@@ -61,7 +61,7 @@ def _addresses(n, step=1 << 20):
     return [(i + 1) * step for i in range(n)]
 
 
-def _fwd(ptr=None, ws=1 << 20, dtype=0, wide=0, **change):
+def _fwd(ptr=None, ws=1 << 24, dtype=0, wide=0, **change):
     d = dict(GOOD, **change)
     p = _addresses(9) if ptr is None else ptr
     lib = _lib.load()
@@ -103,7 +103,8 @@ def test_c_abi_backward_and_step_refuse():
     lib = _lib.load()
     p = _addresses(15)
     p[10] = p[2]  # dv over v
-    assert lib.fpscan_delta_bwd(*p[:14], *GOOD.values(), 1.0, 0, 0, p[14], 1 << 20, None) == 1
+    need = lib.fpscan_delta_workspace_bytes(*GOOD.values(), 0, 0, 1)
+    assert lib.fpscan_delta_bwd(*p[:14], *GOOD.values(), 1.0, 0, 0, p[14], need, None) == 1
     assert b"overlaps" in lib.fpscan_last_error()
     assert lib.fpscan_delta_bwd(*_addresses(14), *GOOD.values(), 1.0, 0, 0, 0, 0, None) == 1
     p = _addresses(8)
