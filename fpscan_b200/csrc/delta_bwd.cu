@@ -851,6 +851,501 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   }
 }
 
+// ------------------------------------------------------------------ gradients of a chunk, tcgen05
+// What delta_grad_kernel computes, for 16-bit results (LV = 1).  The sums are
+// taken transposed, 128 rows of dk by 64 tokens, so that every product has
+// 128 rows, and the strips are operands as they lie (32-byte rows and swizzle,
+// 16 values of k each):
+//     S0 [dO; dV]^T  -> dQ | R,   dS E^T -> W,   [dO; dV] E^T -> [H; X]
+// strip by strip as they arrive, then
+//     K^T [Hb; Xb]^T -> dQ | R,   [K; Q]^T [Xd; Hs] -> W
+// with the matrices that the warps make of H and X.  20 warps: sixteen take the
+// first sums into registers (the next chunk's first products may then start),
+// make the matrices, and turn the results around through shared memory for
+// rows of tokens; one issues the strips' copies and all products, two take
+// <S0, dS> from the strips as they pass, and one loads K, Q and the vectors
+// and closes a chunk (dlog_decay, dbeta) behind the others.
+constexpr int kTcThreads = 640;
+
+template <int NP>
+struct TcGradCfg {
+  static constexpr int NS = 2;
+  // a stage: parts p of [dO; dV] (dO's second part is zeros where NP = 1), E, S0, dS
+  static constexpr int oE = 2 * 2 * kStrip, oS = oE + NS * kStrip, oD = oS + NS * 2 * kStrip;
+  static constexpr int kStage = oD + NS * 2 * kStrip;
+  static constexpr int kTx = (NP + 2 * NS) * kStrip + 2 * NS * 2 * kStrip;
+  // K and Q; two matrices of two parts, then over them three sums of 64 x 128
+  // fp32; the ring; decay vectors, those of the next chunk too
+  static constexpr int oM = NP * kTileKQ, kSum = kChunk * 512;
+  static constexpr int kMatP = 128 * 128;  // a part of [Hb; Xb] or [Xd; Hs]
+  static constexpr int oRing = oM + 3 * kSum;
+  static_assert(2 * NS * kMatP <= 3 * kSum);
+  static constexpr int kVecBytes = kVecCount * kChunk * 4;
+  static constexpr int kRoom = 227 * 1024 - 1024 - 3 * 1024 - 2 * kVecBytes;
+  static constexpr int kStages = (kRoom - oRing) / kStage < 4 ? (kRoom - oRing) / kStage : 4;
+  static constexpr int oVec = oRing + kStages * kStage;
+  static constexpr int kSmem = oVec + 2 * kVecBytes + 1024;
+  static_assert(kStages >= 2 && kSmem + 3 * 1024 <= 227 * 1024);
+};
+
+// K-major operand of strips: 32-byte rows and swizzle, 16 values of k.
+__device__ __forceinline__ uint64_t umma_desc_strip(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(1) << 16) | ((uint64_t)(256 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(6) << 61);
+}
+__host__ __device__ constexpr uint32_t umma_idesc_n(bool ta, bool tb, int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((ta ? 1u : 0u) << 15) | ((tb ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const GradParams p) {
+  constexpr int NP = kParts<T>;
+  using Cfg = TcGradCfg<NP>;
+  constexpr int NS = Cfg::NS, ST = Cfg::kStages;
+  extern __shared__ __align__(128) unsigned char dsm_raw[];
+  unsigned char* dsm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t st = smem_addr(dsm);
+  const uint32_t s_t1 = st + Cfg::oM, s_t2 = s_t1 + NS * Cfg::kMatP;
+  __shared__ __align__(8) uint64_t full[ST], freed[ST], full_kq, full_vec[2], dots[2], done1, mats,
+      done2, used_kq;
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_reads[2][kChunk], s_writes[2][kChunk], s_dot[2][2], s_sum[2][16];
+
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
+  const int strips = (p.dv + 15) / 16;
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&freed[i], 1 + 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full_vec[i], 1);
+      mbar_init(&dots[i], 2);
+    }
+    mbar_init(&full_kq, 1);
+    mbar_init(&done1, 1);
+    mbar_init(&mats, 16);
+    mbar_init(&done2, 1);
+    mbar_init(&used_kq, 16);
+    fence_mbar_init();
+  }
+  if (NP == 1)  // dO's second part
+    for (int i = tid; i < ST * kStrip / 16; i += kTcThreads)
+      sts128(st + Cfg::oRing + i / (kStrip / 16) * Cfg::kStage + 2 * kStrip + i % (kStrip / 16) * 16,
+             make_uint4(0, 0, 0, 0));
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_addr(&s_tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_async();
+  umma_fence_before();
+  __syncthreads();
+  umma_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint32_t t_w = tmem + 128, t_hx = tmem + 192, t_qr2 = tmem + 256, t_w2 = tmem + 384;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int64_t mine = (p.units - blockIdx.x + gridDim.x - 1) / gridDim.x;  // chunks of this CTA
+  bool ok = true;  // as in delta_scan_kernel
+  auto wait = [&](uint64_t* bar, int64_t phase) {
+    if (ok) ok = mbar_wait_soon(bar, (uint32_t)(phase & 1));
+  };
+
+  if (warp == 16) {
+    // ---------------------------------------------------------- copies and products
+    const int64_t total = mine * strips;
+    int64_t next = 0, next_unit = blockIdx.x;
+    int next_strip = 0;
+    auto load = [&]() {  // of the next strip, by one lane
+      const int s = (int)(next % ST);
+      const int64_t at_strip = next_unit * strips + next_strip;
+      const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
+      mbar_expect_tx(&full[s], Cfg::kTx);
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        bulk_in(at + i * 2 * kStrip, p.do_parts + (at_strip * NP + i) * (kStrip / 2), kStrip, &full[s]);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        bulk_in(at + (2 * i + 1) * kStrip, p.dv_parts + (at_strip * NS + i) * (kStrip / 2), kStrip,
+                &full[s]);
+      bulk_in(at + Cfg::oE, p.e_parts + at_strip * NS * (kStrip / 2), NS * kStrip, &full[s]);
+      bulk_in(at + Cfg::oS, p.s_parts + at_strip * NS * kStrip, NS * 2 * kStrip, &full[s]);
+      bulk_in(at + Cfg::oD, p.ds_parts + at_strip * NS * kStrip, NS * 2 * kStrip, &full[s]);
+    };
+    auto advance = [&]() {
+      ++next;
+      if (++next_strip == strips) {
+        next_strip = 0;
+        next_unit += gridDim.x;
+      }
+    };
+    auto test = [&](uint64_t* bar, int64_t phase) {  // one answer for the warp
+      return __shfl_sync(0xffffffffu, mbar_test(bar, (uint32_t)(phase & 1)) ? 1 : 0, 0) != 0;
+    };
+    // Loads what may be, and waits only for the stage of strip `it` itself.
+    auto refill = [&](int64_t it) {
+      while (next < min(total, it + ST)) {
+        const int64_t before = next - ST;
+        if (before >= 0) {
+          if (next <= it)
+            wait(&freed[before % ST], before / ST);
+          else if (!test(&freed[before % ST], before / ST))
+            return;
+        }
+        if (lane == 0) load();
+        advance();
+      }
+    };
+    refill(0);
+    int64_t it = 0;
+    for (int64_t k = 0; k < mine; ++k) {
+      for (int sl = 0; sl < strips; ++sl, ++it) {
+        const int s = (int)(it % ST);
+        wait(&full[s], it / ST);
+        __syncwarp();
+        if (elect_one()) {
+          const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
+          const uint64_t dv = umma_desc_strip(at), e = umma_desc_strip(at + Cfg::oE),
+                         s0 = umma_desc_strip(at + Cfg::oS), ds = umma_desc_strip(at + Cfg::oD);
+          constexpr uint32_t pd = 2 * kStrip >> 4, pe = kStrip >> 4, ps = 2 * kStrip >> 4;  // parts
+          const bool on = sl > 0;
+          umma(tmem, s0 + ps, dv, umma_idesc_n(false, false, 128), on);
+          umma(tmem, s0, dv + pd, umma_idesc_n(false, false, 128), true);
+          umma(tmem, s0, dv, umma_idesc_n(false, false, 128), true);
+          umma(t_w, ds + ps, e, umma_idesc_n(false, false, 64), on);
+          umma(t_w, ds, e + pe, umma_idesc_n(false, false, 64), true);
+          umma(t_w, ds, e, umma_idesc_n(false, false, 64), true);
+          umma(t_hx, dv + pd, e, umma_idesc_n(false, false, 64), on);
+          umma(t_hx, dv, e + pe, umma_idesc_n(false, false, 64), true);
+          umma(t_hx, dv, e, umma_idesc_n(false, false, 64), true);
+          umma_commit(&freed[s]);
+          if (sl == strips - 1) umma_commit(&done1);
+        }
+        __syncwarp();
+        refill(it + 1);
+      }
+      wait(&mats, k);
+      wait(&full_kq, k);
+      umma_fence_after();
+      __syncwarp();
+      if (elect_one()) {
+        const uint64_t kt = umma_desc_a(st, kHalfTile), t1 = umma_desc_a(s_t1, 16), t2 = umma_desc_a(s_t2, 16);
+        bool on = false;
+#pragma unroll
+        for (int lv = 1; lv >= 0; --lv)
+#pragma unroll
+          for (int i = 0; i <= lv && i < NP; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              umma(t_qr2, kt + ((i * kTileKQ + ks * 2048) >> 4),
+                   t1 + (((lv - i) * Cfg::kMatP + ks * 32) >> 4), umma_idesc_n(true, false, 128), on);
+              on = true;
+            }
+        on = false;
+#pragma unroll
+        for (int lv = 1; lv >= 0; --lv)
+#pragma unroll
+          for (int i = 0; i <= lv && i < NP; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+              umma(t_w2, kt + ((i * kTileKQ + ks * 2048) >> 4),
+                   t2 + (((lv - i) * Cfg::kMatP + ks * 2048) >> 4), umma_idesc_n(true, true, 64), on);
+              on = true;
+            }
+        umma_commit(&done2);
+      }
+      __syncwarp();
+    }
+    // No copy may land, and no product run, after the CTA is gone: at once,
+    // unless a wait gave up.
+    if (lane == 0) {
+      for (int64_t j = max((int64_t)0, next - ST); j < next; ++j)
+        mbar_wait_soon(&full[j % ST], (uint32_t)((j / ST) & 1));
+      mbar_wait_soon(&done2, (uint32_t)((mine - 1) & 1));
+    }
+  } else if (warp < 16) {
+    // ---------------------------------------------------------- sums, matrices and rows
+    const int quad = warp & 3, t0c = (warp >> 2) * 16;  // this thread's 16 columns
+    const int row = quad * 32 + lane;  // lane of tensor memory: H, X row; row of dk
+    const uint32_t my = ((uint32_t)(quad * 32) << 16) + t0c;
+    float* st0 = reinterpret_cast<float*>(dsm + Cfg::oM);  // 64 tokens x 128, where the matrices were
+    float* st1 = st0 + kChunk * 128;
+    float* st2 = st1 + kChunk * 128;
+    const int64_t kstride = (int64_t)p.key_heads * p.dk;
+    // four values of K (rows 64..: Q) as fp32 (the sum of their parts)
+    auto kq4 = [&](int r, int col) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = NP - 1; i >= 0; --i) {
+        const uint2 w = *reinterpret_cast<const uint2*>(
+            dsm + i * kTileKQ + (col >> 6) * kHalfTile + tile_at<128>(0, r, (col & 63) / 8) + (col % 8) * 2);
+        v.x += bf16_lo(w.x);
+        v.y += bf16_hi(w.x);
+        v.z += bf16_lo(w.y);
+        v.w += bf16_hi(w.y);
+      }
+      return v;
+    };
+    for (int64_t k = 0; k < mine; ++k) {
+      const int64_t unit = blockIdx.x + k * gridDim.x;
+      const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
+      const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
+      const int64_t t0 = chunk * kChunk;
+      const int rows = (int)min((int64_t)kChunk, p.L - t0);
+      const int buf = (int)(k & 1);
+      const float* vec = reinterpret_cast<const float*>(dsm + Cfg::oVec + buf * Cfg::kVecBytes);
+      const float* enter = vec + kVecEnter * kChunk;
+      const float* beta = vec + kVecBeta * kChunk;
+
+      wait(&full_vec[buf], k >> 1);
+      wait(&done1, k);
+      umma_fence_after();
+      float x[16], dq[16], r[16], w[16];
+      {
+        // H (rows 0..63) or X (64..127), row i, columns j: times D; with each
+        // column times beta to [Hb; Xb], without to [Xd; Hs]
+        tmem_ld(t_hx + my, x);
+        const int i = row & 63;
+        const bool is_h = row < 64;
+        const float* hi = vec + kVecCumHi * kChunk;
+        const float* lo = vec + kVecCumLo * kChunk;
+        const float hi_i = hi[i], lo_i = lo[i], f = is_h ? p.scale : -1.f;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const int j = t0c + c;
+          const float d = i > j ? expf((hi_i - hi[j]) + (lo_i - lo[j])) : 1.f;
+          x[c] = i > j || (i == j && is_h) ? x[c] * (d * f) : 0.f;
+        }
+        split_row<NS>(x, [&](int q, int u, const uint4& v) {
+          sts128(tile_at<128>(s_t2 + q * Cfg::kMatP, row ^ 64, t0c / 8 + u), v);
+        });
+#pragma unroll
+        for (int c = 0; c < 16; ++c) x[c] *= beta[t0c + c];
+        split_row<NS>(x, [&](int q, int u, const uint4& v) {
+          sts128(tile_at<128>(s_t1 + q * Cfg::kMatP, row, t0c / 8 + u), v);
+        });
+      }
+      // the first sums: row of dk, 16 tokens
+      tmem_ld(tmem + my, dq);
+      tmem_ld(tmem + 64 + my, r);
+      tmem_ld(t_w + my, w);
+      fence_async();
+      umma_fence_before();
+      warp_arrive(&mats, lane);
+      const float* leave = vec + kVecLeave * kChunk;
+      float sum = 0.f;
+      wait(&full_kq, k);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const int t = t0c + c;
+        const float e = enter[t];
+        float kv = 0.f;
+#pragma unroll
+        for (int i = NP - 1; i >= 0; --i)
+          kv += __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(
+              dsm + i * kTileKQ + (row >> 6) * kHalfTile + tile_at<128>(0, t, (row & 63) / 8) + (row % 8) * 2));
+        dq[c] *= e * p.scale;
+        r[c] *= -e;
+        w[c] *= leave[t];
+        sum = fmaf(beta[t] * kv, w[c], sum);  // of <S_C, dS>: what the chunk's writes add
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) s_sum[buf][warp] = sum;
+
+      wait(&done2, k);
+      umma_fence_after();
+      tmem_ld(t_qr2 + my, x);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) st0[(t0c + c) * 128 + row] = dq[c] + x[c];
+      tmem_ld(t_qr2 + 64 + my, x);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) st1[(t0c + c) * 128 + row] = r[c] + x[c];
+      tmem_ld(t_w2 + my, x);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) st2[(t0c + c) * 128 + row] = w[c] + x[c];
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+
+      // rows of tokens: 4 a warp, 4 of dk a lane
+      const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
+      auto put = [&](void* dst, float* part, int t, const float4& v) {
+        if (t >= rows || lane * 4 >= p.dk) return;
+        if (p.dq_part != nullptr) {
+          *reinterpret_cast<float4*>(part + ((b * p.L + t0 + t) * p.heads + h) * p.dk + lane * 4) = v;
+        } else {
+          *reinterpret_cast<uint2*>(static_cast<T*>(dst) + kf + (int64_t)t * kstride + lane * 4) =
+              make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+        }
+      };
+      float reads[4], writes[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int t = warp * 4 + q;
+        const float4 a = *reinterpret_cast<const float4*>(st0 + t * 128 + lane * 4);
+        const float4 rr = *reinterpret_cast<const float4*>(st1 + t * 128 + lane * 4);
+        const float4 ww = *reinterpret_cast<const float4*>(st2 + t * 128 + lane * 4);
+        const float4 kv = kq4(t, lane * 4), qv = kq4(kChunk + t, lane * 4);
+        const float be = beta[t];
+        reads[q] = fmaf(qv.x, a.x, fmaf(qv.y, a.y, fmaf(qv.z, a.z, qv.w * a.w)));
+        reads[q] = fmaf(kv.x, rr.x, fmaf(kv.y, rr.y, fmaf(kv.z, rr.z, fmaf(kv.w, rr.w, reads[q]))));
+        writes[q] = fmaf(kv.x, ww.x, fmaf(kv.y, ww.y, fmaf(kv.z, ww.z, kv.w * ww.w)));
+        put(p.dq, p.dq_part, t, a);
+        put(p.dk_out, p.dk_part, t,
+            make_float4(fmaf(be, ww.x, rr.x), fmaf(be, ww.y, rr.y), fmaf(be, ww.z, rr.z), fmaf(be, ww.w, rr.w)));
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          reads[q] += __shfl_xor_sync(0xffffffffu, reads[q], d);
+          writes[q] += __shfl_xor_sync(0xffffffffu, writes[q], d);
+        }
+      if (lane == 0)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          s_reads[buf][warp * 4 + q] = reads[q];
+          s_writes[buf][warp * 4 + q] = writes[q];
+        }
+      warp_arrive(&used_kq, lane);
+      asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums are read: matrices may be written
+    }
+  } else if (warp < 19) {
+    // ---------------------------------------------------------- <S0, dS>
+    const int t = tid - 17 * 32;
+    int64_t it = 0;
+    for (int64_t k = 0; k < mine; ++k) {
+      float dot = 0.f;
+      for (int sl = 0; sl < strips; ++sl, ++it) {
+        const int s = (int)(it % ST);
+        wait(&full[s], it / ST);
+        const uint32_t at = st + Cfg::oRing + s * Cfg::kStage + t * 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[8] = {}, y[8] = {};
+#pragma unroll
+          for (int q = NS - 1; q >= 0; --q) {
+            const uint4 u = lds128(at + Cfg::oS + q * 2 * kStrip + j * 1024);
+            const uint4 v = lds128(at + Cfg::oD + q * 2 * kStrip + j * 1024);
+            const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[2 * e] += bf16_lo(uw[e]);
+              x[2 * e + 1] += bf16_hi(uw[e]);
+              y[2 * e] += bf16_lo(vw[e]);
+              y[2 * e + 1] += bf16_hi(vw[e]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
+        }
+        warp_arrive(&freed[s], lane);
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+      wait(&full_vec[k & 1], k >> 1);  // so the sum of the chunk before the last has been taken
+      if (lane == 0) s_dot[k & 1][warp - 17] = dot;
+      warp_arrive(&dots[k & 1], lane);
+    }
+  } else {
+    // ---------------------------------------------------------- K, Q, vectors; a chunk's last sums
+    auto load_vec = [&](int64_t k) {
+      const int64_t unit = blockIdx.x + k * gridDim.x;
+      mbar_expect_tx(&full_vec[k & 1], Cfg::kVecBytes);
+      bulk_in(st + Cfg::oVec + (int)(k & 1) * Cfg::kVecBytes, p.vecs + unit * (kVecCount * kChunk),
+              Cfg::kVecBytes, &full_vec[k & 1]);
+    };
+    auto load_kq = [&](int64_t k) {
+      const int64_t unit = blockIdx.x + k * gridDim.x;
+      const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
+      const int hk = (int)(bh - b * p.heads) / (p.heads / p.key_heads);
+      const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kTileKQ / 2);
+      mbar_expect_tx(&full_kq, NP * kTileKQ);
+      bulk_in(st, p.kq_tiles + tile, NP * kTileKQ, &full_kq);
+    };
+    if (lane == 0) {
+      load_vec(0);
+      load_kq(0);
+      if (mine > 1) load_vec(1);
+    }
+    for (int64_t k = 0; k < mine; ++k) {
+      const int64_t unit = blockIdx.x + k * gridDim.x;
+      const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
+      const int h = (int)(bh - b * p.heads);
+      const int64_t t0 = chunk * kChunk;
+      const int rows = (int)min((int64_t)kChunk, p.L - t0);
+      const int buf = (int)(k & 1);
+      const float* vec = reinterpret_cast<const float*>(dsm + Cfg::oVec + buf * Cfg::kVecBytes);
+      bool reset[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = 2 * lane + c;
+        // a decay of exactly 0 has no slope in its logarithm
+        reset[c] = i < rows &&
+                   Elem<T>::load(static_cast<const T*>(p.log_decay)[(b * p.L + t0 + i) * p.heads + h]) < kDecayFloor;
+      }
+      wait(&full_vec[buf], k >> 1);
+      wait(&used_kq, k);
+      if (lane == 0 && k + 1 < mine) load_kq(k + 1);
+      wait(&dots[buf], k >> 1);
+      // the suffix sums, two tokens a lane, in 64 bits
+      double dg[2], state = 0.0;
+      float db[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = 2 * lane + c;
+        db[c] = s_writes[buf][i];
+        dg[c] = (double)s_reads[buf][i] - (double)vec[kVecBeta * kChunk + i] * (double)db[c];
+      }
+      if (lane < 16) state = (double)s_sum[buf][lane];
+      if (lane < 2) state += (double)vec[kVecEnter * kChunk + kChunk - 1] * (double)s_dot[buf][lane];
+      double suffix = dg[0] + dg[1];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_down_sync(0xffffffffu, suffix, d);
+        if (lane + d < 32) suffix += o;
+        state += __shfl_xor_sync(0xffffffffu, state, d);
+      }
+      const double out[2] = {suffix + state, suffix - dg[0] + state};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = 2 * lane + c;
+        if (i < rows) {
+          const int64_t o = (b * p.L + t0 + i) * p.heads + h;
+          static_cast<T*>(p.dlog_decay)[o] = Elem<T>::store(reset[c] ? 0.f : (float)out[c]);
+          static_cast<T*>(p.dbeta)[o] = Elem<T>::store(db[c]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && k + 2 < mine) load_vec(k + 2);
+    }
+    if (lane == 0) {
+      mbar_wait_soon(&full_kq, (uint32_t)((mine - 1) & 1));
+      for (int64_t k = max((int64_t)0, mine - 2); k < mine; ++k)
+        mbar_wait_soon(&full_vec[k & 1], (uint32_t)((k >> 1) & 1));
+    }
+  }
+  umma_fence_before();
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
 // ------------------------------------------------------------------ shared key heads
 struct GroupParams {
   const float* src[2];   // (tokens, heads, dk)
@@ -957,12 +1452,20 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   g.dk = (int)a.dk;
   g.dv = (int)a.dv;
   g.scale = a.scale;
-  using GC = GradCfg<NP, LV>;
-  auto kern = delta_grad_kernel<T, NP, LV>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC::kSmem);
-  if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, (unsigned)std::min<int64_t>(g.units, a.num_sms), kGradThreads, GC::kSmem,
-                 a.stream, g);
+  const unsigned grid = (unsigned)std::min<int64_t>(g.units, a.num_sms);
+  if constexpr (LV == 1) {
+    using GC = TcGradCfg<NP>;
+    auto kern = delta_grad_tc_kernel<T>;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC::kSmem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(kern, grid, kTcThreads, GC::kSmem, a.stream, g);
+  } else {
+    using GC = GradCfg<NP, LV>;
+    auto kern = delta_grad_kernel<T, NP, LV>;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC::kSmem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(kern, grid, kGradThreads, GC::kSmem, a.stream, g);
+  }
   if (e != cudaSuccess || !shared) return e;
 
   GroupParams s{};
@@ -973,8 +1476,8 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   s.n = tok * a.key_heads * (a.dk / 4);
   s.group = (int)(a.heads / a.key_heads);
   s.dk4 = (int)(a.dk / 4);
-  const unsigned grid = 2 * (unsigned)std::min<int64_t>((s.n + 255) / 256, 8 * a.num_sms);
-  return launch_pdl(delta_group_kernel<T>, grid, 256, 0, a.stream, s);
+  const unsigned gg = 2 * (unsigned)std::min<int64_t>((s.n + 255) / 256, 8 * a.num_sms);
+  return launch_pdl(delta_group_kernel<T>, gg, 256, 0, a.stream, s);
 }
 
 template <typename T, int LV>
