@@ -861,11 +861,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 //     K^T [Hb; Xb]^T -> dQ | R,   [K; Q]^T [Xd; Hs] -> W
 // with the matrices that the warps make of H and X.  20 warps: sixteen take the
 // first sums into registers (the next chunk's first products may then start),
-// make the matrices, and turn the results around through shared memory for
-// rows of tokens; one issues the strips' copies and all products, two take
-// <S0, dS> from the strips as they pass, and one loads K, Q and the vectors
-// and closes a chunk (dlog_decay, dbeta) behind the others.
-constexpr int kTcThreads = 640;
+// make the matrices, add the second sums and write the gradients from there
+// (a thread has one of dk and 16 tokens: 64 bytes a store, which costs less
+// than turning the sums around through shared memory did); one issues all
+// products, two take <S0, dS> from the strips as they pass (the first of them
+// issues their copies), and one loads K, Q and the vectors and closes a chunk
+// (dlog_decay, dbeta) behind the others.  Copies, like products, are issued by
+// an elected lane of a converged warp: six copies took a lone thread of a
+// divergent branch 900 cycles.
+constexpr int kTcThreads = 640;  // 96 registers a thread; one warp more, and it is 80
 
 template <int NP>
 struct TcGradCfg {
@@ -874,18 +878,17 @@ struct TcGradCfg {
   static constexpr int oE = 2 * 2 * kStrip, oS = oE + NS * kStrip, oD = oS + NS * 2 * kStrip;
   static constexpr int kStage = oD + NS * 2 * kStrip;
   static constexpr int kTx = (NP + 2 * NS) * kStrip + 2 * NS * 2 * kStrip;
-  // K and Q; two matrices of two parts, then over them three sums of 64 x 128
-  // fp32; the ring; decay vectors, those of the next chunk too
-  static constexpr int oM = NP * kTileKQ, kSum = kChunk * 512;
+  // K and Q; two matrices of two parts; the ring; decay vectors, those of the
+  // next chunk too
+  static constexpr int oM = NP * kTileKQ;
   static constexpr int kMatP = 128 * 128;  // a part of [Hb; Xb] or [Xd; Hs]
-  static constexpr int oRing = oM + 3 * kSum;
-  static_assert(2 * NS * kMatP <= 3 * kSum);
+  static constexpr int oRing = oM + 2 * NS * kMatP;
   static constexpr int kVecBytes = kVecCount * kChunk * 4;
-  static constexpr int kRoom = 227 * 1024 - 1024 - 3 * 1024 - 2 * kVecBytes;
+  static constexpr int kRoom = 227 * 1024 - 1024 - 5 * 1024 - 2 * kVecBytes;
   static constexpr int kStages = (kRoom - oRing) / kStage < 4 ? (kRoom - oRing) / kStage : 4;
   static constexpr int oVec = oRing + kStages * kStage;
   static constexpr int kSmem = oVec + 2 * kVecBytes + 1024;
-  static_assert(kStages >= 2 && kSmem + 3 * 1024 <= 227 * 1024);
+  static_assert(kStages >= 2 && kSmem + 5 * 1024 <= 227 * 1024);
 };
 
 // K-major operand of strips: 32-byte rows and swizzle, 16 values of k.
@@ -897,17 +900,17 @@ __host__ __device__ constexpr uint32_t umma_idesc_n(bool ta, bool tb, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((ta ? 1u : 0u) << 15) | ((tb ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
+// Position in a ring of ST stages and how often it has gone round.
+template <int ST>
+struct Ring {
+  int at = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == ST) {
+      at = 0;
+      ++phase;
+    }
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const GradParams p) {
@@ -922,7 +925,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
   __shared__ __align__(8) uint64_t full[ST], freed[ST], full_kq, full_vec[2], dots[2], done1, mats,
       done2, used_kq;
   __shared__ uint32_t s_tmem;
-  __shared__ float s_reads[2][kChunk], s_writes[2][kChunk], s_dot[2][2], s_sum[2][16];
+  // q.dQ + k.R, and k.W, of every token, by quarters of dk
+  __shared__ float s_rows[2][4][2][kChunk], s_dot[2][2], s_sum[2][16];
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
@@ -969,56 +973,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
   };
 
   if (warp == 16) {
-    // ---------------------------------------------------------- copies and products
-    const int64_t total = mine * strips;
-    int64_t next = 0, next_unit = blockIdx.x;
-    int next_strip = 0;
-    auto load = [&]() {  // of the next strip, by one lane
-      const int s = (int)(next % ST);
-      const int64_t at_strip = next_unit * strips + next_strip;
-      const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
-      mbar_expect_tx(&full[s], Cfg::kTx);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        bulk_in(at + i * 2 * kStrip, p.do_parts + (at_strip * NP + i) * (kStrip / 2), kStrip, &full[s]);
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        bulk_in(at + (2 * i + 1) * kStrip, p.dv_parts + (at_strip * NS + i) * (kStrip / 2), kStrip,
-                &full[s]);
-      bulk_in(at + Cfg::oE, p.e_parts + at_strip * NS * (kStrip / 2), NS * kStrip, &full[s]);
-      bulk_in(at + Cfg::oS, p.s_parts + at_strip * NS * kStrip, NS * 2 * kStrip, &full[s]);
-      bulk_in(at + Cfg::oD, p.ds_parts + at_strip * NS * kStrip, NS * 2 * kStrip, &full[s]);
-    };
-    auto advance = [&]() {
-      ++next;
-      if (++next_strip == strips) {
-        next_strip = 0;
-        next_unit += gridDim.x;
-      }
-    };
-    auto test = [&](uint64_t* bar, int64_t phase) {  // one answer for the warp
-      return __shfl_sync(0xffffffffu, mbar_test(bar, (uint32_t)(phase & 1)) ? 1 : 0, 0) != 0;
-    };
-    // Loads what may be, and waits only for the stage of strip `it` itself.
-    auto refill = [&](int64_t it) {
-      while (next < min(total, it + ST)) {
-        const int64_t before = next - ST;
-        if (before >= 0) {
-          if (next <= it)
-            wait(&freed[before % ST], before / ST);
-          else if (!test(&freed[before % ST], before / ST))
-            return;
-        }
-        if (lane == 0) load();
-        advance();
-      }
-    };
-    refill(0);
-    int64_t it = 0;
+    // ---------------------------------------------------------- products
+    Ring<ST> ring;
     for (int64_t k = 0; k < mine; ++k) {
-      for (int sl = 0; sl < strips; ++sl, ++it) {
-        const int s = (int)(it % ST);
-        wait(&full[s], it / ST);
+      for (int sl = 0; sl < strips; ++sl, ring.next()) {
+        const int s = ring.at;
+        wait(&full[s], ring.phase);
+        umma_fence_after();
         __syncwarp();
         if (elect_one()) {
           const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
@@ -1039,7 +1000,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
           if (sl == strips - 1) umma_commit(&done1);
         }
         __syncwarp();
-        refill(it + 1);
       }
       wait(&mats, k);
       wait(&full_kq, k);
@@ -1073,34 +1033,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       }
       __syncwarp();
     }
-    // No copy may land, and no product run, after the CTA is gone: at once,
-    // unless a wait gave up.
-    if (lane == 0) {
-      for (int64_t j = max((int64_t)0, next - ST); j < next; ++j)
-        mbar_wait_soon(&full[j % ST], (uint32_t)((j / ST) & 1));
-      mbar_wait_soon(&done2, (uint32_t)((mine - 1) & 1));
-    }
+    // no product may run after the CTA is gone: at once, unless a wait gave up
+    mbar_wait_soon(&done2, (uint32_t)((mine - 1) & 1));
   } else if (warp < 16) {
     // ---------------------------------------------------------- sums, matrices and rows
     const int quad = warp & 3, t0c = (warp >> 2) * 16;  // this thread's 16 columns
     const int row = quad * 32 + lane;  // lane of tensor memory: H, X row; row of dk
     const uint32_t my = ((uint32_t)(quad * 32) << 16) + t0c;
-    float* st0 = reinterpret_cast<float*>(dsm + Cfg::oM);  // 64 tokens x 128, where the matrices were
-    float* st1 = st0 + kChunk * 128;
-    float* st2 = st1 + kChunk * 128;
-    const int64_t kstride = (int64_t)p.key_heads * p.dk;
-    // four values of K (rows 64..: Q) as fp32 (the sum of their parts)
-    auto kq4 = [&](int r, int col) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int64_t kstride = (int64_t)p.key_heads * p.dk, pstride = (int64_t)p.heads * p.dk;
+    // this thread's row of dk of K (Q: rows from 64), as fp32 (the sum of its parts)
+    auto kq1 = [&](int r) {
+      float v = 0.f;
 #pragma unroll
-      for (int i = NP - 1; i >= 0; --i) {
-        const uint2 w = *reinterpret_cast<const uint2*>(
-            dsm + i * kTileKQ + (col >> 6) * kHalfTile + tile_at<128>(0, r, (col & 63) / 8) + (col % 8) * 2);
-        v.x += bf16_lo(w.x);
-        v.y += bf16_hi(w.x);
-        v.z += bf16_lo(w.y);
-        v.w += bf16_hi(w.y);
-      }
+      for (int i = NP - 1; i >= 0; --i)
+        v += __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(
+            dsm + i * kTileKQ + (row >> 6) * kHalfTile + tile_at<128>(0, r, (row & 63) / 8) + (row % 8) * 2));
       return v;
     };
     for (int64_t k = 0; k < mine; ++k) {
@@ -1111,12 +1058,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       const int rows = (int)min((int64_t)kChunk, p.L - t0);
       const int buf = (int)(k & 1);
       const float* vec = reinterpret_cast<const float*>(dsm + Cfg::oVec + buf * Cfg::kVecBytes);
-      const float* enter = vec + kVecEnter * kChunk;
       const float* beta = vec + kVecBeta * kChunk;
 
       wait(&full_vec[buf], k >> 1);
       wait(&done1, k);
       umma_fence_after();
+      auto vec16 = [&](int which, float (&v)[16]) {  // of this thread's columns
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 f = *reinterpret_cast<const float4*>(vec + which * kChunk + t0c + 4 * c);
+          v[4 * c] = f.x;
+          v[4 * c + 1] = f.y;
+          v[4 * c + 2] = f.z;
+          v[4 * c + 3] = f.w;
+        }
+      };
       float x[16], dq[16], r[16], w[16];
       {
         // H (rows 0..63) or X (64..127), row i, columns j: times D; with each
@@ -1124,20 +1080,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
         tmem_ld(t_hx + my, x);
         const int i = row & 63;
         const bool is_h = row < 64;
-        const float* hi = vec + kVecCumHi * kChunk;
-        const float* lo = vec + kVecCumLo * kChunk;
-        const float hi_i = hi[i], lo_i = lo[i], f = is_h ? p.scale : -1.f;
+        const float hi_i = vec[kVecCumHi * kChunk + i], lo_i = vec[kVecCumLo * kChunk + i];
+        const float f = is_h ? p.scale : -1.f;
+        float hi[16], lo[16];
+        vec16(kVecCumHi, hi);
+        vec16(kVecCumLo, lo);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           const int j = t0c + c;
-          const float d = i > j ? expf((hi_i - hi[j]) + (lo_i - lo[j])) : 1.f;
+          // (an error of 2^-16 of D at the most, where D is above e^-80)
+          const float d = i > j ? __expf((hi_i - hi[c]) + (lo_i - lo[c])) : 1.f;
           x[c] = i > j || (i == j && is_h) ? x[c] * (d * f) : 0.f;
         }
         split_row<NS>(x, [&](int q, int u, const uint4& v) {
           sts128(tile_at<128>(s_t2 + q * Cfg::kMatP, row ^ 64, t0c / 8 + u), v);
         });
+        vec16(kVecBeta, hi);
 #pragma unroll
-        for (int c = 0; c < 16; ++c) x[c] *= beta[t0c + c];
+        for (int c = 0; c < 16; ++c) x[c] *= hi[c];
         split_row<NS>(x, [&](int q, int u, const uint4& v) {
           sts128(tile_at<128>(s_t1 + q * Cfg::kMatP, row, t0c / 8 + u), v);
         });
@@ -1149,120 +1109,151 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       fence_async();
       umma_fence_before();
       warp_arrive(&mats, lane);
-      const float* leave = vec + kVecLeave * kChunk;
-      float sum = 0.f;
-      wait(&full_kq, k);
+      vec16(kVecEnter, x);
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
-        const int t = t0c + c;
-        const float e = enter[t];
-        float kv = 0.f;
-#pragma unroll
-        for (int i = NP - 1; i >= 0; --i)
-          kv += __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(
-              dsm + i * kTileKQ + (row >> 6) * kHalfTile + tile_at<128>(0, t, (row & 63) / 8) + (row % 8) * 2));
-        dq[c] *= e * p.scale;
-        r[c] *= -e;
-        w[c] *= leave[t];
-        sum = fmaf(beta[t] * kv, w[c], sum);  // of <S_C, dS>: what the chunk's writes add
+        dq[c] *= x[c] * p.scale;
+        r[c] *= -x[c];
       }
+      vec16(kVecLeave, x);
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == 0) s_sum[buf][warp] = sum;
-
+      for (int c = 0; c < 16; ++c) w[c] *= x[c];
+      wait(&full_kq, k);
       wait(&done2, k);
       umma_fence_after();
       tmem_ld(t_qr2 + my, x);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) st0[(t0c + c) * 128 + row] = dq[c] + x[c];
+      for (int c = 0; c < 16; ++c) dq[c] += x[c];
       tmem_ld(t_qr2 + 64 + my, x);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) st1[(t0c + c) * 128 + row] = r[c] + x[c];
+      for (int c = 0; c < 16; ++c) r[c] += x[c];
       tmem_ld(t_w2 + my, x);
+      const bool parts = p.dq_part != nullptr;
+      const int n = row < p.dk ? rows - t0c : 0;  // of the 16 tokens to be written
+      const int64_t at = parts ? ((b * p.L + t0 + t0c) * p.heads + h) * p.dk + row
+                               : (b * p.L + t0 + t0c) * kstride + (int64_t)hk * p.dk + row;
+      float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 16; ++c) st2[(t0c + c) * 128 + row] = w[c] + x[c];
-      asm volatile("bar.sync 1, 512;" ::: "memory");
-
-      // rows of tokens: 4 a warp, 4 of dk a lane
-      const int64_t kf = (b * p.L + t0) * kstride + (int64_t)hk * p.dk;
-      auto put = [&](void* dst, float* part, int t, const float4& v) {
-        if (t >= rows || lane * 4 >= p.dk) return;
-        if (p.dq_part != nullptr) {
-          *reinterpret_cast<float4*>(part + ((b * p.L + t0 + t) * p.heads + h) * p.dk + lane * 4) = v;
-        } else {
-          *reinterpret_cast<uint2*>(static_cast<T*>(dst) + kf + (int64_t)t * kstride + lane * 4) =
-              make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+      for (int c = 0; c < 16; ++c) {
+        const float be = beta[t0c + c], kv = kq1(t0c + c), qv = kq1(kChunk + t0c + c);
+        sum = fmaf(be * kv, w[c], sum);  // of <S_C, dS>: what the chunk's writes add
+        w[c] += x[c];
+        const float dk = fmaf(be, w[c], r[c]);
+        if (c < n) {
+          if (parts) {
+            p.dq_part[at + c * pstride] = dq[c];
+            p.dk_part[at + c * pstride] = dk;
+          } else {
+            static_cast<T*>(p.dq)[at + c * kstride] = Elem<T>::store(dq[c]);
+            static_cast<T*>(p.dk_out)[at + c * kstride] = Elem<T>::store(dk);
+          }
         }
-      };
-      float reads[4], writes[4];
+        dq[c] = fmaf(qv, dq[c], kv * r[c]);
+        r[c] = kv * w[c];
+      }
+      // sums over the 32 of dk, the 32 values over the lanes
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int t = warp * 4 + q;
-        const float4 a = *reinterpret_cast<const float4*>(st0 + t * 128 + lane * 4);
-        const float4 rr = *reinterpret_cast<const float4*>(st1 + t * 128 + lane * 4);
-        const float4 ww = *reinterpret_cast<const float4*>(st2 + t * 128 + lane * 4);
-        const float4 kv = kq4(t, lane * 4), qv = kq4(kChunk + t, lane * 4);
-        const float be = beta[t];
-        reads[q] = fmaf(qv.x, a.x, fmaf(qv.y, a.y, fmaf(qv.z, a.z, qv.w * a.w)));
-        reads[q] = fmaf(kv.x, rr.x, fmaf(kv.y, rr.y, fmaf(kv.z, rr.z, fmaf(kv.w, rr.w, reads[q]))));
-        writes[q] = fmaf(kv.x, ww.x, fmaf(kv.y, ww.y, fmaf(kv.z, ww.z, kv.w * ww.w)));
-        put(p.dq, p.dq_part, t, a);
-        put(p.dk_out, p.dk_part, t,
-            make_float4(fmaf(be, ww.x, rr.x), fmaf(be, ww.y, rr.y), fmaf(be, ww.z, rr.z), fmaf(be, ww.w, rr.w)));
+      for (int c = 0; c < 16; ++c) {
+        const float send = lane & 16 ? dq[c] : r[c], keep = lane & 16 ? r[c] : dq[c];
+        x[c] = keep + __shfl_xor_sync(0xffffffffu, send, 16);
       }
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1)
+      for (int m = 8; m > 0; m >>= 1) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          reads[q] += __shfl_xor_sync(0xffffffffu, reads[q], d);
-          writes[q] += __shfl_xor_sync(0xffffffffu, writes[q], d);
+        for (int c = 0; c < m; ++c) {
+          const float send = lane & m ? x[c] : x[c + m], keep = lane & m ? x[c + m] : x[c];
+          x[c] = keep + __shfl_xor_sync(0xffffffffu, send, m);
         }
-      if (lane == 0)
+      }
+      s_rows[buf][quad][lane >> 4][t0c + (lane & 15)] = x[0];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          s_reads[buf][warp * 4 + q] = reads[q];
-          s_writes[buf][warp * 4 + q] = writes[q];
-        }
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) s_sum[buf][warp] = sum;
       warp_arrive(&used_kq, lane);
-      asm volatile("bar.sync 1, 512;" ::: "memory");  // the sums are read: matrices may be written
     }
   } else if (warp < 19) {
     // ---------------------------------------------------------- <S0, dS>
-    const int t = tid - 17 * 32;
-    int64_t it = 0;
+    // The diagonals of products of 16 x 16 blocks with 8 x 16 ones: most of a
+    // product is thrown away, and it still takes a fifth of the instructions
+    // of unpacking the parts.
+    const int half = warp - 17;
+    const int64_t total = mine * strips;
+    int64_t next = 0, next_unit = blockIdx.x;  // strip to be copied
+    int next_sl = 0;
+    Ring<ST> ring, to, left;  // strip at hand, strip to be copied, the strip before the one at hand
+    auto load = [&]() {
+      const int64_t strip = next_unit * strips + next_sl;
+      uint64_t* bar = &full[to.at];
+      const uint32_t at = st + Cfg::oRing + to.at * Cfg::kStage;
+      __syncwarp();
+      if (elect_one()) {
+        mbar_expect_tx(bar, Cfg::kTx);
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          bulk_in(at + i * 2 * kStrip, p.do_parts + (strip * NP + i) * (kStrip / 2), kStrip, bar);
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          bulk_in(at + (2 * i + 1) * kStrip, p.dv_parts + (strip * NS + i) * (kStrip / 2), kStrip, bar);
+        bulk_in(at + Cfg::oE, p.e_parts + strip * (NS * kStrip / 2), NS * kStrip, bar);
+        bulk_in(at + Cfg::oS, p.s_parts + strip * (NS * kStrip), NS * 2 * kStrip, bar);
+        bulk_in(at + Cfg::oD, p.ds_parts + strip * (NS * kStrip), NS * 2 * kStrip, bar);
+      }
+      __syncwarp();
+      ++next;
+      to.next();
+      if (++next_sl == strips) {
+        next_sl = 0;
+        next_unit += gridDim.x;
+      }
+    };
+    if (half == 0)
+      while (next < min((int64_t)ST, total)) load();
     for (int64_t k = 0; k < mine; ++k) {
-      float dot = 0.f;
-      for (int sl = 0; sl < strips; ++sl, ++it) {
-        const int s = (int)(it % ST);
-        wait(&full[s], it / ST);
-        const uint32_t at = st + Cfg::oRing + s * Cfg::kStage + t * 16;
+      float acc[2][2][4] = {};
+      for (int sl = 0; sl < strips; ++sl, ring.next()) {
+        const int s = ring.at;
+        wait(&full[s], ring.phase);
+        const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float x[8] = {}, y[8] = {};
+          const int m0 = (2 * j + half) * 16;
+          uint32_t u[2][4], v[2][4];
 #pragma unroll
-          for (int q = NS - 1; q >= 0; --q) {
-            const uint4 u = lds128(at + Cfg::oS + q * 2 * kStrip + j * 1024);
-            const uint4 v = lds128(at + Cfg::oD + q * 2 * kStrip + j * 1024);
-            const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[2 * e] += bf16_lo(uw[e]);
-              x[2 * e + 1] += bf16_hi(uw[e]);
-              y[2 * e] += bf16_lo(vw[e]);
-              y[2 * e + 1] += bf16_hi(vw[e]);
-            }
+          for (int q = 0; q < 2; ++q) {
+            ldsm4(u[q], strip_a(at + Cfg::oS + q * 2 * kStrip, lane, m0));
+            ldsm4(v[q], strip_b(at + Cfg::oD + q * 2 * kStrip, lane, m0));
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
+          for (int n = 0; n < 2; ++n) {
+            mma_bf16(acc[j & 1][n], u[1], v[0][2 * n], v[0][2 * n + 1]);
+            mma_bf16(acc[j & 1][n], u[0], v[1][2 * n], v[1][2 * n + 1]);
+            mma_bf16(acc[j & 1][n], u[0], v[0][2 * n], v[0][2 * n + 1]);
+          }
         }
         warp_arrive(&freed[s], lane);
+        if (half == 0 && (k > 0 || sl > 0)) {  // the strip before is used up, or nearly
+          if (next < total) {
+            wait(&freed[left.at], left.phase);
+            load();
+          }
+          left.next();
+        }
       }
+      const int g = lane >> 2, c = 2 * (lane & 3);
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        dot += (g == c ? acc[j][0][0] + acc[j][1][2] : 0.f) + (g == c + 1 ? acc[j][0][1] + acc[j][1][3] : 0.f);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
       wait(&full_vec[k & 1], k >> 1);  // so the sum of the chunk before the last has been taken
       if (lane == 0) s_dot[k & 1][warp - 17] = dot;
       warp_arrive(&dots[k & 1], lane);
     }
+    // no copy may land after the CTA is gone: at once, unless a wait gave up
+    if (half == 0)
+      for (int64_t j = max((int64_t)0, next - ST); j < next; ++j)
+        mbar_wait_soon(&full[j % ST], (uint32_t)((j / ST) & 1));
   } else {
     // ---------------------------------------------------------- K, Q, vectors; a chunk's last sums
     auto load_vec = [&](int64_t k) {
@@ -1279,11 +1270,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       mbar_expect_tx(&full_kq, NP * kTileKQ);
       bulk_in(st, p.kq_tiles + tile, NP * kTileKQ, &full_kq);
     };
-    if (lane == 0) {
+    __syncwarp();
+    if (elect_one()) {
       load_vec(0);
       load_kq(0);
       if (mine > 1) load_vec(1);
     }
+    __syncwarp();
     for (int64_t k = 0; k < mine; ++k) {
       const int64_t unit = blockIdx.x + k * gridDim.x;
       const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
@@ -1302,7 +1295,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       }
       wait(&full_vec[buf], k >> 1);
       wait(&used_kq, k);
-      if (lane == 0 && k + 1 < mine) load_kq(k + 1);
+      __syncwarp();
+      if (k + 1 < mine && elect_one()) load_kq(k + 1);
+      __syncwarp();
       wait(&dots[buf], k >> 1);
       // the suffix sums, two tokens a lane, in 64 bits
       double dg[2], state = 0.0;
@@ -1310,8 +1305,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int i = 2 * lane + c;
-        db[c] = s_writes[buf][i];
-        dg[c] = (double)s_reads[buf][i] - (double)vec[kVecBeta * kChunk + i] * (double)db[c];
+        float reads = 0.f;
+        db[c] = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          reads += s_rows[buf][q][0][i];
+          db[c] += s_rows[buf][q][1][i];
+        }
+        dg[c] = (double)reads - (double)vec[kVecBeta * kChunk + i] * (double)db[c];
       }
       if (lane < 16) state = (double)s_sum[buf][lane];
       if (lane < 2) state += (double)vec[kVecEnter * kChunk + kChunk - 1] * (double)s_dot[buf][lane];
@@ -1333,13 +1334,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
         }
       }
       __syncwarp();
-      if (lane == 0 && k + 2 < mine) load_vec(k + 2);
+      if (k + 2 < mine && elect_one()) load_vec(k + 2);
+      __syncwarp();
     }
-    if (lane == 0) {
-      mbar_wait_soon(&full_kq, (uint32_t)((mine - 1) & 1));
-      for (int64_t k = max((int64_t)0, mine - 2); k < mine; ++k)
-        mbar_wait_soon(&full_vec[k & 1], (uint32_t)((k >> 1) & 1));
-    }
+    mbar_wait_soon(&full_kq, (uint32_t)((mine - 1) & 1));
+    for (int64_t k = max((int64_t)0, mine - 2); k < mine; ++k)
+      mbar_wait_soon(&full_vec[k & 1], (uint32_t)((k >> 1) & 1));
   }
   umma_fence_before();
   __syncthreads();
