@@ -137,18 +137,28 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
   pdl_launch_dependents();
 
   // step d handles chunk chunks - 1 - d
-  const bool loads = tid == kRevThreads - 32;
+  // Copies are issued by an elected lane of a converged warp (a lone thread of
+  // a divergent branch takes over 100 cycles for each).
+  const bool loads = warp == kRevThreads / 32 - 1;
   auto load_kq = [&](int64_t d) {
+    __syncwarp();
     const int64_t c = p.chunks - 1 - d;
     const int s = (int)(d % Cfg::kSt);
-    mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
-    bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
-    bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
-            &full_kq[s]);
+    if (elect_one()) {
+      mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
+      bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
+      bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
+              &full_kq[s]);
+    }
+    __syncwarp();
   };
   auto load_n = [&](int64_t d) {
-    mbar_expect_tx(&full_n, Cfg::kNPN);
-    bulk_in(s_npn, p.npn + (unit0 + p.chunks - 1 - d) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
+    __syncwarp();
+    if (elect_one()) {
+      mbar_expect_tx(&full_n, Cfg::kNPN);
+      bulk_in(s_npn, p.npn + (unit0 + p.chunks - 1 - d) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
+    }
+    __syncwarp();
   };
   if (loads) {
     for (int64_t d = 0; d < min((int64_t)Cfg::kSt, p.chunks); ++d) load_kq(d);
@@ -182,20 +192,6 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
            (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * parts + q) * (int64_t)bytes;
   };
 
-  // dS's parts to their strips, by the warps of dO
-  auto keep_ds = [&](int64_t c) {
-    const int have = min(C / 8, strips - slice * (C / 8));
-    char* sp = reinterpret_cast<char*>(p.ds_parts) +
-               ((unit0 + c) * strips + slice * (C / 8)) * (int64_t)(NS * 2 * kStrip);
-    const int t = (warp >> 2) * 64 + (quad - 2) * 32 + lane;  // 0..127
-#pragma unroll 4
-    for (int i = t; i < NS * 128 * (C / 4); i += 128) {
-      const int u = i % (C / 4), r = i / (C / 4) % 128, q = i / (C / 4 * 128);
-      if ((u >> 1) < have)
-        *reinterpret_cast<uint4*>(sp + ((u >> 1) * NS + q) * (2 * kStrip) + strip_at(0, r, u & 1)) =
-            lds128(val_at<C>(s_s + q * Cfg::kPart, r, u));
-    }
-  };
   bool ok = true;  // as in delta_scan_kernel
   auto wait = [&](uint64_t* bar, int64_t phase) {
     if (ok) ok = mbar_wait_soon(bar, (uint32_t)(phase & 1));
@@ -224,12 +220,16 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
       }
       __syncwarp();
     }
+    // dS's parts to their strips, from the registers, while the product runs
+    split_row<NS>(S, [&](int q, int u, const uint4& w) {
+      if ((u & ~1) * 8 < nval)
+        *reinterpret_cast<uint4*>(strip_ptr(p.ds_parts, c, u, NS, q, 2 * kStrip) + strip_at(0, dk, u & 1)) = w;
+    });
     wait(&full_kq[s], d / Cfg::kSt);  // the vectors
     const float ge = vec[kVecEnter * kChunk + tok], total = vec[kVecEnter * kChunk + kChunk - 1];
     const float wb = vec[kVecLeave * kChunk + tok] * vec[kVecBeta * kChunk + tok];
 
     float x[C], g[C];
-    if (Cfg::kOver && !is_y) keep_ds(c);  // before the stacked operand takes its place
     if (!is_y) {
       next_do.take(g);
       split_row<NP>(g, [&](int q, int u, const uint4& w) {
@@ -241,7 +241,6 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
       if (c > 0) load_do(c - 1);
     }
     wait(&done[0], d);
-    if (Cfg::kOver) __syncthreads();  // and has been kept
     umma_fence_after();
     if (is_y) {
       tmem_ld(my_tmem, x);
@@ -264,7 +263,6 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
       }
       __syncwarp();
     }
-    if (!Cfg::kOver && !is_y) keep_ds(c);
     wait(&done[1], d);
     umma_fence_after();
     if (loads && d + 1 < p.chunks) load_n(d + 1);  // N and PN are used up

@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
   const int dv0 = slice * 2 * C + col0;
   const int nval = min(C, p.dv - dv0);  // values of this thread's C that exist (may be <= 0)
+  const int strips = (p.dv + 15) / 16;
   const int64_t vstride = (int64_t)p.heads * p.dv;
   const int64_t tile = (b * p.key_heads + hk) * p.chunks, unit0 = bh * p.chunks;
 
@@ -485,18 +486,27 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
   pdl_wait();
   pdl_launch_dependents();
 
-  // loads, by one thread of the output warps
-  const bool loads = tid == kScanThreads - 32;
+  // Copies are issued by an elected lane of a converged warp (a lone thread of
+  // a divergent branch takes over 100 cycles for each).
+  const bool loads = warp == kScanThreads / 32 - 1;
   auto load_kq = [&](int64_t c) {
+    __syncwarp();
     const int s = (int)(c % Cfg::kSt);
-    mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
-    bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
-    bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
-            &full_kq[s]);
+    if (elect_one()) {
+      mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
+      bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
+      bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
+              &full_kq[s]);
+    }
+    __syncwarp();
   };
   auto load_n = [&](int64_t c) {
-    mbar_expect_tx(&full_n, Cfg::kNPN);
-    bulk_in(s_npn, p.npn + (unit0 + c) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
+    __syncwarp();
+    if (elect_one()) {
+      mbar_expect_tx(&full_n, Cfg::kNPN);
+      bulk_in(s_npn, p.npn + (unit0 + c) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
+    }
+    __syncwarp();
   };
   if (loads) {
     for (int64_t c = 0; c < min((int64_t)Cfg::kSt, p.chunks); ++c) load_kq(c);
@@ -547,20 +557,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
       }
       __syncwarp();
     }
-    if (KEEP && !is_x) {
-      // S0's parts to their strips, by the warps that have no output to work on
-      const int strips = (p.dv + 15) / 16, have = min(C / 8, strips - slice * (C / 8));
-      char* sp = reinterpret_cast<char*>(p.s_parts) +
-                 ((unit0 + c) * strips + slice * (C / 8)) * (int64_t)(NS * 2 * kStrip);
-      const int t = (warp >> 2) * 64 + (quad - 2) * 32 + lane;  // 0..127
-#pragma unroll 4
-      for (int i = t; i < NS * 128 * (C / 4); i += 128) {
-        const int u = i % (C / 4), r = i / (C / 4) % 128, q = i / (C / 4 * 128);
-        if ((u >> 1) < have)
-          *reinterpret_cast<uint4*>(sp + ((u >> 1) * NS + q) * (2 * kStrip) + strip_at(0, r, u & 1)) =
-              lds128(val_at<C>(s_s + q * Cfg::kPartS, r, u));
-      }
-    }
+    if (KEEP)  // S0's parts to their strips, from the registers, while the product runs
+      split_row<NS>(S, [&](int q, int u, const uint4& w) {
+        if ((u & ~1) * 8 < nval)
+          *reinterpret_cast<uint4*>(
+              reinterpret_cast<char*>(p.s_parts) +
+              (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * NS + q) * (int64_t)(2 * kStrip) +
+              strip_at(0, dk, u & 1)) = w;
+      });
     wait(&full_kq[s], c / Cfg::kSt);  // the vectors
     const float ge = vec[kVecEnter * kChunk + tok], total = vec[kVecEnter * kChunk + kChunk - 1];
     const float wb = vec[kVecLeave * kChunk + tok] * vec[kVecBeta * kChunk + tok];
@@ -644,7 +648,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
           if ((u & ~1) * 8 < nval) {
             char* ep = reinterpret_cast<char*>(
                 p.e_parts +
-                (((unit0 + c) * ((p.dv + 15) / 16) + dv0 / 16 + (u >> 1)) * NS + q) * (kStrip / 2));
+                (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * NS + q) * (kStrip / 2));
             *reinterpret_cast<uint4*>(ep + strip_at(0, tok, u & 1)) = w;
           }
         });
