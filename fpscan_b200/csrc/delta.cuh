@@ -239,16 +239,16 @@ __device__ __forceinline__ uint64_t umma_desc_a(uint32_t addr, uint32_t leading)
   return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)((leading >> 4) & 0x3fff) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
+// part: bytes from one part of B to the next, which is the next 2 C columns.
 template <int C>
-__device__ __forceinline__ uint64_t umma_desc_b(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(8 * 4 * C >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(C == 32 ? 2 : 4) << 61);
+__device__ __forceinline__ uint64_t umma_desc_b(uint32_t addr, uint32_t part) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)((part >> 4) & 0x3fff) << 16) |
+         ((uint64_t)(8 * 4 * C >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(C == 32 ? 2 : 4) << 61);
 }
-// fp32 D, bf16 A and B, M = 128, N = 2 C, B MN-major, A MN-major where `ta`.
-template <int C>
-__host__ __device__ constexpr uint32_t umma_idesc(bool ta) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((ta ? 1u : 0u) << 15) | (1u << 16) |
-         ((2 * C >> 3) << 17) | ((128u >> 4) << 24);
+// fp32 D, bf16 A and B, M = 128, n columns; A, B MN-major where `ta`, `tb`.
+__host__ __device__ constexpr uint32_t umma_idesc(bool ta, bool tb, int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((ta ? 1u : 0u) << 15) | ((tb ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 // A wait that is short as a rule: tries for a while before it reads the clock
 // and the limit (a load from global memory), which take longer than the wait.
@@ -289,25 +289,29 @@ __device__ __forceinline__ void umma_fence_before() {
 __device__ __forceinline__ void umma_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// D = sum over parts i of A and j of B, i < NA, i + j <= LV, smallest first,
-// and over KS steps of 16 values of k: a_step / b_step are bytes of one step,
-// a_part / b_part of one part.  SPLIT: A's steps from the fifth on lie a_half
-// further (K-major tiles of 128 columns).
-template <int NA, int LV, int KS, bool SPLIT>
+// D_j = sum over parts i of A, i < NA, i + j <= LV, smallest first, and over KS
+// steps of 16 values of k, of A_i B_j: the parts of B lie side by side as
+// columns of one product, which costs less than a product for each pair
+// (measured cycles of one of 128 rows: 44 for 32 columns, 50 for 64, 66 for
+// 128), and each D_j is summed by itself (tmem_sum adds them up).  The first
+// product sets all columns, the others are as wide as i + j <= LV asks.
+// a_step / b_step are bytes of one step, a_part of one part; b has B's first
+// part.  SPLIT: A's steps from the fifth on lie a_half further (K-major tiles
+// of 128 columns).  TA: A is MN-major.
+template <int C, int NA, int LV, int KS, bool SPLIT, bool TA>
 __device__ __forceinline__ void umma_parts(uint32_t d, uint64_t a, uint64_t b, uint32_t a_part,
-                                           uint32_t b_part, uint32_t a_step, uint32_t b_step,
-                                           uint32_t a_half, uint32_t idesc, int ksteps) {
+                                           uint32_t a_step, uint32_t b_step, uint32_t a_half, int ksteps) {
+  constexpr int top = (NA < LV + 1 ? NA : LV + 1) - 1;
 #pragma unroll
-  for (int lv = LV; lv >= 0; --lv)
+  for (int i = top; i >= 0; --i)
 #pragma unroll
-    for (int i = 0; i <= lv && i < NA; ++i)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if (ks < ksteps) {
-          const uint32_t ao = i * a_part + (SPLIT ? (ks >> 2) * a_half + (ks & 3) * a_step : ks * a_step);
-          const uint32_t bo = (lv - i) * b_part + ks * b_step;
-          umma(d, a + (ao >> 4), b + (bo >> 4), idesc, lv != LV || i != 0 || ks != 0);
-        }
+    for (int ks = 0; ks < KS; ++ks)
+      if (ks < ksteps) {
+        const bool first = i == top && ks == 0;
+        const uint32_t ao = i * a_part + (SPLIT ? (ks >> 2) * a_half + (ks & 3) * a_step : ks * a_step);
+        umma(d, a + (ao >> 4), b + (ks * b_step >> 4),
+             umma_idesc(TA, true, 2 * C * (first ? LV + 1 : LV - i + 1)), !first);
+      }
 }
 
 // 16 or 32 columns of the warp's 32 lanes.
@@ -338,6 +342,24 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Tensor memory of two products of 2 C columns for each of the LV + 1 parts (a
+// power of two of columns).
+template <int LV, int C>
+constexpr int kTmemColumns = (LV + 1) * 4 * C <= 128 ? 128 : (LV + 1) * 4 * C <= 256 ? 256 : 512;
+
+// The sum of what umma_parts left in NS times 2 C columns, smallest first.
+template <int NS, int C>
+__device__ __forceinline__ void tmem_sum(uint32_t addr, float (&x)[C]) {
+  tmem_ld(addr + (NS - 1) * 2 * C, x);
+#pragma unroll
+  for (int j = NS - 2; j >= 0; --j) {
+    float y[C];
+    tmem_ld(addr + j * 2 * C, y);
+#pragma unroll
+    for (int i = 0; i < C; ++i) x[i] += y[i];
+  }
 }
 
 // ---------------------------------------------------------------- bf16 parts

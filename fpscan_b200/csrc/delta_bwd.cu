@@ -89,7 +89,7 @@ struct RevCfg {
 template <typename T, int LV, int C>
 __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevParams p) {
   using Cfg = RevCfg<T, LV, C>;
-  constexpr int kTmem = C == 32 ? 256 : 128;
+  constexpr int kTmem = kTmemColumns<LV, C>;
   constexpr int NP = Cfg::NP, NS = Cfg::NS;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = s_tmem, tmem2 = tmem + NS * 2 * C;  // first and third product; second
   const uint32_t my_tmem = tmem + ((uint32_t)(quad * 32) << 16) + col0;
   pdl_wait();
   pdl_launch_dependents();
@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
       umma_fence_after();
       wait(&full_kq[s], d / Cfg::kSt);
       if (elect_one()) {
-        umma_parts<NP, LV, 8, true>(tmem, umma_desc_a(s_kq, 16), umma_desc_b<C>(s_s), kTileKQ, Cfg::kPart,
-                                    32, 64 * C, kHalfTile, umma_idesc<C>(false), ksteps);
+        umma_parts<C, NP, LV, 8, true, false>(tmem, umma_desc_a(s_kq, 16), umma_desc_b<C>(s_s, Cfg::kPart),
+                                              kTileKQ, 32, 64 * C, kHalfTile, ksteps);
         umma_commit(&done[0]);
       }
       __syncwarp();
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     wait(&done[0], d);
     umma_fence_after();
     if (is_y) {
-      tmem_ld(my_tmem, x);
+      tmem_sum<NS>(my_tmem, x);
 #pragma unroll
       for (int i = 0; i < C; ++i) x[i] *= wb;
       put_tile(tok, x);
@@ -257,8 +257,8 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
       umma_fence_after();
       wait(&full_n, d);
       if (elect_one()) {
-        umma_parts<NS, LV, 8, false>(tmem + 2 * C, umma_desc_a(s_npn, 0), umma_desc_b<C>(s_e), 2 * kMatBytes,
-                                     Cfg::kPart, 2048, 64 * C, 0, umma_idesc<C>(true), 8);
+        umma_parts<C, NS, LV, 8, false, true>(tmem2, umma_desc_a(s_npn, 0), umma_desc_b<C>(s_e, Cfg::kPart),
+                                              2 * kMatBytes, 2048, 64 * C, 0, 8);
         umma_commit(&done[1]);
       }
       __syncwarp();
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     umma_fence_after();
     if (loads && d + 1 < p.chunks) load_n(d + 1);  // N and PN are used up
 
-    tmem_ld(my_tmem + 2 * C, x);  // dV, in both halves of the lanes
+    tmem_sum<NS>(my_tmem + NS * 2 * C, x);  // dV, in both halves of the lanes
     if (is_y) {
 #pragma unroll
       for (int i = 0; i < C; ++i) g[i] = x[i] * -ge;
@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     if (warp == 0) {
       umma_fence_after();
       if (elect_one()) {
-        umma_parts<NP, LV, 8, false>(tmem + 4 * C, umma_desc_a(s_kq, kHalfTile), umma_desc_b<C>(s_e),
-                                     kTileKQ, Cfg::kPart, 2048, 64 * C, 0, umma_idesc<C>(true), 8);
+        umma_parts<C, NP, LV, 8, false, true>(tmem, umma_desc_a(s_kq, kHalfTile),
+                                              umma_desc_b<C>(s_e, Cfg::kPart), kTileKQ, 2048, 64 * C, 0, 8);
         umma_commit(&done[2]);
       }
       __syncwarp();
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     }
     wait(&done[2], d);
     umma_fence_after();
-    tmem_ld(my_tmem + 4 * C, x);
+    tmem_sum<NS>(my_tmem, x);
 #pragma unroll
     for (int i = 0; i < C; ++i) S[i] = fmaf(total, S[i], x[i]);
   }
@@ -894,10 +894,6 @@ __device__ __forceinline__ uint64_t umma_desc_strip(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(1) << 16) | ((uint64_t)(256 >> 4) << 32) |
          (uint64_t(1) << 46) | (uint64_t(6) << 61);
 }
-__host__ __device__ constexpr uint32_t umma_idesc_n(bool ta, bool tb, int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((ta ? 1u : 0u) << 15) | ((tb ? 1u : 0u) << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
-}
 // Position in a ring of ST stages and how often it has gone round.
 template <int ST>
 struct Ring {
@@ -985,15 +981,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
                          s0 = umma_desc_strip(at + Cfg::oS), ds = umma_desc_strip(at + Cfg::oD);
           constexpr uint32_t pd = 2 * kStrip >> 4, pe = kStrip >> 4, ps = 2 * kStrip >> 4;  // parts
           const bool on = sl > 0;
-          umma(tmem, s0 + ps, dv, umma_idesc_n(false, false, 128), on);
-          umma(tmem, s0, dv + pd, umma_idesc_n(false, false, 128), true);
-          umma(tmem, s0, dv, umma_idesc_n(false, false, 128), true);
-          umma(t_w, ds + ps, e, umma_idesc_n(false, false, 64), on);
-          umma(t_w, ds, e + pe, umma_idesc_n(false, false, 64), true);
-          umma(t_w, ds, e, umma_idesc_n(false, false, 64), true);
-          umma(t_hx, dv + pd, e, umma_idesc_n(false, false, 64), on);
-          umma(t_hx, dv, e + pe, umma_idesc_n(false, false, 64), true);
-          umma(t_hx, dv, e, umma_idesc_n(false, false, 64), true);
+          umma(tmem, s0 + ps, dv, umma_idesc(false, false, 128), on);
+          umma(tmem, s0, dv + pd, umma_idesc(false, false, 128), true);
+          umma(tmem, s0, dv, umma_idesc(false, false, 128), true);
+          umma(t_w, ds + ps, e, umma_idesc(false, false, 64), on);
+          umma(t_w, ds, e + pe, umma_idesc(false, false, 64), true);
+          umma(t_w, ds, e, umma_idesc(false, false, 64), true);
+          umma(t_hx, dv + pd, e, umma_idesc(false, false, 64), on);
+          umma(t_hx, dv, e + pe, umma_idesc(false, false, 64), true);
+          umma(t_hx, dv, e, umma_idesc(false, false, 64), true);
           umma_commit(&freed[s]);
           if (sl == strips - 1) umma_commit(&done1);
         }
@@ -1013,7 +1009,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
               umma(t_qr2, kt + ((i * kTileKQ + ks * 2048) >> 4),
-                   t1 + (((lv - i) * Cfg::kMatP + ks * 32) >> 4), umma_idesc_n(true, false, 128), on);
+                   t1 + (((lv - i) * Cfg::kMatP + ks * 32) >> 4), umma_idesc(true, false, 128), on);
               on = true;
             }
         on = false;
@@ -1024,7 +1020,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
               umma(t_w2, kt + ((i * kTileKQ + ks * 2048) >> 4),
-                   t2 + (((lv - i) * Cfg::kMatP + ks * 2048) >> 4), umma_idesc_n(true, true, 64), on);
+                   t2 + (((lv - i) * Cfg::kMatP + ks * 2048) >> 4), umma_idesc(true, true, 64), on);
               on = true;
             }
         umma_commit(&done2);

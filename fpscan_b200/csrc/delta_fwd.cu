@@ -437,7 +437,7 @@ struct ScanCfg {
 template <typename T, int LV, bool KEEP, int C>
 __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanParams p) {
   using Cfg = ScanCfg<T, LV, C>;
-  constexpr int kTmem = C == 32 ? 256 : 128;  // columns: three products of 2 C
+  constexpr int kTmem = kTmemColumns<LV, C>;
   constexpr int NP = Cfg::NP, NS = Cfg::NS;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = s_tmem, tmem2 = tmem + NS * 2 * C;  // first and third product; second
   const uint32_t my_tmem = tmem + ((uint32_t)(quad * 32) << 16) + col0;
   pdl_wait();
   pdl_launch_dependents();
@@ -551,8 +551,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
       umma_fence_after();
       wait(&full_kq[s], c / Cfg::kSt);
       if (elect_one()) {
-        umma_parts<NP, LV, kDkp / 16, true>(tmem, umma_desc_a(s_kq, 16), umma_desc_b<C>(s_s), kTileKQ,
-                                            Cfg::kPartS, 32, 64 * C, kHalfTile, umma_idesc<C>(false), ksteps);
+        umma_parts<C, NP, LV, kDkp / 16, true, false>(tmem, umma_desc_a(s_kq, 16),
+                                                      umma_desc_b<C>(s_s, Cfg::kPartS), kTileKQ, 32, 64 * C,
+                                                      kHalfTile, ksteps);
         umma_commit(&done[0]);
       }
       __syncwarp();
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
     umma_fence_after();
 
     float x[C];
-    tmem_ld(my_tmem, x);
+    tmem_sum<NS>(my_tmem, x);
     // An infinity or a NaN in R (of v, k, or the state) spoils its value from
     // that token on, but the zeros above the diagonals of N and PN would carry
     // it to earlier tokens: it is taken out here and put back into E, O and
@@ -626,9 +627,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
       umma_fence_after();
       wait(&full_n, c);
       if (elect_one()) {
-        umma_parts<NS, LV, kChunk / 16, false>(tmem + 2 * C, umma_desc_a(s_npn, 16), umma_desc_b<C>(s_e),
-                                               2 * kMatBytes, Cfg::kPartE, 32, 64 * C, 0,
-                                               umma_idesc<C>(false), kChunk / 16);
+        umma_parts<C, NS, LV, kChunk / 16, false, false>(tmem2, umma_desc_a(s_npn, 16),
+                                                         umma_desc_b<C>(s_e, Cfg::kPartE), 2 * kMatBytes, 32,
+                                                         64 * C, 0, kChunk / 16);
         umma_commit(&done[1]);
       }
       __syncwarp();
@@ -638,7 +639,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
     if (loads && c + 1 < p.chunks) load_n(c + 1);  // N and PN are used up
 
     if (is_x) {
-      tmem_ld(my_tmem + 2 * C, x);
+      tmem_sum<NS>(my_tmem + NS * 2 * C, x);
       if (KEEP) {
         if (bad)
 #pragma unroll
@@ -664,16 +665,16 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
       if (warp == 0) {
         umma_fence_after();
         if (elect_one()) {
-          umma_parts<NP, LV, kChunk / 16, false>(tmem + 4 * C, umma_desc_a(s_kq, kHalfTile),
-                                                 umma_desc_b<C>(s_e), kTileKQ, Cfg::kPartE, 2048, 64 * C, 0,
-                                                 umma_idesc<C>(true), kChunk / 16);
+          umma_parts<C, NP, LV, kChunk / 16, false, true>(tmem, umma_desc_a(s_kq, kHalfTile),
+                                                          umma_desc_b<C>(s_e, Cfg::kPartE), kTileKQ, 2048,
+                                                          64 * C, 0, kChunk / 16);
           umma_commit(&done[2]);
         }
         __syncwarp();
       }
     } else if (!KEEP) {
       float pe[C];
-      tmem_ld(my_tmem + 2 * C, pe);
+      tmem_sum<NS>(my_tmem + NS * 2 * C, pe);
 #pragma unroll
       for (int i = 0; i < C; ++i) x[i] += pe[i];
       if (bad)
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
     umma_fence_after();
     // The chunk's sum starts at zero and joins the state in one rounded
     // multiply-add.
-    tmem_ld(my_tmem + 4 * C, x);
+    tmem_sum<NS>(my_tmem, x);
 #pragma unroll
     for (int i = 0; i < C; ++i) S[i] = fmaf(total, S[i], x[i]);
     if (bad)
