@@ -205,6 +205,8 @@ at::Tensor delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor
                              s.b, s.l, s.hk, s.h, s.dk, s.dv, (float)scale, s.code,
                              at::cuda::getCurrentCUDAStream().stream()),
            "fpscan_delta_step");
+  // a backward pass that has saved this state must notice
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   return out;
 }
 

@@ -26,6 +26,9 @@
 namespace fpscan {
 
 constexpr int kChunk = 64;
+constexpr int kHalfTile = 2 * kChunk * 128;     // bytes: 64 columns of K's, then Q's rows
+constexpr int kTileKQ = 2 * kHalfTile;          // one part of K and Q
+constexpr int kMatBytes = kChunk * kChunk * 2;  // one part of a 64 x 64 matrix
 
 // Below this log_decay counts as -inf: exp of anything near it is 0, and
 // differences of running sums stay finite.
@@ -96,13 +99,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-// Transposes an 8 x 8 matrix of 16-bit elements held by a warp.
-__device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-
 // Tiles in shared memory: rows of ROWB bytes (a multiple of 128), 16-byte
 // units exchanged by the low bits of the row, so that 8 rows of one unit
 // column (an ldmatrix) fall on 8 different bank groups.
@@ -137,46 +133,18 @@ __device__ __forceinline__ uint32_t at_at(uint32_t base, int lane, int m0, int k
   return tile_at<ROWB>(base, kk * 16 + (m >> 1) * 8 + r, m0 / 8 + (m & 1));
 }
 
-// The parts of the state are kept as two half tiles of dk / 2 columns, one
-// for each chain warp of a strip: rows of DKP bytes (128 or 64).
-template <int DKP>
-__device__ __forceinline__ uint32_t half_at(uint32_t base, int row, int unit) {
-  return DKP == 128 ? base + row * 128 + ((unit ^ (row & 7)) << 4)
-                    : base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
-}
-// A operand, 16 rows, columns 16 kk.. of the half.
-template <int DKP>
-__device__ __forceinline__ uint32_t half_a(uint32_t base, int lane, int kk) {
-  const int m = lane >> 3, r = lane & 7;
-  return half_at<DKP>(base, (m & 1) * 8 + r, kk * 2 + (m >> 1));
-}
-// B operand (transposing load): k = rows 0..15, columns n0..n0+15 of the half.
-template <int DKP>
-__device__ __forceinline__ uint32_t half_bt(uint32_t base, int lane, int n0) {
-  const int m = lane >> 3, r = lane & 7;
-  return half_at<DKP>(base, (m & 1) * 8 + r, n0 / 8 + (m >> 1));
-}
-
-// Strips: 64 tokens x 16 values, rows of 16 values (32 bytes; fp32 64).  A
-// warp's 16 rows of the transposed state meet one strip of v, E, dO or dV.
-// Units are exchanged so that 8 rows of one unit column again fall on 8
-// different bank groups.
+// Strips: the parts of E, dO, dV (64 tokens) and of S0, dS (128 rows of dk) by
+// 16 values, rows of 32 bytes; kept in global memory as they lie in shared
+// memory.  Units are exchanged so that 8 rows of one unit column again fall on
+// 8 different bank groups: the 32-byte swizzle of tcgen05 operands.
 constexpr int kStrip = kChunk * 32;  // bytes of a bf16 strip
 __device__ __forceinline__ uint32_t strip_at(uint32_t base, int row, int unit) {
   return base + row * 32 + ((unit ^ ((row >> 2) & 1)) << 4);
-}
-__device__ __forceinline__ uint32_t strip32_at(uint32_t base, int row, int unit) {
-  return base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
 }
 // A operand with the tokens as its rows (m0..m0+15).
 __device__ __forceinline__ uint32_t strip_a(uint32_t base, int lane, int m0) {
   const int m = lane >> 3, r = lane & 7;
   return strip_at(base, m0 + (m & 1) * 8 + r, m >> 1);
-}
-// A operand with the values as its rows, tokens 16 kk.. (transposing load or store).
-__device__ __forceinline__ uint32_t strip_at_t(uint32_t base, int lane, int kk) {
-  const int m = lane >> 3, r = lane & 7;
-  return strip_at(base, kk * 16 + (m >> 1) * 8 + r, m & 1);
 }
 // B operand with the tokens as its columns n0..n0+15.
 __device__ __forceinline__ uint32_t strip_b(uint32_t base, int lane, int n0) {
@@ -185,11 +153,6 @@ __device__ __forceinline__ uint32_t strip_b(uint32_t base, int lane, int n0) {
 }
 __device__ __forceinline__ void stsm4(uint32_t addr, const uint32_t (&r)[4]) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
-}
-__device__ __forceinline__ void stsm4_t(uint32_t addr, const uint32_t (&r)[4]) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                : "memory");
 }
@@ -205,19 +168,6 @@ __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
                : "memory");
-}
-
-// An accumulator tile, a 16-byte vector per lane.
-__device__ __forceinline__ void sts_acc(uint32_t addr, const float (&c)[4]) {
-  sts128(addr, make_uint4(__float_as_uint(c[0]), __float_as_uint(c[1]), __float_as_uint(c[2]),
-                          __float_as_uint(c[3])));
-}
-__device__ __forceinline__ void lds_acc(uint32_t addr, float (&c)[4]) {
-  const uint4 v = lds128(addr);
-  c[0] = __uint_as_float(v.x);
-  c[1] = __uint_as_float(v.y);
-  c[2] = __uint_as_float(v.z);
-  c[3] = __uint_as_float(v.w);
 }
 
 // ---------------------------------------------------------------- tcgen05
@@ -476,22 +426,6 @@ struct NextRow {
   }
 };
 
-// Tile of ROWS rows of ROWB bytes: row r from src + r * stride (bytes), the
-// first `rows` rows and `units` units of each; the rest is zeros.  src must
-// be a valid pointer even where nothing of it is read.
-template <int ROWS, int ROWB, int NTH>
-__device__ __forceinline__ void load_tile(uint32_t dst, const void* src, int64_t stride, int rows,
-                                          int units, int tid) {
-  constexpr int U = ROWB / 16;
-  const char* s = static_cast<const char*>(src);
-#pragma unroll 4
-  for (int i = tid; i < ROWS * U; i += NTH) {
-    const int r = i / U, u = i % U;
-    const bool in = r < rows && u < units;
-    cp16(tile_at<ROWB>(dst, r, u), in ? s + r * stride + u * 16 : s, in);
-  }
-}
-
 // The kept tiles move between global and shared memory as they lie there, by
 // bulk copies.  Stores: what the warp wrote is made visible to the copy
 // engine, then one lane stores and commits; before the bytes are written
@@ -530,21 +464,6 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
-// A strip of T from token rows: rows [0, rows) and `units` 16-byte units of
-// each from src + r * stride (bytes), zeros elsewhere.  One warp.
-template <typename T>
-__device__ __forceinline__ void load_strip(uint32_t dst, const void* src, int64_t stride, int rows,
-                                           int units, int lane) {
-  constexpr int U = (int)sizeof(T);  // 16 values: 2 or 4 units
-  const char* s = static_cast<const char*>(src);
-#pragma unroll
-  for (int i = 0; i < kChunk * U / 32; ++i) {
-    const int r = (i * 32 + lane) / U, u = (i * 32 + lane) % U;
-    const bool in = r < rows && u < units;
-    cp16(U == 2 ? strip_at(dst, r, u) : strip32_at(dst, r, u), in ? s + r * stride + u * 16 : s, in);
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <>
@@ -565,30 +484,6 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-
-// Stores an accumulator tile that holds 16 rows of values (dv) x 8 tokens as
-// token rows: element (token, dv) at out[token * stride + dv].  Tokens
-// [0, ntok) and values [0, nval) of the tile are written.
-template <typename T>
-__device__ __forceinline__ void store_t(T* out, int64_t stride, const float (&c)[4], int lane,
-                                        int ntok, int nval) {
-  const int g = lane >> 2, t = lane & 3;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int tok = 2 * t + (q & 1), val = g + (q >> 1) * 8;
-      if (tok < ntok && val < nval) out[tok * stride + val] = c[q];
-    }
-  } else {
-    const uint32_t lo = movmatrix_t(pack2<T>(c[0], c[1]));
-    const uint32_t hi = movmatrix_t(pack2<T>(c[2], c[3]));
-    if (g < ntok) {
-      T* p = out + g * stride + 2 * t;
-      if (nval > 0) *reinterpret_cast<uint32_t*>(p) = lo;
-      if (nval > 8) *reinterpret_cast<uint32_t*>(p + 8) = hi;
-    }
-  }
 }
 
 }  // namespace fpscan

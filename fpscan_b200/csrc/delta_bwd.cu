@@ -32,10 +32,6 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
 
 namespace {
 
-constexpr int kHalfTile = 2 * kChunk * 128;    // 64 columns of K's, then Q's rows
-constexpr int kTileKQ = 2 * kHalfTile;         // one part of K and Q
-constexpr int kMatBytes = kChunk * kChunk * 2; // one part of N or PN
-
 // ------------------------------------------------------------------ along the chunks, backwards
 struct RevParams {
   const __nv_bfloat16* kq_tiles;
@@ -345,45 +341,39 @@ struct GradParams {
 
 constexpr int kGradThreads = 512;
 
-// 16 warps.  The three 64 x dk sums (dQ, R, W) are cut into tiles of 32
-// rows x 16 columns, H and X into tiles of 16 x 16; all stay in registers
-// while dO, dV, E, S0 and dS pass once through a ring of bulk copies, KS
-// strips of 16 values at a time.  One CTA per SM takes chunk after chunk, and
-// the ring runs on into the next chunk during the second phase: with a CTA
-// per chunk the copies of a chunk and its products took turns.
-template <int NP, int LV>
+// For 32-bit results (LV = 2; the sums of each step of 16 values have to be
+// rounded, see Step, which products summed in tensor memory are not).  16
+// warps.  The three 64 x dk sums (dQ, R, W) are cut into tiles of 32 rows x 16
+// columns, H and X into tiles of 16 x 16; all stay in registers while dO, dV,
+// E, S0 and dS pass once through a ring of bulk copies, a strip of 16 values
+// at a time.  One CTA per SM takes chunk after chunk, and the ring runs on
+// into the next chunk during the second phase.
+template <int NP>
 struct GradCfg {
-  static constexpr int NS = LV + 1;
+  static constexpr int LV = 2, NS = LV + 1;
   static constexpr int MT = 2;     // m tiles of a warp in the 64 x dk sums
   static constexpr int kColW = 8;  // warps side by side there
   static constexpr int kMat = kMatBytes;
   static constexpr int kRows = 2 * kStrip;  // a strip of a part of S0 or dS
-  static constexpr int kOne = (NP + 2 * NS) * kStrip + 2 * NS * kRows;  // one strip's share
-  static constexpr int KS = 1;
   // a stage of the ring
-  static constexpr int oV = KS * NP * kStrip;
-  static constexpr int oE = oV + KS * NS * kStrip;
-  static constexpr int oS = oE + KS * NS * kStrip;
-  static constexpr int oD = oS + NS * KS * kRows;
-  static constexpr int kStage = oD + NS * KS * kRows;
-  static_assert(kStage == KS * kOne);
-  // K, Q and the decay vectors; the matrices of the second phase (two at a
-  // time where four do not fit); the ring
+  static constexpr int oV = NP * kStrip, oE = oV + NS * kStrip, oS = oE + NS * kStrip;
+  static constexpr int oD = oS + NS * kRows, kStage = oD + NS * kRows;
+  // K, Q and the decay vectors; two matrices of the second phase; the ring
   static constexpr int oVec = NP * kTileKQ;
   static constexpr int kVecBytes = kVecCount * kChunk * 4;
   static constexpr int oMats = oVec + (kVecBytes + 127) / 128 * 128;
-  static constexpr int kSets = LV == 1 ? 2 : 1;  // of two matrices
-  static constexpr int oRing = oMats + kSets * 2 * NS * kMat;
+  static constexpr int oRing = oMats + 2 * NS * kMat;
   static constexpr int kRoom = 227 * 1024 - 8192 - 128 - oRing;
   static constexpr int kStages = kRoom / kStage < 4 ? kRoom / kStage : 4;
   static constexpr int kSmem = oRing + kStages * kStage + 128;
   static_assert(kStages >= 1 && kSmem + 8192 <= 227 * 1024);
 };
 
-template <typename T, int NP, int LV>
+template <typename T>
 __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradParams p) {
-  using Cfg = GradCfg<NP, LV>;
-  constexpr int NS = Cfg::NS, NTH = kGradThreads, MROW = kChunk * 2, KS = Cfg::KS;
+  constexpr int NP = kParts<T>;
+  using Cfg = GradCfg<NP>;
+  constexpr int LV = Cfg::LV, NS = Cfg::NS, NTH = kGradThreads, MROW = kChunk * 2;
   constexpr int MT = Cfg::MT, ST = Cfg::kStages, CW = Cfg::kColW;
   extern __shared__ __align__(128) unsigned char dsm_raw[];
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
@@ -398,12 +388,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   const int row0 = warp / CW * 16 * MT, col0 = warp % CW * 16;  // in the 64 x dk sums
   const int hr = (warp >> 2) * 16, hc = (warp & 3) * 16;        // in H and X
   // The tiles of H and X above the diagonal are not needed: their 6 warps
-  // take <S0, dS> instead, and one of them (thread kLoader) issues the copies.
+  // take <S0, dS> instead, and one thread of them (kLoader) issues the copies
+  // (a whole warp with an elected lane spilled more: 29 us against 26).
   const bool lower = hc <= hr;
   constexpr int kLoader = 3 * 32;
   const int above = warp < 4 ? warp - 1 : warp < 8 ? warp - 3 : 5;  // 0..5 among those
   const int64_t kstride = (int64_t)p.key_heads * p.dk;
-  const int strips = (p.dv + 15) / 16, slices = (strips + KS - 1) / KS;
+  const int strips = (p.dv + 15) / 16;
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&full[i], 1);
@@ -416,31 +407,28 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   pdl_wait();
   pdl_launch_dependents();
 
-  // the copies: slice by slice, over this CTA's chunks
+  // the copies: strip by strip, over this CTA's chunks
   const int64_t mine = (p.units - blockIdx.x + gridDim.x - 1) / gridDim.x;  // chunks of this CTA
-  const int64_t total = mine * slices;
-  int64_t next = 0;      // slices issued
+  const int64_t total = mine * strips;
+  int64_t next = 0;      // strips issued
   int64_t next_unit = blockIdx.x;
-  int next_slice = 0;
+  int next_strip = 0;
   auto issue = [&]() {
     const int s = (int)(next % ST);
-    if (next >= ST && !mbar_wait_soon(&freed[s], (uint32_t)((next / ST - 1) & 1))) return false;
-    const int64_t unit = next_unit;
-    const int v0 = next_slice * KS, n = min(KS, strips - v0);
+    if (next >= ST && !mbar_wait_soon(&freed[s], (uint32_t)((next / ST - 1) & 1))) return;
+    const int64_t strip = next_unit * strips + next_strip;
     const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
-    mbar_expect_tx(&full[s], n * Cfg::kOne);
-    bulk_in(at, p.do_parts + (unit * strips + v0) * NP * (kStrip / 2), n * NP * kStrip, &full[s]);
-    bulk_in(at + Cfg::oV, p.dv_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
-    bulk_in(at + Cfg::oE, p.e_parts + (unit * strips + v0) * NS * (kStrip / 2), n * NS * kStrip, &full[s]);
-    const int64_t sv = (unit * strips + v0) * NS * (Cfg::kRows / 2);
-    bulk_in(at + Cfg::oS, p.s_parts + sv, n * NS * Cfg::kRows, &full[s]);
-    bulk_in(at + Cfg::oD, p.ds_parts + sv, n * NS * Cfg::kRows, &full[s]);
+    mbar_expect_tx(&full[s], Cfg::kStage);
+    bulk_in(at, p.do_parts + strip * (NP * kStrip / 2), NP * kStrip, &full[s]);
+    bulk_in(at + Cfg::oV, p.dv_parts + strip * (NS * kStrip / 2), NS * kStrip, &full[s]);
+    bulk_in(at + Cfg::oE, p.e_parts + strip * (NS * kStrip / 2), NS * kStrip, &full[s]);
+    bulk_in(at + Cfg::oS, p.s_parts + strip * (NS * Cfg::kRows / 2), NS * Cfg::kRows, &full[s]);
+    bulk_in(at + Cfg::oD, p.ds_parts + strip * (NS * Cfg::kRows / 2), NS * Cfg::kRows, &full[s]);
     ++next;
-    if (++next_slice == slices) {
-      next_slice = 0;
+    if (++next_strip == strips) {
+      next_strip = 0;
       next_unit += gridDim.x;
     }
-    return true;
   };
   auto issue_kq = [&](int64_t unit) {
     const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
@@ -451,12 +439,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     bulk_in(st + Cfg::oVec, p.vecs + unit * (kVecCount * kChunk), Cfg::kVecBytes, &full_kq);
   };
   if (tid == kLoader) {
-    while (next < min((int64_t)ST, total)) issue();
+    const int64_t ahead = min((int64_t)ST, total);
+    for (int64_t i = 0; i < ahead; ++i) issue();
     issue_kq(blockIdx.x);
   }
 
   bool ok = true;
-  int64_t it = 0;  // slices consumed
+  int64_t it = 0;  // strips consumed
   for (int64_t done = 0; done < mine; ++done) {
     const int64_t unit = blockIdx.x + done * gridDim.x;
     const int64_t bh = unit / p.chunks, chunk = unit - bh * p.chunks, b = bh / p.heads;
@@ -475,24 +464,22 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       }
     float dot = 0.f;  // this thread's share of <S0, dS>
 
-    for (int sl = 0; sl < slices; ++sl, ++it) {
-      const int s_id = (int)(it % ST), n = min(KS, strips - sl * KS);
+    for (int sl = 0; sl < strips; ++sl, ++it) {
+      const int s_id = (int)(it % ST);
       const uint32_t at = st + Cfg::oRing + s_id * Cfg::kStage;
-      // refill the stage of the slice before: every warp is done with it, or nearly
+      // refill the stage of the strip before: every warp is done with it, or nearly
       if (tid == kLoader && ST > 1 && it > 0 && next < total) issue();
       ok = __all_sync(0xffffffffu, mbar_wait_soon(&full[s_id], (uint32_t)((it / ST) & 1)));
       if (!ok) break;
-      for (int kk = 0; kk < n; ++kk) {
-        const uint32_t a_g = at + kk * NP * kStrip, a_v = at + Cfg::oV + kk * NS * kStrip,
-                       a_e = at + Cfg::oE + kk * NS * kStrip;
-        const uint32_t s_strip = at + kk * NS * Cfg::kRows;  // S0's and dS's (plus oS, oD)
+      {
+        const uint32_t a_v = at + Cfg::oV, a_e = at + Cfg::oE;
         if (lower) {
           uint32_t ag[NP][4], av[NS][4];
 #pragma unroll
-          for (int i = 0; i < NP; ++i) ldsm4(ag[i], strip_a(a_g + i * kStrip, lane, hr));
+          for (int i = 0; i < NP; ++i) ldsm4(ag[i], strip_a(at + i * kStrip, lane, hr));
 #pragma unroll
           for (int i = 0; i < NS; ++i) ldsm4(av[i], strip_a(a_v + i * kStrip, lane, hr));
-          Step<LV == 2, 4> s;
+          Step<true, 4> s;
 #pragma unroll
           for (int j = LV; j >= 0; --j) {
             uint32_t eb[4];
@@ -516,15 +503,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           uint32_t sb[NS][4];
 #pragma unroll
           for (int j = 0; j < NS; ++j)
-            ldsm4(sb[j], strip_b(s_strip + Cfg::oS + j * Cfg::kRows, lane, col0));
+            ldsm4(sb[j], strip_b(at + Cfg::oS + j * Cfg::kRows, lane, col0));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             uint32_t ag[NP][4], av[NS][4];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) ldsm4(ag[i], strip_a(a_g + i * kStrip, lane, row0 + m * 16));
+            for (int i = 0; i < NP; ++i) ldsm4(ag[i], strip_a(at + i * kStrip, lane, row0 + m * 16));
 #pragma unroll
             for (int i = 0; i < NS; ++i) ldsm4(av[i], strip_a(a_v + i * kStrip, lane, row0 + m * 16));
-            Step<LV == 2, 4> s;
+            Step<true, 4> s;
 #pragma unroll
             for (int j = LV; j >= 0; --j)
 #pragma unroll
@@ -546,13 +533,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           uint32_t db[NS][4];
 #pragma unroll
           for (int j = 0; j < NS; ++j)
-            ldsm4(db[j], strip_b(s_strip + Cfg::oD + j * Cfg::kRows, lane, col0));
+            ldsm4(db[j], strip_b(at + Cfg::oD + j * Cfg::kRows, lane, col0));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             uint32_t ae[NS][4];
 #pragma unroll
             for (int i = 0; i < NS; ++i) ldsm4(ae[i], strip_a(a_e + i * kStrip, lane, row0 + m * 16));
-            Step<LV == 2, 2> s;
+            Step<true, 2> s;
 #pragma unroll
             for (int j = LV; j >= 0; --j)
 #pragma unroll
@@ -565,8 +552,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           }
         }
       }
-      // <S0, dS> over this slice (the same place of every part: swizzle does not matter)
-      for (int i = above * 32 + lane; !lower && i < n * Cfg::kRows / 16; i += 6 * 32) {
+      // <S0, dS> over this strip (the same place of every part: swizzle does not matter)
+      for (int i = above * 32 + lane; !lower && i < Cfg::kRows / 16; i += 6 * 32) {
         float x[8] = {}, y[8] = {};
 #pragma unroll
         for (int q = NS - 1; q >= 0; --q) {
@@ -604,8 +591,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     const float* hi = s_vec + kVecCumHi * kChunk;
     const float* lo = s_vec + kVecCumLo * kChunk;
     // H and X times D: rows i, columns j, in the order of an A operand's
-    // registers.  As parts in shared memory with each column times beta (set
-    // 0, row operands of dQ and R) or without (set 1, column operands of W).
+    // registers.  As parts in shared memory first with each column times beta
+    // (set 0, row operands of dQ and R), then without (set 1, column operands
+    // of W).
     float2 hd[4], xd[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -624,7 +612,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       }
     }
     auto put_mats = [&](int set) {
-      const uint32_t base = st + Cfg::oMats + (Cfg::kSets == 2 ? set : 0) * 2 * NS * Cfg::kMat;
+      const uint32_t base = st + Cfg::oMats;
       uint32_t wh[4][NS], wx[4][NS];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -642,7 +630,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       }
     };
     put_mats(0);
-    if (Cfg::kSets == 2) put_mats(1);
     // an element pair of K or Q as fp32 (the sum of its parts)
     auto kq_pair = [&](int row, int col) {  // Q: rows 64..
       float2 v = make_float2(0.f, 0.f);
@@ -695,7 +682,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       for (int j = 0; j < NP; ++j) ldsm4_t(kb[j], at_bt<128>(kq_cols + j * kTileKQ, lane, col0 & 63, kk));
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        Step<LV == 2, 4> s;
+        Step<true, 4> s;
 #pragma unroll
         for (int i = LV; i >= 0; --i) {
           uint32_t fh[4], fx[4];
@@ -717,11 +704,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
         s.add(3, ar[m][1]);
       }
     }
-    if (Cfg::kSets == 1) {
-      __syncthreads();
-      put_mats(1);
-      __syncthreads();
-    }
+    __syncthreads();
+    put_mats(1);
+    __syncthreads();
     // W += Hs^T Q + Xd^T K: rows j, columns i >= j
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
@@ -734,12 +719,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        Step<LV == 2, 4> s;
+        Step<true, 4> s;
 #pragma unroll
         for (int i = LV; i >= 0; --i) {
           uint32_t fh[4], fx[4];
-          const uint32_t base =
-              st + Cfg::oMats + (Cfg::kSets == 2 ? 2 * NS * Cfg::kMat : 0) + i * Cfg::kMat;
+          const uint32_t base = st + Cfg::oMats + i * Cfg::kMat;
           ldsm4_t(fh, at_at<MROW>(base, lane, row0 + m * 16, kk));
           ldsm4_t(fx, at_at<MROW>(base + NS * Cfg::kMat, lane, row0 + m * 16, kk));
 #pragma unroll
@@ -1454,8 +1438,8 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
     if (e != cudaSuccess) return e;
     e = launch_pdl(kern, grid, kTcThreads, GC::kSmem, a.stream, g);
   } else {
-    using GC = GradCfg<NP, LV>;
-    auto kern = delta_grad_kernel<T, NP, LV>;
+    using GC = GradCfg<NP>;
+    auto kern = delta_grad_kernel<T>;
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC::kSmem);
     if (e != cudaSuccess) return e;
     e = launch_pdl(kern, grid, kGradThreads, GC::kSmem, a.stream, g);

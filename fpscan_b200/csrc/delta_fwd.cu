@@ -42,12 +42,9 @@ struct PrepParams {
 };
 
 constexpr int kPrepThreads = 128;
-constexpr int kMatBytes = kChunk * kChunk * 2;  // one part of N or P
 constexpr int kPad = kChunk + 4;  // fp32 rows in shared memory: 16-byte vectors on distinct banks
 
 constexpr int kDkp = 128;                          // dk, padded
-constexpr int kHalfTile = 2 * kChunk * 128;        // 64 columns of K's, then Q's rows
-constexpr int kTileKQ = 2 * kHalfTile;             // one part of K and Q
 
 // K and Q, and behind them M diag(beta); over K and Q, once they are used up,
 // the inverse; behind that, over all else, the images of N and PN.

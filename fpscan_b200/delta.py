@@ -162,6 +162,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     _launch(v.get_device(), "fpscan_delta_step", q.data_ptr(), k.data_ptr(), v.data_ptr(),
             log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), out.data_ptr(), state.data_ptr(),
             *_sizes(q, v), _scale(scale, q), DTYPE_CODES[v.dtype])
+    if not state.is_inference():  # a backward pass that has saved this state must notice
+        torch.autograd.graph.increment_version(state)
     return out
 
 
@@ -190,8 +192,8 @@ def gated_delta_backward(q, k, v, log_decay, beta, grad_out, initial_state=None,
 
 
 class GatedDelta(torch.autograd.Function):
-    """Differentiable gated delta rule (the compiled binding has the same one).  Saves its inputs (q, k and v in 8 bits with ``checkpoint8``) and
-    recomputes the chunks' states in the backward pass."""
+    """Differentiable gated delta rule (the compiled binding has the same one).  Saves its inputs (q, k and v
+    in 8 bits with ``checkpoint8``) and recomputes the chunks' states in the backward pass."""
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, beta, state, scale, return_state, checkpoint8):
