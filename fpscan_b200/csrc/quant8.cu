@@ -48,28 +48,36 @@ template <typename T>
 __global__ void __launch_bounds__(256) quantize8_kernel(const Quant8Params p) {
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t units = (p.n + kBlock8 - 1) / kBlock8 * 8;  // whole blocks: all lanes of a group stay
+  const int64_t units = (p.n + kBlock8 - 1) / kBlock8 * 4;  // whole blocks: all lanes of a group stay
   const int64_t step = (int64_t)gridDim.x * blockDim.x;
   const T* src = static_cast<const T*>(p.x);
-  // the loop's bound is a multiple of 8 lanes, not of 32: the shuffles name their group
-  const unsigned mask = 0xffu << (threadIdx.x & 24);
+  // the loop's bound is a multiple of 4 lanes, not of 32: the shuffles name their group
+  const unsigned mask = 0xfu << (threadIdx.x & 28);
   for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += step) {
-    const int64_t i = u * 8, left = p.n - i;
-    float x[8];
-    load8(src + i, left, x);
+    const int64_t i = u * 16, left = p.n - i;
+    float x[2][8];
+    load8(src + i, left, x[0]);
+    load8(src + i + 8, left - 8, x[1]);
     uint32_t most = 0;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) most = max(most, __float_as_uint(x[c]) & 0x7fffffffu);
+    for (int c = 0; c < 8; ++c)
+      most = max(most, max(__float_as_uint(x[0][c]) & 0x7fffffffu, __float_as_uint(x[1][c]) & 0x7fffffffu));
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) most = max(most, __shfl_xor_sync(mask, most, d));
-    const Quant8 q = quant8_block(most);
-    const uint2 code = make_uint2(quant8_codes(q, x[0], x[1], x[2], x[3]),
-                                  quant8_codes(q, x[4], x[5], x[6], x[7]));
-    if (left >= 8)
-      *reinterpret_cast<uint2*>(p.codes + i) = code;
+    for (int d = 1; d < 4; d <<= 1) most = max(most, __shfl_xor_sync(mask, most, d));
+    const Quant8 q = quant8_block<T>(most);
+    uint32_t w[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float* y = x[c / 2] + c % 2 * 4;
+      w[c] = quant8_codes<T>(q, y[0], y[1], y[2], y[3]);
+    }
+    if (left >= 16)
+      *reinterpret_cast<uint4*>(p.codes + i) = make_uint4(w[0], w[1], w[2], w[3]);
     else
-      for (int c = 0; c < left; ++c) p.codes[i + c] = (int8_t)((c < 4 ? code.x : code.y) >> (8 * (c & 3)));
-    if ((u & 7) == 0) p.steps[u / 8] = q.step;
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        if (c < left) p.codes[i + c] = (int8_t)(w[c / 4] >> (8 * (c & 3)));
+    if ((u & 3) == 0) p.steps[u / 4] = q.step;
   }
 }
 

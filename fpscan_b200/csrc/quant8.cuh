@@ -4,20 +4,31 @@
 //
 // The code is the rounding of the quotient x * 127 / most.  Times a rounded
 // reciprocal alone it would not be: half of a block's largest value, common
-// in bf16, is a tie, and the product may land on either side of it.  So the
+// in bf16, is a tie, and the product may land on either side of it.
+//
+// bf16: one multiply-add, x r + 1.5 * 2^23 with r = 127 / most rounded up,
+// rounds the product itself to an integer.  It is off by 2^-23 of the quotient
+// at most and never towards zero, and a quotient that is no tie is at least
+// 2^-19 of itself away from one.  A tie has 254 x = (2 n + 1) most with odd 2 n + 1, so the
+// prime 127 divides most's significand (which has 8 bits: then it is a power
+// of two times 127, and r is exact) or 2 n + 1 (then 2 n + 1 = 127, the value
+// is most / 2, and its tie 63.5 goes to 64, even and away from zero).
+// fp16 and fp32: a significand may hold 127 times an odd number, so the
 // quotient is corrected once by its residual (Markstein, 1990: with the
 // correctly rounded reciprocal y of b and q near a / b, q + (a - q b) y
-// rounds to the quotient), three multiply-adds in place of a division: the
-// kernels below read and write about 3 bytes for a value and have some 20
-// instructions for it before they are bound by them.  For fp16 and bf16
-// x * 127 is exact and a quotient that is not a tie is at least 2^-19 of
-// itself away from one, so the codes are those of real arithmetic; for fp32
-// they are those of fp32 arithmetic.
+// rounds to the quotient), three multiply-adds in place of a division.  For
+// fp16 x * 127 is exact, and the codes are those of real arithmetic as in
+// bf16; for fp32 they are those of fp32 arithmetic.
+//
+// The kernels read and write about 3 bytes for a value and have some 20
+// instructions for it before these bound them.
 //
 // Magnitudes near the ends of fp32 are brought to its middle by a power of
 // two.  A block that holds an infinity or a NaN has a step that is not finite
 // and codes of 0: all of it reads back as NaN.
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -25,26 +36,29 @@ namespace fpscan {
 
 struct Quant8 {
   float step;       // most / 127
-  float mul;        // 127 times the power of two
-  float most, inv;  // the largest magnitude times the power of two, its reciprocal
+  float mul;        // the power of two; but for bf16, 127 times that
+  float most, inv;  // the largest magnitude times the power of two, its reciprocal (bf16: 127 / most)
   uint32_t keep;    // all ones; 0: every code is 0
 };
 
 // `bits`: the largest magnitude of the block, as the bits of its absolute
 // value (compared as integers, a NaN is above everything).
+template <typename T>
 __device__ __forceinline__ Quant8 quant8_block(uint32_t bits) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   Quant8 q;
   const float most = __uint_as_float(bits);
   q.step = most / 127.f;
   q.keep = bits != 0 && bits < 0x7f800000u ? ~0u : 0u;
   const float up = most > 0x1p100f ? 0x1p-60f : most < 0x1p-80f ? 0x1p80f : 1.f;
-  q.mul = 127.f * up;
+  q.mul = kBf16 ? up : 127.f * up;
   q.most = q.keep ? most * up : 1.f;
-  q.inv = __frcp_rn(q.most);
+  q.inv = kBf16 ? __fdiv_ru(127.f, q.most) : __frcp_rn(q.most);
   return q;
 }
 
 // Codes of four values, one byte each.
+template <typename T>
 __device__ __forceinline__ uint32_t quant8_codes(const Quant8& q, float a, float b, float c,
                                                  float d) {
   const float x[4] = {a, b, c, d};
@@ -52,11 +66,15 @@ __device__ __forceinline__ uint32_t quant8_codes(const Quant8& q, float a, float
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float t = x[i] * q.mul;
-    float r = t * q.inv;
-    r = fmaf(fmaf(-r, q.most, t), q.inv, r);
     // adding 1.5 * 2^23 rounds to an integer, ties to even, whose low byte
     // in two's complement is the sum's
-    w[i] = __float_as_uint(r + 12582912.f);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      w[i] = __float_as_uint(fmaf(t, q.inv, 12582912.f));
+    } else {
+      float r = t * q.inv;
+      r = fmaf(fmaf(-r, q.most, t), q.inv, r);
+      w[i] = __float_as_uint(r + 12582912.f);
+    }
   }
   return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410) &
          q.keep;

@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(NTH, 1)
         for (int c = 0; c < V; ++c)
           most = max(most, __float_as_uint(y[c]) & (blk0 + i < L ? 0x7fffffffu : 0u));
       }
-      const Quant8 q8 = quant8_block(most);
+      const Quant8 q8 = quant8_block<T>(most);
       if (lane_ok && blk0 < L) p.steps[(b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv] = q8.step;
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(NTH, 1)
         uint32_t w[V / 4];
 #pragma unroll
         for (int c = 0; c < V; c += 4)
-          w[c / 4] = quant8_codes(q8, y[c], y[c + 1], y[c + 2], y[c + 3]);
+          w[c / 4] = quant8_codes<T>(q8, y[c], y[c + 1], y[c + 2], y[c + 3]);
         if (lane_ok && blk0 + i < L) {
           int8_t* o = p.codes + (b * L + blk0 + i) * p.code_stride + cv * V;
           if constexpr (V == 8)
