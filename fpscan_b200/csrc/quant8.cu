@@ -26,22 +26,20 @@ struct Quant8Params {
   int64_t n;
 };
 
-// Eight values from p; those at or past `left` are 0.
+// A 16-byte vector from p; values at or past `left` are 0.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t left, float (&x)[8]) {
+__device__ __forceinline__ uint4 load_vec(const T* p, int64_t left) {
   constexpr int V = Elem<T>::kVec;
-  if (left >= 8) {
-#pragma unroll
-    for (int j = 0; j < 8 / V; ++j) {
-      Vec16<T> v;
-      v.raw = *reinterpret_cast<const uint4*>(p + j * V);
-#pragma unroll
-      for (int c = 0; c < V; ++c) x[j * V + c] = Elem<T>::load(v.e[c]);
-    }
+  Vec16<T> v;
+  v.raw = make_uint4(0, 0, 0, 0);
+  if (left >= V) {
+    v.raw = *reinterpret_cast<const uint4*>(p);
   } else {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) x[c] = c < left ? Elem<T>::load(p[c]) : 0.f;
+    for (int c = 0; c < V; ++c)
+      if (c < left) v.e[c] = p[c];
   }
+  return v.raw;
 }
 
 template <typename T>
@@ -55,21 +53,24 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const Quant8Params p) {
   const unsigned mask = 0xfu << (threadIdx.x & 28);
   for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += step) {
     const int64_t i = u * 16, left = p.n - i;
-    float x[2][8];
-    load8(src + i, left, x[0]);
-    load8(src + i + 8, left - 8, x[1]);
+    constexpr int V = Elem<T>::kVec;
+    uint4 raw[16 / V];
+#pragma unroll
+    for (int j = 0; j < 16 / V; ++j) raw[j] = load_vec(src + i + j * V, left - j * V);
     uint32_t most = 0;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      most = max(most, max(__float_as_uint(x[0][c]) & 0x7fffffffu, __float_as_uint(x[1][c]) & 0x7fffffffu));
+    for (int j = 0; j < 16 / V; ++j) most = quant8_max<T>(most, quant8_max<T>(raw[j]));
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) most = max(most, __shfl_xor_sync(mask, most, d));
-    const Quant8 q = quant8_block<T>(most);
+    for (int d = 1; d < 4; d <<= 1) most = quant8_max<T>(most, __shfl_xor_sync(mask, most, d));
+    const Quant8 q = quant8_block<T>(quant8_bits<T>(most));
     uint32_t w[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float* y = x[c / 2] + c % 2 * 4;
-      w[c] = quant8_codes<T>(q, y[0], y[1], y[2], y[3]);
+      Vec16<T> v;
+      v.raw = raw[4 * c / V];
+      const T* y = v.e + 4 * c % V;
+      w[c] = quant8_codes<T>(q, Elem<T>::load(y[0]), Elem<T>::load(y[1]), Elem<T>::load(y[2]),
+                             Elem<T>::load(y[3]));
     }
     if (left >= 16)
       *reinterpret_cast<uint4*>(p.codes + i) = make_uint4(w[0], w[1], w[2], w[3]);

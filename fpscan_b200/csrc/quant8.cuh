@@ -41,6 +41,30 @@ struct Quant8 {
   uint32_t keep;    // all ones; 0: every code is 0
 };
 
+// Largest magnitudes, as the bits of absolute values compared as integers (so
+// a NaN is above everything); 16-bit types two at a time.
+template <typename T>
+__device__ __forceinline__ uint32_t quant8_max(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) return max(a, b);
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t quant8_max(const uint4& x) {
+  constexpr uint32_t m = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  return quant8_max<T>(quant8_max<T>(x.x & m, x.y & m), quant8_max<T>(x.z & m, x.w & m));
+}
+// The same as the bits of one fp32 magnitude.
+template <typename T>
+__device__ __forceinline__ uint32_t quant8_bits(uint32_t most) {
+  if constexpr (sizeof(T) == 4) return most;
+  const uint32_t one = max(most >> 16, most & 0xffffu);
+  if constexpr (std::is_same<T, __half>::value)
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)one)));
+  return one << 16;
+}
+
 // `bits`: the largest magnitude of the block, as the bits of its absolute
 // value (compared as integers, a NaN is above everything).
 template <typename T>
@@ -61,16 +85,21 @@ __device__ __forceinline__ Quant8 quant8_block(uint32_t bits) {
 template <typename T>
 __device__ __forceinline__ uint32_t quant8_codes(const Quant8& q, float a, float b, float c,
                                                  float d) {
-  const float x[4] = {a, b, c, d};
+  float x[4] = {a, b, c, d};
   uint32_t w[4];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if (q.mul != 1.f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] *= q.mul;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float t = x[i] * q.mul;
     // adding 1.5 * 2^23 rounds to an integer, ties to even, whose low byte
     // in two's complement is the sum's
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      w[i] = __float_as_uint(fmaf(t, q.inv, 12582912.f));
+      w[i] = __float_as_uint(fmaf(x[i], q.inv, 12582912.f));
     } else {
+      const float t = x[i] * q.mul;
       float r = t * q.inv;
       r = fmaf(fmaf(-r, q.most, t), q.inv, r);
       w[i] = __float_as_uint(r + 12582912.f);

@@ -340,14 +340,8 @@ __global__ void __launch_bounds__(NTH, 1)
       // rows past L and vectors past dim were read as zeros and hold zeros
       uint32_t most = 0;
 #pragma unroll
-      for (int i = 0; i < TW; ++i) {
-        float y[V];
-        unpack<T>(kept[i], y);
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-          most = max(most, __float_as_uint(y[c]) & (blk0 + i < L ? 0x7fffffffu : 0u));
-      }
-      const Quant8 q8 = quant8_block<T>(most);
+      for (int i = 0; i < TW; ++i) most = quant8_max<T>(most, blk0 + i < L ? quant8_max<T>(kept[i]) : 0);
+      const Quant8 q8 = quant8_block<T>(quant8_bits<T>(most));
       if (lane_ok && blk0 < L) p.steps[(b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv] = q8.step;
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
