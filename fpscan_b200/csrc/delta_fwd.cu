@@ -17,7 +17,11 @@
 // warps read the result from tensor memory (a thread holds C values of one
 // token, or of one row of the state), and write the next operand's parts to
 // shared memory: warps of lanes 0..63 work on X and E, those of 64..127 on the
-// output, all on the state.
+// output, all on the state.  What bounds it is this chain, 4500 to 6000 cycles
+// a chunk, about 40% of them products, and with 64 heads or more the bytes.
+// Measured, dk = dv = 128: two prompts of 8192, 16 heads, bf16 with states 340
+// us; 4 x 4096 tokens of 16 heads, bf16 198 us, and 243 us kept for the
+// backward pass (1 GB, 4 TB/s).
 #include <algorithm>
 
 #include "delta.cuh"
@@ -41,6 +45,11 @@ struct PrepParams {
   float scale;
 };
 
+// One chunk per CTA of four warps, four CTAs on an SM: a chunk is a chain of
+// short steps (load, two 64 x 64 x 128 products, the inverse by blocks of 16,
+// P N) with a barrier after each, and what one CTA waits for the others
+// cover (with fewer CTAs on an SM 153 us against 128).  4 x 4096 tokens of 16
+// heads, dk = 128: bf16 137 us (400 MB, 3 TB/s), 2 x 8192 with three parts 166 us.
 constexpr int kPrepThreads = 128;
 constexpr int kPad = kChunk + 4;  // fp32 rows in shared memory: 16-byte vectors on distinct banks
 
@@ -119,8 +128,10 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   float* s_n = reinterpret_cast<float*>(dsm);              // the inverse
   float* s_a = reinterpret_cast<float*>(dsm + Cfg::oA);  // M diag(beta), strictly lower
   float* s_vec = reinterpret_cast<float*>(dsm + Cfg::oVec);
+  __shared__ int s_bad;  // first row of M that is not finite
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_bad = kChunk;
   const int64_t bh = blockIdx.x / p.chunks, chunk = blockIdx.x - bh * p.chunks;
   const int64_t b = bh / p.heads;
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
@@ -222,6 +233,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   };
   float acc[8][4];
   with_k(0, acc);
+  float probe[2] = {0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -232,12 +244,27 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
       for (int c = 0; c < 2; ++c) {
         const int j = j0 + c;
         a[c] = i > j ? acc[n][2 * r + c] * expf((hi[i] - hi[j]) + (lo[i] - lo[j])) * be[j] : 0.f;
+        probe[r] = fmaf(a[c], 0.f, probe[r]);
       }
       *reinterpret_cast<float2*>(&s_a[i * kPad + j0]) = make_float2(a[0], a[1]);
     }
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+    if (probe[r] != 0.f) atomicMin(&s_bad, warp * 16 + g4 + r * 8);
   with_k(kChunk, acc);
   if (keeper) bulk_wait_read<0>();
   __syncthreads();  // K and Q are used up
+  // An infinity or a NaN (of k, beta, log_decay; or an overflow) would reach
+  // the rows of N before its own through zeros times it.  From that row on M
+  // counts as zeros here, and what reads the state as NaN, which
+  // delta_scan_kernel carries to all that follows.
+  if (s_bad < kChunk) {  // uniform
+    for (int i = s_bad * kPad + tid; i < kChunk * kPad; i += kPrepThreads) s_a[i] = 0.f;
+    for (int i = s_bad + tid; i < kChunk; i += kPrepThreads)
+      p.vecs[(bh * p.chunks + chunk) * (kVecCount * kChunk) + kVecEnter * kChunk + i] =
+          __int_as_float(0x7fc00000);
+    __syncthreads();
+  }
   uint32_t pf[4][NS][4];  // P's 16 rows of this warp, as an A operand
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
@@ -729,9 +756,10 @@ cudaError_t launch_scan_as(const DeltaArgs& a, ScanParams& p, int64_t bh) {
 }
 
 // 32 values per CTA while every CTA gets an SM of its own (fewer values,
-// shorter steps: two prompts of 8192, 32 heads, 411 us against 574 us), 64
-// beyond (more work for each operand read: 64 heads of 4096 kept for the
-// backward pass 208 us against 220 us with two CTAs of 32 values on an SM).
+// shorter steps: two prompts of 8192, 16 heads with states, 340 us against
+// 532 us), 64 beyond (more work for each operand read: 4 x 4096 of 16 heads
+// 198 us against 280 us, kept for the backward pass 243 us against 300 us,
+// delta_rev_kernel 284 us against 325 us).
 template <typename T, int LV, bool KEEP>
 cudaError_t launch_scan(const DeltaArgs& a, ScanParams& p, int64_t bh) {
   return bh * ((a.dv + 31) / 32) <= a.num_sms ? launch_scan_as<T, LV, KEEP, 16>(a, p, bh)

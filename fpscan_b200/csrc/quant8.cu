@@ -1,10 +1,11 @@
 // quantize8 / dequantize8: a tensor kept in 8 bits for the backward pass, in
 // blocks of 64 consecutive values (format in quant8.cuh).
 //
-// Bound by memory: the value's bytes and one more in each direction.  Eight
-// lanes share a block, eight values each, so a lane reads 16 (fp32: 32)
-// bytes and writes 8, a block's magnitude is three shuffles, and no shared
-// memory or second pass is needed.
+// Bound by memory: the value's bytes and one more in each direction.  To 8
+// bits, four lanes share a block, 16 values each: the block's quotients are
+// worked out by every lane (with eight lanes they cost 113 us instead of 85),
+// its magnitude is two shuffles, and no shared memory or second pass is
+// needed.  32768 x 4096 bf16: to 8 bits 85 us (4.8 TB/s), back 71 us (5.7 TB/s).
 #include <algorithm>
 
 #include "internal.h"

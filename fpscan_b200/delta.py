@@ -19,6 +19,11 @@ are float32 (batch, heads, dv, dk).  dk: a multiple of 8 up to 128; dv: a multip
 ``log_decay`` is usually <= 0 and may be -inf: the state before that token counts no more, which is how a
 sequence packed behind another begins (the gradient with respect to that ``log_decay`` is 0).
 
+An infinity or a NaN spoils nothing before its token: in q it spoils that token's output, in v its column of
+the outputs from there on, in k, log_decay or beta its head from there on, a reset or not.  So what pads a
+batch behind a sequence does not reach its outputs; for its final state and its gradients it has to be
+finite (beta 0 writes nothing).
+
 Sums, states and the decay's running sums are held in 32 bits or more.  The products run on 16-bit tensor
 cores with operands cut into exact parts: to 2^-16 relative where everything that comes out has 16 bits, to
 2^-24 where a float32 tensor does (float32 data, or a state that is taken, returned or differentiated).

@@ -183,3 +183,21 @@ def test_a_state_changed_by_a_step_is_noticed():
         fp.gated_delta_step(*(t[:, :1].contiguous() for t in x), s1)
     fp.gated_delta_step(*(t[:, :1].contiguous() for t in x), s1)  # made there, used here
 
+
+
+@pytest.mark.parametrize("heads", [2, 160])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["q", "k", "log_decay", "beta"])
+def test_a_bad_value_reaches_no_earlier_token(which, dtype, heads):
+    x, s0 = make(1, 140, heads, 1, 40, 24, dtype, seed=11, state=True)
+    clean = fp.gated_delta_forward(*x, initial_state=s0)
+    i = "q k v log_decay beta".split().index(which)
+    x[i].view(1, 140, heads, -1)[0, 70, 1, -1] = math.nan
+    o = fp.gated_delta_forward(*x, initial_state=s0)
+    assert torch.equal(o[:, :70], clean[:, :70])
+    assert torch.equal(o[:, :, 0], clean[:, :, 0]) and torch.equal(o[:, :, 2:], clean[:, :, 2:])
+    assert torch.isnan(o[0, 70, 1]).all()
+    if which == "q":
+        assert torch.equal(o[:, 71:], clean[:, 71:])
+    else:
+        assert torch.isnan(o[0, 71:, 1]).all()
