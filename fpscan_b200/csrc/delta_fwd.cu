@@ -49,7 +49,8 @@ struct PrepParams {
 // short steps (load, two 64 x 64 x 128 products, the inverse by blocks of 16,
 // P N) with a barrier after each, and what one CTA waits for the others
 // cover (with fewer CTAs on an SM 153 us against 128).  4 x 4096 tokens of 16
-// heads, dk = 128: bf16 137 us (400 MB, 3 TB/s), 2 x 8192 with three parts 166 us.
+// heads, dk = 128: bf16 133 us (400 MB, 3 TB/s), 2 x 8192 with three parts 167
+// us.  Giving the long rows to another warp in every CTA was no faster.
 constexpr int kPrepThreads = 128;
 constexpr int kPad = kChunk + 4;  // fp32 rows in shared memory: 16-byte vectors on distinct banks
 
@@ -233,9 +234,16 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   };
   float acc[8][4];
   with_k(0, acc);
+  // D; with 16-bit results a fast exponential will do (off by 2^-16 at the
+  // most where D is above e^-80)
+  auto decay = [&](int i, int j) {
+    const float x = (hi[i] - hi[j]) + (lo[i] - lo[j]);
+    return LV == 1 ? __expf(x) : expf(x);
+  };
   float probe[2] = {0.f, 0.f};
 #pragma unroll
-  for (int n = 0; n < 8; ++n)
+  for (int n = 0; n < 8; ++n) {
+    if (n > 2 * warp + 1) break;  // above the diagonal, and not read
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int i = warp * 16 + g4 + r * 8, j0 = n * 8 + 2 * t4;
@@ -243,11 +251,12 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int j = j0 + c;
-        a[c] = i > j ? acc[n][2 * r + c] * expf((hi[i] - hi[j]) + (lo[i] - lo[j])) * be[j] : 0.f;
+        a[c] = i > j ? acc[n][2 * r + c] * decay(i, j) * be[j] : 0.f;
         probe[r] = fmaf(a[c], 0.f, probe[r]);
       }
       *reinterpret_cast<float2*>(&s_a[i * kPad + j0]) = make_float2(a[0], a[1]);
     }
+  }
 #pragma unroll
   for (int r = 0; r < 2; ++r)
     if (probe[r] != 0.f) atomicMin(&s_bad, warp * 16 + g4 + r * 8);
@@ -267,7 +276,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   }
   uint32_t pf[4][NS][4];  // P's 16 rows of this warp, as an A operand
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk)
+  for (int kk = 0; kk < 4; ++kk) {
+    if (kk > warp) break;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int n = 2 * kk + (q >> 1), r = q & 1;
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int j = j0 + c;
-        const float d = i == j ? 1.f : i > j ? expf((hi[i] - hi[j]) + (lo[i] - lo[j])) : 0.f;
+        const float d = i > j ? decay(i, j) : 1.f;
         v[c] = i >= j ? acc[n][2 * r + c] * d * p.scale * be[j] : 0.f;
       }
       uint32_t w[NS];
@@ -284,6 +294,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
 #pragma unroll
       for (int o = 0; o < NS; ++o) pf[kk][o][q] = w[o];
     }
+  }
 
   // N = (I + A)^-1.  16 x 16 blocks on the diagonal by substitution, a column
   // a lane; then [[B, 0], [C, D]]^-1 = [[B', 0], [-D' C B', D']] twice.
