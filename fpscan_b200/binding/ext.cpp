@@ -7,6 +7,7 @@
 // call costs what the reference's does instead of a Python + ctypes round
 // trip.  All work is done by libfpscan_b200.so; this file has no kernels.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -262,6 +263,23 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
+// Gradients of a backward pass that is not differentiable itself: taken with
+// create_graph, they raise when they are differentiated instead of counting
+// as constants.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const at::Tensor& g : grads)
+    if (g.defined()) in.push_back(g.detach().set_requires_grad(true));
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " is differentiable once", (int64_t)in.size());
+  const variable_list out = (*error)(std::move(in));
+  size_t i = 0;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
+}
+
 struct GatedDelta : public torch::autograd::Function<GatedDelta> {
   static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k,
                                const Variable& v, const Variable& log_decay, const Variable& beta,
@@ -321,7 +339,7 @@ struct GatedDelta : public torch::autograd::Function<GatedDelta> {
                        ctx->saved_data["scale"].toDouble(), need);
     at::Tensor dstate;
     if (di) dstate = di->to((at::ScalarType)state_dtype);
-    return {dq, dk, dv, dg, db, dstate, none, none, none};
+    return once({dq, dk, dv, dg, db, dstate, none, none, none}, "gated_delta");
   }
 };
 
@@ -428,7 +446,7 @@ struct Scan8 : public torch::autograd::Function<Scan8> {
                                    at::cuda::getCurrentCUDAStream().stream()),
                "fpscan_scan_bwd_cl8");
     }
-    return {dgates, dtokens};
+    return once({dgates, dtokens}, "pscan_channels_last with checkpoint8");
   }
 };
 

@@ -7,7 +7,7 @@ For each head, with a state S of ``(dv, dk)`` and ``a[t] = exp(log_decay[t])``,
 
 where the scan of ops.py has one number per channel.  The reference has no such operator.
 
-* ``gated_delta``          -- differentiable (training)
+* ``gated_delta``          -- differentiable, once (training)
 * ``gated_delta_forward``  -- no autograd (a prompt: state in, state out)
 * ``gated_delta_step``     -- token by token, the state updated in place (serving)
 
@@ -36,7 +36,7 @@ import torch
 
 from . import _lib
 from .checkpoint8 import dequantize8, quantize8
-from .ops import _EXT, DTYPE_CODES, NVTX, _check_input, _fn, _launch, nvtx_range
+from .ops import _EXT, DTYPE_CODES, NVTX, _check_input, _fn, _launch, _once, nvtx_range
 
 __all__ = ["gated_delta", "gated_delta_forward", "gated_delta_step"]
 
@@ -225,7 +225,7 @@ class GatedDelta(torch.autograd.Function):
                                                   ctx.scale, need_initial=ctx.needs_input_grad[5])
         if dstate is not None:
             dstate = dstate.to(ctx.state_dtype)
-        return (*grads, dstate, None, None, None)
+        return (*_once((*grads, dstate), "gated_delta"), None, None, None)
 
 
 def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,

@@ -549,6 +549,26 @@ def _cl8_workspace(t: torch.Tensor, backward: bool) -> torch.Tensor:
     return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=t.device)
 
 
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, *grads):
+        ctx.what = what
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what} is differentiable once")
+
+
+def _once(grads, what):
+    """Gradients of a backward pass that is not differentiable itself: taken with create_graph, they raise
+    when they are differentiated instead of counting as constants."""
+    if not torch.is_grad_enabled():
+        return grads
+    out = iter(_Once.apply(what, *(g.detach().requires_grad_() for g in grads if g is not None)))
+    return tuple(None if g is None else next(out) for g in grads)
+
+
 class PScanChannelsLast8(torch.autograd.Function):
     """``PScanChannelsLast`` that keeps its output for the backward pass in 8 bits, written and read inside
     the scan kernels: one step per block of 8 timesteps x one 16-byte channel vector.  (The compiled binding
@@ -586,7 +606,7 @@ class PScanChannelsLast8(torch.autograd.Function):
                     codes.data_ptr(), steps.data_ptr(), grad_output.data_ptr(), dgates.data_ptr(),
                     dtokens.data_ptr(), b, l, d, DTYPE_CODES[grad_output.dtype], ws.data_ptr(),
                     ws.numel())
-        return dgates, dtokens
+        return _once((dgates, dtokens), "pscan_channels_last with checkpoint8")
 
 
 def pscan_channels_last(gates: torch.Tensor, tokens: torch.Tensor,

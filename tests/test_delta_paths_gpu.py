@@ -201,3 +201,24 @@ def test_a_bad_value_reaches_no_earlier_token(which, dtype, heads):
         assert torch.equal(o[:, 71:], clean[:, 71:])
     else:
         assert torch.isnan(o[0, 71:, 1]).all()
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_second_derivatives_are_refused(binding, monkeypatch):
+    if not binding:
+        for m in (ops, delta, checkpoint8):
+            monkeypatch.setattr(m, "_EXT", None)
+    x, s0 = make(1, 66, 1, 1, 16, 16, torch.float32, seed=12, state=True)
+    leaves = [t.requires_grad_() for t in (*x, s0)]
+    o = fp.gated_delta(*leaves[:5], initial_state=leaves[5])
+    plain = torch.autograd.grad(o.square().sum(), leaves, retain_graph=True)
+    grads = torch.autograd.grad(o.square().sum(), leaves, create_graph=True)
+    for a, b in zip(plain, grads):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="gated_delta is differentiable once"):
+        sum(t.sum() for t in grads).backward()  # (grad() finds the inputs unused, and says so)
+    g = torch.rand(1, 40, 8, device="cuda").requires_grad_()
+    y = fp.pscan_channels_last(g, torch.ones_like(g), checkpoint8=True)
+    d, = torch.autograd.grad(y.sum(), g, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        d.sum().backward()
