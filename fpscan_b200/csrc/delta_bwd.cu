@@ -9,10 +9,19 @@
 //     dK = diag(beta) W + R,  R = -exp(G) dV S0 - Xd diag(beta) K,
 //          W = Hs^T Q - Xd^T K + exp(G_C - G) E dS,
 //     dbeta_i = k_i . W_i,
-//     dlog_decay_t = sum_{i >= t} (q_i.dQ_i + k_i.R_i - beta_i dbeta_i) + <S_C, dS>.
-// The last two hold because beta and k scale a write alike, and because a
-// decay scales what is read after it like q and k do: no quotient of a
-// gradient by beta or by a decay appears, so zeros of both are harmless.
+//     dlog_decay_t = sum_{i >= t > j} A_ij + sum_{i >= t} reads_i + sum_{j < t} writes_j
+//                    + exp(G_C) <S0, dS>,
+//          A_ij = beta_j (Hs_ij q_i.k_j - Xd_ij k_i.k_j),
+//          reads_i = q_i.(scale exp(G_i) S0^T dO_i) - k_i.(exp(G_i) S0^T dV_i),
+//          writes_j = beta_j k_j.(exp(G_C - G_j) dS^T E_j).
+// beta and k scale a write alike, hence dbeta: no quotient of a gradient by
+// beta or by a decay appears, so zeros of both are harmless.  dlog_decay_t has
+// what crosses t and nothing else, and every term carries its own decay: what a
+// strong decay or a reset leaves of it is as accurate as any other.  (The sums
+// over i >= t of q_i.dQ_i + k_i.R_i - beta_i dbeta_i, plus <S_C, dS>, are the
+// same number, but there everything behind t appears twice with opposite
+// signs, rounded twice, and drowns it: half of it was noise at a log_decay of
+// -10.)
 //
 //   delta_rev_kernel    from the last chunk to the first, as
 //                       delta_scan_kernel; writes dV, and dV, dO, dS as parts.
@@ -353,7 +362,8 @@ constexpr int kGradThreads = 512;
 // at a time.  One CTA per SM takes chunk after chunk, and the ring runs on
 // into the next chunk during the second phase.  Bound by mma.sync and its
 // loads from shared memory (4 x 4096 tokens of 16 heads took its form for 16
-// bits 542 us); 2 x 200 tokens of 4 heads, dk = dv = 64, fp32: 26 us.
+// bits 542 us); 2 x 200 tokens of 4 heads, dk = dv = 64, fp32: 34 us (30 us
+// with the sums that cancel in dlog_decay).
 template <int NP>
 struct GradCfg {
   static constexpr int LV = 2, NS = LV + 1;
@@ -375,6 +385,28 @@ struct GradCfg {
   static_assert(kStages >= 1 && kSmem + 8192 <= 227 * 1024);
 };
 
+// sum_{i >= t} reads_i + sum_{j < t} writes_j for t = 2 lane, 2 lane + 1, of
+// which the lane holds the values.
+__device__ __forceinline__ void crossing_sums(const double (&reads)[2], const double (&writes)[2], int lane,
+                                              double (&out)[2]) {
+  double suffix = reads[0] + reads[1], prefix = writes[0] + writes[1];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const double r = __shfl_down_sync(0xffffffffu, suffix, d);
+    if (lane + d < 32) suffix += r;
+    const double w = __shfl_up_sync(0xffffffffu, prefix, d);
+    if (lane >= d) prefix += w;
+  }
+  // (lane by lane: a difference would let in what does not cross t)
+  double behind = __shfl_down_sync(0xffffffffu, suffix, 1), before = __shfl_up_sync(0xffffffffu, prefix, 1);
+  if (lane == 31) behind = 0.0;
+  if (lane == 0) before = 0.0;
+  out[0] = suffix + before;
+  out[1] = (reads[1] + behind) + (before + writes[0]);
+}
+
+constexpr int kPadA = kChunk + 4;  // fp32 rows of A in shared memory: columns of eight rows on distinct banks
+
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradParams p) {
   constexpr int NP = kParts<T>;
@@ -385,8 +417,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   unsigned char* dsm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(dsm_raw) + 127) & ~uintptr_t(127));
   const uint32_t st = smem_addr(dsm);
-  __shared__ float s_red[3][CW][kChunk];
-  __shared__ float s_dot[NTH / 32];
+  __shared__ float s_red[3][CW][kChunk];  // reads, k.W and writes / beta, by warp columns
+  __shared__ float s_dot[NTH / 32], s_cross[kChunk];
   __shared__ __align__(8) uint64_t full[ST], freed[ST], full_kq;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -395,7 +427,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
   const int hr = (warp >> 2) * 16, hc = (warp & 3) * 16;        // in H and X
   // The tiles of H and X above the diagonal are not needed: their 6 warps
   // take <S0, dS> instead, and one thread of them (kLoader) issues the copies
-  // (a whole warp with an elected lane spilled more: 29 us against 26).
+  // (a whole warp with an elected lane spilled more: 29 us against 26 at 2 x 200 tokens).
   const bool lower = hc <= hr;
   constexpr int kLoader = 3 * 32;
   const int above = warp < 4 ? warp - 1 : warp < 8 ? warp - 3 : 5;  // 0..5 among those
@@ -635,7 +667,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
         stsm4(at_a<MROW>(base + (NS + q) * Cfg::kMat, lane, hr, hc / 16), x);
       }
     };
-    put_mats(0);
     // an element pair of K or Q as fp32 (the sum of its parts)
     auto kq_pair = [&](int row, int col) {  // Q: rows 64..
       float2 v = make_float2(0.f, 0.f);
@@ -651,6 +682,81 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     };
     // this warp's columns of K (and, 64 rows on, Q) as a B operand
     const uint32_t kq_cols = st + (col0 >> 6) * kHalfTile;
+    // A, the sum of its rows up to each t, and of those over i >= t (in the
+    // room of the matrices).  The tokens' products are made here a second time:
+    // the first were for the forward pass, in another kernel.
+    float* s_a = reinterpret_cast<float*>(dsm + Cfg::oMats);
+    {
+      float2 z[4] = {};
+      if (lower) {
+        const int ksteps = (p.dk + 15) / 16;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {  // K K^T, Q K^T
+          float t[2][4] = {};
+          for (int kk = 0; kk < ksteps; ++kk) {
+            const uint32_t half = st + (kk >> 2) * kHalfTile;
+            Step<true, 2> sum;
+#pragma unroll
+            for (int j = NP - 1; j >= 0; --j) {
+              uint32_t kb[4];
+              ldsm4(kb, at_b<128>(half + j * kTileKQ, lane, hc, kk & 3));
+#pragma unroll
+              for (int i = NP - 1; i >= 0; --i) {
+                if (i + j > LV) continue;
+                uint32_t a[4];
+                ldsm4(a, at_a<128>(half + i * kTileKQ, lane, which * kChunk + hr, kk & 3));
+                sum.mma(0, t[0], a, kb[0], kb[1]);
+                sum.mma(1, t[1], a, kb[2], kb[3]);
+              }
+            }
+            sum.add(0, t[0]);
+            sum.add(1, t[1]);
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = which ? hd[q] : xd[q];
+            z[q].x = fmaf(f.x, t[q >> 1][2 * (q & 1)], z[q].x);
+            z[q].y = fmaf(f.y, t[q >> 1][2 * (q & 1) + 1], z[q].y);
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = hr + (q & 1) * 8 + g4, j0 = hc + (q >> 1) * 8 + 2 * t4;
+        const float2 w = *reinterpret_cast<const float2*>(beta + j0);
+        *reinterpret_cast<float2*>(&s_a[i * kPadA + j0]) =
+            make_float2(i > j0 ? z[q].x * w.x : 0.f, i > j0 + 1 ? z[q].y * w.y : 0.f);
+      }
+      __syncthreads();
+      const int i = tid >> 3, part = tid & 7;  // a row, eight of its columns
+      float a[8], sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float v = s_a[i * kPadA + part * 8 + c];
+        a[c] = sum;
+        sum += v;
+      }
+      float left = sum;
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) {
+        const float o = __shfl_up_sync(0xffffffffu, left, d, 8);
+        if (part >= d) left += o;
+      }
+      left = __shfl_up_sync(0xffffffffu, left, 1, 8);
+      if (part == 0) left = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        s_a[i * kPadA + part * 8 + c] = part * 8 + c <= i ? left + a[c] : 0.f;
+      __syncthreads();
+      float cross = 0.f;  // t = i: rows part, part + 8, ..
+#pragma unroll
+      for (int c = 0; c < 8; ++c) cross += s_a[(part + 8 * c) * kPadA + i];
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) cross += __shfl_xor_sync(0xffffffffu, cross, d);
+      if (part == 0) s_cross[i] = cross;
+      __syncthreads();
+    }
+    put_mats(0);
     // sums over a warp's columns of a row, one value per row and warp column
     auto put_row = [&](int which, int row, float v) {
       v += __shfl_xor_sync(0xffffffffu, v, 1);
@@ -663,19 +769,23 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       for (int r = 0; r < 2; ++r) {
         const int i = row0 + m * 16 + r * 8 + g4;
         const float ge = enter[i], gl = leave[i];
-        float sum = 0.f;
+        float reads = 0.f, writes = 0.f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const float2 kv = kq_pair(i, col0 + n * 8 + 2 * t4);
+          const float2 qv = kq_pair(kChunk + i, col0 + n * 8 + 2 * t4);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             aq[m][n][2 * r + c] *= ge * p.scale;
             ar[m][n][2 * r + c] *= -ge;
             aw[m][n][2 * r + c] *= gl;
-            sum = fmaf(aw[m][n][2 * r + c], c ? kv.y : kv.x, sum);
+            reads = fmaf(aq[m][n][2 * r + c], c ? qv.y : qv.x, reads);
+            reads = fmaf(ar[m][n][2 * r + c], c ? kv.y : kv.x, reads);
+            writes = fmaf(aw[m][n][2 * r + c], c ? kv.y : kv.x, writes);
           }
         }
-        put_row(2, i, sum);
+        put_row(0, i, reads);
+        put_row(2, i, writes);
       }
     __syncthreads();
 
@@ -755,16 +865,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
       for (int r = 0; r < 2; ++r) {
         const int i = row0 + m * 16 + r * 8 + g4;
         const float be = beta[i];
-        float reads = 0.f, writes = 0.f;
+        float kw = 0.f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int col = col0 + n * 8 + 2 * t4;
-          const float2 kv = kq_pair(i, col), qv = kq_pair(kChunk + i, col);
+          const float2 kv = kq_pair(i, col);
           const float q0 = aq[m][n][2 * r], q1 = aq[m][n][2 * r + 1];
           const float r0 = ar[m][n][2 * r], r1 = ar[m][n][2 * r + 1];
           const float w0 = aw[m][n][2 * r], w1 = aw[m][n][2 * r + 1];
-          reads = fmaf(qv.x, q0, fmaf(qv.y, q1, fmaf(kv.x, r0, fmaf(kv.y, r1, reads))));
-          writes = fmaf(kv.x, w0, fmaf(kv.y, w1, writes));
+          kw = fmaf(kv.x, w0, fmaf(kv.y, w1, kw));
           const float k0 = fmaf(be, w0, r0), k1 = fmaf(be, w1, r1);
           if (i < rows && col < p.dk) {
             if (p.dq_part != nullptr) {
@@ -785,14 +894,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
             }
           }
         }
-        put_row(0, i, reads);
-        put_row(1, i, writes);
+        put_row(1, i, kw);
       }
     __syncthreads();
 
-    // dbeta, and the suffix sums of dlog_decay: one warp, two tokens a lane, in 64 bits
+    // dbeta, and the sums of dlog_decay: one warp, two tokens a lane, in 64 bits
     if (warp == 0) {
-      double dg[2], state = 0.0;
+      double reads[2], writes[2], state = 0.0;
       float db[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -802,19 +910,17 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
         for (int w = 0; w < CW; ++w)
 #pragma unroll
           for (int q = 0; q < 3; ++q) sum[q] += s_red[q][w][i];
+        reads[c] = sum[0];
         db[c] = sum[1];
-        dg[c] = (double)sum[0] - (double)beta[i] * (double)sum[1];
-        state += (double)beta[i] * (double)sum[2];
+        writes[c] = (double)beta[i] * (double)sum[2];
       }
-      if (lane < NTH / 32) state += (double)enter[kChunk - 1] * (double)s_dot[lane];
-      double suffix = dg[0] + dg[1];
+      if (lane < NTH / 32) state = (double)enter[kChunk - 1] * (double)s_dot[lane];
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_down_sync(0xffffffffu, suffix, d);
-        if (lane + d < 32) suffix += o;
-        state += __shfl_xor_sync(0xffffffffu, state, d);
-      }
-      const double out[2] = {suffix + state, suffix - dg[0] + state};
+      for (int d = 1; d < 32; d <<= 1) state += __shfl_xor_sync(0xffffffffu, state, d);
+      double out[2];
+      crossing_sums(reads, writes, lane, out);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) out[c] += state + (double)s_cross[2 * lane + c];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int i = 2 * lane + c;
@@ -844,10 +950,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 // taken transposed, 128 rows of dk by 64 tokens, so that every product has
 // 128 rows, and the strips are operands as they lie (32-byte rows and swizzle,
 // 16 values of k each):
-//     S0 [dO; dV]^T  -> dQ | R,   dS E^T -> W,   [dO; dV] E^T -> [H; X]
+//     S0 [dV; dO]^T  -> R | dQ,   dS E^T -> W,   [dV; dO] E^T -> [X; H]
 // strip by strip as they arrive, then
-//     K^T [Hb; Xb]^T -> dQ | R,   [K; Q]^T [Xd; Hs] -> W
-// with the matrices that the warps make of H and X.  20 warps: sixteen take the
+//     K^T [Xb; Hb]^T -> R | dQ,   [K; Q]^T [Xd; Hs] -> W
+// with the matrices that the warps make of H and X, and [K; Q] K^T, which makes
+// A of them.  20 warps: sixteen take the
 // first sums into registers (the next chunk's first products may then start),
 // make the matrices, add the second sums and write the gradients from there
 // (a thread has one of dk and 16 tokens: 64 bytes a store, which costs less
@@ -858,28 +965,30 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
 // an elected lane of a converged warp: six copies took a lone thread of a
 // divergent branch 900 cycles.  What bounds it: reading operands from shared
 // memory, 640 KB a chunk at 128 bytes a cycle, and the warps' steps between
-// the two phases.  4 x 4096 tokens of 16 heads, dk = dv = 128, bf16: 292 us
-// (1.1 GB, 3.9 TB/s), 2 x 2048 with two value heads to a key head 83 us.
+// the two phases.  4 x 4096 tokens of 16 heads, dk = dv = 128, bf16: 346 us
+// (1.1 GB, 3.2 TB/s), 2 x 2048 with two value heads to a key head 91 us; A and
+// what crosses each token cost 43 and 8 us of that over sums that cancel.
 constexpr int kTcThreads = 640;  // 96 registers a thread; one warp more, and it is 80
 
 template <int NP>
 struct TcGradCfg {
   static constexpr int NS = 2;
-  // a stage: parts p of [dO; dV] (dO's second part is zeros where NP = 1), E, S0, dS
+  // a stage: parts p of [dV; dO] (dO's second part is zeros where NP = 1), E, S0, dS
   static constexpr int oE = 2 * 2 * kStrip, oS = oE + NS * kStrip, oD = oS + NS * 2 * kStrip;
   static constexpr int kStage = oD + NS * 2 * kStrip;
   static constexpr int kTx = (NP + 2 * NS) * kStrip + 2 * NS * 2 * kStrip;
   // K and Q; two matrices of two parts; the ring; decay vectors, those of the
-  // next chunk too
+  // next chunk too.  kStatic bytes besides (the kernel's __shared__ variables)
+  static constexpr int kStatic = 11 * 1024 + 512;
   static constexpr int oM = NP * kTileKQ;
-  static constexpr int kMatP = 128 * 128;  // a part of [Hb; Xb] or [Xd; Hs]
+  static constexpr int kMatP = 128 * 128;  // a part of [Xb; Hb] or [Xd; Hs]
   static constexpr int oRing = oM + 2 * NS * kMatP;
   static constexpr int kVecBytes = kVecCount * kChunk * 4;
-  static constexpr int kRoom = 227 * 1024 - 1024 - 5 * 1024 - 2 * kVecBytes;
+  static constexpr int kRoom = 227 * 1024 - 1024 - kStatic - 2 * kVecBytes;
   static constexpr int kStages = (kRoom - oRing) / kStage < 4 ? (kRoom - oRing) / kStage : 4;
   static constexpr int oVec = oRing + kStages * kStage;
   static constexpr int kSmem = oVec + 2 * kVecBytes + 1024;
-  static_assert(kStages >= 2 && kSmem + 5 * 1024 <= 227 * 1024);
+  static_assert(kStages >= 2 && kSmem + kStatic <= 227 * 1024);
 };
 
 // K-major operand of strips: 32-byte rows and swizzle, 16 values of k.
@@ -899,6 +1008,19 @@ struct Ring {
   }
 };
 
+// 16 values of every lane summed over each half of the warp: lane l keeps the
+// sum of the values l & 15 of its half, in x[0].
+__device__ __forceinline__ void over_lanes(float (&x)[16], int lane) {
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) {
+#pragma unroll
+    for (int c = 0; c < m; ++c) {
+      const float send = lane & m ? x[c] : x[c + m], keep = lane & m ? x[c + m] : x[c];
+      x[c] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+    }
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const GradParams p) {
   constexpr int NP = kParts<T>;
@@ -912,8 +1034,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
   __shared__ __align__(8) uint64_t full[ST], freed[ST], full_kq, full_vec[2], dots[2], done1, mats,
       done2, used_kq;
   __shared__ uint32_t s_tmem;
-  // q.dQ + k.R, and k.W, of every token, by quarters of dk
-  __shared__ float s_rows[2][4][2][kChunk], s_dot[2][2], s_sum[2][16];
+  // reads, writes / beta and k.W of every token, by quarters of dk; the sum of
+  // A over its 16 columns from t & ~15 up to t and 32 rows i >= t
+  __shared__ float s_rows[2][4][4][kChunk], s_dot[2][2];
+  __shared__ float s_a[2][3][128];  // A's rows (X's share, H's share), summed over 16 columns
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
@@ -936,7 +1060,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
   }
   if (NP == 1)  // dO's second part
     for (int i = tid; i < ST * kStrip / 16; i += kTcThreads)
-      sts128(st + Cfg::oRing + i / (kStrip / 16) * Cfg::kStage + 2 * kStrip + i % (kStrip / 16) * 16,
+      sts128(st + Cfg::oRing + i / (kStrip / 16) * Cfg::kStage + 3 * kStrip + i % (kStrip / 16) * 16,
              make_uint4(0, 0, 0, 0));
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
@@ -949,7 +1073,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
   __syncthreads();
   umma_fence_after();
   const uint32_t tmem = s_tmem;
-  const uint32_t t_w = tmem + 128, t_hx = tmem + 192, t_qr2 = tmem + 256, t_w2 = tmem + 384;
+  const uint32_t t_w = tmem + 128, t_xh = tmem + 192, t_rq2 = tmem + 256, t_w2 = tmem + 384;
+  const uint32_t t_kk = tmem + 448;
   pdl_wait();
   pdl_launch_dependents();
 
@@ -980,16 +1105,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
           umma(t_w, ds + ps, e, umma_idesc(false, false, 64), on);
           umma(t_w, ds, e + pe, umma_idesc(false, false, 64), true);
           umma(t_w, ds, e, umma_idesc(false, false, 64), true);
-          umma(t_hx, dv + pd, e, umma_idesc(false, false, 64), on);
-          umma(t_hx, dv, e + pe, umma_idesc(false, false, 64), true);
-          umma(t_hx, dv, e, umma_idesc(false, false, 64), true);
+          umma(t_xh, dv + pd, e, umma_idesc(false, false, 64), on);
+          umma(t_xh, dv, e + pe, umma_idesc(false, false, 64), true);
+          umma(t_xh, dv, e, umma_idesc(false, false, 64), true);
           umma_commit(&freed[s]);
           if (sl == strips - 1) umma_commit(&done1);
         }
         __syncwarp();
       }
-      wait(&mats, k);
+      // (the warps were through with the chunk before's when K and Q were loaded)
       wait(&full_kq, k);
+      umma_fence_after();
+      __syncwarp();
+      if (elect_one()) {
+        const uint64_t kq = umma_desc_a(st, 16);
+        bool on = false;
+#pragma unroll
+        for (int lv = 1; lv >= 0; --lv)
+#pragma unroll
+          for (int i = 0; i <= lv; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              if (i < NP && lv - i < NP) {
+                const uint32_t at = (ks >> 2) * kHalfTile + (ks & 3) * 32;
+                umma(t_kk, kq + ((i * kTileKQ + at) >> 4), kq + (((lv - i) * kTileKQ + at) >> 4),
+                     umma_idesc(false, false, 64), on);
+                on = true;
+              }
+      }
+      __syncwarp();
+      wait(&mats, k);
       umma_fence_after();
       __syncwarp();
       if (elect_one()) {
@@ -1001,7 +1146,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
           for (int i = 0; i <= lv && i < NP; ++i)
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-              umma(t_qr2, kt + ((i * kTileKQ + ks * 2048) >> 4),
+              umma(t_rq2, kt + ((i * kTileKQ + ks * 2048) >> 4),
                    t1 + (((lv - i) * Cfg::kMatP + ks * 32) >> 4), umma_idesc(true, false, 128), on);
               on = true;
             }
@@ -1025,7 +1170,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
   } else if (warp < 16) {
     // ---------------------------------------------------------- sums, matrices and rows
     const int quad = warp & 3, t0c = (warp >> 2) * 16;  // this thread's 16 columns
-    const int row = quad * 32 + lane;  // lane of tensor memory: H, X row; row of dk
+    const int row = quad * 32 + lane;  // lane of tensor memory: X, H row; row of dk
     const uint32_t my = ((uint32_t)(quad * 32) << 16) + t0c;
     const int64_t kstride = (int64_t)p.key_heads * p.dk, pstride = (int64_t)p.heads * p.dk;
     // this thread's row of dk of K (Q: rows from 64), as fp32 (the sum of its parts)
@@ -1062,11 +1207,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       };
       float x[16], dq[16], r[16], w[16];
       {
-        // H (rows 0..63) or X (64..127), row i, columns j: times D; with each
-        // column times beta to [Hb; Xb], without to [Xd; Hs]
-        tmem_ld(t_hx + my, x);
+        // X (rows 0..63) or H (64..127), row i, columns j: times D; with each
+        // column times beta to [Xb; Hb], without to [Xd; Hs]
+        tmem_ld(t_xh + my, x);
         const int i = row & 63;
-        const bool is_h = row < 64;
+        const bool is_h = row >= 64;
         const float hi_i = vec[kVecCumHi * kChunk + i], lo_i = vec[kVecCumLo * kChunk + i];
         const float f = is_h ? p.scale : -1.f;
         float hi[16], lo[16];
@@ -1080,7 +1225,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
           x[c] = i > j || (i == j && is_h) ? x[c] * (d * f) : 0.f;
         }
         split_row<NS>(x, [&](int q, int u, const uint4& v) {
-          sts128(tile_at<128>(s_t2 + q * Cfg::kMatP, row ^ 64, t0c / 8 + u), v);
+          sts128(tile_at<128>(s_t2 + q * Cfg::kMatP, row, t0c / 8 + u), v);
         });
         vec16(kVecBeta, hi);
 #pragma unroll
@@ -1090,8 +1235,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
         });
       }
       // the first sums: row of dk, 16 tokens
-      tmem_ld(tmem + my, dq);
-      tmem_ld(tmem + 64 + my, r);
+      tmem_ld(tmem + my, r);
+      tmem_ld(tmem + 64 + my, dq);
       tmem_ld(t_w + my, w);
       fence_async();
       umma_fence_before();
@@ -1106,26 +1251,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
 #pragma unroll
       for (int c = 0; c < 16; ++c) w[c] *= x[c];
       wait(&full_kq, k);
+      // reads and writes: sums over the 32 of dk, the 32 values over the lanes
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const float kv = kq1(t0c + c), qv = kq1(kChunk + t0c + c);
+        const float reads = fmaf(qv, dq[c], kv * r[c]), writes = kv * w[c];
+        x[c] = (lane & 16 ? writes : reads) + __shfl_xor_sync(0xffffffffu, lane & 16 ? reads : writes, 16);
+      }
+      over_lanes(x, lane);
+      s_rows[buf][quad][lane >> 4][t0c + (lane & 15)] = x[0];
       wait(&done2, k);
       umma_fence_after();
-      tmem_ld(t_qr2 + my, x);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) dq[c] += x[c];
-      tmem_ld(t_qr2 + 64 + my, x);
+      tmem_ld(t_rq2 + my, x);
 #pragma unroll
       for (int c = 0; c < 16; ++c) r[c] += x[c];
+      tmem_ld(t_rq2 + 64 + my, x);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) dq[c] += x[c];
       tmem_ld(t_w2 + my, x);
       const bool parts = p.dq_part != nullptr;
       const int n = row < p.dk ? rows - t0c : 0;  // of the 16 tokens to be written
       const int64_t at = parts ? ((b * p.L + t0 + t0c) * p.heads + h) * p.dk + row
                                : (b * p.L + t0 + t0c) * kstride + (int64_t)hk * p.dk + row;
-      float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
-        const float be = beta[t0c + c], kv = kq1(t0c + c), qv = kq1(kChunk + t0c + c);
-        sum = fmaf(be * kv, w[c], sum);  // of <S_C, dS>: what the chunk's writes add
         w[c] += x[c];
-        const float dk = fmaf(be, w[c], r[c]);
+        const float dk = fmaf(beta[t0c + c], w[c], r[c]);
         if (c < n) {
           if (parts) {
             p.dq_part[at + c * pstride] = dq[c];
@@ -1135,27 +1286,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
             static_cast<T*>(p.dk_out)[at + c * kstride] = Elem<T>::store(dk);
           }
         }
-        dq[c] = fmaf(qv, dq[c], kv * r[c]);
-        r[c] = kv * w[c];
+        x[c] = kq1(t0c + c) * w[c];
       }
-      // sums over the 32 of dk, the 32 values over the lanes
+      over_lanes(x, lane);
+      x[0] += __shfl_xor_sync(0xffffffffu, x[0], 16);
+      if (lane < 16) s_rows[buf][quad][2][t0c + lane] = x[0];
+      {
+        // A's row i (X's or H's share), 16 columns: this thread's [Xb; Hb] times
+        // [K; Q] K^T.  Summed over the columns j < t for each t, and that over
+        // the rows i >= t.
+        const int i = row & 63;
+        tmem_ld(t_kk + my, dq);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float send = lane & 16 ? dq[c] : r[c], keep = lane & 16 ? r[c] : dq[c];
-        x[c] = keep + __shfl_xor_sync(0xffffffffu, send, 16);
-      }
+        for (int u = 0; u < 2; ++u) {
+          const uint4 a = lds128(tile_at<128>(s_t1, row, t0c / 8 + u));
+          const uint4 b = lds128(tile_at<128>(s_t1 + Cfg::kMatP, row, t0c / 8 + u));
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int m = 8; m > 0; m >>= 1) {
-#pragma unroll
-        for (int c = 0; c < m; ++c) {
-          const float send = lane & m ? x[c] : x[c + m], keep = lane & m ? x[c + m] : x[c];
-          x[c] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+          for (int e = 0; e < 4; ++e) {
+            r[8 * u + 2 * e] = bf16_lo(aw[e]) + bf16_lo(bw[e]);
+            r[8 * u + 2 * e + 1] = bf16_hi(aw[e]) + bf16_hi(bw[e]);
+          }
         }
-      }
-      s_rows[buf][quad][lane >> 4][t0c + (lane & 15)] = x[0];
+        float sum = 0.f;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == 0) s_sum[buf][warp] = sum;
+        for (int c = 0; c < 16; ++c) {
+          x[c] = i >= t0c + c ? sum : 0.f;
+          sum += i > t0c + c ? r[c] * dq[c] : 0.f;
+        }
+        if (t0c < 48) s_a[buf][t0c / 16][row] = sum;
+        over_lanes(x, lane);
+        x[0] += __shfl_xor_sync(0xffffffffu, x[0], 16);
+        if (lane < 16) s_rows[buf][quad][3][t0c + lane] = x[0];
+        umma_fence_before();
+      }
       warp_arrive(&used_kq, lane);
     }
   } else if (warp < 19) {
@@ -1177,10 +1341,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
         mbar_expect_tx(bar, Cfg::kTx);
 #pragma unroll
         for (int i = 0; i < NP; ++i)
-          bulk_in(at + i * 2 * kStrip, p.do_parts + (strip * NP + i) * (kStrip / 2), kStrip, bar);
+          bulk_in(at + (2 * i + 1) * kStrip, p.do_parts + (strip * NP + i) * (kStrip / 2), kStrip, bar);
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-          bulk_in(at + (2 * i + 1) * kStrip, p.dv_parts + (strip * NS + i) * (kStrip / 2), kStrip, bar);
+          bulk_in(at + i * 2 * kStrip, p.dv_parts + (strip * NS + i) * (kStrip / 2), kStrip, bar);
         bulk_in(at + Cfg::oE, p.e_parts + strip * (NS * kStrip / 2), NS * kStrip, bar);
         bulk_in(at + Cfg::oS, p.s_parts + strip * (NS * kStrip), NS * 2 * kStrip, bar);
         bulk_in(at + Cfg::oD, p.ds_parts + strip * (NS * kStrip), NS * 2 * kStrip, bar);
@@ -1286,31 +1450,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       if (k + 1 < mine && elect_one()) load_kq(k + 1);
       __syncwarp();
       wait(&dots[buf], k >> 1);
-      // the suffix sums, two tokens a lane, in 64 bits
-      double dg[2], state = 0.0;
+      // dbeta, and the sums of dlog_decay: two tokens a lane, in 64 bits
+      double reads[2], writes[2], cross[2], state = 0.0;
       float db[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int i = 2 * lane + c;
-        float reads = 0.f;
-        db[c] = 0.f;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          reads += s_rows[buf][q][0][i];
-          db[c] += s_rows[buf][q][1][i];
-        }
-        dg[c] = (double)reads - (double)vec[kVecBeta * kChunk + i] * (double)db[c];
-      }
-      if (lane < 16) state = (double)s_sum[buf][lane];
-      if (lane < 2) state += (double)vec[kVecEnter * kChunk + kChunk - 1] * (double)s_dot[buf][lane];
-      double suffix = dg[0] + dg[1];
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_down_sync(0xffffffffu, suffix, d);
-        if (lane + d < 32) suffix += o;
-        state += __shfl_xor_sync(0xffffffffu, state, d);
+          for (int o = 0; o < 4; ++o) sum[o] += s_rows[buf][q][o][i];
+        reads[c] = sum[0];
+        writes[c] = (double)vec[kVecBeta * kChunk + i] * (double)sum[1];
+        db[c] = sum[2];
+        cross[c] = sum[3];
       }
-      const double out[2] = {suffix + state, suffix - dg[0] + state};
+      // A's columns left of those 16 that t belongs to, rows i >= t
+#pragma unroll
+      for (int g = 0; g < 3; ++g) {
+        double v[2], suffix[2];
+        const double none[2] = {0.0, 0.0};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) v[c] = (double)s_a[buf][g][2 * lane + c] + (double)s_a[buf][g][64 + 2 * lane + c];
+        crossing_sums(v, none, lane, suffix);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (g < lane >> 3) cross[c] += suffix[c];
+      }
+      if (lane < 2) state = (double)vec[kVecEnter * kChunk + kChunk - 1] * (double)s_dot[buf][lane];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) state += __shfl_xor_sync(0xffffffffu, state, d);
+      double out[2];
+      crossing_sums(reads, writes, lane, out);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) out[c] += state + cross[c];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int i = 2 * lane + c;

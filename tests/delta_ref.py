@@ -59,3 +59,38 @@ def tolerance(dtype, wide, products):
     steps, truncated to 24 bits, are off by 16 x 2^-23 at most (wide: rounded and stepwise, 8 x 2^-24)."""
     unit = 3 * 2 ** -25 + 8 * 2 ** -24 if wide or dtype == torch.float32 else 3 * 2 ** -17 + 16 * 2 ** -23
     return half_step(dtype) + products * unit
+
+
+def decay_gradient_sizes(x, state, go, gs, scale):
+    """How large the terms of dlog_decay are that cross each token t: the sum over i >= t > j of the norms that
+    meet in them, a token's own error and gradient counted with all that they are differences of.  go, gs:
+    gradients of the output and of the last state (or None).  In 64 bits, the whole sequence at once."""
+    q, k, v, g, beta = (t.detach().double() for t in x)
+    b, l, h, dv = v.shape
+    group = h // q.shape[2]
+    norm = lambda t: t.norm(dim=-1).transpose(1, 2)  # noqa: E731  (b, h, l)
+    q, k = norm(q).repeat_interleave(group, 1), norm(k).repeat_interleave(group, 1)
+    v, go, beta = norm(v), norm(go.double()), beta.transpose(1, 2)
+    cum = g.clamp(min=-10000.0).transpose(1, 2).cumsum(-1)
+    lower = torch.ones(l, l, dtype=torch.bool, device=v.device).tril()
+    d = torch.where(lower, torch.exp(torch.where(lower, cum[..., :, None] - cum[..., None, :], 0.0)), 0.0)
+    strict = d.tril(-1)
+    first = 0.0 if state is None else state.double().flatten(2).norm(dim=-1)[..., None]
+    last = 0.0 if gs is None else gs.double().flatten(2).norm(dim=-1)[..., None]
+    enter, leave = cum.exp(), (cum[..., -1:] - cum).exp()
+    # e_j = v_j - what the state says; dv_i = what e_i's write is read for
+    kk = strict * k[..., :, None] * (beta * k)[..., None, :]
+    e = v + enter * k * first
+    for _ in range(3):  # each write is read by the next ones' errors, and so on: three rounds are enough for a size
+        e = v + enter * k * first + (kk @ e[..., None])[..., 0]
+    reads = (d * (scale * q * go)[..., :, None]).sum(-2) * beta * k + leave * beta * k * last
+    dv = reads
+    for _ in range(3):
+        dv = reads + (kk.mT @ dv[..., None])[..., 0]
+    a = strict * (scale * q * go + k * dv)[..., :, None] * (beta * k * e)[..., None, :]
+    left = a.cumsum(-1) - a  # of the columns before t (sums of positive numbers)
+    t = torch.where(lower, left, 0.0).sum(-2)
+    t = t + (enter * (scale * q * go + k * dv) * first).flip(-1).cumsum(-1).flip(-1)
+    w = leave * beta * k * e * last
+    t = t + (w.cumsum(-1) - w) + enter[..., -1:] * first * last
+    return t.transpose(1, 2)
