@@ -191,6 +191,13 @@ at::Tensor delta_workspace(const at::Tensor& v, const DeltaSizes& s, bool wide, 
   return at::empty({std::max<int64_t>(n, 16)}, v.options().dtype(at::kByte));
 }
 
+// One token of `heads` values, or one sequence of a batch, starts anywhere: a
+// contiguous tensor that does not start on 16 bytes, as the sequence kernels'
+// operands must, is copied.
+at::Tensor aligned(const at::Tensor& t) {
+  return t.numel() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
+}
+
 float* state_ptr(const c10::optional<at::Tensor>& t) {
   return t && t->numel() ? t->data_ptr<float>() : nullptr;
 }
@@ -212,11 +219,12 @@ at::Tensor delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor
 }
 
 std::tuple<at::Tensor, c10::optional<at::Tensor>> delta_forward(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
-    const at::Tensor& beta, const c10::optional<at::Tensor>& initial, double scale,
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay_,
+    const at::Tensor& beta_, const c10::optional<at::Tensor>& initial, double scale,
     bool return_state, const c10::optional<at::Tensor>& out_) {
-  const DeltaSizes s = check_delta(q, k, v, log_decay, beta, initial, out_);
+  const DeltaSizes s = check_delta(q, k, v, log_decay_, beta_, initial, out_);
   const c10::cuda::CUDAGuard guard(v.device());
+  const at::Tensor log_decay = aligned(log_decay_), beta = aligned(beta_);
   const bool wide = initial || return_state;
   at::Tensor out = out_ ? *out_ : at::empty_like(v);
   c10::optional<at::Tensor> last;
@@ -232,12 +240,15 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> delta_forward(
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, c10::optional<at::Tensor>>
 delta_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-               const at::Tensor& log_decay, const at::Tensor& beta, const at::Tensor& grad_out,
+               const at::Tensor& log_decay_, const at::Tensor& beta_, const at::Tensor& grad_out_,
                const c10::optional<at::Tensor>& initial,
-               const c10::optional<at::Tensor>& grad_final, double scale, bool need_initial) {
-  const DeltaSizes s = check_delta(q, k, v, log_decay, beta, initial, grad_out);
-  if (grad_final) check_delta(q, k, v, log_decay, beta, grad_final, c10::nullopt);
+               const c10::optional<at::Tensor>& grad_final_, double scale, bool need_initial) {
+  const DeltaSizes s = check_delta(q, k, v, log_decay_, beta_, initial, grad_out_);
+  if (grad_final_) check_delta(q, k, v, log_decay_, beta_, grad_final_, c10::nullopt);
   const c10::cuda::CUDAGuard guard(v.device());
+  const at::Tensor log_decay = aligned(log_decay_), beta = aligned(beta_), grad_out = aligned(grad_out_);
+  c10::optional<at::Tensor> grad_final;
+  if (grad_final_) grad_final = aligned(*grad_final_);
   const bool wide = initial || grad_final || need_initial;
   at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v),
              dg = at::empty_like(log_decay), db = at::empty_like(beta);
@@ -434,7 +445,8 @@ struct Scan8 : public torch::autograd::Function<Scan8> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list kept = ctx->get_saved_variables();
-    const at::Tensor gates = kept[0], go = grads[0].contiguous();
+    const at::Tensor gates = kept[0];
+    const at::Tensor go = aligned(grads[0].contiguous());
     check(gates, go);
     const c10::cuda::CUDAGuard guard(go.device());
     at::Tensor dgates = at::empty_like(go), dtokens = at::empty_like(go);

@@ -132,10 +132,10 @@ int check_dtype(int dtype) {
   return FPSCAN_OK;
 }
 
-int check_ptr(const void* p, const char* name) {
+int check_ptr(const void* p, const char* name, int align = 16) {
   if (p == nullptr) return fail(FPSCAN_ERR_INVALID, "%s is NULL", name);
-  if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
-    return fail(FPSCAN_ERR_INVALID, "%s must be 16-byte aligned", name);
+  if (reinterpret_cast<uintptr_t>(p) % align != 0)
+    return fail(FPSCAN_ERR_INVALID, "%s must be %d-byte aligned", name, align);
   return FPSCAN_OK;
 }
 
@@ -783,20 +783,22 @@ int fpscan_scan_bwd_cl(const void* gates, const void* y, const void* grad_out, v
 // ------------------------------------------------------------------ gated delta rule
 namespace {
 
-// One tensor of a call: its name, address, bytes, and whether it is written.
+// One tensor of a call: its name, address, bytes, whether it is written, and
+// the alignment that the kernels' accesses to it need.
 struct Operand {
   const char* name;
   const void* ptr;
   int64_t bytes;
   bool written;
+  int align = 16;
 };
 
-// Every operand present (ptr non-null), 16-byte aligned, and none that is
-// written overlapping another.
+// Every operand present (ptr non-null), aligned, and none that is written
+// overlapping another.
 template <size_t N>
 int check_operands(const Operand (&ops)[N]) {
   for (const Operand& o : ops)
-    if (o.bytes > 0) FPSCAN_TRY(check_ptr(o.ptr, o.name));
+    if (o.bytes > 0) FPSCAN_TRY(check_ptr(o.ptr, o.name, o.align));
   for (size_t i = 0; i < N; ++i)
     for (size_t j = 0; j < i; ++j) {
       const Operand &a = ops[i], &b = ops[j];
@@ -962,13 +964,14 @@ int fpscan_delta_step(const void* q, const void* k, const void* v, const void* l
   if (batch == 0) return ok();
   const int64_t es = dtype_size(dtype), tok = batch * seqlen, st = batch * heads * dv * dk * 4;
   const bool in_place = initial != nullptr && initial == final_state;
+  const int each = (int)es;  // read or written one element at a time
   const Operand ops[] = {{"q", q, tok * key_heads * dk * es, false},
                          {"k", k, tok * key_heads * dk * es, false},
-                         {"v", v, tok * heads * dv * es, false},
-                         {"log_decay", log_decay, tok * heads * es, false},
-                         {"beta", beta, tok * heads * es, false},
+                         {"v", v, tok * heads * dv * es, false, each},
+                         {"log_decay", log_decay, tok * heads * es, false, each},
+                         {"beta", beta, tok * heads * es, false, each},
                          {"initial", initial, initial && !in_place ? st : 0, false},
-                         {"out", out, tok * heads * dv * es, true},
+                         {"out", out, tok * heads * dv * es, true, each},
                          {"final_state", final_state, final_state ? st : 0, true}};
   FPSCAN_TRY(check_operands(ops));
   DeltaArgs a{};

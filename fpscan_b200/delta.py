@@ -15,6 +15,8 @@ where the scan of ops.py has one number per channel.  The reference has no such 
 ``beta``: (batch, seqlen, heads); contiguous CUDA tensors of one dtype, float32 / float16 / bfloat16.
 ``heads`` is a multiple of ``key_heads``: value head h uses key head ``h // (heads // key_heads)``.  States
 are float32 (batch, heads, dv, dk).  dk: a multiple of 8 up to 128; dv: a multiple of 8; any seqlen >= 1.
+q, k, v, states and ``out`` start on 16 bytes (in a step only q, k and the state); ``log_decay`` and ``beta``
+may be slices that start anywhere, which a call over a sequence copies.
 
 ``log_decay`` is usually <= 0 and may be -inf: the state before that token counts no more, which is how a
 sequence packed behind another begins (the gradient with respect to that ``log_decay`` is 0).
@@ -36,7 +38,7 @@ import torch
 
 from . import _lib
 from .checkpoint8 import dequantize8, quantize8
-from .ops import _EXT, DTYPE_CODES, NVTX, _check_input, _fn, _launch, _once, nvtx_range
+from .ops import _EXT, DTYPE_CODES, NVTX, _aligned, _check_input, _fn, _launch, _once, nvtx_range
 
 __all__ = ["gated_delta", "gated_delta_forward", "gated_delta_step"]
 
@@ -127,7 +129,7 @@ def _run_forward(q, k, v, log_decay, beta, state, scale, return_state, out=None)
         return _EXT.delta_forward(q, k, v, log_decay, beta, _state_in(state), scale, return_state, out)
     _lib.load()
     validate_delta(q, k, v, log_decay, beta, state, out)
-    state = _state_in(state)
+    state, log_decay, beta = _state_in(state), _aligned(log_decay), _aligned(beta)
     wide = state is not None or return_state
     if out is None:
         out = torch.empty_like(v)
@@ -184,6 +186,8 @@ def gated_delta_backward(q, k, v, log_decay, beta, grad_out, initial_state=None,
     if grad_final is not None:
         validate_delta_layout(q, k, v, log_decay, beta, grad_final)
     state, grad_final = _state_in(initial_state), _state_in(grad_final)
+    grad_final = None if grad_final is None else _aligned(grad_final)
+    log_decay, beta, grad_out = _aligned(log_decay), _aligned(beta), _aligned(grad_out)
     b, l, hk, h, dk, dv = _sizes(q, v)
     wide = state is not None or grad_final is not None or need_initial
     grads = [torch.empty_like(t) for t in (q, k, v, log_decay, beta)]

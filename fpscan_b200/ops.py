@@ -549,6 +549,12 @@ def _cl8_workspace(t: torch.Tensor, backward: bool) -> torch.Tensor:
     return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=t.device)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    # one token of a few heads, or a part of another tensor's gradient, starts anywhere; the kernels that load
+    # 16 bytes at a time get a copy then
+    return t.clone() if t.numel() and t.data_ptr() % 16 else t
+
+
 class _Once(torch.autograd.Function):
     @staticmethod
     def forward(ctx, what, *grads):
@@ -595,7 +601,7 @@ class PScanChannelsLast8(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_output):
         gates, codes, steps = ctx.saved_tensors
-        grad_output = grad_output.contiguous()
+        grad_output = _aligned(grad_output.contiguous())
         validate_channels_last(gates, grad_output)
         dgates = torch.empty_like(grad_output)
         dtokens = torch.empty_like(grad_output)

@@ -247,7 +247,8 @@ FPSCAN_API int fpscan_delta_bwd(const void* q, const void* k, const void* v, con
 /* fpscan_delta_fwd token by token, for one or a few tokens (a serving step):
  * fp32 arithmetic, no workspace.  final_state may be `initial` itself (the
  * state is updated in place); otherwise no written operand may overlap
- * another. */
+ * another.  v, log_decay, beta and out need no more than their element's
+ * alignment. */
 FPSCAN_API int fpscan_delta_step(const void* q, const void* k, const void* v,
                                  const void* log_decay, const void* beta, const float* initial,
                                  void* out, float* final_state, int64_t batch, int64_t seqlen,

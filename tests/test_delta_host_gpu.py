@@ -1,0 +1,98 @@
+"""Gated delta rule and 8-bit checkpoints on the GPU: slices of larger tensors, and what the host keeps or refuses."""
+import pytest
+import torch
+
+import fpscan_b200 as fp
+from fpscan_b200 import _lib, checkpoint8, delta, ops
+from delta_ref import make
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(autouse=True)
+def _healthy():
+    yield
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+@pytest.fixture(params=["binding", "ctypes"])
+def path(request, monkeypatch):
+    if request.param == "ctypes":
+        for m in (ops, delta, checkpoint8):
+            monkeypatch.setattr(m, "_EXT", None)
+    return request.param
+
+
+def _shifted(t, by=1):
+    """The same values in memory that starts `by` elements behind a 16-byte boundary."""
+    s = torch.empty(t.numel() + by, dtype=t.dtype, device=t.device)[by:].view(t.shape)
+    return s.copy_(t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [1, 3, 6])
+def test_slices_along_time_and_batch(heads, dtype, path):
+    # a server steps through a packed (1, L, heads) tensor; a batch's sequences one by one
+    x, s0 = make(1, 7, heads, 1, 16, 24, dtype, seed=1, state=True)
+    whole, state = s0.clone(), s0.clone()
+    want = fp.gated_delta_step(*x, whole)
+    got = torch.cat([fp.gated_delta_step(*(t[:, i:i + 1] for t in x), state) for i in range(7)], 1)
+    assert torch.equal(got, want) and torch.equal(state, whole)
+    y, t0 = make(3, 33, heads, 1, 16, 24, dtype, seed=2, state=True)
+    o, last = fp.gated_delta_forward(*y, initial_state=t0, return_state=True)
+    for i in range(3):
+        p, one = fp.gated_delta_forward(*(t[i:i + 1] for t in y), initial_state=t0[i:i + 1], return_state=True)
+        assert torch.equal(p, o[i:i + 1]) and torch.equal(one, last[i:i + 1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_step_takes_values_from_anywhere(dtype, path):
+    x, s0 = make(2, 2, 1, 3, 16, 24, dtype, seed=3, state=True)
+    want = fp.gated_delta_step(*x, s0.clone())
+    out = _shifted(torch.zeros_like(x[2]), 3)
+    got = fp.gated_delta_step(*x[:2], *(_shifted(t) for t in x[2:]), s0.clone(), out=out)
+    assert got is out and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_that_are_slices(dtype, path):
+    # the outputs are part of a flat vector whose gradient is cut up again
+    x, s0 = make(2, 70, 1, 2, 16, 24, dtype, seed=4, state=True)
+    go, gs = torch.randn_like(x[2]), torch.randn_like(s0)
+    decays = [_shifted(t) for t in x[3:]]
+    want = delta.gated_delta_backward(*x, go, s0, gs, need_initial=True)
+    for a, b in zip(delta.gated_delta_backward(*x[:3], *decays, _shifted(go), s0, _shifted(gs), need_initial=True), want):
+        assert torch.equal(a, b)
+    for eight in (False, True):
+        leaves = [t.clone().requires_grad_() for t in x]
+        o = fp.gated_delta(*leaves, checkpoint8=eight)
+        want = torch.autograd.grad(o, leaves, go, retain_graph=True)
+        flat = torch.cat([torch.zeros(1, dtype=dtype, device="cuda"), o.flatten()])
+        got = torch.autograd.grad(flat[1:], leaves, go.flatten(), retain_graph=True)
+        some = torch.autograd.grad(flat, leaves, torch.cat([go.new_zeros(1), go.flatten()]))
+        for a, b, c in zip(got, some, want):
+            assert torch.equal(a, c) and torch.equal(b, c)
+    g, t = (torch.rand(2, 50, 24, device="cuda").to(dtype).requires_grad_() for _ in range(2))
+    y = fp.pscan_channels_last(g, t, checkpoint8=True)
+    go = torch.randn_like(y)
+    want = torch.autograd.grad(y, (g, t), go, retain_graph=True)
+    flat = torch.cat([go.new_zeros(1), y.flatten()])
+    for a, b in zip(torch.autograd.grad(flat, (g, t), torch.cat([go.new_zeros(1), go.flatten()])), want):
+        assert torch.equal(a, b)
+
+
+def test_operands_that_stay_refused(path):
+    x, s0 = make(1, 4, 2, 1, 16, 16, torch.float32, seed=5, state=True)
+    for i in (0, 1, 2):
+        y = list(x)
+        y[i] = _shifted(x[i])
+        with pytest.raises(RuntimeError, match="aligned"):
+            fp.gated_delta_forward(*y)
+        if i < 2:
+            with pytest.raises(RuntimeError, match="aligned"):
+                fp.gated_delta_step(*y, s0.clone())
+    with pytest.raises(RuntimeError, match="aligned"):
+        fp.gated_delta_step(*x, _shifted(s0))
