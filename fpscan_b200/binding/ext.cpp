@@ -354,10 +354,20 @@ struct GatedDelta : public torch::autograd::Function<GatedDelta> {
   }
 };
 
+// Whether a backward pass can follow: without one no checkpoint is made.
+bool wanted(std::initializer_list<const at::Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : inputs)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
 std::tuple<at::Tensor, c10::optional<at::Tensor>> gated_delta(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
     const at::Tensor& beta, const c10::optional<at::Tensor>& state, double scale,
     bool return_state, bool checkpoint8) {
+  const at::Tensor none;
+  checkpoint8 = checkpoint8 && wanted({&q, &k, &v, &log_decay, &beta, state ? &*state : &none});
   const variable_list r =
       GatedDelta::apply(q, k, v, log_decay, beta, state, scale, return_state, checkpoint8);
   if (return_state) return {r[0], r[1]};
@@ -422,12 +432,23 @@ struct Scan8 : public torch::autograd::Function<Scan8> {
     return at::empty({std::max<int64_t>(n, 256)}, t.options().dtype(at::kByte).requires_grad(false));
   }
 
-  static Variable forward(AutogradContext* ctx, const Variable& gates, const Variable& tokens) {
+  // keep: a backward pass can follow
+  static Variable forward(AutogradContext* ctx, const Variable& gates, const Variable& tokens, bool keep) {
     check(gates, tokens);
     const c10::cuda::CUDAGuard guard(tokens.device());
     const int64_t b = tokens.size(0), l = tokens.size(1), d = tokens.size(2);
     const auto opts = tokens.options().requires_grad(false);
     at::Tensor out = at::empty_like(tokens);
+    if (!keep) {
+      if (b && d) {
+        const at::Tensor ws = workspace_of(tokens, false);
+        raise_on(fpscan_scan_fwd_cl(gates.data_ptr(), tokens.data_ptr(), out.data_ptr(), b, l, d,
+                                    dtype_code(tokens), 0, ws.data_ptr(), ws.numel(),
+                                    at::cuda::getCurrentCUDAStream().stream()),
+                 "fpscan_scan_fwd_cl");
+      }
+      return out;
+    }
     // rows of codes start on 16-byte boundaries, as the kernels' tile copies need
     at::Tensor codes = at::empty({b, l, (d + 15) / 16 * 16}, opts.dtype(at::kChar));
     at::Tensor steps = at::empty({b, (l + 7) / 8, d * tokens.element_size() / 16}, opts.dtype(at::kFloat));
@@ -458,7 +479,7 @@ struct Scan8 : public torch::autograd::Function<Scan8> {
                                    at::cuda::getCurrentCUDAStream().stream()),
                "fpscan_scan_bwd_cl8");
     }
-    return once({dgates, dtokens}, "pscan_channels_last with checkpoint8");
+    return once({dgates, dtokens, at::Tensor()}, "pscan_channels_last with checkpoint8");
   }
 };
 
@@ -480,7 +501,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "gated_delta(q, k, v, log_decay, beta, state, scale, return_state, checkpoint8) -> (out, final),"
         " differentiable");
   m.def("pscan_channels_last8",
-        [](const at::Tensor& gates, const at::Tensor& tokens) { return Scan8::apply(gates, tokens); },
+        [](const at::Tensor& gates, const at::Tensor& tokens) {
+          return Scan8::apply(gates, tokens, wanted({&gates, &tokens}));
+        },
         "pscan_channels_last8(gates, tokens) -> out, differentiable, the output kept in 8 bits");
   m.def("quantize8", &quantize8, "quantize8(x) -> (codes, steps)");
   m.def("dequantize8", [](const at::Tensor& codes, const at::Tensor& steps, py::object dtype) {

@@ -38,7 +38,8 @@ import torch
 
 from . import _lib
 from .checkpoint8 import dequantize8, quantize8
-from .ops import _EXT, DTYPE_CODES, NVTX, _aligned, _check_input, _fn, _launch, _once, nvtx_range
+from .ops import (_EXT, DTYPE_CODES, NVTX, _aligned, _check_input, _fn, _launch, _once, _wanted,
+                  nvtx_range)
 
 __all__ = ["gated_delta", "gated_delta_forward", "gated_delta_step"]
 
@@ -238,10 +239,11 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: to
                 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Differentiable gated delta rule over a sequence: ``out``, or ``(out, final_state)`` with
     ``return_state``; differentiable in all five inputs, the initial and the final state.
-    ``checkpoint8=True`` keeps q, k and v for the backward pass in 8 bits (``quantize8``): gradients are
-    those of the rule at the values that these stand for."""
+    ``checkpoint8=True`` keeps q, k and v for the backward pass, where one can follow, in 8 bits
+    (``quantize8``): gradients are those of the rule at the values that these stand for."""
     scale, return_state, checkpoint8 = _scale(scale, q), bool(return_state), bool(checkpoint8)
     if not NVTX and _tensors(q, k, v, log_decay, beta, initial_state):
         out, final = _EXT.gated_delta(q, k, v, log_decay, beta, initial_state, scale, return_state, checkpoint8)
         return (out, final) if return_state else out
+    checkpoint8 = checkpoint8 and _wanted(q, k, v, log_decay, beta, initial_state)
     return GatedDelta.apply(q, k, v, log_decay, beta, initial_state, scale, return_state, checkpoint8)

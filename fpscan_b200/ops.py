@@ -555,6 +555,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.numel() and t.data_ptr() % 16 else t
 
 
+def _wanted(*tensors) -> bool:
+    # whether a backward pass can follow: without one no checkpoint is made
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
 class _Once(torch.autograd.Function):
     @staticmethod
     def forward(ctx, what, *grads):
@@ -581,11 +586,17 @@ class PScanChannelsLast8(torch.autograd.Function):
     has the same one.)"""
 
     @staticmethod
-    def forward(ctx, gates, tokens):
+    def forward(ctx, gates, tokens, keep):  # keep: a backward pass can follow
         _lib.load()
         validate_channels_last(gates, tokens)
         out = torch.empty_like(tokens)
         b, l, d = tokens.shape
+        if not keep:
+            if b and d:
+                ws = _cl8_workspace(tokens, False)
+                _launch(tokens.get_device(), "fpscan_scan_fwd_cl", gates.data_ptr(), tokens.data_ptr(),
+                        out.data_ptr(), b, l, d, DTYPE_CODES[tokens.dtype], 0, ws.data_ptr(), ws.numel())
+            return out
         # rows of codes start on 16-byte boundaries, as the kernels' tile copies need
         codes = torch.empty(b, l, (d + 15) // 16 * 16, dtype=torch.int8, device=tokens.device)
         steps = torch.empty(b, (l + 7) // 8, d * tokens.element_size() // 16, dtype=torch.float32,
@@ -612,15 +623,16 @@ class PScanChannelsLast8(torch.autograd.Function):
                     codes.data_ptr(), steps.data_ptr(), grad_output.data_ptr(), dgates.data_ptr(),
                     dtokens.data_ptr(), b, l, d, DTYPE_CODES[grad_output.dtype], ws.data_ptr(),
                     ws.numel())
-        return _once((dgates, dtokens), "pscan_channels_last with checkpoint8")
+        return (*_once((dgates, dtokens), "pscan_channels_last with checkpoint8"), None)
 
 
 def pscan_channels_last(gates: torch.Tensor, tokens: torch.Tensor,
                         checkpoint8: bool = False) -> torch.Tensor:
     """Differentiable scan along dim 1 of (batch, seqlen, dim) tensors.  ``checkpoint8=True`` keeps the
-    output for the backward pass in 8 bits: grad_gates is then that of the values these stand for."""
+    output for the backward pass in 8 bits, where one can follow: grad_gates is then that of the values these
+    stand for."""
     if checkpoint8:
         if _EXT is not None and not NVTX and isinstance(gates, torch.Tensor) and isinstance(tokens, torch.Tensor):
             return _EXT.pscan_channels_last8(gates, tokens)
-        return PScanChannelsLast8.apply(gates, tokens)
+        return PScanChannelsLast8.apply(gates, tokens, _wanted(gates, tokens))
     return PScanChannelsLast.apply(gates, tokens)

@@ -96,3 +96,53 @@ def test_operands_that_stay_refused(path):
                 fp.gated_delta_step(*y, s0.clone())
     with pytest.raises(RuntimeError, match="aligned"):
         fp.gated_delta_step(*x, _shifted(s0))
+
+
+@pytest.mark.parametrize("mode", ["no_grad", "inference", "no leaf"])
+def test_no_checkpoint_without_a_backward_pass(mode, path):
+    # what the call leaves allocated besides its results, at most and in the end, is what it needs without one
+    x, s0 = make(2, 200, 2, 1, 64, 64, torch.bfloat16, seed=6, state=True)
+    g, t = (torch.rand(2, 600, 2048, device="cuda").to(torch.bfloat16) for _ in range(2))
+    want = fp.gated_delta_forward(*x, initial_state=s0, return_state=True), fp.scan_forward_channels_last(g, t)
+    if mode != "no leaf":
+        for y in (*x, s0, g, t):
+            y.requires_grad_()
+    guard = {"no_grad": torch.no_grad, "inference": torch.inference_mode, "no leaf": torch.enable_grad}[mode]
+
+    def peak(call):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        res = call()
+        return res, torch.cuda.max_memory_allocated() - before
+
+    with guard():
+        for eight in (False, True):
+            fp.gated_delta(*x, initial_state=s0, return_state=True, checkpoint8=eight)
+            fp.pscan_channels_last(g, t, checkpoint8=eight)
+        (o, s1), most = peak(lambda: fp.gated_delta(*x, initial_state=s0, return_state=True, checkpoint8=True))
+        _, plain = peak(lambda: fp.gated_delta(*x, initial_state=s0, return_state=True))
+        assert most == plain
+        y, most = peak(lambda: fp.pscan_channels_last(g, t, checkpoint8=True))
+        _, plain = peak(lambda: fp.pscan_channels_last(g, t))
+        # a workspace of its own, as every call with checkpoint8 has; the codes would be half of the output
+        assert most <= plain + _lib.load().fpscan_cl_workspace_bytes(2, 600, 2048, 2, 0) + 1024 < plain + y.numel()
+    assert not o.requires_grad and not y.requires_grad
+    assert torch.equal(o, want[0][0]) and torch.equal(s1, want[0][1]) and torch.equal(y, want[1])
+
+
+def test_a_checkpoint_where_one_input_asks_for_it(path):
+    x, s0 = make(1, 70, 1, 1, 16, 16, torch.bfloat16, seed=7, state=True)
+    go = torch.randn_like(x[2])
+    kept = [fp.dequantize8(*fp.quantize8(t), torch.bfloat16) for t in x[:3]]
+    want = delta.gated_delta_backward(*kept, *x[3:], go, s0, need_initial=True)
+    for i, t in enumerate((*x, s0)):
+        leaves = [y.clone() for y in (*x, s0)]
+        leaves[i].requires_grad_()
+        o = fp.gated_delta(*leaves[:5], initial_state=leaves[5], checkpoint8=True)
+        assert torch.equal(torch.autograd.grad(o, leaves[i], go)[0], want[i])
+    g, t = (torch.rand(1, 40, 8, device="cuda") for _ in range(2))
+    for a, b in ((g.clone().requires_grad_(), t), (g, t.clone().requires_grad_())):
+        y = fp.pscan_channels_last(a, b, checkpoint8=True)
+        leaf = a if a.requires_grad else b
+        assert torch.isfinite(torch.autograd.grad(y.sum(), leaf)[0]).all()
