@@ -158,10 +158,13 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
                      beta: torch.Tensor, state: torch.Tensor, scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gated delta rule for the next token, or the next few (seqlen of the inputs), of each sequence:
-    returns the outputs and updates ``state`` in place (float32, contiguous).  No autograd."""
+    returns the outputs and updates ``state`` in place (float32, contiguous).  No autograd: in grad mode a state
+    that requires a gradient, as the last one of ``gated_delta`` does, is refused (detach it)."""
     if not (isinstance(state, torch.Tensor) and state.is_cuda and state.dtype == torch.float32
             and state.is_contiguous()):
         raise RuntimeError("state must be a contiguous float32 CUDA tensor")
+    if state.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("state requires a gradient, which an update in place would lose: detach it")
     if _tensors(q, k, v, log_decay, beta, out):
         return _EXT.delta_step(q, k, v, log_decay, beta, state, _scale(scale, q), out)
     validate_delta(q, k, v, log_decay, beta, state, out)

@@ -146,3 +146,20 @@ def test_a_checkpoint_where_one_input_asks_for_it(path):
         y = fp.pscan_channels_last(a, b, checkpoint8=True)
         leaf = a if a.requires_grad else b
         assert torch.isfinite(torch.autograd.grad(y.sum(), leaf)[0]).all()
+
+
+def test_a_step_does_not_overwrite_a_state_that_has_a_gradient(path):
+    x, s0 = make(1, 66, 1, 1, 16, 16, torch.float32, seed=8, state=True)
+    one = [t[:, :1].contiguous() for t in x]
+    leaf = s0.clone().requires_grad_()
+    _, last = fp.gated_delta(*x, initial_state=leaf, return_state=True)
+    for state in (leaf, last):
+        held = state.detach().clone()
+        with pytest.raises(RuntimeError, match="gradient"):
+            fp.gated_delta_step(*one, state)
+        assert torch.equal(state, held)
+    state = last.detach().clone()
+    want = fp.gated_delta_step(*one, state)
+    with torch.no_grad():  # as torch's own operations in place
+        assert torch.equal(fp.gated_delta_step(*one, last), want)
+    assert torch.equal(fp.gated_delta_step(*one, last.detach()), fp.gated_delta_step(*one, state))
