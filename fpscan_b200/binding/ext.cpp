@@ -198,6 +198,11 @@ at::Tensor aligned(const at::Tensor& t) {
   return t.numel() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
 }
 
+// A backward pass that has saved a tensor must notice that it is overwritten.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 float* state_ptr(const c10::optional<at::Tensor>& t) {
   return t && t->numel() ? t->data_ptr<float>() : nullptr;
 }
@@ -213,8 +218,8 @@ at::Tensor delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor
                              s.b, s.l, s.hk, s.h, s.dk, s.dv, (float)scale, s.code,
                              at::cuda::getCurrentCUDAStream().stream()),
            "fpscan_delta_step");
-  // a backward pass that has saved this state must notice
-  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  written(state);
+  if (out_) written(out);
   return out;
 }
 
@@ -235,6 +240,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> delta_forward(
                             s.b, s.l, s.hk, s.h, s.dk, s.dv, (float)scale, s.code, wide,
                             ws.data_ptr(), ws.numel(), at::cuda::getCurrentCUDAStream().stream()),
            "fpscan_delta_fwd");
+  if (out_) written(out);
   return {out, last};
 }
 

@@ -93,6 +93,18 @@ def validate_delta_layout(q, k, v, log_decay, beta, state=None, out=None) -> Non
             raise RuntimeError("out must be contiguous")
 
 
+def _check_out(out) -> None:
+    if isinstance(out, torch.Tensor) and out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("out requires a gradient, which writing it here would lose: detach it")
+
+
+def _written(*tensors) -> None:
+    # a backward pass that has saved one of these must notice
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _sizes(q, v):
     b, l, h, dv = v.shape
     return b, l, q.shape[2], h, q.shape[3], dv
@@ -132,6 +144,7 @@ def _run_forward(q, k, v, log_decay, beta, state, scale, return_state, out=None)
     validate_delta(q, k, v, log_decay, beta, state, out)
     state, log_decay, beta = _state_in(state), _aligned(log_decay), _aligned(beta)
     wide = state is not None or return_state
+    given = out
     if out is None:
         out = torch.empty_like(v)
     b, l, hk, h, dk, dv = _sizes(q, v)
@@ -140,6 +153,7 @@ def _run_forward(q, k, v, log_decay, beta, state, scale, return_state, out=None)
     _launch(v.get_device(), "fpscan_delta_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
             log_decay.data_ptr(), beta.data_ptr(), _ptr(state), out.data_ptr(), _ptr(final),
             b, l, hk, h, dk, dv, scale, DTYPE_CODES[v.dtype], 1 if wide else 0, ws.data_ptr(), ws.numel())
+    _written(given)
     return out, final
 
 
@@ -150,6 +164,7 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
                         ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """The gated delta rule over a sequence (no autograd): ``out``, or ``(out, final_state)`` with
     ``return_state``.  ``scale`` defaults to ``dk ** -0.5``; ``initial_state`` to zero."""
+    _check_out(out)
     out, final = _run_forward(q, k, v, log_decay, beta, initial_state, _scale(scale, q), bool(return_state), out)
     return (out, final) if return_state else out
 
@@ -165,16 +180,17 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         raise RuntimeError("state must be a contiguous float32 CUDA tensor")
     if state.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("state requires a gradient, which an update in place would lose: detach it")
+    _check_out(out)
     if _tensors(q, k, v, log_decay, beta, out):
         return _EXT.delta_step(q, k, v, log_decay, beta, state, _scale(scale, q), out)
     validate_delta(q, k, v, log_decay, beta, state, out)
+    given = out
     if out is None:
         out = torch.empty_like(v)
     _launch(v.get_device(), "fpscan_delta_step", q.data_ptr(), k.data_ptr(), v.data_ptr(),
             log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), out.data_ptr(), state.data_ptr(),
             *_sizes(q, v), _scale(scale, q), DTYPE_CODES[v.dtype])
-    if not state.is_inference():  # a backward pass that has saved this state must notice
-        torch.autograd.graph.increment_version(state)
+    _written(state, given)
     return out
 
 

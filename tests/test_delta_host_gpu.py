@@ -163,3 +163,24 @@ def test_a_step_does_not_overwrite_a_state_that_has_a_gradient(path):
     with torch.no_grad():  # as torch's own operations in place
         assert torch.equal(fp.gated_delta_step(*one, last), want)
     assert torch.equal(fp.gated_delta_step(*one, last.detach()), fp.gated_delta_step(*one, state))
+
+
+def test_an_output_written_over_a_saved_tensor_is_noticed(path):
+    x, s0 = make(1, 66, 1, 1, 16, 16, torch.float32, seed=9, state=True)
+    one = [t[:, :1].contiguous() for t in x]
+    for y, call in ((x, lambda out: fp.gated_delta_forward(*x, out=out)),
+                    (one, lambda out: fp.gated_delta_step(*one, s0.clone(), out=out))):
+        leaf = torch.ones_like(y[2]).requires_grad_()
+        held = torch.zeros_like(y[2])
+        product = (leaf * held).sum()
+        assert call(held) is held
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+        with pytest.raises(RuntimeError, match="gradient"):
+            call(leaf)
+        with torch.no_grad():
+            assert torch.equal(call(leaf), held)
+        with torch.inference_mode():
+            made = torch.zeros_like(y[2])
+            call(made)
+        assert torch.equal(call(made), held)
