@@ -8,8 +8,9 @@ What a recurrence keeps for its backward pass can be kept in 8 bits:
 * ``gated_delta(..., checkpoint8=True)`` (delta.py) keeps q, k and v so.
 
 A block's step is its largest magnitude over 127 and a value becomes the nearest multiple of it (ties to
-even), so it is off by at most half a step: 2^-8 of the block's largest magnitude.  A block that holds an
-infinity or a NaN reads back as NaN.  The reference saves its tensors as they are (fpscan/ops.py:64-67).
+even), so it is off by at most half a step, 1/254 of the block's largest magnitude, before it is rounded to
+the type it is read back in (steps are fp32 numbers: magnitudes below 2^-119 are off by up to 2^-143
+besides).  A block that holds an infinity or a NaN reads back as NaN.  The reference saves its tensors as they are (fpscan/ops.py:64-67).
 """
 from __future__ import annotations
 

@@ -24,7 +24,9 @@
 // instructions for it before these bound them.
 //
 // Magnitudes near the ends of fp32 are brought to its middle by a power of
-// two.  A block that holds an infinity or a NaN has a step that is not finite
+// two.  The step of the largest fp32 number is rounded towards zero: rounded
+// up, 127 times it would be infinite.  A step below 2^-126 is subnormal and off
+// by up to 2^-150, so what it stands for is off by up to 127 * 2^-150.  A block that holds an infinity or a NaN has a step that is not finite
 // and codes of 0: all of it reads back as NaN.
 #pragma once
 
@@ -73,6 +75,7 @@ __device__ __forceinline__ Quant8 quant8_block(uint32_t bits) {
   Quant8 q;
   const float most = __uint_as_float(bits);
   q.step = most / 127.f;
+  if (sizeof(T) == 4 && bits == 0x7f7fffffu) q.step = __fdiv_rz(most, 127.f);
   q.keep = bits != 0 && bits < 0x7f800000u ? ~0u : 0u;
   const float up = most > 0x1p100f ? 0x1p-60f : most < 0x1p-80f ? 0x1p80f : 1.f;
   q.mul = kBf16 ? up : 127.f * up;
