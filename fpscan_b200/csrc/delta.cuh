@@ -25,6 +25,13 @@
 
 namespace fpscan {
 
+// Debug builds: n elements of type T at p, aligned to ALIGN bytes, inside a
+// tensor of `total` elements from `base`.
+template <typename T, int ALIGN = 16>
+__device__ __forceinline__ bool within(const void* p, int64_t n, const void* base, int64_t total) {
+  return in_bounds<ALIGN>(p, n * sizeof(T), base, static_cast<const T*>(base) + total);
+}
+
 constexpr int kChunk = 64;
 constexpr int kHalfTile = 2 * kChunk * 128;     // bytes: 64 columns of K's, then Q's rows
 constexpr int kTileKQ = 2 * kHalfTile;          // one part of K and Q
@@ -367,10 +374,11 @@ __device__ __forceinline__ void split_row(const float (&x)[C], F put) {
 }
 
 template <typename T, int C>
-__device__ __forceinline__ void store_row(T* p, int n, const float (&x)[C]) {
+__device__ __forceinline__ void store_row(T* p, int n, const float (&x)[C]
+                                          FPSCAN_DEBUG_ONLY(, const void* base, int64_t total)) {
 #pragma unroll
   for (int i = 0; i < C / Elem<T>::kVec; ++i)
-    if (i * Elem<T>::kVec < n)
+    if (i * Elem<T>::kVec < n FPSCAN_DEBUG_ONLY(&& within<T>(p + i * Elem<T>::kVec, Elem<T>::kVec, base, total)))
       *reinterpret_cast<uint4*>(p + i * Elem<T>::kVec) = pack_vec<T>(x + i * Elem<T>::kVec);
 }
 
@@ -400,10 +408,10 @@ struct NextRow {
   uint32_t at;
   __device__ __forceinline__ NextRow(uint32_t room, int thread) : at(room + thread * 16) {}
   // the first `n` values (a multiple of 8, may be <= 0) from p, zeros behind them
-  __device__ __forceinline__ void fetch(const T* p, int n, const T* valid) {
+  __device__ __forceinline__ void fetch(const T* p, int n, const T* valid FPSCAN_DEBUG_ONLY(, int64_t total)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const bool in = i * V < n;
+      const bool in = i * V < n FPSCAN_DEBUG_ONLY(&& within<T>(p + i * V, V, valid, total));
       if constexpr (sizeof(T) == 2)
         cp16(at + i * 128 * 16, in ? p + i * V : valid, in);
       else

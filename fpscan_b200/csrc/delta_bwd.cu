@@ -58,6 +58,7 @@ struct RevParams {
   int64_t L, chunks;
   int key_heads, heads, dk, dv, slices;
   float scale;
+  int64_t nb;  // sequences (bounds checks of debug builds)
 };
 
 constexpr int kRevThreads = 256;
@@ -123,6 +124,8 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
   const int strips = (p.dv + 15) / 16;
   const int64_t vstride = (int64_t)p.heads * p.dv;
   const int64_t tile = (b * p.key_heads + hk) * p.chunks, unit0 = bh * p.chunks;
+  FPSCAN_DEBUG_ONLY(const int64_t n_units = p.nb * p.heads * p.chunks, n_tiles = p.nb * p.key_heads * p.chunks,
+                    n_v = p.nb * p.L * vstride, n_state = p.nb * p.heads * p.dv * p.dk;)
 
   if (tid == 0) {
     mbar_init(&full_kq[0], 1);
@@ -155,9 +158,14 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     const int s = (int)(d % Cfg::kSt);
     if (elect_one()) {
       mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
+      // (a copy left out: the wait for it gives up and is recorded too)
+      FPSCAN_DEBUG_ONLY(if (within<char>(p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, p.kq_tiles, n_tiles * Cfg::kKQ) &&
+                            within<float>(p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec / 4, p.vecs,
+                                          n_units * (kVecCount * kChunk))) {)
       bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
       bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
               &full_kq[s]);
+      FPSCAN_DEBUG_ONLY(})
     }
     __syncwarp();
   };
@@ -165,6 +173,8 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     __syncwarp();
     if (elect_one()) {
       mbar_expect_tx(&full_n, Cfg::kNPN);
+      FPSCAN_DEBUG_ONLY(if (within<char>(p.npn + (unit0 + p.chunks - 1 - d) * (Cfg::kNPN / 2), Cfg::kNPN, p.npn,
+                                         n_units * Cfg::kNPN)))
       bulk_in(s_npn, p.npn + (unit0 + p.chunks - 1 - d) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
     }
     __syncwarp();
@@ -178,14 +188,15 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
   NextRow<T, C> next_do(sm0 + Cfg::oRow, (warp >> 2) * 64 + tok);
   auto load_do = [&](int64_t c) {
     next_do.fetch(static_cast<const T*>(p.grad) + row0 + c * kChunk * vstride,
-                  c * kChunk + tok < p.L ? nval : 0, static_cast<const T*>(p.grad));
+                  c * kChunk + tok < p.L ? nval : 0, static_cast<const T*>(p.grad) FPSCAN_DEBUG_ONLY(, n_v));
   };
   if (!is_y) load_do(p.chunks - 1);
 
   float S[C];  // dS, one row of dk
 #pragma unroll
   for (int i = 0; i < C; ++i)
-    S[i] = p.grad_final != nullptr && dk < p.dk && i < nval
+    S[i] = p.grad_final != nullptr && dk < p.dk && i < nval FPSCAN_DEBUG_ONLY(
+               && within<float, 4>(p.grad_final + (bh * p.dv + dv0 + i) * p.dk + dk, 1, p.grad_final, n_state))
                ? p.grad_final[(bh * p.dv + dv0 + i) * p.dk + dk]
                : 0.f;
   const int ksteps = (p.dk + 15) / 16;
@@ -231,7 +242,9 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     }
     // dS's parts to their strips, from the registers, while the product runs
     split_row<NS>(S, [&](int q, int u, const uint4& w) {
-      if ((u & ~1) * 8 < nval)
+      if ((u & ~1) * 8 < nval FPSCAN_DEBUG_ONLY(
+                                  && within<char>(strip_ptr(p.ds_parts, c, u, NS, q, 2 * kStrip) + strip_at(0, dk, u & 1), 16,
+                                                  p.ds_parts, n_units * strips * NS * 2 * kStrip)))
         *reinterpret_cast<uint4*>(strip_ptr(p.ds_parts, c, u, NS, q, 2 * kStrip) + strip_at(0, dk, u & 1)) = w;
     });
     wait(&full_kq[s], d / Cfg::kSt);  // the vectors
@@ -242,7 +255,9 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     if (!is_y) {
       next_do.take(g);
       split_row<NP>(g, [&](int q, int u, const uint4& w) {
-        if ((u & ~1) * 8 < nval)
+        if ((u & ~1) * 8 < nval FPSCAN_DEBUG_ONLY(
+                                    && within<char>(strip_ptr(p.do_parts, c, u, NP, q, kStrip) + strip_at(0, tok, u & 1), 16,
+                                                    p.do_parts, n_units * strips * NP * kStrip)))
           *reinterpret_cast<uint4*>(strip_ptr(p.do_parts, c, u, NP, q, kStrip) +
                                     strip_at(0, tok, u & 1)) = w;
       });
@@ -301,12 +316,15 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
     // meanwhile: dV to the caller and as parts
     if (is_y) {
       split_row<NS>(x, [&](int q, int u, const uint4& w) {
-        if ((u & ~1) * 8 < nval)
+        if ((u & ~1) * 8 < nval FPSCAN_DEBUG_ONLY(
+                                    && within<char>(strip_ptr(p.dv_parts, c, u, NS, q, kStrip) + strip_at(0, tok, u & 1), 16,
+                                                    p.dv_parts, n_units * strips * NS * kStrip)))
           *reinterpret_cast<uint4*>(strip_ptr(p.dv_parts, c, u, NS, q, kStrip) +
                                     strip_at(0, tok, u & 1)) = w;
       });
     } else if (c * kChunk + tok < p.L) {
-      store_row<T>(static_cast<T*>(p.dv_out) + row0 + c * kChunk * vstride, nval, x);
+      store_row<T>(static_cast<T*>(p.dv_out) + row0 + c * kChunk * vstride, nval,
+                   x FPSCAN_DEBUG_ONLY(, p.dv_out, n_v));
     }
     wait(&done[2], d);
     umma_fence_after();
@@ -318,7 +336,9 @@ __global__ void __launch_bounds__(kRevThreads, 1) delta_rev_kernel(const RevPara
   if (p.dinitial != nullptr && ok && dk < p.dk)
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (i < nval) p.dinitial[(bh * p.dv + dv0 + i) * p.dk + dk] = S[i];
+      if (i < nval FPSCAN_DEBUG_ONLY(
+                       && within<float, 4>(p.dinitial + (bh * p.dv + dv0 + i) * p.dk + dk, 1, p.dinitial, n_state)))
+        p.dinitial[(bh * p.dv + dv0 + i) * p.dk + dk] = S[i];
   // No copy may land after the CTA is gone: at once, unless a wait gave up.
   if (loads) {
     for (int64_t d = max((int64_t)0, p.chunks - Cfg::kSt); d < p.chunks; ++d)
@@ -350,7 +370,47 @@ struct GradParams {
   int64_t L, chunks, units;  // units: chunks of all heads
   int key_heads, heads, dk, dv;
   float scale;
+  int64_t nb;  // sequences (bounds checks of debug builds)
 };
+
+#ifdef FPSCAN_DEBUG_BOUNDS
+// A strip of every kept tensor, K's and Q's tile and the vectors of a unit,
+// inside what the call keeps.
+template <int NP, int NS>
+__device__ __forceinline__ bool strip_within(const GradParams& p, int64_t strip, int strips) {
+  const int64_t n = p.units * strips;
+  return within<char>(p.do_parts + strip * (NP * kStrip / 2), NP * kStrip, p.do_parts, n * NP * kStrip) &&
+         within<char>(p.dv_parts + strip * (NS * kStrip / 2), NS * kStrip, p.dv_parts, n * NS * kStrip) &&
+         within<char>(p.e_parts + strip * (NS * kStrip / 2), NS * kStrip, p.e_parts, n * NS * kStrip) &&
+         within<char>(p.s_parts + strip * (NS * kStrip), NS * 2 * kStrip, p.s_parts, n * NS * 2 * kStrip) &&
+         within<char>(p.ds_parts + strip * (NS * kStrip), NS * 2 * kStrip, p.ds_parts, n * NS * 2 * kStrip);
+}
+// N elements of dq, dk (`at`) or of their parts (`part`); an element of the decays and their gradients.
+template <typename T, int N>
+__device__ __forceinline__ bool grads_within(const GradParams& p, int64_t part, int64_t at) {
+  const int64_t n = p.nb * p.L * p.dk;
+  if (p.dq_part != nullptr)
+    return within<float, 4 * N>(p.dq_part + part, N, p.dq_part, n * p.heads) &&
+           within<float, 4 * N>(p.dk_part + part, N, p.dk_part, n * p.heads);
+  return within<T, sizeof(T) * N>(static_cast<T*>(p.dq) + at, N, p.dq, n * p.key_heads) &&
+         within<T, sizeof(T) * N>(static_cast<T*>(p.dk_out) + at, N, p.dk_out, n * p.key_heads);
+}
+template <typename T>
+__device__ __forceinline__ bool decays_within(const GradParams& p, int64_t at) {
+  const int64_t n = p.nb * p.L * p.heads;
+  return within<T, sizeof(T)>(static_cast<const T*>(p.log_decay) + at, 1, p.log_decay, n) &&
+         within<T, sizeof(T)>(static_cast<T*>(p.dlog_decay) + at, 1, p.dlog_decay, n) &&
+         within<T, sizeof(T)>(static_cast<T*>(p.dbeta) + at, 1, p.dbeta, n);
+}
+template <int NP>
+__device__ __forceinline__ bool tile_within(const GradParams& p, int64_t tile) {
+  return within<char>(p.kq_tiles + tile, NP * kTileKQ, p.kq_tiles, p.nb * p.key_heads * p.chunks * NP * kTileKQ);
+}
+__device__ __forceinline__ bool vecs_within(const GradParams& p, int64_t unit) {
+  return within<float>(p.vecs + unit * (kVecCount * kChunk), kVecCount * kChunk, p.vecs,
+                       p.units * (kVecCount * kChunk));
+}
+#endif
 
 constexpr int kGradThreads = 512;
 
@@ -457,11 +517,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     const int64_t strip = next_unit * strips + next_strip;
     const uint32_t at = st + Cfg::oRing + s * Cfg::kStage;
     mbar_expect_tx(&full[s], Cfg::kStage);
+    FPSCAN_DEBUG_ONLY(if (strip_within<NP, NS>(p, strip, strips)) {)
     bulk_in(at, p.do_parts + strip * (NP * kStrip / 2), NP * kStrip, &full[s]);
     bulk_in(at + Cfg::oV, p.dv_parts + strip * (NS * kStrip / 2), NS * kStrip, &full[s]);
     bulk_in(at + Cfg::oE, p.e_parts + strip * (NS * kStrip / 2), NS * kStrip, &full[s]);
     bulk_in(at + Cfg::oS, p.s_parts + strip * (NS * Cfg::kRows / 2), NS * Cfg::kRows, &full[s]);
     bulk_in(at + Cfg::oD, p.ds_parts + strip * (NS * Cfg::kRows / 2), NS * Cfg::kRows, &full[s]);
+    FPSCAN_DEBUG_ONLY(})
     ++next;
     if (++next_strip == strips) {
       next_strip = 0;
@@ -473,6 +535,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
     const int hk = (int)(bh - b * p.heads) / (p.heads / p.key_heads);
     const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kTileKQ / 2);
     mbar_expect_tx(&full_kq, NP * kTileKQ + Cfg::kVecBytes);
+    FPSCAN_DEBUG_ONLY(if (!tile_within<NP>(p, tile) || !vecs_within(p, unit)) return;)
     bulk_in(st, p.kq_tiles + tile, NP * kTileKQ, &full_kq);
     bulk_in(st + Cfg::oVec, p.vecs + unit * (kVecCount * kChunk), Cfg::kVecBytes, &full_kq);
   };
@@ -875,7 +938,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
           const float w0 = aw[m][n][2 * r], w1 = aw[m][n][2 * r + 1];
           kw = fmaf(kv.x, w0, fmaf(kv.y, w1, kw));
           const float k0 = fmaf(be, w0, r0), k1 = fmaf(be, w1, r1);
-          if (i < rows && col < p.dk) {
+          if (i < rows && col < p.dk FPSCAN_DEBUG_ONLY(
+                              && grads_within<T, 2>(p, ((b * p.L + t0 + i) * p.heads + h) * p.dk + col,
+                                                    kf + (int64_t)i * kstride + col))) {
             if (p.dq_part != nullptr) {
               const int64_t o = ((b * p.L + t0 + i) * p.heads + h) * p.dk + col;
               *reinterpret_cast<float2*>(p.dq_part + o) = make_float2(q0, q1);
@@ -926,6 +991,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) delta_grad_kernel(const GradP
         const int i = 2 * lane + c;
         if (i < rows) {
           const int64_t o = (b * p.L + t0 + i) * p.heads + h;
+          FPSCAN_DEBUG_ONLY(if (!decays_within<T>(p, o)) continue;)
           // a decay of exactly 0 has no slope in its logarithm
           const bool reset = Elem<T>::load(static_cast<const T*>(p.log_decay)[o]) < kDecayFloor;
           static_cast<T*>(p.dlog_decay)[o] = Elem<T>::store(reset ? 0.f : (float)out[c]);
@@ -1277,7 +1343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       for (int c = 0; c < 16; ++c) {
         w[c] += x[c];
         const float dk = fmaf(beta[t0c + c], w[c], r[c]);
-        if (c < n) {
+        if (c < n FPSCAN_DEBUG_ONLY(&& grads_within<T, 1>(p, at + c * pstride, at + c * kstride))) {
           if (parts) {
             p.dq_part[at + c * pstride] = dq[c];
             p.dk_part[at + c * pstride] = dk;
@@ -1339,6 +1405,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       __syncwarp();
       if (elect_one()) {
         mbar_expect_tx(bar, Cfg::kTx);
+        FPSCAN_DEBUG_ONLY(if (strip_within<NP, NS>(p, strip, strips)) {)
 #pragma unroll
         for (int i = 0; i < NP; ++i)
           bulk_in(at + (2 * i + 1) * kStrip, p.do_parts + (strip * NP + i) * (kStrip / 2), kStrip, bar);
@@ -1348,6 +1415,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
         bulk_in(at + Cfg::oE, p.e_parts + strip * (NS * kStrip / 2), NS * kStrip, bar);
         bulk_in(at + Cfg::oS, p.s_parts + strip * (NS * kStrip), NS * 2 * kStrip, bar);
         bulk_in(at + Cfg::oD, p.ds_parts + strip * (NS * kStrip), NS * 2 * kStrip, bar);
+        FPSCAN_DEBUG_ONLY(})
       }
       __syncwarp();
       ++next;
@@ -1410,6 +1478,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
     auto load_vec = [&](int64_t k) {
       const int64_t unit = blockIdx.x + k * gridDim.x;
       mbar_expect_tx(&full_vec[k & 1], Cfg::kVecBytes);
+      FPSCAN_DEBUG_ONLY(if (vecs_within(p, unit)))
       bulk_in(st + Cfg::oVec + (int)(k & 1) * Cfg::kVecBytes, p.vecs + unit * (kVecCount * kChunk),
               Cfg::kVecBytes, &full_vec[k & 1]);
     };
@@ -1419,6 +1488,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       const int hk = (int)(bh - b * p.heads) / (p.heads / p.key_heads);
       const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kTileKQ / 2);
       mbar_expect_tx(&full_kq, NP * kTileKQ);
+      FPSCAN_DEBUG_ONLY(if (tile_within<NP>(p, tile)))
       bulk_in(st, p.kq_tiles + tile, NP * kTileKQ, &full_kq);
     };
     __syncwarp();
@@ -1441,7 +1511,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
       for (int c = 0; c < 2; ++c) {
         const int i = 2 * lane + c;
         // a decay of exactly 0 has no slope in its logarithm
-        reset[c] = i < rows &&
+        reset[c] = i < rows FPSCAN_DEBUG_ONLY(&& decays_within<T>(p, (b * p.L + t0 + i) * p.heads + h)) &&
                    Elem<T>::load(static_cast<const T*>(p.log_decay)[(b * p.L + t0 + i) * p.heads + h]) < kDecayFloor;
       }
       wait(&full_vec[buf], k >> 1);
@@ -1490,6 +1560,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_grad_tc_kernel(const Grad
         const int i = 2 * lane + c;
         if (i < rows) {
           const int64_t o = (b * p.L + t0 + i) * p.heads + h;
+          FPSCAN_DEBUG_ONLY(if (!decays_within<T>(p, o)) continue;)
           static_cast<T*>(p.dlog_decay)[o] = Elem<T>::store(reset[c] ? 0.f : (float)out[c]);
           static_cast<T*>(p.dbeta)[o] = Elem<T>::store(db[c]);
         }
@@ -1525,6 +1596,11 @@ __global__ void __launch_bounds__(256) delta_group_kernel(const GroupParams p) {
   for (int64_t i = (int64_t)(blockIdx.x / 2) * blockDim.x + threadIdx.x; i < p.n; i += step) {
     const int64_t head = i / p.dk4;
     const int c = (int)(i - head * p.dk4);
+    FPSCAN_DEBUG_ONLY(
+        if (!within<float>(p.src[which] + (head * p.group * p.dk4 + c) * 4, 4, p.src[which], p.n * p.group * 4) ||
+            !within<float>(p.src[which] + ((head + 1) * p.group - 1) * p.dk4 * 4 + c * 4, 4, p.src[which],
+                           p.n * p.group * 4) ||
+            !within<T, 4 * sizeof(T)>(static_cast<T*>(p.dst[which]) + i * 4, 4, p.dst[which], p.n * 4)) continue;)
     const float4* src = reinterpret_cast<const float4*>(p.src[which]) + head * p.group * p.dk4 + c;
     float4 s = src[0];
     for (int q = 1; q < p.group; ++q) {
@@ -1583,6 +1659,7 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   r.dk = (int)a.dk;
   r.dv = (int)a.dv;
   r.scale = a.scale;
+  r.nb = nb;
   // as launch_scan chooses
   e = bh * ((a.dv + 31) / 32) <= a.num_sms ? launch_rev_as<T, LV, 16>(a, r, bh)
                                            : launch_rev_as<T, LV, 32>(a, r, bh);
@@ -1614,6 +1691,7 @@ cudaError_t bwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, int64_
   g.dk = (int)a.dk;
   g.dv = (int)a.dv;
   g.scale = a.scale;
+  g.nb = nb;
   const unsigned grid = (unsigned)std::min<int64_t>(g.units, a.num_sms);
   if constexpr (LV == 1) {
     using GC = TcGradCfg<NP>;

@@ -43,6 +43,7 @@ struct PrepParams {
   int64_t L, chunks;
   int key_heads, heads, dk;
   float scale;
+  int64_t nb;  // sequences (bounds checks of debug builds)
 };
 
 // One chunk per CTA of four warps, four CTAs on an SM: a chunk is a chain of
@@ -76,13 +77,14 @@ __device__ __forceinline__ uint32_t kq_at(uint32_t base, int r, int u) {
 // The chunk's rows of x as parts, from row r0 of the tile on.
 template <typename T, int NP>
 __device__ __forceinline__ void split_tile(uint32_t dst, int r0, const T* x, int64_t stride,
-                                           int rows, int units, int tid) {
+                                           int rows, int units, int tid
+                                           FPSCAN_DEBUG_ONLY(, const void* base, int64_t total)) {
   constexpr int U = kDkp / 8, N = kChunk * U / kPrepThreads, V = Elem<T>::kVec;
   if constexpr (NP == 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = (tid + i * kPrepThreads) / U, u = (tid + i * kPrepThreads) % U;
-      const bool in = r < rows && u < units;
+      const bool in = r < rows && u < units FPSCAN_DEBUG_ONLY(&& within<T>(x + r * stride + u * 8, 8, base, total));
       cp16(kq_at(dst, r0 + r, u), in ? x + r * stride + u * 8 : x, in);
     }
   } else {
@@ -92,7 +94,8 @@ __device__ __forceinline__ void split_tile(uint32_t dst, int r0, const T* x, int
       const int r = (tid + i * kPrepThreads) / U, u = (tid + i * kPrepThreads) % U;
 #pragma unroll
       for (int j = 0; j < 8 / V; ++j)
-        raw[i][j] = r < rows && u < units
+        raw[i][j] = r < rows && u < units FPSCAN_DEBUG_ONLY(
+                                              && within<T>(x + r * stride + u * 8 + j * V, V, base, total))
                         ? *reinterpret_cast<const uint4*>(x + r * stride + u * 8 + j * V)
                         : make_uint4(0, 0, 0, 0);
     }
@@ -143,8 +146,10 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   pdl_launch_dependents();
   const int64_t tok_stride = (int64_t)p.key_heads * p.dk;
   const int64_t first = (b * p.L + t0) * tok_stride + (int64_t)hk * p.dk;
-  split_tile<T, NP>(s_kq, 0, static_cast<const T*>(p.k) + first, tok_stride, rows, p.dk / 8, tid);
-  split_tile<T, NP>(s_kq, kChunk, static_cast<const T*>(p.q) + first, tok_stride, rows, p.dk / 8, tid);
+  split_tile<T, NP>(s_kq, 0, static_cast<const T*>(p.k) + first, tok_stride, rows, p.dk / 8, tid
+                    FPSCAN_DEBUG_ONLY(, p.k, p.nb * p.L * tok_stride));
+  split_tile<T, NP>(s_kq, kChunk, static_cast<const T*>(p.q) + first, tok_stride, rows, p.dk / 8, tid
+                    FPSCAN_DEBUG_ONLY(, p.q, p.nb * p.L * tok_stride));
   cp_commit();
 
   // decay vectors: one warp, two tokens a lane; the running sum in 64 bits
@@ -156,6 +161,9 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int t = 2 * lane + j;
+      FPSCAN_DEBUG_ONLY(const int64_t n_dec = p.nb * p.L * p.heads;
+                        if (t < rows && (!within<T, sizeof(T)>(g + (int64_t)t * p.heads, 1, p.log_decay, n_dec) ||
+                                         !within<T, sizeof(T)>(bt + (int64_t)t * p.heads, 1, p.beta, n_dec))) continue;)
       float v = t < rows ? Elem<T>::load(g[(int64_t)t * p.heads]) : 0.f;
       if (v < kDecayFloor) v = kDecayFloor;  // NaN stays NaN
       x[j] = v;
@@ -179,6 +187,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
 #pragma unroll
       for (int q = 0; q < kVecCount; ++q) {
         s_vec[q * kChunk + t] = v[q];
+        FPSCAN_DEBUG_ONLY(if (within<float, 4>(out + q * kChunk + t, 1, p.vecs,
+                                               p.nb * p.heads * p.chunks * (kVecCount * kChunk))))
         out[q * kChunk + t] = v[q];
       }
     }
@@ -190,6 +200,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   const bool keeper = tid == 0 && h % (p.heads / p.key_heads) == 0;
   if (keeper) {
     const int64_t tile = ((b * p.key_heads + hk) * p.chunks + chunk) * NP * (kTileKQ / 2);
+    FPSCAN_DEBUG_ONLY(if (within<char>(p.kq_tiles + tile, NP * kTileKQ, p.kq_tiles,
+                                       p.nb * p.key_heads * p.chunks * NP * kTileKQ)))
     bulk_s2g(p.kq_tiles + tile, s_kq, NP * kTileKQ);
     bulk_commit();
   }
@@ -270,6 +282,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   if (s_bad < kChunk) {  // uniform
     for (int i = s_bad * kPad + tid; i < kChunk * kPad; i += kPrepThreads) s_a[i] = 0.f;
     for (int i = s_bad + tid; i < kChunk; i += kPrepThreads)
+      FPSCAN_DEBUG_ONLY(if (within<float, 4>(p.vecs + (bh * p.chunks + chunk) * (kVecCount * kChunk) + kVecEnter * kChunk + i,
+                                             1, p.vecs, p.nb * p.heads * p.chunks * (kVecCount * kChunk))))
       p.vecs[(bh * p.chunks + chunk) * (kVecCount * kChunk) + kVecEnter * kChunk + i] =
           __int_as_float(0x7fc00000);
     __syncthreads();
@@ -426,6 +440,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) delta_prep_kernel(const PrepP
   fence_async();
   __syncthreads();
   if (tid == 0) {
+    FPSCAN_DEBUG_ONLY(if (within<char>(p.npn + (bh * p.chunks + chunk) * NS * (2 * kChunk * kChunk), 2 * NS * kMatBytes,
+                                       p.npn, p.nb * p.heads * p.chunks * 2 * NS * kMatBytes)))
     bulk_s2g(p.npn + (bh * p.chunks + chunk) * NS * (2 * kChunk * kChunk), s_img, 2 * NS * kMatBytes);
     bulk_commit();
     bulk_wait_all();
@@ -446,6 +462,7 @@ struct ScanParams {
   int64_t L, chunks;
   int key_heads, heads, dk, dv, slices;
   float scale;
+  int64_t nb;  // sequences (bounds checks of debug builds)
 };
 
 constexpr int kScanThreads = 256;
@@ -498,6 +515,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
   const int strips = (p.dv + 15) / 16;
   const int64_t vstride = (int64_t)p.heads * p.dv;
   const int64_t tile = (b * p.key_heads + hk) * p.chunks, unit0 = bh * p.chunks;
+  FPSCAN_DEBUG_ONLY(const int64_t n_units = p.nb * p.heads * p.chunks, n_tiles = p.nb * p.key_heads * p.chunks,
+                    n_v = p.nb * p.L * vstride, n_state = p.nb * p.heads * p.dv * p.dk;)
 
   if (tid == 0) {
     mbar_init(&full_kq[0], 1);
@@ -529,9 +548,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
     const int s = (int)(c % Cfg::kSt);
     if (elect_one()) {
       mbar_expect_tx(&full_kq[s], Cfg::kKQ + Cfg::kVec);
+      // (a copy left out: the wait for it gives up and is recorded too)
+      FPSCAN_DEBUG_ONLY(if (within<char>(p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, p.kq_tiles, n_tiles * Cfg::kKQ) &&
+                            within<float>(p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec / 4, p.vecs,
+                                          n_units * (kVecCount * kChunk))) {)
       bulk_in(sm0 + s * Cfg::kKQ, p.kq_tiles + (tile + c) * (Cfg::kKQ / 2), Cfg::kKQ, &full_kq[s]);
       bulk_in(sm0 + Cfg::oVec + s * Cfg::kVec, p.vecs + (unit0 + c) * (kVecCount * kChunk), Cfg::kVec,
               &full_kq[s]);
+      FPSCAN_DEBUG_ONLY(})
     }
     __syncwarp();
   };
@@ -539,6 +563,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
     __syncwarp();
     if (elect_one()) {
       mbar_expect_tx(&full_n, Cfg::kNPN);
+      FPSCAN_DEBUG_ONLY(if (within<char>(p.npn + (unit0 + c) * (Cfg::kNPN / 2), Cfg::kNPN, p.npn, n_units * Cfg::kNPN)))
       bulk_in(s_npn, p.npn + (unit0 + c) * (Cfg::kNPN / 2), Cfg::kNPN, &full_n);
     }
     __syncwarp();
@@ -550,12 +575,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
 
   const T* v_row = static_cast<const T*>(p.v) + (b * p.L + tok) * vstride + (int64_t)h * p.dv + dv0;
   NextRow<T, C> v_next(sm0 + Cfg::oRow, (warp >> 2) * 64 + tok);
-  if (is_x) v_next.fetch(v_row, tok < p.L ? nval : 0, static_cast<const T*>(p.v));
+  if (is_x) v_next.fetch(v_row, tok < p.L ? nval : 0, static_cast<const T*>(p.v) FPSCAN_DEBUG_ONLY(, n_v));
 
   float S[C];
 #pragma unroll
   for (int i = 0; i < C; ++i)
-    S[i] = p.initial != nullptr && dk < p.dk && i < nval
+    S[i] = p.initial != nullptr && dk < p.dk && i < nval FPSCAN_DEBUG_ONLY(
+               && within<float, 4>(p.initial + (bh * p.dv + dv0 + i) * p.dk + dk, 1, p.initial, n_state))
                ? p.initial[(bh * p.dv + dv0 + i) * p.dk + dk]
                : 0.f;
   const int ksteps = (p.dk + 15) / 16;
@@ -595,11 +621,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
     }
     if (KEEP)  // S0's parts to their strips, from the registers, while the product runs
       split_row<NS>(S, [&](int q, int u, const uint4& w) {
-        if ((u & ~1) * 8 < nval)
-          *reinterpret_cast<uint4*>(
-              reinterpret_cast<char*>(p.s_parts) +
-              (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * NS + q) * (int64_t)(2 * kStrip) +
-              strip_at(0, dk, u & 1)) = w;
+        if ((u & ~1) * 8 < nval) {
+          char* sp = reinterpret_cast<char*>(p.s_parts) +
+                     (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * NS + q) * (int64_t)(2 * kStrip) +
+                     strip_at(0, dk, u & 1);
+          FPSCAN_DEBUG_ONLY(if (within<char>(sp, 16, p.s_parts, n_units * strips * NS * 2 * kStrip)))
+          *reinterpret_cast<uint4*>(sp) = w;
+        }
       });
     wait(&full_kq[s], c / Cfg::kSt);  // the vectors
     const float ge = vec[kVecEnter * kChunk + tok], total = vec[kVecEnter * kChunk + kChunk - 1];
@@ -630,7 +658,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
       // v of the next chunk
       if (c + 1 < p.chunks) {
         v_row += kChunk * vstride;
-        v_next.fetch(v_row, (c + 1) * kChunk + tok < p.L ? nval : 0, static_cast<const T*>(p.v));
+        v_next.fetch(v_row, (c + 1) * kChunk + tok < p.L ? nval : 0,
+                     static_cast<const T*>(p.v) FPSCAN_DEBUG_ONLY(, n_v));
       }
     } else {
 #pragma unroll
@@ -685,6 +714,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
             char* ep = reinterpret_cast<char*>(
                 p.e_parts +
                 (((unit0 + c) * strips + dv0 / 16 + (u >> 1)) * NS + q) * (kStrip / 2));
+            FPSCAN_DEBUG_ONLY(if (within<char>(ep + strip_at(0, tok, u & 1), 16, p.e_parts, n_units * strips * NS * kStrip)))
             *reinterpret_cast<uint4*>(ep + strip_at(0, tok, u & 1)) = w;
           }
         });
@@ -719,7 +749,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
       if (c * kChunk + tok < p.L)
         store_row<T>(static_cast<T*>(p.out) + (b * p.L + c * kChunk + tok) * vstride +
                          (int64_t)h * p.dv + dv0,
-                     nval, x);
+                     nval, x FPSCAN_DEBUG_ONLY(, p.out, n_v));
     }
     wait(&done[2], c);
     umma_fence_after();
@@ -737,7 +767,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) delta_scan_kernel(const ScanP
   if (!KEEP && p.final_state != nullptr && ok && dk < p.dk)
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (i < nval) p.final_state[(bh * p.dv + dv0 + i) * p.dk + dk] = S[i];
+      if (i < nval FPSCAN_DEBUG_ONLY(&& within<float, 4>(p.final_state + (bh * p.dv + dv0 + i) * p.dk + dk, 1,
+                                                         p.final_state, n_state)))
+        p.final_state[(bh * p.dv + dv0 + i) * p.dk + dk] = S[i];
   // No copy may land after the CTA is gone: at once, unless a wait gave up.
   if (loads) {
     for (int64_t c = max((int64_t)0, p.chunks - Cfg::kSt); c < p.chunks; ++c)
@@ -804,6 +836,7 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   pp.heads = (int)a.heads;
   pp.dk = (int)a.dk;
   pp.scale = a.scale;
+  pp.nb = nb;
   auto prep = delta_prep_kernel<T, NP, LV>;
   constexpr int prep_smem = PrepCfg<NP, LV + 1>::kSmem;
   cudaError_t e = configure(prep, prep_smem);
@@ -828,6 +861,7 @@ cudaError_t delta_fwd_pass(const DeltaArgs& a, const DeltaPlan& pl, int64_t b0, 
   p.dk = (int)a.dk;
   p.dv = (int)a.dv;
   p.scale = a.scale;
+  p.nb = nb;
   return keep ? launch_scan<T, LV, true>(a, p, bh) : launch_scan<T, LV, false>(a, p, bh);
 }
 

@@ -32,6 +32,7 @@ struct StepParams {
   int64_t L;
   int key_heads, heads, dk, dv, blocks;  // blocks: CTAs along dv
   float scale;
+  int64_t batch;  // bounds checks of debug builds
 };
 
 constexpr int kStepThreads = 128;
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const StepPara
   const int h = (int)(bh - b * p.heads), hk = h / (p.heads / p.key_heads);
   pdl_wait();
   pdl_launch_dependents();
+  FPSCAN_DEBUG_ONLY(const int64_t n_tok = p.batch * p.L, n_state = p.batch * p.heads * p.dv * p.dk;)
 
   float4 S[kStepRows][VEC];
 #pragma unroll
@@ -72,7 +74,8 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const StepPara
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int c = (i * 8 + part) * 4;
-      S[r][i] = p.initial != nullptr && row < p.dv && c < p.dk
+      S[r][i] = p.initial != nullptr && row < p.dv && c < p.dk FPSCAN_DEBUG_ONLY(
+                                                                  && in_bounds(src + c, 16, p.initial, p.initial + n_state))
                     ? __ldcs(reinterpret_cast<const float4*>(src + c))
                     : make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -87,20 +90,28 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const StepPara
     for (int i = 0; i < VEC; ++i) {
       const int c = (i * 8 + part) * 4;
       k[i] = q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (c < p.dk) {
+      if (c < p.dk FPSCAN_DEBUG_ONLY(
+                       && within<T, 4 * sizeof(T)>(kp + c, 4, p.k, n_tok * p.key_heads * p.dk)
+                       && within<T, 4 * sizeof(T)>(qp + c, 4, p.q, n_tok * p.key_heads * p.dk))) {
         k[i] = load4(kp + c);
         q[i] = load4(qp + c);
       }
       qk = dot4(k[i], q[i], qk);
     }
+    FPSCAN_DEBUG_ONLY(
+        if (!within<T, sizeof(T)>(static_cast<const T*>(p.log_decay) + tok * p.heads + h, 1, p.log_decay, n_tok * p.heads) ||
+            !within<T, sizeof(T)>(static_cast<const T*>(p.beta) + tok * p.heads + h, 1, p.beta, n_tok * p.heads)) return;)
     const float a = expf(Elem<T>::load(static_cast<const T*>(p.log_decay)[tok * p.heads + h]));
     const float beta = Elem<T>::load(static_cast<const T*>(p.beta)[tok * p.heads + h]);
     float v[kStepRows], sk[kStepRows], sq[kStepRows];
 #pragma unroll
     for (int r = 0; r < kStepRows; ++r) {
       const int row = row0 + r * (kStepThreads / 8);
-      v[r] = row < p.dv ? Elem<T>::load(static_cast<const T*>(p.v)[(tok * p.heads + h) * p.dv + row])
-                        : 0.f;
+      v[r] = row < p.dv FPSCAN_DEBUG_ONLY(
+                 && within<T, sizeof(T)>(static_cast<const T*>(p.v) + (tok * p.heads + h) * p.dv + row, 1, p.v,
+                                         n_tok * p.heads * p.dv))
+                 ? Elem<T>::load(static_cast<const T*>(p.v)[(tok * p.heads + h) * p.dv + row])
+                 : 0.f;
       sk[r] = sq[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -132,7 +143,9 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const StepPara
         S[r][i].z = fmaf(u, k[i].z, S[r][i].z);
         S[r][i].w = fmaf(u, k[i].w, S[r][i].w);
       }
-      if (part == 0 && row < p.dv)
+      if (part == 0 && row < p.dv FPSCAN_DEBUG_ONLY(
+                           && within<T, sizeof(T)>(static_cast<T*>(p.out) + (tok * p.heads + h) * p.dv + row, 1, p.out,
+                                                   n_tok * p.heads * p.dv)))
         static_cast<T*>(p.out)[(tok * p.heads + h) * p.dv + row] =
             Elem<T>::store(p.scale * fmaf(u, qk, sq[r]));
     }
@@ -145,7 +158,9 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const StepPara
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int c = (i * 8 + part) * 4;
-      if (row < p.dv && c < p.dk) __stcs(reinterpret_cast<float4*>(dst + c), S[r][i]);
+      if (row < p.dv && c < p.dk FPSCAN_DEBUG_ONLY(
+                            && in_bounds(dst + c, 16, p.final_state, p.final_state + n_state)))
+        __stcs(reinterpret_cast<float4*>(dst + c), S[r][i]);
     }
   }
 }
@@ -170,7 +185,7 @@ cudaError_t step_t(const DeltaArgs& a, const StepParams& p) {
 cudaError_t launch_delta_step(const DeltaArgs& a) {
   StepParams p{a.q, a.k, a.v, a.log_decay, a.beta, a.initial, a.final_state, a.out, a.seqlen,
                (int)a.key_heads, (int)a.heads, (int)a.dk, (int)a.dv,
-               (int)((a.dv + kStepCta - 1) / kStepCta), a.scale};
+               (int)((a.dv + kStepCta - 1) / kStepCta), a.scale, a.batch};
   switch (a.dtype) {
     case kF32:
       return step_t<float>(a, p);

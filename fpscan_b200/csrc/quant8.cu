@@ -29,10 +29,11 @@ struct Quant8Params {
 
 // A 16-byte vector from p; values at or past `left` are 0.
 template <typename T>
-__device__ __forceinline__ uint4 load_vec(const T* p, int64_t left) {
+__device__ __forceinline__ uint4 load_vec(const T* p, int64_t left FPSCAN_DEBUG_ONLY(, const T* lo, const T* hi)) {
   constexpr int V = Elem<T>::kVec;
   Vec16<T> v;
   v.raw = make_uint4(0, 0, 0, 0);
+  FPSCAN_DEBUG_ONLY(if (left > 0 && !in_bounds(p, (left < V ? left : V) * sizeof(T), lo, hi)) return v.raw;)
   if (left >= V) {
     v.raw = *reinterpret_cast<const uint4*>(p);
   } else {
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const Quant8Params p) {
     constexpr int V = Elem<T>::kVec;
     uint4 raw[16 / V];
 #pragma unroll
-    for (int j = 0; j < 16 / V; ++j) raw[j] = load_vec(src + i + j * V, left - j * V);
+    for (int j = 0; j < 16 / V; ++j) raw[j] = load_vec(src + i + j * V, left - j * V FPSCAN_DEBUG_ONLY(, src, src + p.n));
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 16 / V; ++j) most = quant8_max<T>(most, quant8_max<T>(raw[j]));
@@ -73,13 +74,17 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const Quant8Params p) {
       w[c] = quant8_codes<T>(q, Elem<T>::load(y[0]), Elem<T>::load(y[1]), Elem<T>::load(y[2]),
                              Elem<T>::load(y[3]));
     }
+    // (a block's lanes behind the tensor's end hold nothing)
+    FPSCAN_DEBUG_ONLY(if (left > 0 && !in_bounds(p.codes + i, left < 16 ? left : 16, p.codes, p.codes + p.n)) continue;)
     if (left >= 16)
       *reinterpret_cast<uint4*>(p.codes + i) = make_uint4(w[0], w[1], w[2], w[3]);
     else
 #pragma unroll
       for (int c = 0; c < 16; ++c)
         if (c < left) p.codes[i + c] = (int8_t)(w[c / 4] >> (8 * (c & 3)));
-    if ((u & 3) == 0) p.steps[u / 4] = q.step;
+    if ((u & 3) == 0 FPSCAN_DEBUG_ONLY(
+                         && in_bounds<4>(p.steps + u / 4, 4, p.steps, p.steps + (p.n + kBlock8 - 1) / kBlock8)))
+      p.steps[u / 4] = q.step;
   }
 }
 
@@ -91,6 +96,11 @@ __global__ void __launch_bounds__(256) dequantize8_kernel(const Quant8Params p) 
   T* dst = static_cast<T*>(p.out);
   for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += step) {
     const int64_t i = u * 8, left = p.n - i;
+    FPSCAN_DEBUG_ONLY(
+        const int64_t some = left < 8 ? left : 8;
+        if (!in_bounds<4>(p.steps_in + u / 8, 4, p.steps_in, p.steps_in + (p.n + kBlock8 - 1) / kBlock8) ||
+            !in_bounds<8>(p.codes_in + i, some, p.codes_in, p.codes_in + p.n) ||
+            !in_bounds(dst + i, some * sizeof(T), dst, dst + p.n)) continue;)
     const float s = p.steps_in[u / 8];
     if (left >= 8) {
       const uint2 w = *reinterpret_cast<const uint2*>(p.codes_in + i);

@@ -184,6 +184,9 @@ __global__ void __launch_bounds__(NTH, 1)
   T* out2 = static_cast<T*>(p.out2);
   const int64_t row_elems = p.dv * V;
   const int64_t base = (b * L) * row_elems + cv * V;
+  // elements of the 8-bit format's tensors
+  FPSCAN_DEBUG_ONLY(const int64_t n_seq = p.n_el / (L * row_elems); const int64_t n_steps = n_seq * ((L + 7) / 8) * p.dv;
+                    const int64_t n_codes = n_seq * L * p.code_stride;)
 
   float seg_a[V];  // SPLIT 1: product of the segment's gates (thread group NG-1)
 #pragma unroll
@@ -203,8 +206,10 @@ __global__ void __launch_bounds__(NTH, 1)
     float y_step = 0.f, y_step_prev = 0.f;
     if (BWD && Q8 && SPLIT != 1 && lane_ok && blk0 < L) {
       const float* sp = p.steps + (b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv;
+      FPSCAN_DEBUG_ONLY(if (in_bounds<4>(sp, 4, p.steps, p.steps + n_steps)))
       y_step = sp[0];
-      if (blk0 > 0) y_step_prev = sp[-p.dv];
+      if (blk0 > 0 FPSCAN_DEBUG_ONLY(&& in_bounds<4>(sp - p.dv, 4, p.steps, p.steps + n_steps)))
+        y_step_prev = sp[-p.dv];
     }
     const bool ok = mbar_wait_bounded(&s_bar[s], phase);
     const uint4* s_a = reinterpret_cast<const uint4*>(csm + s * Cfg::kStageBytes);
@@ -345,7 +350,11 @@ __global__ void __launch_bounds__(NTH, 1)
 #pragma unroll
       for (int i = 0; i < TW; ++i) most = quant8_max<T>(most, blk0 + i < L ? quant8_max<T>(kept[i]) : 0);
       const Quant8 q8 = quant8_block<T>(quant8_bits<T>(most));
-      if (lane_ok && blk0 < L) p.steps[(b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv] = q8.step;
+      if (lane_ok && blk0 < L) {
+        float* sp = p.steps + (b * ((L + 7) / 8) + blk0 / 8) * p.dv + cv;
+        FPSCAN_DEBUG_ONLY(if (in_bounds<4>(sp, 4, p.steps, p.steps + n_steps)))
+        *sp = q8.step;
+      }
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
         float y[V];
@@ -356,6 +365,7 @@ __global__ void __launch_bounds__(NTH, 1)
           w[c / 4] = quant8_codes<T>(q8, y[c], y[c + 1], y[c + 2], y[c + 3]);
         if (lane_ok && blk0 + i < L) {
           int8_t* o = p.codes + (b * L + blk0 + i) * p.code_stride + cv * V;
+          FPSCAN_DEBUG_ONLY(if (!in_bounds<V>(o, V, p.codes, p.codes + n_codes)) continue;)
           if constexpr (V == 8)
             *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
           else
