@@ -203,6 +203,11 @@ void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+void check_written(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+              " requires a gradient, which writing it here would lose: detach it");
+}
+
 float* state_ptr(const c10::optional<at::Tensor>& t) {
   return t && t->numel() ? t->data_ptr<float>() : nullptr;
 }
@@ -211,6 +216,8 @@ at::Tensor delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor
                       const at::Tensor& log_decay, const at::Tensor& beta, at::Tensor state,
                       double scale, const c10::optional<at::Tensor>& out_) {
   const DeltaSizes s = check_delta(q, k, v, log_decay, beta, state, out_);
+  check_written(state, "state");
+  if (out_) check_written(*out_, "out");
   const c10::cuda::CUDAGuard guard(v.device());
   at::Tensor out = out_ ? *out_ : at::empty_like(v);
   raise_on(fpscan_delta_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
@@ -228,6 +235,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> delta_forward(
     const at::Tensor& beta_, const c10::optional<at::Tensor>& initial, double scale,
     bool return_state, const c10::optional<at::Tensor>& out_) {
   const DeltaSizes s = check_delta(q, k, v, log_decay_, beta_, initial, out_);
+  if (out_) check_written(*out_, "out");
   const c10::cuda::CUDAGuard guard(v.device());
   const at::Tensor log_decay = aligned(log_decay_), beta = aligned(beta_);
   const bool wide = initial || return_state;

@@ -132,10 +132,11 @@ int check_dtype(int dtype) {
   return FPSCAN_OK;
 }
 
-int check_ptr(const void* p, const char* name, int align = 16) {
+// align: a power of two
+int check_ptr(const void* p, const char* name, uintptr_t align = 16) {
   if (p == nullptr) return fail(FPSCAN_ERR_INVALID, "%s is NULL", name);
-  if (reinterpret_cast<uintptr_t>(p) % align != 0)
-    return fail(FPSCAN_ERR_INVALID, "%s must be %d-byte aligned", name, align);
+  if ((reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0)
+    return fail(FPSCAN_ERR_INVALID, "%s must be %d-byte aligned", name, (int)align);
   return FPSCAN_OK;
 }
 
@@ -790,7 +791,7 @@ struct Operand {
   const void* ptr;
   int64_t bytes;
   bool written;
-  int align = 16;
+  uintptr_t align = 16;
 };
 
 // Every operand present (ptr non-null), aligned, and none that is written
@@ -964,7 +965,7 @@ int fpscan_delta_step(const void* q, const void* k, const void* v, const void* l
   if (batch == 0) return ok();
   const int64_t es = dtype_size(dtype), tok = batch * seqlen, st = batch * heads * dv * dk * 4;
   const bool in_place = initial != nullptr && initial == final_state;
-  const int each = (int)es;  // read or written one element at a time
+  const uintptr_t each = (uintptr_t)es;  // read or written one element at a time
   const Operand ops[] = {{"q", q, tok * key_heads * dk * es, false},
                          {"k", k, tok * key_heads * dk * es, false},
                          {"v", v, tok * heads * dv * es, false, each},

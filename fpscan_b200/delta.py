@@ -93,9 +93,9 @@ def validate_delta_layout(q, k, v, log_decay, beta, state=None, out=None) -> Non
             raise RuntimeError("out must be contiguous")
 
 
-def _check_out(out) -> None:
-    if isinstance(out, torch.Tensor) and out.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("out requires a gradient, which writing it here would lose: detach it")
+def _check_written(t: Optional[torch.Tensor], name: str) -> None:
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, which writing it here would lose: detach it")
 
 
 def _written(*tensors) -> None:
@@ -142,6 +142,7 @@ def _run_forward(q, k, v, log_decay, beta, state, scale, return_state, out=None)
         return _EXT.delta_forward(q, k, v, log_decay, beta, _state_in(state), scale, return_state, out)
     _lib.load()
     validate_delta(q, k, v, log_decay, beta, state, out)
+    _check_written(out, "out")
     state, log_decay, beta = _state_in(state), _aligned(log_decay), _aligned(beta)
     wide = state is not None or return_state
     given = out
@@ -164,7 +165,6 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_d
                         ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """The gated delta rule over a sequence (no autograd): ``out``, or ``(out, final_state)`` with
     ``return_state``.  ``scale`` defaults to ``dk ** -0.5``; ``initial_state`` to zero."""
-    _check_out(out)
     out, final = _run_forward(q, k, v, log_decay, beta, initial_state, _scale(scale, q), bool(return_state), out)
     return (out, final) if return_state else out
 
@@ -178,12 +178,11 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     if not (isinstance(state, torch.Tensor) and state.is_cuda and state.dtype == torch.float32
             and state.is_contiguous()):
         raise RuntimeError("state must be a contiguous float32 CUDA tensor")
-    if state.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("state requires a gradient, which an update in place would lose: detach it")
-    _check_out(out)
     if _tensors(q, k, v, log_decay, beta, out):
         return _EXT.delta_step(q, k, v, log_decay, beta, state, _scale(scale, q), out)
     validate_delta(q, k, v, log_decay, beta, state, out)
+    _check_written(state, "state")
+    _check_written(out, "out")
     given = out
     if out is None:
         out = torch.empty_like(v)
