@@ -106,9 +106,12 @@ struct StreamParams {
 // backward reads that in place of y (tm_c covers the codes).  A block of the
 // format is what one thread holds in a chunk, 8 timesteps x one 16-byte
 // channel vector, so its magnitude needs no exchange between threads.
-// 8 x 8192 x 2048 bf16: forward 231 us (0.95 GB, 4.1 TB/s; 256 columns are
-// 1.7 waves of one CTA per SM, and eight warps issue for half of the time),
-// backward 273 us (1.2 GB, 4.5 TB/s).
+// 8 x 8192 x 2048 bf16: forward 231 us (0.95 GB, 4.1 TB/s), backward 273 us
+// (1.2 GB, 4.5 TB/s), against 161 and 231 us without the format: it saves
+// memory, not time.  What it costs is its instructions on an SM's eight warps
+// (8 x 2048 x 2048, forward: 30.8 million a launch against 19.3, 68.5 us
+// against 49.7, issuing in half of the cycles both times); 256 columns are 1.7
+// waves of one CTA per SM with it and without.
 template <typename T, int MODE, int TW, int S, int NTH, int SPLIT = 0, bool Q8 = false>
 __global__ void __launch_bounds__(NTH, 1)
     scan_cl_stream_kernel(const __grid_constant__ StreamParams p) {
